@@ -1,0 +1,785 @@
+// Products with weights in MX4 (csrc/mx4.h has their layout): y = x W^T, and the experts' products of tokens routed to them.
+//
+// A weight is a 4-bit code times a power of two: exact in bf16, which the matrix cores multiply at full rate with sums
+// in 32 bits.  Activations are taken as one, two or three bf16 numbers each (bf16, f16, f32: 8, 11, 24 bits of
+// significand in parts of 8), so every product is exact in every type.  Codes become bf16 pairs with one instruction a pair, which
+// also multiplies by the scale, in the registers of the wave that uses them: what comes from memory is 17 bytes for 32 weights.
+#include <algorithm>
+#include <new>
+
+#include "mx4.h"
+
+namespace tetris {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// What a launch writes: numbers of a type, or (between the experts' products) bf16 parts of numbers.
+enum { kOutF32 = TETRIS_F32, kOutF16 = TETRIS_F16, kOutBF16 = TETRIS_BF16, kOutParts2, kOutParts3 };
+
+struct Product {
+  const void* x;         // rows of ldx elements that start on 16 bytes; elements k .. k8 - 1 of a row are zero
+  int64_t ldx, part;     // part: elements between the parts' arrays
+  int parts, k8, rows;   // rows of all groups together
+  const i32x4* codes;    // laid-out weights
+  const uint8_t* scales;
+  int row_tiles, col_tiles, n, gated;
+  // Rows in groups, one for each expert: positions offsets[e] .. offsets[e + 1] - 1 are expert e's, position p standing for slot
+  // order[p].  NULL: one group, position = row.
+  const int* offsets;
+  const int* order;
+  int experts;
+  int from_div;          // > 0: position p reads row order[p] / from_div; 0: row p
+  int to_slot;           // position p writes row order[p], else row p
+  int max_tiles;         // of rows, over all groups
+  void* y;
+  int64_t ldy, y_part;
+  int out, vec_out;      // vec_out: four neighbouring outputs may be stored at once
+  const float* bias;
+};
+
+// Which rows a workgroup has: tile `tile` of the groups' tiles of `size` rows, numbered through.  Every wave finds it for itself.
+__device__ inline bool find_tile(const Product& a, int tile, int size, int* expert, int* first, int* count) {
+  if (!a.offsets) {
+    *expert = 0;
+    *first = tile * size;
+    *count = min(size, a.rows - tile * size);
+    return *count > 0;
+  }
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int base = 0; base < a.experts; base += 64) {
+    const int e = base + lane;
+    const int lo = a.offsets[min(e, a.experts)], hi = a.offsets[min(e + 1, a.experts)];
+    const int tiles = (hi - lo + size - 1) / size;
+    int sum = tiles;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int v = __shfl_up(sum, d);
+      if (lane >= d) sum += v;
+    }
+    const unsigned long long here = __ballot(tile < before + sum);
+    if (here) {
+      const int l = __builtin_ctzll(here);
+      const int t = tile - before - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(tiles, l));
+      *expert = base + l;
+      *first = __builtin_amdgcn_readlane(lo, l) + t * size;
+      *count = min(size, __builtin_amdgcn_readlane(hi, l) - *first);
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(sum, 63);
+  }
+  return false;
+}
+
+// Eight codes and their scale's exponent bits to bf16.
+__device__ inline bf16x8 weights8(int codes, float scale) {
+  i32x4 v;
+  v.x = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)codes, scale, 0));
+  v.y = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)codes, scale, 1));
+  v.z = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)codes, scale, 2));
+  v.w = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)codes, scale, 3));
+  return __builtin_bit_cast(bf16x8, v);
+}
+
+__device__ inline float silu(float v) { return v / (1.f + expf(-v)); }
+
+// the leading 16 bits of v that are a bf16 number, and what is left (csrc/mx4_quantize.hip, split)
+__device__ inline unsigned leading(float& v) {
+  unsigned u = __float_as_uint(v);
+  if ((u & 0x7f800000u) == 0x7f800000u) {
+    if (u & 0x007fffffu) u |= 0x00400000u;
+    v = 0.f;
+  } else {
+    v -= __uint_as_float(u & 0xffff0000u);
+  }
+  return u >> 16;
+}
+
+__device__ inline void store1(const Product& a, int64_t at, float v) {
+  switch (a.out) {
+    case kOutF32: static_cast<float*>(a.y)[at] = v; break;
+    case kOutF16: static_cast<_Float16*>(a.y)[at] = (_Float16)v; break;
+    case kOutBF16: static_cast<__bf16*>(a.y)[at] = (__bf16)v; break;
+    default:
+      for (int p = 0; p < (a.out == kOutParts2 ? 2 : 3); ++p)
+        static_cast<unsigned short*>(a.y)[at + p * a.y_part] = (unsigned short)leading(v);
+  }
+}
+
+// four neighbouring outputs
+__device__ inline void store4(const Product& a, int64_t at, const float (&v)[4]) {
+  switch (a.out) {
+    case kOutF32: *reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + at) = f32x4{v[0], v[1], v[2], v[3]}; break;
+    case kOutF16: {
+      typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+      *reinterpret_cast<half4*>(static_cast<_Float16*>(a.y) + at) = half4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+      break;
+    }
+    case kOutBF16: {
+      typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+      *reinterpret_cast<bf16x4*>(static_cast<__bf16*>(a.y) + at) = bf16x4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+      break;
+    }
+    default: {
+      float w[4] = {v[0], v[1], v[2], v[3]};
+      for (int p = 0; p < (a.out == kOutParts2 ? 2 : 3); ++p) {
+        uint2 u;
+        u.x = leading(w[0]); u.x |= leading(w[1]) << 16;
+        u.y = leading(w[2]); u.y |= leading(w[3]) << 16;
+        *reinterpret_cast<uint2*>(static_cast<unsigned short*>(a.y) + at + p * a.y_part) = u;
+      }
+    }
+  }
+}
+
+// Four outputs of one row from feature f on.  A gated launch writes all of a tile's features: its rows are padded, and those past
+// the last feature have to be zero for the product that reads them.
+__device__ inline void put4(const Product& a, int64_t row, int f, float (&v)[4]) {
+  const int n = a.gated ? a.n / 2 : a.n;
+  if (a.bias) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += f + i < n ? a.bias[f + i] : 0.f;
+  }
+  const int64_t at = row * a.ldy + f;
+  if (a.gated) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = f + i < n ? v[i] : 0.f;
+    store4(a, at, v);
+  } else if (a.vec_out && f + 4 <= n) {
+    store4(a, at, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (f + i < n) store1(a, at + i, v[i]);
+  }
+}
+
+// ---- many rows: tiles through LDS ---------------------------------------------------------------------------------
+//
+// A workgroup computes BM = 32 WT WM rows by 32 WR WN features.  Rows come in steps of 64 columns, 128 bytes of each row
+// in one stretch, through registers into one of two LDS buffers while the other is multiplied; weights come straight
+// from memory to the registers that use them, a step ahead.  Row r's 16-byte piece p lies at piece p ^ (r / 2 % 8) of its
+// 128 bytes: the sixteen lanes that an LDS read serves at once then touch all 64 banks.
+template <int WT, int WR, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Product a) {
+  constexpr int kRows = 32 * WT * WM, kThreads = 64 * WM * WN, kLoads = kRows * 8 / kThreads;
+  __shared__ i32x4 lds[2][kRows * 8];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave % WM, wn = wave / WM;
+
+  const int row_blocks = (a.row_tiles + WR * WN - 1) / (WR * WN);
+  const int id = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);  // neighbouring tiles on one of the eight L2s
+  if (id >= row_blocks * a.max_tiles) return;
+  constexpr int kBand = 4;  // tiles of rows that share the weights they read
+  const int band = id / (row_blocks * kBand), in_band = id - band * row_blocks * kBand;
+  const int wide = min(kBand, a.max_tiles - band * kBand);
+  const int block = in_band / wide, tile = band * kBand + in_band - block * wide;
+  int expert, first, count;
+  if (!find_tile(a, tile, kRows, &expert, &first, &count)) return;
+
+  const __bf16* from[kLoads];
+  int column[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int q = i * kThreads + threadIdx.x, r = q >> 3, piece = (q & 7) ^ ((r >> 1) & 7);
+    const int p = first + min(r, count - 1);
+    const int64_t row = a.from_div ? a.order[p] / a.from_div : p;
+    column[i] = piece * 8;
+    from[i] = static_cast<const __bf16*>(a.x) + row * a.ldx + column[i];
+  }
+  const i32x4* codes[WR];
+  const uint8_t* scales[WR];
+#pragma unroll
+  for (int r = 0; r < WR; ++r) {
+    const int64_t t = (int64_t)expert * a.row_tiles + min((block * WN + wn) * WR + r, a.row_tiles - 1);
+    codes[r] = a.codes + t * a.col_tiles * 64 + lane;
+    scales[r] = a.scales + t * a.col_tiles * 64 + lane * 2;
+  }
+
+  f32x16 acc[WT][WR];
+#pragma unroll
+  for (int t = 0; t < WT; ++t)
+#pragma unroll
+    for (int r = 0; r < WR; ++r) acc[t][r] = f32x16{};
+
+  i32x4 next_x[kLoads], next_w[WR], w[WR];
+  unsigned next_s[WR];
+  float s[WR];
+  int col = 0, part = 0;
+  auto fetch = [&]() {  // column tile `col` of part `part`
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const bool in = col * 64 + column[i] < a.k8;
+      const i32x4 v = *reinterpret_cast<const i32x4*>(from[i] + part * a.part + (in ? col * 64 : -column[i]));
+      next_x[i] = in ? v : i32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int r = 0; r < WR; ++r) {
+      next_w[r] = codes[r][(int64_t)col * 64];
+      next_s[r] = scales[r][(int64_t)(col >> 1) * 128 + (col & 1)];
+    }
+    if (++part == a.parts) part = 0, ++col;
+  };
+  auto keep = [&](int buffer) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) lds[buffer][i * kThreads + threadIdx.x] = next_x[i];
+#pragma unroll
+    for (int r = 0; r < WR; ++r) w[r] = next_w[r], s[r] = __uint_as_float(next_s[r] << 23);
+  };
+
+  const int steps = a.col_tiles * a.parts;
+  const int row_in = wm * WT * 32 + (lane & 31), turn = (lane >> 1) & 7, half = lane >> 5;
+  fetch();
+  keep(0);
+  for (int step = 0; step < steps; ++step) {
+    __syncthreads();
+    if (step + 1 < steps) fetch();
+    const i32x4* in = lds[step & 1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      bf16x8 xs[WT], ws[WR];
+#pragma unroll
+      for (int t = 0; t < WT; ++t) xs[t] = __builtin_bit_cast(bf16x8, in[(row_in + t * 32) * 8 + ((half * 4 + j) ^ turn)]);
+#pragma unroll
+      for (int r = 0; r < WR; ++r) ws[r] = weights8(w[r][j], s[r]);
+#pragma unroll
+      for (int t = 0; t < WT; ++t)
+#pragma unroll
+        for (int r = 0; r < WR; ++r) acc[t][r] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ws[r], xs[t], acc[t][r], 0, 0, 0);
+    }
+    if (step + 1 < steps) keep((step + 1) & 1);
+  }
+
+#pragma unroll
+  for (int t = 0; t < WT; ++t) {
+    const int r_in = row_in + t * 32;
+    if (r_in >= count) continue;
+    const int64_t row = a.to_slot ? a.order[first + r_in] : first + r_in;
+#pragma unroll
+    for (int r = 0; r < WR; ++r) {
+      const int row_tile = (block * WN + wn) * WR + r;
+      if (row_tile >= a.row_tiles) continue;
+      if (a.gated) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          float v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] = silu(acc[t][r][q * 4 + i]) * acc[t][r][8 + q * 4 + i];
+          put4(a, row, row_tile * 16 + q * 8 + half * 4, v);
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v[4] = {acc[t][r][q * 4], acc[t][r][q * 4 + 1], acc[t][r][q * 4 + 2], acc[t][r][q * 4 + 3]};
+          put4(a, row, row_tile * 32 + q * 8 + half * 4, v);
+        }
+      }
+    }
+  }
+}
+
+// ---- few rows: weights streamed once -----------------------------------------------------------------------------------
+//
+// A workgroup computes 16 RT features for up to 16 TT rows; its waves take turns at stretches of 128 columns and add their sums
+// in LDS at the end, in the order of the waves.  Bound by the weights' bytes: a lane loads 16 bytes of codes, whose
+// 32 weights feed four 16 x 16 x 32 products, and the rows' numbers come from the caches, split into parts in registers.
+template <int TYPE>
+__device__ inline void parts8(const typename Elem<TYPE>::type* p, bool in, bf16x8 (&out)[TYPE == TETRIS_F32 ? 3 : TYPE == TETRIS_F16 ? 2 : 1]) {
+  if constexpr (TYPE == TETRIS_BF16) {
+    out[0] = __builtin_bit_cast(bf16x8, in ? *reinterpret_cast<const i32x4*>(p) : i32x4{0, 0, 0, 0});
+  } else {
+    constexpr int P = TYPE == TETRIS_F32 ? 3 : 2;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (in) {
+      if constexpr (TYPE == TETRIS_F32) {
+        const f32x4 u = reinterpret_cast<const f32x4*>(p)[0], t = reinterpret_cast<const f32x4*>(p)[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = u[i], v[4 + i] = t[i];
+      } else {
+        typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+        const half8 u = *reinterpret_cast<const half8*>(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)u[i];
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+      i32x4 o;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned lo = leading(v[2 * i]), hi = leading(v[2 * i + 1]);
+        o[i] = (int)(lo | hi << 16);
+      }
+      out[q] = __builtin_bit_cast(bf16x8, o);
+    }
+  }
+}
+
+template <int TYPE, int TT, int RT>
+__global__ __launch_bounds__(TT == 1 ? 1024 : 512) void stream_kernel(Product a) {
+  using T = typename Elem<TYPE>::type;
+  constexpr int P = TYPE == TETRIS_F32 ? 3 : TYPE == TETRIS_F16 ? 2 : 1;
+  extern __shared__ float sums[];  // [wave][RT][TT][4][64]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int halves = a.row_tiles * 2, blocks = (halves + RT - 1) / RT;
+  const int tile = blockIdx.x / blocks, block = blockIdx.x - tile * blocks;
+  int expert, first, count;
+  if (!find_tile(a, tile, 16 * TT, &expert, &first, &count)) return;
+
+  const int r16 = lane & 15, g = lane >> 4;
+  const T* from[TT];
+  bool have[TT];
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+    have[t] = t * 16 + r16 < count;
+    const int p = first + min(t * 16 + r16, count - 1);
+    const int64_t row = a.from_div ? a.order[p] / a.from_div : p;
+    from[t] = static_cast<const T*>(a.x) + row * a.ldx + 32 * g;
+  }
+  const i32x4* codes[RT];
+  const uint8_t* scales[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int h = min(block * RT + r, halves - 1);
+    const int64_t t = ((int64_t)expert * a.row_tiles + (h >> 1)) * a.col_tiles;
+    const int l = (g & 1) * 32 + (h & 1) * 16 + r16;
+    codes[r] = a.codes + (t + (g >> 1)) * 64 + l;
+    scales[r] = a.scales + t * 64 + l * 2 + (g >> 1);
+  }
+  f32x4 acc[RT][TT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int t = 0; t < TT; ++t) acc[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const int chunks = a.col_tiles >> 1;
+  for (int c = wave; c < chunks; c += waves) {
+    i32x4 w[RT];
+    float s[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      w[r] = codes[r][(int64_t)c * 128];
+      s[r] = __uint_as_float((unsigned)scales[r][(int64_t)c * 128] << 23);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      bf16x8 ws[RT];
+#pragma unroll
+      for (int r = 0; r < RT; ++r) ws[r] = weights8(w[r][j], s[r]);
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        bf16x8 xs[P];
+        parts8<TYPE>(from[t] + c * 128 + j * 8, have[t] && c * 128 + 32 * g + j * 8 < a.k8, xs);
+#pragma unroll
+        for (int q = 0; q < P; ++q)
+#pragma unroll
+          for (int r = 0; r < RT; ++r) acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ws[r], xs[q], acc[r][t], 0, 0, 0);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sums[(((wave * RT + r) * TT + t) * 4 + i) * 64 + lane] = acc[r][t][i];
+  __syncthreads();
+
+  const int n = a.gated ? a.n / 2 : a.n;
+  auto sum = [&](int r, int row, int f) {
+    const int at = ((r * TT + (row >> 4)) * 4 + (f & 3)) * 64 + (f >> 2) * 16 + (row & 15);
+    float v = 0.f;
+    for (int w = 0; w < waves; ++w) v += sums[w * (RT * TT * 256) + at];
+    return v;
+  };
+  if (a.gated) {
+    if constexpr (RT == 2) {
+      for (int i = threadIdx.x; i < TT * 256; i += blockDim.x) {
+        const int row = i >> 4, f = i & 15;
+        if (row >= count) break;
+        const float v = silu(sum(0, row, f)) * sum(1, row, f);
+        const int64_t to = a.to_slot ? a.order[first + row] : first + row;
+        store1(a, to * a.ldy + block * 16 + f, block * 16 + f < n ? v : 0.f);
+      }
+    }
+  } else {
+    for (int i = threadIdx.x; i < RT * TT * 256; i += blockDim.x) {
+      const int row = i / (16 * RT), f = i - row * (16 * RT), feature = block * RT * 16 + f;
+      if (row >= count) break;
+      if (feature >= n) continue;
+      const float v = sum(f >> 4, row, f & 15) + (a.bias ? a.bias[feature] : 0.f);
+      const int64_t to = a.to_slot ? a.order[first + row] : first + row;
+      store1(a, to * a.ldy + feature, v);
+    }
+  }
+}
+
+// ---- routed rows ---------------------------------------------------------------------------------------------------------
+
+// Slots (token, j) in the order of their experts, those of one expert in the order of the slots.  Workgroup e finds expert e's: it
+// counts the slots of lower experts, which is where its own begin, and the matches in each wave's stretch of the slots,
+// then goes through them again and writes.  Slots of no expert are in no group.  No atomics: the order is always the same.
+__global__ __launch_bounds__(1024) void plan_kernel(const int* __restrict__ index, int slots, int experts, int* __restrict__ offsets,
+                                                    int* __restrict__ order) {
+  __shared__ int lower_of[16], match_of[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, e = blockIdx.x;
+  const int stretch = ((slots + waves - 1) / waves + 63) & ~63;
+  const int begin = min(wave * stretch, slots), end = min(begin + stretch, slots);
+  int lower = 0, match = 0;
+  for (int i = begin + lane; i < end; i += 64) {
+    const int v = index[i];
+    lower += v >= 0 && v < e;
+    match += v == e;
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    lower += __shfl_xor(lower, d);
+    match += __shfl_xor(match, d);
+  }
+  if (lane == 0) lower_of[wave] = lower, match_of[wave] = match;
+  __syncthreads();
+  int at = 0, all = 0;
+  for (int w = 0; w < waves; ++w) {
+    at += lower_of[w] + (w < wave ? match_of[w] : 0);
+    all += lower_of[w] + match_of[w];
+  }
+  if (threadIdx.x == 0) {
+    if (e == 0) offsets[0] = 0;
+    offsets[e + 1] = all;
+  }
+  for (int i = begin; i < end; i += 64) {
+    const bool mine = i + lane < end && index[i + lane] == e;
+    const unsigned long long found = __ballot(mine);
+    if (mine) order[at + __builtin_popcountll(found & ((1ull << lane) - 1))] = i + lane;
+    at += __builtin_popcountll(found);
+  }
+}
+
+// y[t] = sum over j of weight[t][j] rows[t top + j], four columns a thread; bound by the rows' bytes.
+template <int TYPE>
+__global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ rows, int64_t ld_rows, const int* __restrict__ index,
+                                                      const float* __restrict__ weight, int tokens, int top, int experts, int width,
+                                                      typename Elem<TYPE>::type* __restrict__ y, int64_t ldy, int vec) {
+  using T = typename Elem<TYPE>::type;
+  const int quads = (width + 3) / 4;
+  const int64_t total = (int64_t)tokens * quads;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t t = i / quads;
+    const int c = (int)(i - t * quads) * 4;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < top; ++j) {
+      const int e = index[t * top + j];
+      if (e < 0 || e >= experts) continue;
+      const f32x4 r = *reinterpret_cast<const f32x4*>(rows + (t * top + j) * ld_rows + c);
+      const float w = weight[t * top + j];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] = fmaf(w, r[q], v[q]);
+    }
+    T* out = y + t * ldy + c;
+    if (vec && c + 4 <= width) {
+      typedef T T4 __attribute__((ext_vector_type(4)));
+      *reinterpret_cast<T4*>(out) = T4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    } else {
+      for (int q = 0; q < 4 && c + q < width; ++q) out[q] = (T)v[q];
+    }
+  }
+}
+
+// ---- launches ------------------------------------------------------------------------------------------------------------
+
+constexpr int kStreamRows = 64;  // up to so many rows of a matrix are streamed
+
+template <int WT, int WR, int WM, int WN>
+int launch_tile(Product& a, hipStream_t stream) {
+  const int size = 32 * WT * WM, row_blocks = ceil_div(a.row_tiles, WR * WN);
+  a.max_tiles = a.offsets ? std::min(a.rows, a.rows / size + std::min(a.experts, a.rows)) : ceil_div(a.rows, size);
+  const int64_t blocks = round_up((int64_t)row_blocks * a.max_tiles, 8);
+  if (blocks > 0x7fffffff / 2) return fail(TETRIS_EINVAL, "%d rows by %d features are too many for one launch", a.rows, a.n);
+  hipLaunchKernelGGL((tile_kernel<WT, WR, WM, WN>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream, a);
+  TETRIS_HIP(hipGetLastError());
+  return TETRIS_OK;
+}
+
+template <int TYPE, int TT, int RT>
+int launch_stream(Product& a, hipStream_t stream) {
+  const int size = 16 * TT, blocks = ceil_div(a.row_tiles * 2, RT);
+  a.max_tiles = a.offsets ? std::min(a.rows, a.rows / size + std::min(a.experts, a.rows)) : ceil_div(a.rows, size);
+  const int64_t grid = (int64_t)blocks * a.max_tiles;
+  if (grid > 0x7fffffff / 2) return fail(TETRIS_EINVAL, "%d rows by %d features are too many for one launch", a.rows, a.n);
+  const int chunks = a.col_tiles / 2;
+  int waves = 8;
+  while (waves > 1 && waves > chunks) waves >>= 1;
+  hipLaunchKernelGGL((stream_kernel<TYPE, TT, RT>), dim3((unsigned)grid), dim3(64 * waves), (size_t)waves * RT * TT * 1024, stream, a);
+  TETRIS_HIP(hipGetLastError());
+  return TETRIS_OK;
+}
+
+template <int TYPE>
+int launch_stream_typed(Product& a, int rows_a_group, hipStream_t stream) {
+  if (a.gated) {
+    if (rows_a_group <= 16) return launch_stream<TYPE, 1, 2>(a, stream);
+    return launch_stream<TYPE, 2, 2>(a, stream);
+  }
+  if (rows_a_group <= 16) return launch_stream<TYPE, 1, 1>(a, stream);
+  return launch_stream<TYPE, 2, 2>(a, stream);
+}
+
+int launch_stream_any(Product& a, int type, int rows_a_group, hipStream_t stream) {
+  if (type == TETRIS_F32) return launch_stream_typed<TETRIS_F32>(a, rows_a_group, stream);
+  if (type == TETRIS_F16) return launch_stream_typed<TETRIS_F16>(a, rows_a_group, stream);
+  return launch_stream_typed<TETRIS_BF16>(a, rows_a_group, stream);
+}
+
+int launch_tile_any(Product& a, int rows_a_group, hipStream_t stream) {
+  (void)rows_a_group;
+  return launch_tile<4, 2, 2, 4>(a, stream);
+}
+
+void set_weights(Product* a, const tetris_mx4* w) {
+  a->codes = reinterpret_cast<const i32x4*>(w->codes);
+  a->scales = w->scales;
+  a->row_tiles = w->row_tiles;
+  a->col_tiles = w->col_tiles;
+  a->n = w->n;
+  a->gated = w->gated;
+}
+
+// Whether the kernels can read rows as they lie.
+bool lies_well(const void* x, int64_t ld, int k, int type) {
+  return (reinterpret_cast<size_t>(x) & 15) == 0 && (ld * elem_size(type)) % 16 == 0 && k % 8 == 0;
+}
+
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+// The workspace of (handle, stream), at least `need` bytes.  A buffer that has to grow is replaced and kept until the handle goes: a
+// captured graph may hold its address.
+int workspace(tetris_mx4* w, hipStream_t stream, size_t need, uint8_t** out) {
+  *out = nullptr;
+  if (!need) return TETRIS_OK;
+  try {
+    std::lock_guard<std::mutex> lock(w->mu);
+    tetris_mx4::Space& s = w->space[stream];
+    if (s.bytes < need) {
+      hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+      if (hipStreamIsCapturing(stream, &cap) == hipSuccess && cap != hipStreamCaptureStatusNone)
+        return fail(TETRIS_EINVAL, "this launch would allocate its workspace: prepare it before capturing");
+      w->retired.reserve(w->retired.size() + 1);
+      void* d = nullptr;
+      TETRIS_HIP(hipMalloc(&d, need));
+      if (s.ptr) w->retired.push_back(s.ptr);
+      s.ptr = d;
+      s.bytes = need;
+    }
+    *out = static_cast<uint8_t*>(s.ptr);
+    return TETRIS_OK;
+  } catch (const std::exception& e) {
+    return fail(TETRIS_EINVAL, "%s", e.what());
+  }
+}
+
+bool streams(int rows) { return rows <= kStreamRows; }
+
+// bytes that rows made ready for a product take at most
+size_t staged_bytes(int rows, int k, int type, bool rounded, bool stream) {
+  const size_t padded = (size_t)rows * round_up(k, kMxPad);
+  if (rounded) return padded * 2;
+  return padded * (stream ? elem_size(type) : 2 * parts_of(type));
+}
+
+// Points `a` at rows x of `type`, made ready in d_ready where they have to be.  *as: the type the product reads.
+int ready_rows(Product* a, const void* x, int type, int rows, int k, int64_t ld, bool rounded, bool stream, uint8_t* d_ready, int* as,
+               hipStream_t s) {
+  const int64_t padded = round_up(k, kMxPad);
+  a->rows = rows;
+  a->parts = 1;
+  a->part = 0;
+  *as = type;
+  if (rounded) {
+    a->x = d_ready;
+    a->ldx = padded;
+    a->k8 = (int)padded;
+    *as = TETRIS_BF16;
+    return mx4_quantize_to(kMxValues, x, type, rows, k, ld, d_ready, nullptr, s);
+  }
+  if (lies_well(x, ld, k, type) && (stream || type == TETRIS_BF16)) {
+    a->x = x;
+    a->ldx = ld;
+    a->k8 = k;
+    return TETRIS_OK;
+  }
+  a->x = d_ready;
+  a->ldx = padded;
+  a->k8 = (int)padded;
+  if (stream || type == TETRIS_BF16) return stage_rows(x, type, rows, k, ld, 0, d_ready, s);
+  a->parts = parts_of(type);
+  a->part = rows * padded;
+  *as = TETRIS_BF16;
+  return stage_rows(x, type, rows, k, ld, a->parts, d_ready, s);
+}
+
+int launch_product(Product& a, int as, int rows_a_group, bool stream, hipStream_t s) {
+  return stream ? launch_stream_any(a, as, rows_a_group, s) : launch_tile_any(a, rows_a_group, s);
+}
+
+int check_rows(const void* x, int type, int rows, int64_t ld, int k, const char* what) {
+  if (!x) return fail(TETRIS_EINVAL, "null argument");
+  if (ld < k) return fail(TETRIS_EINVAL, "%s: leading dimension %lld below the %d columns", what, (long long)ld, k);
+  if (reinterpret_cast<size_t>(x) % elem_size(type)) return fail(TETRIS_EINVAL, "%s not aligned to its elements", what);
+  return TETRIS_OK;
+}
+
+}  // namespace
+}  // namespace tetris
+
+using namespace tetris;
+
+extern "C" int tetris_mx4_prepare(tetris_mx4* w, int m, int type, int mx4_input, void* stream) {
+  if (!w) return fail(TETRIS_EINVAL, "null argument");
+  if (bad_type(type)) return fail(TETRIS_EINVAL, "type %d is not TETRIS_F32, TETRIS_F16 or TETRIS_BF16", type);
+  if (m < 0) return fail(TETRIS_EINVAL, "%d rows", m);
+  uint8_t* d;
+  return workspace(w, static_cast<hipStream_t>(stream), staged_bytes(m, w->k, type, mx4_input, streams(m)), &d);
+}
+
+extern "C" int tetris_mx4_linear(tetris_mx4* w, const void* d_x, int type, int m, int64_t ldx, void* d_y, int64_t ldy,
+                                 const float* d_bias, int mx4_input, void* stream) {
+  if (!w) return fail(TETRIS_EINVAL, "null argument");
+  if (bad_type(type)) return fail(TETRIS_EINVAL, "type %d is not TETRIS_F32, TETRIS_F16 or TETRIS_BF16", type);
+  if (w->gated || w->experts != 1) return fail(TETRIS_EINVAL, "one matrix that is not gated is needed, these are %d%s", w->experts, w->gated ? ", gated" : "");
+  if (m < 0) return fail(TETRIS_EINVAL, "%d rows", m);
+  if (m == 0) return TETRIS_OK;
+  int rc = check_rows(d_x, type, m, ldx, w->k, "input");
+  if (!rc) rc = check_rows(d_y, type, m, ldy, w->n, "output");
+  if (rc) return rc;
+  if (reinterpret_cast<size_t>(d_bias) & 3) return fail(TETRIS_EINVAL, "bias not aligned to its elements");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool stream_it = streams(m);
+  const bool as_it_lies = !mx4_input && lies_well(d_x, ldx, w->k, type) && (stream_it || type == TETRIS_BF16);
+  uint8_t* d = nullptr;
+  if (!as_it_lies && (rc = workspace(w, s, staged_bytes(m, w->k, type, mx4_input, stream_it), &d))) return rc;
+  Product a{};
+  set_weights(&a, w);
+  int as;
+  if ((rc = ready_rows(&a, d_x, type, m, w->k, ldx, mx4_input, stream_it, d, &as, s))) return rc;
+  a.y = d_y;
+  a.ldy = ldy;
+  a.out = type;
+  a.vec_out = ldy % 4 == 0 && (reinterpret_cast<size_t>(d_y) & (4 * elem_size(type) - 1)) == 0;
+  a.bias = d_bias;
+  return launch_product(a, as, m, stream_it, s);
+}
+
+namespace {
+
+struct ExpertSpace {
+  size_t offsets, order, hidden, rows, ready, all;
+};
+
+ExpertSpace expert_space(const tetris_mx4* up, const tetris_mx4* down, int tokens, int top, int type, bool stream) {
+  const size_t slots = (size_t)tokens * top;
+  ExpertSpace e;
+  e.offsets = 0;
+  e.order = up256(e.offsets + 4 * ((size_t)up->experts + 1));
+  e.hidden = up256(e.order + 4 * slots);
+  e.rows = up256(e.hidden + slots * round_up(down->k, kMxPad) * (stream ? elem_size(type) : 2 * parts_of(type)));
+  e.ready = up256(e.rows + slots * round_up(down->n, 4) * 4);
+  e.all = e.ready + staged_bytes(tokens, up->k, type, false, stream);
+  return e;
+}
+
+int experts_check(const tetris_mx4* up, const tetris_mx4* down, int tokens, int top, int type) {
+  if (!up || !down) return fail(TETRIS_EINVAL, "null argument");
+  if (bad_type(type)) return fail(TETRIS_EINVAL, "type %d is not TETRIS_F32, TETRIS_F16 or TETRIS_BF16", type);
+  if (!up->gated || down->gated || up->experts != down->experts || up->n != 2 * down->k || up->k != down->n)
+    return fail(TETRIS_EINVAL, "experts of %d x %d x %d%s and %d x %d x %d%s do not follow each other", up->experts, up->n, up->k,
+                up->gated ? " gated" : "", down->experts, down->n, down->k, down->gated ? " gated" : "");
+  if (tokens < 0 || top <= 0 || top > 1024 || (int64_t)tokens * top > (1 << 28)) return fail(TETRIS_EINVAL, "%d tokens of %d experts each", tokens, top);
+  return TETRIS_OK;
+}
+
+// rows of a group, were all groups alike
+int rows_a_group(const tetris_mx4* up, int tokens, int top) { return (int)(((int64_t)tokens * top + up->experts - 1) / up->experts); }
+
+}  // namespace
+
+extern "C" int tetris_experts_prepare(tetris_mx4* up, tetris_mx4* down, int tokens, int top, int type, void* stream) {
+  const int rc = experts_check(up, down, tokens, top, type);
+  if (rc || tokens == 0) return rc;
+  uint8_t* d;
+  return workspace(up, static_cast<hipStream_t>(stream), expert_space(up, down, tokens, top, type, streams(rows_a_group(up, tokens, top))).all, &d);
+}
+
+extern "C" int tetris_experts(tetris_mx4* up, tetris_mx4* down, const void* d_x, int type, int tokens, int64_t ldx, int top,
+                              const int32_t* d_index, const float* d_weight, void* d_y, int64_t ldy, void* stream) {
+  int rc = experts_check(up, down, tokens, top, type);
+  if (rc) return rc;
+  if (tokens == 0) return TETRIS_OK;
+  if ((rc = check_rows(d_x, type, tokens, ldx, up->k, "input"))) return rc;
+  if ((rc = check_rows(d_y, type, tokens, ldy, down->n, "output"))) return rc;
+  if (!d_index || !d_weight) return fail(TETRIS_EINVAL, "null argument");
+  if ((reinterpret_cast<size_t>(d_index) | reinterpret_cast<size_t>(d_weight)) & 3) return fail(TETRIS_EINVAL, "index or weights not aligned to their elements");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int slots = tokens * top, each = rows_a_group(up, tokens, top);
+  const bool stream_it = streams(each);
+  const ExpertSpace e = expert_space(up, down, tokens, top, type, stream_it);
+  uint8_t* d;
+  if ((rc = workspace(up, s, e.all, &d))) return rc;
+  int* offsets = reinterpret_cast<int*>(d + e.offsets);
+  int* order = reinterpret_cast<int*>(d + e.order);
+  const int threads = std::min(1024, (int)round_up(slots, 64));
+  hipLaunchKernelGGL(plan_kernel, dim3(up->experts), dim3(threads), 0, s, d_index, slots, up->experts, offsets, order);
+  TETRIS_HIP(hipGetLastError());
+
+  Product a{};
+  set_weights(&a, up);
+  int as;
+  if ((rc = ready_rows(&a, d_x, type, tokens, up->k, ldx, false, stream_it, d + e.ready, &as, s))) return rc;
+  a.rows = slots;
+  a.offsets = offsets;
+  a.order = order;
+  a.experts = up->experts;
+  a.from_div = top;
+  a.y = d + e.hidden;
+  a.ldy = round_up(down->k, kMxPad);
+  a.y_part = slots * a.ldy;
+  a.out = stream_it || type == TETRIS_BF16 ? type : type == TETRIS_F16 ? (int)kOutParts2 : (int)kOutParts3;
+  if ((rc = launch_product(a, as, each, stream_it, s))) return rc;
+
+  Product b{};
+  set_weights(&b, down);
+  b.x = d + e.hidden;
+  b.ldx = a.ldy;
+  b.part = a.y_part;
+  b.parts = stream_it ? 1 : parts_of(type);
+  b.k8 = (int)round_up(down->k, 8);
+  b.rows = slots;
+  b.offsets = offsets;
+  b.order = order;
+  b.experts = up->experts;
+  b.to_slot = 1;
+  b.y = d + e.rows;
+  b.ldy = round_up(down->n, 4);
+  b.out = kOutF32;
+  b.vec_out = 1;
+  if ((rc = launch_product(b, stream_it ? type : (int)TETRIS_BF16, each, stream_it, s))) return rc;
+
+  const int vec = ldy % 4 == 0 && (reinterpret_cast<size_t>(d_y) & (4 * elem_size(type) - 1)) == 0;
+  const float* rows = reinterpret_cast<const float*>(d + e.rows);
+  const dim3 grid((unsigned)std::min<int64_t>(((int64_t)tokens * ceil_div(down->n, 4) + 255) / 256, 256 * 64));
+  if (type == TETRIS_F32)
+    hipLaunchKernelGGL(combine_kernel<TETRIS_F32>, grid, dim3(256), 0, s, rows, b.ldy, d_index, d_weight, tokens, top, up->experts, down->n,
+                       static_cast<float*>(d_y), ldy, vec);
+  else if (type == TETRIS_F16)
+    hipLaunchKernelGGL(combine_kernel<TETRIS_F16>, grid, dim3(256), 0, s, rows, b.ldy, d_index, d_weight, tokens, top, up->experts, down->n,
+                       static_cast<_Float16*>(d_y), ldy, vec);
+  else
+    hipLaunchKernelGGL(combine_kernel<TETRIS_BF16>, grid, dim3(256), 0, s, rows, b.ldy, d_index, d_weight, tokens, top, up->experts, down->n,
+                       static_cast<__bf16*>(d_y), ldy, vec);
+  TETRIS_HIP(hipGetLastError());
+  return TETRIS_OK;
+}

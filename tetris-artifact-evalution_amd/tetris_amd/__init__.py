@@ -519,3 +519,7 @@ def TensorEqual(x, y):
     x = np.ascontiguousarray(x, np.float32).ravel()
     y = np.ascontiguousarray(y, np.float32).ravel()
     return int(_lib.tetris_tensor_first_mismatch(x, y, x.size)) == -1
+
+
+from .mx4 import (BF16, F16, F32, GROUP_MAX, GROUP_TWO, SCORE_SIGMOID, SCORE_SOFTMAX, ExpertLayer, MX4Weights, Router,  # noqa: E402
+                  mx4_code_bytes, mx4_dequantize, mx4_quantize, mx4_scale_bytes)
