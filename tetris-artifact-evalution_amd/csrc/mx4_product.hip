@@ -27,7 +27,7 @@ struct Product {
   int parts, k8, rows;   // rows of all groups together
   const i32x4* codes;    // laid-out weights
   const uint8_t* scales;
-  int row_tiles, col_tiles, n, gated;
+  int row_tiles, col_tiles, n;
   // Rows in groups, one for each expert: positions offsets[e] .. offsets[e + 1] - 1 are expert e's, position p standing for slot
   // order[p].  NULL: one group, position = row.
   const int* offsets;
@@ -38,7 +38,7 @@ struct Product {
   int max_tiles;         // of rows, over all groups
   void* y;
   int64_t ldy, y_part;
-  int out, vec_out;      // vec_out: four neighbouring outputs may be stored at once
+  int vec_out;           // four neighbouring outputs may be stored at once
   const float* bias;
 };
 
@@ -100,62 +100,54 @@ __device__ inline unsigned leading(float& v) {
   return u >> 16;
 }
 
+template <int OUT>
 __device__ inline void store1(const Product& a, int64_t at, float v) {
-  switch (a.out) {
-    case kOutF32: static_cast<float*>(a.y)[at] = v; break;
-    case kOutF16: static_cast<_Float16*>(a.y)[at] = (_Float16)v; break;
-    case kOutBF16: static_cast<__bf16*>(a.y)[at] = (__bf16)v; break;
-    default:
-      for (int p = 0; p < (a.out == kOutParts2 ? 2 : 3); ++p)
-        static_cast<unsigned short*>(a.y)[at + p * a.y_part] = (unsigned short)leading(v);
+  if constexpr (OUT <= kOutBF16) {
+    static_cast<typename Elem<OUT>::type*>(a.y)[at] = (typename Elem<OUT>::type)v;
+  } else {
+#pragma unroll
+    for (int p = 0; p < (OUT == kOutParts2 ? 2 : 3); ++p) static_cast<unsigned short*>(a.y)[at + p * a.y_part] = (unsigned short)leading(v);
   }
 }
 
 // four neighbouring outputs
-__device__ inline void store4(const Product& a, int64_t at, const float (&v)[4]) {
-  switch (a.out) {
-    case kOutF32: *reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + at) = f32x4{v[0], v[1], v[2], v[3]}; break;
-    case kOutF16: {
-      typedef _Float16 half4 __attribute__((ext_vector_type(4)));
-      *reinterpret_cast<half4*>(static_cast<_Float16*>(a.y) + at) = half4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
-      break;
-    }
-    case kOutBF16: {
-      typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-      *reinterpret_cast<bf16x4*>(static_cast<__bf16*>(a.y) + at) = bf16x4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
-      break;
-    }
-    default: {
-      float w[4] = {v[0], v[1], v[2], v[3]};
-      for (int p = 0; p < (a.out == kOutParts2 ? 2 : 3); ++p) {
-        uint2 u;
-        u.x = leading(w[0]); u.x |= leading(w[1]) << 16;
-        u.y = leading(w[2]); u.y |= leading(w[3]) << 16;
-        *reinterpret_cast<uint2*>(static_cast<unsigned short*>(a.y) + at + p * a.y_part) = u;
-      }
+template <int OUT>
+__device__ inline void store4(const Product& a, int64_t at, f32x4 v) {
+  if constexpr (OUT <= kOutBF16) {
+    using T = typename Elem<OUT>::type;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<T4*>(static_cast<T*>(a.y) + at) = T4{(T)v.x, (T)v.y, (T)v.z, (T)v.w};
+  } else {
+    float w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int p = 0; p < (OUT == kOutParts2 ? 2 : 3); ++p) {
+      uint2 u;
+      u.x = leading(w[0]); u.x |= leading(w[1]) << 16;
+      u.y = leading(w[2]); u.y |= leading(w[3]) << 16;
+      *reinterpret_cast<uint2*>(static_cast<unsigned short*>(a.y) + at + p * a.y_part) = u;
     }
   }
 }
 
 // Four outputs of one row from feature f on.  A gated launch writes all of a tile's features: its rows are padded, and those past
 // the last feature have to be zero for the product that reads them.
-__device__ inline void put4(const Product& a, int64_t row, int f, float (&v)[4]) {
-  const int n = a.gated ? a.n / 2 : a.n;
-  if (a.bias) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] += f + i < n ? a.bias[f + i] : 0.f;
-  }
+template <int OUT, bool GATED>
+__device__ inline void put4(const Product& a, int64_t row, int f, f32x4 v) {
   const int64_t at = row * a.ldy + f;
-  if (a.gated) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = f + i < n ? v[i] : 0.f;
-    store4(a, at, v);
-  } else if (a.vec_out && f + 4 <= n) {
-    store4(a, at, v);
+  if constexpr (GATED) {
+    const int left = a.n / 2 - f;
+    store4<OUT>(a, at, f32x4{left > 0 ? v.x : 0.f, left > 1 ? v.y : 0.f, left > 2 ? v.z : 0.f, left > 3 ? v.w : 0.f});
   } else {
+    const int left = a.n - f;
+    if (a.vec_out && left >= 4) {
+      if (a.bias) v += f32x4{a.bias[f], a.bias[f + 1], a.bias[f + 2], a.bias[f + 3]};
+      store4<OUT>(a, at, v);
+    } else {
+      const float w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (f + i < n) store1(a, at + i, v[i]);
+      for (int i = 0; i < 4; ++i)
+        if (i < left) store1<OUT>(a, at + i, w[i] + (a.bias ? a.bias[f + i] : 0.f));
+    }
   }
 }
 
@@ -165,9 +157,10 @@ __device__ inline void put4(const Product& a, int64_t row, int f, float (&v)[4])
 // in one stretch, through registers into one of two LDS buffers while the other is multiplied; weights come straight
 // from memory to the registers that use them, a step ahead.  Row r's 16-byte piece p lies at piece p ^ (r / 2 % 8) of its
 // 128 bytes: the sixteen lanes that an LDS read serves at once then touch all 64 banks.
-template <int WT, int WR, int WM, int WN>
+template <int WT, int WR, int WM, int WN, int OUT, bool GATED>
 __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Product a) {
   constexpr int kRows = 32 * WT * WM, kThreads = 64 * WM * WN, kLoads = kRows * 8 / kThreads;
+  static_assert(kThreads / 8 % 16 == 0, "a thread's pieces lie in the same columns");
   __shared__ i32x4 lds[2][kRows * 8];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, wn = wave / WM;
@@ -182,15 +175,13 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Product a) {
   int expert, first, count;
   if (!find_tile(a, tile, kRows, &expert, &first, &count)) return;
 
+  const int column = ((threadIdx.x & 7) ^ ((threadIdx.x >> 4) & 7)) * 8;
   const __bf16* from[kLoads];
-  int column[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
-    const int q = i * kThreads + threadIdx.x, r = q >> 3, piece = (q & 7) ^ ((r >> 1) & 7);
-    const int p = first + min(r, count - 1);
+    const int p = first + min((int)(i * kThreads + threadIdx.x) >> 3, count - 1);
     const int64_t row = a.from_div ? a.order[p] / a.from_div : p;
-    column[i] = piece * 8;
-    from[i] = static_cast<const __bf16*>(a.x) + row * a.ldx + column[i];
+    from[i] = static_cast<const __bf16*>(a.x) + row * a.ldx;
   }
   const i32x4* codes[WR];
   const uint8_t* scales[WR];
@@ -210,14 +201,13 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Product a) {
   i32x4 next_x[kLoads], next_w[WR], w[WR];
   unsigned next_s[WR];
   float s[WR];
+  bool next_in = true;
   int col = 0, part = 0;
-  auto fetch = [&]() {  // column tile `col` of part `part`
+  auto fetch = [&]() {  // column tile `col` of part `part`; past a row's end its beginning, of which nothing is kept
+    next_in = col * 64 + column < a.k8;
+    const int64_t at = part * a.part + (next_in ? col * 64 + column : 0);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const bool in = col * 64 + column[i] < a.k8;
-      const i32x4 v = *reinterpret_cast<const i32x4*>(from[i] + part * a.part + (in ? col * 64 : -column[i]));
-      next_x[i] = in ? v : i32x4{0, 0, 0, 0};
-    }
+    for (int i = 0; i < kLoads; ++i) next_x[i] = *reinterpret_cast<const i32x4*>(from[i] + at);
 #pragma unroll
     for (int r = 0; r < WR; ++r) {
       next_w[r] = codes[r][(int64_t)col * 64];
@@ -227,7 +217,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Product a) {
   };
   auto keep = [&](int buffer) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) lds[buffer][i * kThreads + threadIdx.x] = next_x[i];
+    for (int i = 0; i < kLoads; ++i) lds[buffer][i * kThreads + threadIdx.x] = next_in ? next_x[i] : i32x4{0, 0, 0, 0};
 #pragma unroll
     for (int r = 0; r < WR; ++r) w[r] = next_w[r], s[r] = __uint_as_float(next_s[r] << 23);
   };
@@ -239,18 +229,24 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Product a) {
   for (int step = 0; step < steps; ++step) {
     __syncthreads();
     if (step + 1 < steps) fetch();
-    const i32x4* in = lds[step & 1];
+    const i32x4* in = lds[step & 1] + row_in * 8;
+    bf16x8 xs[2][WT], ws[2][WR];
+#pragma unroll
+    for (int t = 0; t < WT; ++t) xs[0][t] = __builtin_bit_cast(bf16x8, in[t * 256 + ((half * 4) ^ turn)]);
+#pragma unroll
+    for (int r = 0; r < WR; ++r) ws[0][r] = weights8(w[r][0], s[r]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      bf16x8 xs[WT], ws[WR];
+      if (j < 3) {
 #pragma unroll
-      for (int t = 0; t < WT; ++t) xs[t] = __builtin_bit_cast(bf16x8, in[(row_in + t * 32) * 8 + ((half * 4 + j) ^ turn)]);
+        for (int t = 0; t < WT; ++t) xs[(j + 1) & 1][t] = __builtin_bit_cast(bf16x8, in[t * 256 + ((half * 4 + j + 1) ^ turn)]);
 #pragma unroll
-      for (int r = 0; r < WR; ++r) ws[r] = weights8(w[r][j], s[r]);
+        for (int r = 0; r < WR; ++r) ws[(j + 1) & 1][r] = weights8(w[r][j + 1], s[r]);
+      }
 #pragma unroll
       for (int t = 0; t < WT; ++t)
 #pragma unroll
-        for (int r = 0; r < WR; ++r) acc[t][r] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ws[r], xs[t], acc[t][r], 0, 0, 0);
+        for (int r = 0; r < WR; ++r) acc[t][r] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ws[j & 1][r], xs[j & 1][t], acc[t][r], 0, 0, 0);
     }
     if (step + 1 < steps) keep((step + 1) & 1);
   }
@@ -258,25 +254,19 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Product a) {
 #pragma unroll
   for (int t = 0; t < WT; ++t) {
     const int r_in = row_in + t * 32;
-    if (r_in >= count) continue;
-    const int64_t row = a.to_slot ? a.order[first + r_in] : first + r_in;
+    if (r_in < count) {
+      const int64_t row = a.to_slot ? a.order[first + r_in] : first + r_in;
 #pragma unroll
-    for (int r = 0; r < WR; ++r) {
-      const int row_tile = (block * WN + wn) * WR + r;
-      if (row_tile >= a.row_tiles) continue;
-      if (a.gated) {
+      for (int r = 0; r < WR; ++r) {
+        const int row_tile = (block * WN + wn) * WR + r;
+        if (row_tile < a.row_tiles) {
+          const f32x16& v = acc[t][r];
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          float v[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = silu(acc[t][r][q * 4 + i]) * acc[t][r][8 + q * 4 + i];
-          put4(a, row, row_tile * 16 + q * 8 + half * 4, v);
-        }
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float v[4] = {acc[t][r][q * 4], acc[t][r][q * 4 + 1], acc[t][r][q * 4 + 2], acc[t][r][q * 4 + 3]};
-          put4(a, row, row_tile * 32 + q * 8 + half * 4, v);
+          for (int q = 0; q < (GATED ? 2 : 4); ++q) {
+            f32x4 u = {v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]};
+            if constexpr (GATED) u = f32x4{silu(u.x) * v[8 + q * 4], silu(u.y) * v[9 + q * 4], silu(u.z) * v[10 + q * 4], silu(u.w) * v[11 + q * 4]};
+            put4<OUT, GATED>(a, row, row_tile * (GATED ? 16 : 32) + q * 8 + half * 4, u);
+          }
         }
       }
     }
@@ -320,7 +310,7 @@ __device__ inline void parts8(const typename Elem<TYPE>::type* p, bool in, bf16x
   }
 }
 
-template <int TYPE, int TT, int RT>
+template <int TYPE, int TT, int RT, int OUT, bool GATED>
 __global__ __launch_bounds__(TT == 1 ? 1024 : 512) void stream_kernel(Product a) {
   using T = typename Elem<TYPE>::type;
   constexpr int P = TYPE == TETRIS_F32 ? 3 : TYPE == TETRIS_F16 ? 2 : 1;
@@ -390,22 +380,21 @@ __global__ __launch_bounds__(TT == 1 ? 1024 : 512) void stream_kernel(Product a)
       for (int i = 0; i < 4; ++i) sums[(((wave * RT + r) * TT + t) * 4 + i) * 64 + lane] = acc[r][t][i];
   __syncthreads();
 
-  const int n = a.gated ? a.n / 2 : a.n;
+  const int n = GATED ? a.n / 2 : a.n;
   auto sum = [&](int r, int row, int f) {
     const int at = ((r * TT + (row >> 4)) * 4 + (f & 3)) * 64 + (f >> 2) * 16 + (row & 15);
     float v = 0.f;
     for (int w = 0; w < waves; ++w) v += sums[w * (RT * TT * 256) + at];
     return v;
   };
-  if (a.gated) {
-    if constexpr (RT == 2) {
-      for (int i = threadIdx.x; i < TT * 256; i += blockDim.x) {
-        const int row = i >> 4, f = i & 15;
-        if (row >= count) break;
-        const float v = silu(sum(0, row, f)) * sum(1, row, f);
-        const int64_t to = a.to_slot ? a.order[first + row] : first + row;
-        store1(a, to * a.ldy + block * 16 + f, block * 16 + f < n ? v : 0.f);
-      }
+  if constexpr (GATED) {
+    static_assert(RT == 2, "a gate's rows and what they gate");
+    for (int i = threadIdx.x; i < TT * 256; i += blockDim.x) {
+      const int row = i >> 4, f = i & 15;
+      if (row >= count) break;
+      const float v = silu(sum(0, row, f)) * sum(1, row, f);
+      const int64_t to = a.to_slot ? a.order[first + row] : first + row;
+      store1<OUT>(a, to * a.ldy + block * 16 + f, block * 16 + f < n ? v : 0.f);
     }
   } else {
     for (int i = threadIdx.x; i < RT * TT * 256; i += blockDim.x) {
@@ -414,7 +403,7 @@ __global__ __launch_bounds__(TT == 1 ? 1024 : 512) void stream_kernel(Product a)
       if (feature >= n) continue;
       const float v = sum(f >> 4, row, f & 15) + (a.bias ? a.bias[feature] : 0.f);
       const int64_t to = a.to_slot ? a.order[first + row] : first + row;
-      store1(a, to * a.ldy + feature, v);
+      store1<OUT>(a, to * a.ldy + feature, v);
     }
   }
 }
@@ -494,18 +483,18 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ 
 
 constexpr int kStreamRows = 64;  // up to so many rows of a matrix are streamed
 
-template <int WT, int WR, int WM, int WN>
+template <int WT, int WR, int WM, int WN, int OUT, bool GATED>
 int launch_tile(Product& a, hipStream_t stream) {
   const int size = 32 * WT * WM, row_blocks = ceil_div(a.row_tiles, WR * WN);
   a.max_tiles = a.offsets ? std::min(a.rows, a.rows / size + std::min(a.experts, a.rows)) : ceil_div(a.rows, size);
   const int64_t blocks = round_up((int64_t)row_blocks * a.max_tiles, 8);
   if (blocks > 0x7fffffff / 2) return fail(TETRIS_EINVAL, "%d rows by %d features are too many for one launch", a.rows, a.n);
-  hipLaunchKernelGGL((tile_kernel<WT, WR, WM, WN>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream, a);
+  hipLaunchKernelGGL((tile_kernel<WT, WR, WM, WN, OUT, GATED>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream, a);
   TETRIS_HIP(hipGetLastError());
   return TETRIS_OK;
 }
 
-template <int TYPE, int TT, int RT>
+template <int TYPE, int TT, int RT, int OUT, bool GATED>
 int launch_stream(Product& a, hipStream_t stream) {
   const int size = 16 * TT, blocks = ceil_div(a.row_tiles * 2, RT);
   a.max_tiles = a.offsets ? std::min(a.rows, a.rows / size + std::min(a.experts, a.rows)) : ceil_div(a.rows, size);
@@ -514,30 +503,22 @@ int launch_stream(Product& a, hipStream_t stream) {
   const int chunks = a.col_tiles / 2;
   int waves = 8;
   while (waves > 1 && waves > chunks) waves >>= 1;
-  hipLaunchKernelGGL((stream_kernel<TYPE, TT, RT>), dim3((unsigned)grid), dim3(64 * waves), (size_t)waves * RT * TT * 1024, stream, a);
+  hipLaunchKernelGGL((stream_kernel<TYPE, TT, RT, OUT, GATED>), dim3((unsigned)grid), dim3(64 * waves), (size_t)waves * RT * TT * 1024, stream, a);
   TETRIS_HIP(hipGetLastError());
   return TETRIS_OK;
 }
 
-template <int TYPE>
-int launch_stream_typed(Product& a, int rows_a_group, hipStream_t stream) {
-  if (a.gated) {
-    if (rows_a_group <= 16) return launch_stream<TYPE, 1, 2>(a, stream);
-    return launch_stream<TYPE, 2, 2>(a, stream);
-  }
-  if (rows_a_group <= 16) return launch_stream<TYPE, 1, 1>(a, stream);
-  return launch_stream<TYPE, 2, 2>(a, stream);
+// The rows of `a` are of TYPE and streamed; rows_a_group: as many as a group has on average.
+template <int TYPE, int OUT, bool GATED>
+int stream_rows(Product& a, int rows_a_group, hipStream_t stream) {
+  if (rows_a_group <= 16) return launch_stream<TYPE, 1, GATED ? 2 : 1, OUT, GATED>(a, stream);
+  return launch_stream<TYPE, 2, 2, OUT, GATED>(a, stream);
 }
 
-int launch_stream_any(Product& a, int type, int rows_a_group, hipStream_t stream) {
-  if (type == TETRIS_F32) return launch_stream_typed<TETRIS_F32>(a, rows_a_group, stream);
-  if (type == TETRIS_F16) return launch_stream_typed<TETRIS_F16>(a, rows_a_group, stream);
-  return launch_stream_typed<TETRIS_BF16>(a, rows_a_group, stream);
-}
-
-int launch_tile_any(Product& a, int rows_a_group, hipStream_t stream) {
+template <int OUT, bool GATED>
+int tile_rows(Product& a, int rows_a_group, hipStream_t stream) {
   (void)rows_a_group;
-  return launch_tile<4, 2, 2, 4>(a, stream);
+  return launch_tile<4, 2, 2, 4, OUT, GATED>(a, stream);
 }
 
 void set_weights(Product* a, const tetris_mx4* w) {
@@ -546,7 +527,6 @@ void set_weights(Product* a, const tetris_mx4* w) {
   a->row_tiles = w->row_tiles;
   a->col_tiles = w->col_tiles;
   a->n = w->n;
-  a->gated = w->gated;
 }
 
 // Whether the kernels can read rows as they lie.
@@ -622,8 +602,32 @@ int ready_rows(Product* a, const void* x, int type, int rows, int k, int64_t ld,
   return stage_rows(x, type, rows, k, ld, a->parts, d_ready, s);
 }
 
-int launch_product(Product& a, int as, int rows_a_group, bool stream, hipStream_t s) {
-  return stream ? launch_stream_any(a, as, rows_a_group, s) : launch_tile_any(a, rows_a_group, s);
+// Which of the three products it is: numbers of a type; the gated product of the experts, which writes what the next
+// reads; and that one, which writes numbers of 32 bits.
+enum Role { kLinear, kUp, kDown };
+
+// `as`: the type of the rows; `type`: that of the operator.
+int launch_product(Product& a, Role role, int as, int type, int rows_a_group, bool stream, hipStream_t s) {
+  if (stream) {
+    if (as == TETRIS_F32)
+      return role == kUp ? stream_rows<TETRIS_F32, kOutF32, true>(a, rows_a_group, s) : stream_rows<TETRIS_F32, kOutF32, false>(a, rows_a_group, s);
+    if (as == TETRIS_F16)
+      return role == kUp     ? stream_rows<TETRIS_F16, kOutF16, true>(a, rows_a_group, s)
+             : role == kDown ? stream_rows<TETRIS_F16, kOutF32, false>(a, rows_a_group, s)
+                             : stream_rows<TETRIS_F16, kOutF16, false>(a, rows_a_group, s);
+    if (role == kUp) return stream_rows<TETRIS_BF16, kOutBF16, true>(a, rows_a_group, s);
+    if (role == kDown || type == TETRIS_F32) return stream_rows<TETRIS_BF16, kOutF32, false>(a, rows_a_group, s);
+    if (type == TETRIS_F16) return stream_rows<TETRIS_BF16, kOutF16, false>(a, rows_a_group, s);
+    return stream_rows<TETRIS_BF16, kOutBF16, false>(a, rows_a_group, s);
+  }
+  if (role == kUp) {
+    if (type == TETRIS_F32) return tile_rows<kOutParts3, true>(a, rows_a_group, s);
+    if (type == TETRIS_F16) return tile_rows<kOutParts2, true>(a, rows_a_group, s);
+    return tile_rows<kOutBF16, true>(a, rows_a_group, s);
+  }
+  if (role == kDown || type == TETRIS_F32) return tile_rows<kOutF32, false>(a, rows_a_group, s);
+  if (type == TETRIS_F16) return tile_rows<kOutF16, false>(a, rows_a_group, s);
+  return tile_rows<kOutBF16, false>(a, rows_a_group, s);
 }
 
 int check_rows(const void* x, int type, int rows, int64_t ld, int k, const char* what) {
@@ -668,10 +672,9 @@ extern "C" int tetris_mx4_linear(tetris_mx4* w, const void* d_x, int type, int m
   if ((rc = ready_rows(&a, d_x, type, m, w->k, ldx, mx4_input, stream_it, d, &as, s))) return rc;
   a.y = d_y;
   a.ldy = ldy;
-  a.out = type;
   a.vec_out = ldy % 4 == 0 && (reinterpret_cast<size_t>(d_y) & (4 * elem_size(type) - 1)) == 0;
   a.bias = d_bias;
-  return launch_product(a, as, m, stream_it, s);
+  return launch_product(a, kLinear, as, type, m, stream_it, s);
 }
 
 namespace {
@@ -747,8 +750,7 @@ extern "C" int tetris_experts(tetris_mx4* up, tetris_mx4* down, const void* d_x,
   a.y = d + e.hidden;
   a.ldy = round_up(down->k, kMxPad);
   a.y_part = slots * a.ldy;
-  a.out = stream_it || type == TETRIS_BF16 ? type : type == TETRIS_F16 ? (int)kOutParts2 : (int)kOutParts3;
-  if ((rc = launch_product(a, as, each, stream_it, s))) return rc;
+  if ((rc = launch_product(a, kUp, as, type, each, stream_it, s))) return rc;
 
   Product b{};
   set_weights(&b, down);
@@ -764,9 +766,8 @@ extern "C" int tetris_experts(tetris_mx4* up, tetris_mx4* down, const void* d_x,
   b.to_slot = 1;
   b.y = d + e.rows;
   b.ldy = round_up(down->n, 4);
-  b.out = kOutF32;
   b.vec_out = 1;
-  if ((rc = launch_product(b, stream_it ? type : (int)TETRIS_BF16, each, stream_it, s))) return rc;
+  if ((rc = launch_product(b, kDown, stream_it ? type : (int)TETRIS_BF16, type, each, stream_it, s))) return rc;
 
   const int vec = ldy % 4 == 0 && (reinterpret_cast<size_t>(d_y) & (4 * elem_size(type) - 1)) == 0;
   const float* rows = reinterpret_cast<const float*>(d + e.rows);
