@@ -22,6 +22,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 enum { kOutF32 = TETRIS_F32, kOutF16 = TETRIS_F16, kOutBF16 = TETRIS_BF16, kOutParts2, kOutParts3 };
 
 struct Product {
+  const uint8_t* x_scales;  // of rows in MX4
   const void* x;         // rows of ldx elements that start on 16 bytes; elements k .. k8 - 1 of a row are zero
   int64_t ldx, part;     // part: elements between the parts' arrays
   int parts, k8, rows;   // rows of all groups together
@@ -151,6 +152,44 @@ __device__ inline void put4(const Product& a, int64_t row, int f, f32x4 v) {
   }
 }
 
+// What a wave has of a tile: 32 WT rows from row_in - lane % 32 of the workgroup's on, WR row tiles of features from row_tile0 on.
+template <int WT, int WR, int OUT, bool GATED>
+__device__ inline void put_tile(const Product& a, const f32x16 (&acc)[WT][WR], int row_in, int half, int first, int count, int row_tile0) {
+#pragma unroll
+  for (int t = 0; t < WT; ++t) {
+    const int r_in = row_in + t * 32;
+    if (r_in < count) {
+      const int64_t row = a.to_slot ? a.order[first + r_in] : first + r_in;
+#pragma unroll
+      for (int r = 0; r < WR; ++r) {
+        const int row_tile = row_tile0 + r;
+        if (row_tile < a.row_tiles) {
+          const f32x16& v = acc[t][r];
+#pragma unroll
+          for (int q = 0; q < (GATED ? 2 : 4); ++q) {
+            f32x4 u = {v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]};
+            if constexpr (GATED) u = f32x4{silu(u.x) * v[8 + q * 4], silu(u.y) * v[9 + q * 4], silu(u.z) * v[10 + q * 4], silu(u.w) * v[11 + q * 4]};
+            put4<OUT, GATED>(a, row, row_tile * (GATED ? 16 : 32) + q * 8 + half * 4, u);
+          }
+        }
+      }
+    }
+  }
+}
+
+// Which tile a workgroup has: neighbours on one of the eight L2s share the weights of kBand tiles of rows.
+__device__ inline bool place_tile(const Product& a, int row_tiles_each, int* block, int* tile) {
+  constexpr int kBand = 4;
+  const int row_blocks = (a.row_tiles + row_tiles_each - 1) / row_tiles_each;
+  const int id = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  if (id >= row_blocks * a.max_tiles) return false;
+  const int band = id / (row_blocks * kBand), in_band = id - band * row_blocks * kBand;
+  const int wide = min(kBand, a.max_tiles - band * kBand);
+  *block = in_band / wide;
+  *tile = band * kBand + in_band - *block * wide;
+  return true;
+}
+
 // ---- many rows: tiles through LDS ---------------------------------------------------------------------------------
 //
 // A workgroup computes BM = 32 WT WM rows by 32 WR WN features.  Rows come in steps of 64 columns, 128 bytes of each row
@@ -165,13 +204,8 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Product a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, wn = wave / WM;
 
-  const int row_blocks = (a.row_tiles + WR * WN - 1) / (WR * WN);
-  const int id = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);  // neighbouring tiles on one of the eight L2s
-  if (id >= row_blocks * a.max_tiles) return;
-  constexpr int kBand = 4;  // tiles of rows that share the weights they read
-  const int band = id / (row_blocks * kBand), in_band = id - band * row_blocks * kBand;
-  const int wide = min(kBand, a.max_tiles - band * kBand);
-  const int block = in_band / wide, tile = band * kBand + in_band - block * wide;
+  int block, tile;
+  if (!place_tile(a, WR * WN, &block, &tile)) return;
   int expert, first, count;
   if (!find_tile(a, tile, kRows, &expert, &first, &count)) return;
 
@@ -243,6 +277,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Product a) {
 #pragma unroll
         for (int r = 0; r < WR; ++r) ws[(j + 1) & 1][r] = weights8(w[r][j + 1], s[r]);
       }
+      __builtin_amdgcn_sched_barrier(0);  // the next reads stay ahead of these products
 #pragma unroll
       for (int t = 0; t < WT; ++t)
 #pragma unroll
@@ -251,26 +286,96 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Product a) {
     if (step + 1 < steps) keep((step + 1) & 1);
   }
 
+  put_tile<WT, WR, OUT, GATED>(a, acc, row_in, half, first, count, (block * WN + wn) * WR);
+}
+
+// The same for rows that are in MX4 as well, in the weights' layout (csrc/mx4.h): products of 4-bit numbers with both blocks' scales
+// applied by the matrix cores, four times the rate of bf16.  Rows come in steps of 128 columns through LDS, as they lie; a wave's
+// reads of it are one contiguous kilobyte.
+template <int WT, int WR, int WM, int WN, int OUT>
+__global__ __launch_bounds__(64 * WM * WN) void rounded_kernel(Product a) {
+  constexpr int kTiles = WT * WM, kThreads = 64 * WM * WN, kLoads = kTiles * 128 / kThreads;
+  __shared__ i32x4 lds[2][kTiles * 128];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave % WM, wn = wave / WM;
+  int block, tile;
+  if (!place_tile(a, WR * WN, &block, &tile)) return;
+  const int first = tile * kTiles * 32, count = min(kTiles * 32, a.rows - first);
+  const int last = (a.rows - 1) >> 5, tile0 = first >> 5;
+
+  const i32x4* from[kLoads];
 #pragma unroll
-  for (int t = 0; t < WT; ++t) {
-    const int r_in = row_in + t * 32;
-    if (r_in < count) {
-      const int64_t row = a.to_slot ? a.order[first + r_in] : first + r_in;
-#pragma unroll
-      for (int r = 0; r < WR; ++r) {
-        const int row_tile = (block * WN + wn) * WR + r;
-        if (row_tile < a.row_tiles) {
-          const f32x16& v = acc[t][r];
-#pragma unroll
-          for (int q = 0; q < (GATED ? 2 : 4); ++q) {
-            f32x4 u = {v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]};
-            if constexpr (GATED) u = f32x4{silu(u.x) * v[8 + q * 4], silu(u.y) * v[9 + q * 4], silu(u.z) * v[10 + q * 4], silu(u.w) * v[11 + q * 4]};
-            put4<OUT, GATED>(a, row, row_tile * (GATED ? 16 : 32) + q * 8 + half * 4, u);
-          }
-        }
-      }
-    }
+  for (int i = 0; i < kLoads; ++i) {
+    const int q = i * kThreads + threadIdx.x;
+    from[i] = static_cast<const i32x4*>(a.x) + (int64_t)min(tile0 + (q >> 7), last) * a.col_tiles * 64 + (q & 127);
   }
+  const unsigned short* x_scales[WT];
+#pragma unroll
+  for (int t = 0; t < WT; ++t)
+    x_scales[t] = reinterpret_cast<const unsigned short*>(a.x_scales) + (int64_t)min(tile0 + wm * WT + t, last) * a.col_tiles * 32 + lane;
+  const i32x4* codes[WR];
+  const unsigned short* scales[WR];
+#pragma unroll
+  for (int r = 0; r < WR; ++r) {
+    const int64_t t = min((block * WN + wn) * WR + r, a.row_tiles - 1);
+    codes[r] = a.codes + t * a.col_tiles * 64 + lane;
+    scales[r] = reinterpret_cast<const unsigned short*>(a.scales) + t * a.col_tiles * 32 + lane;
+  }
+  f32x16 acc[WT][WR];
+#pragma unroll
+  for (int t = 0; t < WT; ++t)
+#pragma unroll
+    for (int r = 0; r < WR; ++r) acc[t][r] = f32x16{};
+
+  i32x4 next_x[kLoads], next_w[WR][2], w[WR][2];
+  int next_xs[WT], xs[WT], next_ws[WR], ws[WR];
+  auto fetch = [&](int step) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) next_x[i] = from[i][(int64_t)step * 128];
+#pragma unroll
+    for (int r = 0; r < WR; ++r) {
+      next_w[r][0] = codes[r][(int64_t)step * 128];
+      next_w[r][1] = codes[r][(int64_t)step * 128 + 64];
+      next_ws[r] = scales[r][(int64_t)step * 64];
+    }
+#pragma unroll
+    for (int t = 0; t < WT; ++t) next_xs[t] = x_scales[t][(int64_t)step * 64];
+  };
+  auto keep = [&](int buffer) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) lds[buffer][i * kThreads + threadIdx.x] = next_x[i];
+#pragma unroll
+    for (int r = 0; r < WR; ++r) w[r][0] = next_w[r][0], w[r][1] = next_w[r][1], ws[r] = next_ws[r];
+#pragma unroll
+    for (int t = 0; t < WT; ++t) xs[t] = next_xs[t];
+  };
+  auto wide = [](i32x4 v) { return i32x8{v.x, v.y, v.z, v.w, 0, 0, 0, 0}; };
+
+  const int steps = a.col_tiles >> 1;
+  fetch(0);
+  keep(0);
+  for (int step = 0; step < steps; ++step) {
+    __syncthreads();
+    if (step + 1 < steps) fetch(step + 1);
+    const i32x4* in = lds[step & 1] + wm * WT * 128 + lane;
+    i32x4 x0[WT], x1[WT];
+#pragma unroll
+    for (int t = 0; t < WT; ++t) x0[t] = in[t * 128];
+#pragma unroll
+    for (int t = 0; t < WT; ++t) x1[t] = in[t * 128 + 64];
+#pragma unroll
+    for (int t = 0; t < WT; ++t)
+#pragma unroll
+      for (int r = 0; r < WR; ++r)
+        acc[t][r] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(w[r][0]), wide(x0[t]), acc[t][r], 4, 4, 0, ws[r], 0, xs[t]);
+#pragma unroll
+    for (int t = 0; t < WT; ++t)
+#pragma unroll
+      for (int r = 0; r < WR; ++r)
+        acc[t][r] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(w[r][1]), wide(x1[t]), acc[t][r], 4, 4, 1, ws[r], 1, xs[t]);
+    if (step + 1 < steps) keep((step + 1) & 1);
+  }
+  put_tile<WT, WR, OUT, false>(a, acc, wm * WT * 32 + (lane & 31), lane >> 5, first, count, (block * WN + wn) * WR);
 }
 
 // ---- few rows: weights streamed once -----------------------------------------------------------------------------------
@@ -494,6 +599,16 @@ int launch_tile(Product& a, hipStream_t stream) {
   return TETRIS_OK;
 }
 
+template <int WT, int WR, int WM, int WN, int OUT>
+int launch_rounded(Product& a, hipStream_t stream) {
+  a.max_tiles = ceil_div(a.rows, 32 * WT * WM);
+  const int64_t blocks = round_up((int64_t)ceil_div(a.row_tiles, WR * WN) * a.max_tiles, 8);
+  if (blocks > 0x7fffffff / 2) return fail(TETRIS_EINVAL, "%d rows by %d features are too many for one launch", a.rows, a.n);
+  hipLaunchKernelGGL((rounded_kernel<WT, WR, WM, WN, OUT>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream, a);
+  TETRIS_HIP(hipGetLastError());
+  return TETRIS_OK;
+}
+
 template <int TYPE, int TT, int RT, int OUT, bool GATED>
 int launch_stream(Product& a, hipStream_t stream) {
   const int size = 16 * TT, blocks = ceil_div(a.row_tiles * 2, RT);
@@ -567,7 +682,7 @@ bool streams(int rows) { return rows <= kStreamRows; }
 // bytes that rows made ready for a product take at most
 size_t staged_bytes(int rows, int k, int type, bool rounded, bool stream) {
   const size_t padded = (size_t)rows * round_up(k, kMxPad);
-  if (rounded) return padded * 2;
+  if (rounded) return stream ? padded * 2 : (size_t)round_up(rows, 32) * round_up(k, kMxPad) / 32 * 17;
   return padded * (stream ? elem_size(type) : 2 * parts_of(type));
 }
 
@@ -584,7 +699,10 @@ int ready_rows(Product* a, const void* x, int type, int rows, int k, int64_t ld,
     a->ldx = padded;
     a->k8 = (int)padded;
     *as = TETRIS_BF16;
-    return mx4_quantize_to(kMxValues, x, type, rows, k, ld, d_ready, nullptr, s);
+    if (stream) return mx4_quantize_to(kMxValues, x, type, rows, k, ld, d_ready, nullptr, s);
+    uint8_t* scales = d_ready + round_up(rows, 32) * padded / 2;
+    a->x_scales = scales;
+    return mx4_quantize_to(kMxTiles, x, type, rows, k, ld, d_ready, scales, s);
   }
   if (lies_well(x, ld, k, type) && (stream || type == TETRIS_BF16)) {
     a->x = x;
@@ -619,6 +737,11 @@ int launch_product(Product& a, Role role, int as, int type, int rows_a_group, bo
     if (role == kDown || type == TETRIS_F32) return stream_rows<TETRIS_BF16, kOutF32, false>(a, rows_a_group, s);
     if (type == TETRIS_F16) return stream_rows<TETRIS_BF16, kOutF16, false>(a, rows_a_group, s);
     return stream_rows<TETRIS_BF16, kOutBF16, false>(a, rows_a_group, s);
+  }
+  if (a.x_scales) {
+    if (type == TETRIS_F32) return launch_rounded<4, 2, 2, 4, kOutF32>(a, s);
+    if (type == TETRIS_F16) return launch_rounded<4, 2, 2, 4, kOutF16>(a, s);
+    return launch_rounded<4, 2, 2, 4, kOutBF16>(a, s);
   }
   if (role == kUp) {
     if (type == TETRIS_F32) return tile_rows<kOutParts3, true>(a, rows_a_group, s);
