@@ -177,11 +177,12 @@ __device__ inline void put_tile(const Product& a, const f32x16 (&acc)[WT][WR], i
   }
 }
 
-// Which tile a workgroup has: neighbours on one of the eight L2s share the weights of kBand tiles of rows.
+// Which tile a workgroup has.  Workgroups go to the eight L2s in turn; runs of 32 tiles, one for each of its compute units, stay on one of them
+// and share weights between kBand tiles of rows.  (Eighths of the whole grid would leave the last L2 the groups' empty tiles.)
 __device__ inline bool place_tile(const Product& a, int row_tiles_each, int* block, int* tile) {
   constexpr int kBand = 4;
   const int row_blocks = (a.row_tiles + row_tiles_each - 1) / row_tiles_each;
-  const int id = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  const int id = (((blockIdx.x >> 8) * 8 + (blockIdx.x & 7)) << 5) + ((blockIdx.x >> 3) & 31);
   if (id >= row_blocks * a.max_tiles) return false;
   const int band = id / (row_blocks * kBand), in_band = id - band * row_blocks * kBand;
   const int wide = min(kBand, a.max_tiles - band * kBand);
@@ -192,28 +193,30 @@ __device__ inline bool place_tile(const Product& a, int row_tiles_each, int* blo
 
 // ---- many rows: tiles through LDS ---------------------------------------------------------------------------------
 //
-// A workgroup computes BM = 32 WT WM rows by 32 WR WN features.  Rows come in steps of 64 columns, 128 bytes of each row
-// in one stretch, through registers into one of two LDS buffers while the other is multiplied; weights come straight
-// from memory to the registers that use them, a step ahead.  Row r's 16-byte piece p lies at piece p ^ (r / 2 % 8) of its
-// 128 bytes: the sixteen lanes that an LDS read serves at once then touch all 64 banks.
-template <int WT, int WR, int WM, int WN, int OUT, bool GATED>
+// A workgroup computes BM = 32 WT WM rows by 32 WR WN features.  Rows come in steps of 64 KS columns, 128 KS bytes of each
+// row in one stretch, through registers into one of two LDS buffers while the other is multiplied; weights come straight
+// from memory to the registers that use them, a step ahead, once for all parts of the rows.  A row's 16-byte pieces are permuted in LDS
+// (by turn_of, exclusive or) so that the sixteen lanes that an LDS read serves at once touch all 64 banks.
+template <int KS>
+__device__ inline int turn_of(int row) { return KS == 1 ? (row >> 1) & 7 : row & 15; }
+
+template <int WT, int WR, int WM, int WN, int KS, int OUT, bool GATED>
 __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Product a) {
-  constexpr int kRows = 32 * WT * WM, kThreads = 64 * WM * WN, kLoads = kRows * 8 / kThreads;
-  static_assert(kThreads / 8 % 16 == 0, "a thread's pieces lie in the same columns");
-  __shared__ i32x4 lds[2][kRows * 8];
+  constexpr int kRows = 32 * WT * WM, kThreads = 64 * WM * WN, kPieces = 8 * KS, kLoads = kRows * kPieces / kThreads;
+  static_assert(kThreads / kPieces % 16 == 0, "a thread's pieces lie in the same columns");
+  __shared__ i32x4 lds[2][kRows * kPieces];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, wn = wave / WM;
-
   int block, tile;
   if (!place_tile(a, WR * WN, &block, &tile)) return;
   int expert, first, count;
   if (!find_tile(a, tile, kRows, &expert, &first, &count)) return;
 
-  const int column = ((threadIdx.x & 7) ^ ((threadIdx.x >> 4) & 7)) * 8;
+  const int column = ((threadIdx.x % kPieces) ^ turn_of<KS>(threadIdx.x / kPieces)) * 8;
   const __bf16* from[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
-    const int p = first + min((int)(i * kThreads + threadIdx.x) >> 3, count - 1);
+    const int p = first + min((int)(i * kThreads + threadIdx.x) / kPieces, count - 1);
     const int64_t row = a.from_div ? a.order[p] / a.from_div : p;
     from[i] = static_cast<const __bf16*>(a.x) + row * a.ldx;
   }
@@ -232,50 +235,64 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Product a) {
 #pragma unroll
     for (int r = 0; r < WR; ++r) acc[t][r] = f32x16{};
 
-  i32x4 next_x[kLoads], next_w[WR], w[WR];
+  i32x4 next_x[kLoads], next_w[WR][KS], w[WR][KS];
   unsigned next_s[WR];
-  float s[WR];
+  float s[WR][KS];
   bool next_in = true;
-  int col = 0, part = 0;
-  auto fetch = [&]() {  // column tile `col` of part `part`; past a row's end its beginning, of which nothing is kept
+  int col = 0, part = 0;  // of the step fetched last, and then of the next one
+  auto fetch = [&]() {    // past a row's end its beginning, of which nothing is kept
     next_in = col * 64 + column < a.k8;
     const int64_t at = part * a.part + (next_in ? col * 64 + column : 0);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) next_x[i] = *reinterpret_cast<const i32x4*>(from[i] + at);
+    if (part == 0) {
 #pragma unroll
-    for (int r = 0; r < WR; ++r) {
-      next_w[r] = codes[r][(int64_t)col * 64];
-      next_s[r] = scales[r][(int64_t)(col >> 1) * 128 + (col & 1)];
+      for (int r = 0; r < WR; ++r) {
+#pragma unroll
+        for (int c = 0; c < KS; ++c) next_w[r][c] = codes[r][(int64_t)(col + c) * 64];
+        if constexpr (KS == 1)
+          next_s[r] = scales[r][(int64_t)(col >> 1) * 128 + (col & 1)];
+        else
+          next_s[r] = *reinterpret_cast<const unsigned short*>(scales[r] + (int64_t)col * 64);
+      }
     }
-    if (++part == a.parts) part = 0, ++col;
   };
   auto keep = [&](int buffer) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) lds[buffer][i * kThreads + threadIdx.x] = next_in ? next_x[i] : i32x4{0, 0, 0, 0};
+    if (part == 0) {
 #pragma unroll
-    for (int r = 0; r < WR; ++r) w[r] = next_w[r], s[r] = __uint_as_float(next_s[r] << 23);
+      for (int r = 0; r < WR; ++r)
+#pragma unroll
+        for (int c = 0; c < KS; ++c) {
+          w[r][c] = next_w[r][c];
+          s[r][c] = __uint_as_float((next_s[r] >> (8 * c)) << 23);  // (the sign bit of a scale is not looked at)
+        }
+    }
+    if (++part == a.parts) part = 0, col += KS;
   };
 
-  const int steps = a.col_tiles * a.parts;
-  const int row_in = wm * WT * 32 + (lane & 31), turn = (lane >> 1) & 7, half = lane >> 5;
+  const int steps = a.col_tiles / KS * a.parts;
+  const int row_in = wm * WT * 32 + (lane & 31), turn = turn_of<KS>(lane & 31), half = lane >> 5;
   fetch();
   keep(0);
   for (int step = 0; step < steps; ++step) {
     __syncthreads();
     if (step + 1 < steps) fetch();
-    const i32x4* in = lds[step & 1] + row_in * 8;
+    const i32x4* in = lds[step & 1] + row_in * kPieces;
+    auto piece = [&](int j) { return ((j >> 2) * 8 + half * 4 + (j & 3)) ^ turn; };
     bf16x8 xs[2][WT], ws[2][WR];
 #pragma unroll
-    for (int t = 0; t < WT; ++t) xs[0][t] = __builtin_bit_cast(bf16x8, in[t * 256 + ((half * 4) ^ turn)]);
+    for (int t = 0; t < WT; ++t) xs[0][t] = __builtin_bit_cast(bf16x8, in[t * 32 * kPieces + piece(0)]);
 #pragma unroll
-    for (int r = 0; r < WR; ++r) ws[0][r] = weights8(w[r][0], s[r]);
+    for (int r = 0; r < WR; ++r) ws[0][r] = weights8(w[r][0][0], s[r][0]);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (j < 3) {
+    for (int j = 0; j < 4 * KS; ++j) {
+      if (j + 1 < 4 * KS) {
 #pragma unroll
-        for (int t = 0; t < WT; ++t) xs[(j + 1) & 1][t] = __builtin_bit_cast(bf16x8, in[t * 256 + ((half * 4 + j + 1) ^ turn)]);
+        for (int t = 0; t < WT; ++t) xs[(j + 1) & 1][t] = __builtin_bit_cast(bf16x8, in[t * 32 * kPieces + piece(j + 1)]);
 #pragma unroll
-        for (int r = 0; r < WR; ++r) ws[(j + 1) & 1][r] = weights8(w[r][j + 1], s[r]);
+        for (int r = 0; r < WR; ++r) ws[(j + 1) & 1][r] = weights8(w[r][(j + 1) >> 2][(j + 1) & 3], s[r][(j + 1) >> 2]);
       }
       __builtin_amdgcn_sched_barrier(0);  // the next reads stay ahead of these products
 #pragma unroll
@@ -285,7 +302,6 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Product a) {
     }
     if (step + 1 < steps) keep((step + 1) & 1);
   }
-
   put_tile<WT, WR, OUT, GATED>(a, acc, row_in, half, first, count, (block * WN + wn) * WR);
 }
 
@@ -586,15 +602,15 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ 
 
 // ---- launches ------------------------------------------------------------------------------------------------------------
 
-constexpr int kStreamRows = 64;  // up to so many rows of a matrix are streamed
+constexpr int kStreamRows = 16;  // up to so many rows of a matrix are streamed
 
-template <int WT, int WR, int WM, int WN, int OUT, bool GATED>
+template <int WT, int WR, int WM, int WN, int KS, int OUT, bool GATED>
 int launch_tile(Product& a, hipStream_t stream) {
   const int size = 32 * WT * WM, row_blocks = ceil_div(a.row_tiles, WR * WN);
   a.max_tiles = a.offsets ? std::min(a.rows, a.rows / size + std::min(a.experts, a.rows)) : ceil_div(a.rows, size);
-  const int64_t blocks = round_up((int64_t)row_blocks * a.max_tiles, 8);
+  const int64_t blocks = round_up((int64_t)row_blocks * a.max_tiles, 256);
   if (blocks > 0x7fffffff / 2) return fail(TETRIS_EINVAL, "%d rows by %d features are too many for one launch", a.rows, a.n);
-  hipLaunchKernelGGL((tile_kernel<WT, WR, WM, WN, OUT, GATED>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream, a);
+  hipLaunchKernelGGL((tile_kernel<WT, WR, WM, WN, KS, OUT, GATED>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream, a);
   TETRIS_HIP(hipGetLastError());
   return TETRIS_OK;
 }
@@ -602,7 +618,7 @@ int launch_tile(Product& a, hipStream_t stream) {
 template <int WT, int WR, int WM, int WN, int OUT>
 int launch_rounded(Product& a, hipStream_t stream) {
   a.max_tiles = ceil_div(a.rows, 32 * WT * WM);
-  const int64_t blocks = round_up((int64_t)ceil_div(a.row_tiles, WR * WN) * a.max_tiles, 8);
+  const int64_t blocks = round_up((int64_t)ceil_div(a.row_tiles, WR * WN) * a.max_tiles, 256);
   if (blocks > 0x7fffffff / 2) return fail(TETRIS_EINVAL, "%d rows by %d features are too many for one launch", a.rows, a.n);
   hipLaunchKernelGGL((rounded_kernel<WT, WR, WM, WN, OUT>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream, a);
   TETRIS_HIP(hipGetLastError());
@@ -632,8 +648,10 @@ int stream_rows(Product& a, int rows_a_group, hipStream_t stream) {
 
 template <int OUT, bool GATED>
 int tile_rows(Product& a, int rows_a_group, hipStream_t stream) {
-  (void)rows_a_group;
-  return launch_tile<4, 2, 2, 4, OUT, GATED>(a, stream);
+  if (rows_a_group <= 40) return launch_tile<1, 2, 1, 4, 2, OUT, GATED>(a, stream);
+  if (rows_a_group <= 80) return launch_tile<2, 2, 1, 4, 2, OUT, GATED>(a, stream);
+  if (rows_a_group <= 300) return launch_tile<4, 2, 1, 4, 2, OUT, GATED>(a, stream);
+  return launch_tile<4, 2, 2, 4, 1, OUT, GATED>(a, stream);
 }
 
 void set_weights(Product* a, const tetris_mx4* w) {
