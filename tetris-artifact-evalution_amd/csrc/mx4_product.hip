@@ -6,6 +6,7 @@
 // also multiplies by the scale, in the registers of the wave that uses them: what comes from memory is 17 bytes for 32 weights.
 #include <algorithm>
 #include <new>
+#include <type_traits>
 
 #include "mx4.h"
 
@@ -85,6 +86,16 @@ __device__ inline bf16x8 weights8(int codes, float scale) {
   v.z = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)codes, scale, 2));
   v.w = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)codes, scale, 3));
   return __builtin_bit_cast(bf16x8, v);
+}
+
+// the same for the i-th pair
+__device__ inline int pair_of(int codes, float scale, int i) {
+  switch (i) {  // (a constant where this is used)
+    case 0: return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)codes, scale, 0));
+    case 1: return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)codes, scale, 1));
+    case 2: return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)codes, scale, 2));
+    default: return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)codes, scale, 3));
+  }
 }
 
 __device__ inline float silu(float v) { return v / (1.f + expf(-v)); }
@@ -201,7 +212,7 @@ template <int KS>
 __device__ inline int turn_of(int row) { return KS == 1 ? (row >> 1) & 7 : row & 15; }
 
 template <int WT, int WR, int WM, int WN, int KS, int OUT, bool GATED>
-__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Product a) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
   constexpr int kRows = 32 * WT * WM, kThreads = 64 * WM * WN, kPieces = 8 * KS, kLoads = kRows * kPieces / kThreads;
   static_assert(kThreads / kPieces % 16 == 0, "a thread's pieces lie in the same columns");
   __shared__ i32x4 lds[2][kRows * kPieces];
@@ -235,73 +246,88 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Product a) {
 #pragma unroll
     for (int r = 0; r < WR; ++r) acc[t][r] = f32x16{};
 
-  i32x4 next_x[kLoads], next_w[WR][KS], w[WR][KS];
-  unsigned next_s[WR];
-  float s[WR][KS];
-  bool next_in = true;
-  int col = 0, part = 0;  // of the step fetched last, and then of the next one
-  auto fetch = [&]() {    // past a row's end its beginning, of which nothing is kept
-    next_in = col * 64 + column < a.k8;
-    const int64_t at = part * a.part + (next_in ? col * 64 + column : 0);
+  // Steps alternate between two sets of registers for weights, so that nothing is copied.
+  i32x4 next_x[kLoads], w[2][WR][KS];
+  unsigned s[2][WR];
+  int col = 0, part = 0, next_col = 0;
+  auto fetch = [&](int set) {  // past a row's end its beginning, of which nothing is kept; past the last step that one again
+    next_col = min(col, a.col_tiles - KS);
+    const int at = next_col * 64 + column;
+    const int64_t from_row = part * a.part + (at < a.k8 ? at : 0);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) next_x[i] = *reinterpret_cast<const i32x4*>(from[i] + at);
-    if (part == 0) {
+    for (int i = 0; i < kLoads; ++i) next_x[i] = *reinterpret_cast<const i32x4*>(from[i] + from_row);
 #pragma unroll
-      for (int r = 0; r < WR; ++r) {
+    for (int r = 0; r < WR; ++r) {
 #pragma unroll
-        for (int c = 0; c < KS; ++c) next_w[r][c] = codes[r][(int64_t)(col + c) * 64];
-        if constexpr (KS == 1)
-          next_s[r] = scales[r][(int64_t)(col >> 1) * 128 + (col & 1)];
-        else
-          next_s[r] = *reinterpret_cast<const unsigned short*>(scales[r] + (int64_t)col * 64);
-      }
-    }
-  };
-  auto keep = [&](int buffer) {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) lds[buffer][i * kThreads + threadIdx.x] = next_in ? next_x[i] : i32x4{0, 0, 0, 0};
-    if (part == 0) {
-#pragma unroll
-      for (int r = 0; r < WR; ++r)
-#pragma unroll
-        for (int c = 0; c < KS; ++c) {
-          w[r][c] = next_w[r][c];
-          s[r][c] = __uint_as_float((next_s[r] >> (8 * c)) << 23);  // (the sign bit of a scale is not looked at)
-        }
+      for (int c = 0; c < KS; ++c) w[set][r][c] = codes[r][(int64_t)(next_col + c) * 64];
+      if constexpr (KS == 1)
+        s[set][r] = scales[r][(int64_t)(next_col >> 1) * 128 + (next_col & 1)];
+      else
+        s[set][r] = *reinterpret_cast<const unsigned short*>(scales[r] + (int64_t)next_col * 64);
     }
     if (++part == a.parts) part = 0, col += KS;
+  };
+  auto keep = [&](int buffer) {
+    if (next_col * 64 + 64 * KS > a.k8) {
+      const bool in = next_col * 64 + column < a.k8;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) next_x[i] = in ? next_x[i] : i32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) lds[buffer][i * kThreads + threadIdx.x] = next_x[i];
   };
 
   const int steps = a.col_tiles / KS * a.parts;
   const int row_in = wm * WT * 32 + (lane & 31), turn = turn_of<KS>(lane & 31), half = lane >> 5;
-  fetch();
-  keep(0);
-  for (int step = 0; step < steps; ++step) {
-    __syncthreads();
-    if (step + 1 < steps) fetch();
-    const i32x4* in = lds[step & 1] + row_in * kPieces;
-    auto piece = [&](int j) { return ((j >> 2) * 8 + half * 4 + (j & 3)) ^ turn; };
-    bf16x8 xs[2][WT], ws[2][WR];
+  constexpr int kRounds = 4 * KS, kProducts = WT * WR, kPairs = 4 * WR;
+  i32x4 xs[2][WT], ws[2][WR];
+  auto read = [&](int buffer, int j) {  // the rows' share in round j of a step's products
+    const i32x4* in = lds[buffer] + row_in * kPieces + (((j >> 2) * 8 + half * 4 + (j & 3)) ^ turn);
 #pragma unroll
-    for (int t = 0; t < WT; ++t) xs[0][t] = __builtin_bit_cast(bf16x8, in[t * 32 * kPieces + piece(0)]);
+    for (int t = 0; t < WT; ++t) xs[j & 1][t] = in[t * 32 * kPieces];
+  };
+  auto convert = [&](int set, int j, int i) {  // (the sign bit of a scale is not looked at)
+    const float scale = __uint_as_float((s[set][i >> 2] >> (8 * (j >> 2))) << 23);
+    ws[j & 1][i >> 2][i & 3] = pair_of(w[set][i >> 2][j >> 2][j & 3], scale, i & 3);
+  };
+  // The weights' pairs of the next round are made between the products of this one: a conversion takes the vector unit for 16 cycles, a
+  // product the matrix unit for 32.  A step's last round runs behind the barrier, while the next step's first reads are under
+  // way; the next step's numbers go to LDS in the last but one, and those of the step after it are asked for.  All reads
+  // of a buffer have ended when its step's barrier is passed, so two buffers are enough.
+  auto multiply = [&](int set) {
 #pragma unroll
-    for (int r = 0; r < WR; ++r) ws[0][r] = weights8(w[r][0][0], s[r][0]);
+    for (int j = 0; j < kRounds; ++j) {
+      const bool last = j + 1 == kRounds;
+      if (last) __syncthreads();
+      read(last ? set ^ 1 : set, last ? 0 : j + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int j = 0; j < 4 * KS; ++j) {
-      if (j + 1 < 4 * KS) {
+      for (int i = 0; i < kProducts; ++i) {
+        const int t = i / WR, r = i % WR;
+        acc[t][r] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ws[j & 1][r]), __builtin_bit_cast(bf16x8, xs[j & 1][t]), acc[t][r], 0, 0, 0);
 #pragma unroll
-        for (int t = 0; t < WT; ++t) xs[(j + 1) & 1][t] = __builtin_bit_cast(bf16x8, in[t * 32 * kPieces + piece(j + 1)]);
-#pragma unroll
-        for (int r = 0; r < WR; ++r) ws[(j + 1) & 1][r] = weights8(w[r][(j + 1) >> 2][(j + 1) & 3], s[r][(j + 1) >> 2]);
+        for (int c = i * kPairs / kProducts; c < (i + 1) * kPairs / kProducts; ++c) convert(last ? set ^ 1 : set, last ? 0 : j + 1, c);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);  // the next reads stay ahead of these products
-#pragma unroll
-      for (int t = 0; t < WT; ++t)
-#pragma unroll
-        for (int r = 0; r < WR; ++r) acc[t][r] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ws[j & 1][r], xs[j & 1][t], acc[t][r], 0, 0, 0);
+      if (j + 2 == kRounds) {
+        keep(set ^ 1);
+        fetch(set);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
-    if (step + 1 < steps) keep((step + 1) & 1);
+  };
+  fetch(0);
+  keep(0);
+  fetch(1);
+  __syncthreads();
+  read(0, 0);
+#pragma unroll
+  for (int c = 0; c < kPairs; ++c) convert(0, 0, c);
+  for (int step = 0; step + 1 < steps; step += 2) {
+    multiply(0);
+    multiply(1);
   }
+  if (steps & 1) multiply(0);
   put_tile<WT, WR, OUT, GATED>(a, acc, row_in, half, first, count, (block * WN + wn) * WR);
 }
 
@@ -344,7 +370,7 @@ __global__ __launch_bounds__(64 * WM * WN) void rounded_kernel(Product a) {
     for (int r = 0; r < WR; ++r) acc[t][r] = f32x16{};
 
   i32x4 next_x[kLoads], next_w[WR][2], w[WR][2];
-  int next_xs[WT], xs[WT], next_ws[WR], ws[WR];
+  int next_xs[WT], x_s[WT], next_ws[WR], ws[WR];
   auto fetch = [&](int step) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) next_x[i] = from[i][(int64_t)step * 128];
@@ -363,33 +389,50 @@ __global__ __launch_bounds__(64 * WM * WN) void rounded_kernel(Product a) {
 #pragma unroll
     for (int r = 0; r < WR; ++r) w[r][0] = next_w[r][0], w[r][1] = next_w[r][1], ws[r] = next_ws[r];
 #pragma unroll
-    for (int t = 0; t < WT; ++t) xs[t] = next_xs[t];
+    for (int t = 0; t < WT; ++t) x_s[t] = next_xs[t];
   };
   auto wide = [](i32x4 v) { return i32x8{v.x, v.y, v.z, v.w, 0, 0, 0, 0}; };
 
   const int steps = a.col_tiles >> 1;
+  i32x4 xs[2][WT], w1[WR];
+  int xs1[WT], ws1[WR];
+  auto read = [&](int buffer, int j) {
+    const i32x4* in = lds[buffer] + wm * WT * 128 + lane + j * 64;
+#pragma unroll
+    for (int t = 0; t < WT; ++t) xs[j][t] = in[t * 128];
+  };
+  // the order of things as in tile_kernel, with two rounds of products a step
   fetch(0);
   keep(0);
+  if (steps > 1) fetch(1);
+  __syncthreads();
+  read(0, 0);
   for (int step = 0; step < steps; ++step) {
-    __syncthreads();
-    if (step + 1 < steps) fetch(step + 1);
-    const i32x4* in = lds[step & 1] + wm * WT * 128 + lane;
-    i32x4 x0[WT], x1[WT];
-#pragma unroll
-    for (int t = 0; t < WT; ++t) x0[t] = in[t * 128];
-#pragma unroll
-    for (int t = 0; t < WT; ++t) x1[t] = in[t * 128 + 64];
+    const bool more = step + 1 < steps;
+    read(step & 1, 1);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int t = 0; t < WT; ++t)
 #pragma unroll
       for (int r = 0; r < WR; ++r)
-        acc[t][r] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(w[r][0]), wide(x0[t]), acc[t][r], 4, 4, 0, ws[r], 0, xs[t]);
+        acc[t][r] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(w[r][0]), wide(xs[0][t]), acc[t][r], 4, 4, 0, ws[r], 0, x_s[t]);
+#pragma unroll
+    for (int r = 0; r < WR; ++r) w1[r] = w[r][1], ws1[r] = ws[r];
+#pragma unroll
+    for (int t = 0; t < WT; ++t) xs1[t] = x_s[t];
+    if (more) {
+      keep((step + 1) & 1);
+      if (step + 2 < steps) fetch(step + 2);
+      __syncthreads();
+      read((step + 1) & 1, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int t = 0; t < WT; ++t)
 #pragma unroll
       for (int r = 0; r < WR; ++r)
-        acc[t][r] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(w[r][1]), wide(x1[t]), acc[t][r], 4, 4, 1, ws[r], 1, xs[t]);
-    if (step + 1 < steps) keep((step + 1) & 1);
+        acc[t][r] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(w1[r]), wide(xs[1][t]), acc[t][r], 4, 4, 1, ws1[r], 1, xs1[t]);
+    __builtin_amdgcn_sched_barrier(0);
   }
   put_tile<WT, WR, OUT, false>(a, acc, wm * WT * 32 + (lane & 31), lane >> 5, first, count, (block * WN + wn) * WR);
 }
