@@ -49,7 +49,8 @@ struct tetris_mx4 {
   bool gated = false;
   int row_tiles = 0, col_tiles = 0;  // of one matrix
   uint8_t* codes = nullptr;
-  uint8_t* scales = nullptr;
+  uint8_t* scales = nullptr;  // zeros behind them
+  uint8_t* zeros = nullptr;
   std::mutex mu;
   struct Space { void* ptr = nullptr; size_t bytes = 0; };
   std::map<hipStream_t, Space> space;

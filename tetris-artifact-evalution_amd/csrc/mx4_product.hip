@@ -24,6 +24,7 @@ enum { kOutF32 = TETRIS_F32, kOutF16 = TETRIS_F16, kOutBF16 = TETRIS_BF16, kOutP
 
 struct Product {
   const uint8_t* x_scales;  // of rows in MX4
+  const void* zeros;     // sixteen bytes of them
   const void* x;         // rows of ldx elements that start on 16 bytes; elements k .. k8 - 1 of a row are zero
   int64_t ldx, part;     // part: elements between the parts' arrays
   int parts, k8, rows;   // rows of all groups together
@@ -40,7 +41,7 @@ struct Product {
   int max_tiles;         // of rows, over all groups
   void* y;
   int64_t ldy, y_part;
-  int vec_out;           // four neighbouring outputs may be stored at once
+  int vec_out;           // rows of outputs start on 16 bytes
   const float* bias;
 };
 
@@ -122,68 +123,111 @@ __device__ inline void store1(const Product& a, int64_t at, float v) {
   }
 }
 
-// four neighbouring outputs
+// Four outputs of one row from feature f on, at the edge of a matrix or where rows lie badly.
 template <int OUT>
-__device__ inline void store4(const Product& a, int64_t at, f32x4 v) {
-  if constexpr (OUT <= kOutBF16) {
-    using T = typename Elem<OUT>::type;
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    *reinterpret_cast<T4*>(static_cast<T*>(a.y) + at) = T4{(T)v.x, (T)v.y, (T)v.z, (T)v.w};
-  } else {
-    float w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int p = 0; p < (OUT == kOutParts2 ? 2 : 3); ++p) {
-      uint2 u;
-      u.x = leading(w[0]); u.x |= leading(w[1]) << 16;
-      u.y = leading(w[2]); u.y |= leading(w[3]) << 16;
-      *reinterpret_cast<uint2*>(static_cast<unsigned short*>(a.y) + at + p * a.y_part) = u;
-    }
-  }
-}
-
-// Four outputs of one row from feature f on.  A gated launch writes all of a tile's features: its rows are padded, and those past
-// the last feature have to be zero for the product that reads them.
-template <int OUT, bool GATED>
 __device__ inline void put4(const Product& a, int64_t row, int f, f32x4 v) {
   const int64_t at = row * a.ldy + f;
-  if constexpr (GATED) {
-    const int left = a.n / 2 - f;
-    store4<OUT>(a, at, f32x4{left > 0 ? v.x : 0.f, left > 1 ? v.y : 0.f, left > 2 ? v.z : 0.f, left > 3 ? v.w : 0.f});
-  } else {
-    const int left = a.n - f;
-    if (a.vec_out && left >= 4) {
-      if (a.bias) v += f32x4{a.bias[f], a.bias[f + 1], a.bias[f + 2], a.bias[f + 3]};
-      store4<OUT>(a, at, v);
-    } else {
-      const float w[4] = {v.x, v.y, v.z, v.w};
+  const float w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i < left) store1<OUT>(a, at + i, w[i] + (a.bias ? a.bias[f + i] : 0.f));
-    }
-  }
+  for (int i = 0; i < 4; ++i)
+    if (f + i < a.n) store1<OUT>(a, at + i, w[i] + (a.bias ? a.bias[f + i] : 0.f));
 }
 
-// What a wave has of a tile: 32 WT rows from row_in - lane % 32 of the workgroup's on, WR row tiles of features from row_tile0 on.
-template <int WT, int WR, int OUT, bool GATED>
-__device__ inline void put_tile(const Product& a, const f32x16 (&acc)[WT][WR], int row_in, int half, int first, int count, int row_tile0) {
+// What a wave has of a tile: 32 WT rows from row0 of the workgroup's on, two row tiles of features from row_tile0 on.  Whole
+// tiles go through 4 KiB of LDS of the wave's own, 32 rows of 128 bytes at a time, so that a store writes whole lines: stored from
+// the sums' layout, 16 bytes of a row at once, 4096 x 8192 outputs took 20 us of a product of 190.  A 16-byte piece of row r lies at
+// piece ^ (r / 2 % 8).
+template <int WT, int OUT, bool GATED>
+__device__ inline void put_tile(const Product& a, const f32x16 (&acc)[WT][2], int row0, int first, int count, int row_tile0, i32x4* stage) {
+  constexpr bool kWide = OUT == kOutF32;                         // four bytes an output
+  constexpr int kParts = OUT == kOutParts2 ? 2 : OUT == kOutParts3 ? 3 : 1;
+  constexpr int kQuads = GATED ? 2 : 4;                          // of outputs a lane has in a row tile
+  constexpr int kTimes = (kWide ? 2 : 1) * kParts;               // through LDS for 32 rows
+  constexpr int kWidth = GATED ? 32 : kWide ? 32 : 64;           // features at a time
+  constexpr int kPieces = kWidth * (kWide ? 4 : 2) / 16, kEach = 64 / kPieces;
+  static_assert(!(GATED && kWide), "what a gated product writes has 16 bits");
+  const int lane = threadIdx.x & 63, half = lane >> 5, n = GATED ? a.n / 2 : a.n, f0 = row_tile0 * (GATED ? 16 : 32);
+  const bool whole = GATED || (a.vec_out && f0 + 64 <= n);
+  f32x4 bias[GATED ? 1 : 2][GATED ? 1 : 4] = {};
+  if constexpr (!GATED) {
+    if (whole && a.bias) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) bias[r][q][i] = a.bias[f0 + r * 32 + q * 8 + half * 4 + i];
+    }
+  }
 #pragma unroll
   for (int t = 0; t < WT; ++t) {
-    const int r_in = row_in + t * 32;
-    if (r_in < count) {
-      const int64_t row = a.to_slot ? a.order[first + r_in] : first + r_in;
+    f32x4 v[2][kQuads];
 #pragma unroll
-      for (int r = 0; r < WR; ++r) {
-        const int row_tile = row_tile0 + r;
-        if (row_tile < a.row_tiles) {
-          const f32x16& v = acc[t][r];
+    for (int r = 0; r < 2; ++r)
 #pragma unroll
-          for (int q = 0; q < (GATED ? 2 : 4); ++q) {
-            f32x4 u = {v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]};
-            if constexpr (GATED) u = f32x4{silu(u.x) * v[8 + q * 4], silu(u.y) * v[9 + q * 4], silu(u.z) * v[10 + q * 4], silu(u.w) * v[11 + q * 4]};
-            put4<OUT, GATED>(a, row, row_tile * (GATED ? 16 : 32) + q * 8 + half * 4, u);
-          }
+      for (int q = 0; q < kQuads; ++q) {
+        const f32x16& u = acc[t][r];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (GATED)
+            v[r][q][i] = f0 + r * 16 + q * 8 + half * 4 + i < n ? silu(u[q * 4 + i]) * u[8 + q * 4 + i] : 0.f;
+          else
+            v[r][q][i] = u[q * 4 + i] + bias[r][q][i];
         }
       }
+    if constexpr (!GATED) {
+      if (!whole) {
+        const int r_in = row0 + t * 32 + (lane & 31);
+        if (r_in < count) {
+          const int64_t row = a.to_slot ? a.order[first + r_in] : first + r_in;
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int q = 0; q < kQuads; ++q) put4<OUT>(a, row, f0 + r * 32 + q * 8 + half * 4, v[r][q]);
+        }
+        continue;
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < kTimes; ++c) {
+      const int row = lane & 31, turn = (row >> 1) & 7;
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+#pragma unroll
+        for (int q = 0; q < kQuads; ++q) {
+          if constexpr (kWide) {
+            if (r == c) stage[row * 8 + ((q * 2 + half) ^ turn)] = __builtin_bit_cast(i32x4, v[r][q]);
+          } else {
+            const int piece = r * kQuads + q;
+            uint2 u;
+            if constexpr (kParts > 1) {
+              float w[4] = {v[r][q].x, v[r][q].y, v[r][q].z, v[r][q].w};
+              u.x = leading(w[0]); u.x |= leading(w[1]) << 16;
+              u.y = leading(w[2]); u.y |= leading(w[3]) << 16;
+              v[r][q] = f32x4{w[0], w[1], w[2], w[3]};
+            } else {
+              using T = typename Elem<OUT == kOutF16 ? TETRIS_F16 : TETRIS_BF16>::type;
+              typedef T T4 __attribute__((ext_vector_type(4)));
+              u = __builtin_bit_cast(uint2, T4{(T)v[r][q].x, (T)v[r][q].y, (T)v[r][q].z, (T)v[r][q].w});
+            }
+            reinterpret_cast<uint2*>(stage)[(row * 8 + (piece ^ turn)) * 2 + half] = u;
+          }
+        }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+      for (int i = 0; i < 32 / kEach; ++i) {
+        const int out_row = i * kEach + lane / kPieces, piece = lane % kPieces;
+        const i32x4 u = stage[out_row * 8 + (piece ^ ((out_row >> 1) & 7))];
+        const int r_in = row0 + t * 32 + out_row, f = f0 + (kWide ? c * 32 + piece * 4 : piece * 8);
+        if (r_in < count && f < a.row_tiles * (GATED ? 16 : 32)) {
+          const int64_t to = (a.to_slot ? a.order[first + r_in] : first + r_in) * a.ldy + f;
+          if constexpr (kWide)
+            *reinterpret_cast<i32x4*>(static_cast<float*>(a.y) + to) = u;
+          else
+            *reinterpret_cast<i32x4*>(static_cast<unsigned short*>(a.y) + to + (kParts > 1 ? c * a.y_part : 0)) = u;
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
   }
 }
@@ -202,6 +246,21 @@ __device__ inline bool place_tile(const Product& a, int row_tiles_each, int* blo
   return true;
 }
 
+// Sixteen bytes a lane from memory to LDS, to `to` (the same for the whole wave) + lane.
+__device__ inline void to_lds(const void* from, i32x4* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+// A barrier behind which the LDS of the whole workgroup may be read and written over: this wave's reads of it have ended, and all its loads
+// have arrived but the N issued last.  (__syncthreads would wait for those as well.)
+template <int N>
+__device__ inline void barrier_but() {
+  static_assert(N < 64, "a six-bit counter");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0070);  // vmcnt(N) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // ---- many rows: tiles through LDS ---------------------------------------------------------------------------------
 //
 // A workgroup computes BM = 32 WT WM rows by 32 WR WN features.  Rows come in steps of 64 KS columns, 128 KS bytes of each
@@ -215,7 +274,7 @@ template <int WT, int WR, int WM, int WN, int KS, int OUT, bool GATED>
 __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
   constexpr int kRows = 32 * WT * WM, kThreads = 64 * WM * WN, kPieces = 8 * KS, kLoads = kRows * kPieces / kThreads;
   static_assert(kThreads / kPieces % 16 == 0, "a thread's pieces lie in the same columns");
-  __shared__ i32x4 lds[2][kRows * kPieces];
+  __shared__ i32x4 lds0[kRows * kPieces], lds1[kRows * kPieces], stage[WM * WN][256];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, wn = wave / WM;
   int block, tile;
@@ -246,43 +305,39 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
 #pragma unroll
     for (int r = 0; r < WR; ++r) acc[t][r] = f32x16{};
 
-  // Steps alternate between two sets of registers for weights, so that nothing is copied.
-  i32x4 next_x[kLoads], w[2][WR][KS];
+  // Steps alternate between two LDS buffers and two sets of registers for weights, so that nothing is copied.
+  i32x4 w[2][WR][KS];
   unsigned s[2][WR];
-  int col = 0, part = 0, next_col = 0;
-  auto fetch = [&](int set) {  // past a row's end its beginning, of which nothing is kept; past the last step that one again
-    next_col = min(col, a.col_tiles - KS);
-    const int at = next_col * 64 + column;
-    const int64_t from_row = part * a.part + (at < a.k8 ? at : 0);
+  int w_step = 0, x_col = 0, x_part = 0, w_col = 0;
+  // past the last step that one again
+  auto fetch_rows = [&](int set) {  // straight to LDS; zeros past a row's end
+    const int at = min(x_col, a.col_tiles - KS) * 64 + column;
+    const int64_t from_row = x_part * a.part + at;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) next_x[i] = *reinterpret_cast<const i32x4*>(from[i] + from_row);
+    for (int i = 0; i < kLoads; ++i) to_lds(at < a.k8 ? from[i] + from_row : static_cast<const __bf16*>(a.zeros), (set ? lds1 : lds0) + i * kThreads + wave * 64);
+    if (++x_part == a.parts) x_part = 0, x_col += KS;
+  };
+  auto fetch_weights = [&](int set) {
+    const int c0 = min(w_col, a.col_tiles - KS);
 #pragma unroll
     for (int r = 0; r < WR; ++r) {
 #pragma unroll
-      for (int c = 0; c < KS; ++c) w[set][r][c] = codes[r][(int64_t)(next_col + c) * 64];
+      for (int c = 0; c < KS; ++c) w[set][r][c] = codes[r][(int64_t)(c0 + c) * 64];
       if constexpr (KS == 1)
-        s[set][r] = scales[r][(int64_t)(next_col >> 1) * 128 + (next_col & 1)];
+        s[set][r] = scales[r][(int64_t)(c0 >> 1) * 128 + (c0 & 1)];
       else
-        s[set][r] = *reinterpret_cast<const unsigned short*>(scales[r] + (int64_t)next_col * 64);
+        s[set][r] = *reinterpret_cast<const unsigned short*>(scales[r] + (int64_t)c0 * 64);
     }
-    if (++part == a.parts) part = 0, col += KS;
+    if (++w_step == a.parts) w_step = 0, w_col += KS;
   };
-  auto keep = [&](int buffer) {
-    if (next_col * 64 + 64 * KS > a.k8) {
-      const bool in = next_col * 64 + column < a.k8;
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) next_x[i] = in ? next_x[i] : i32x4{0, 0, 0, 0};
-    }
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) lds[buffer][i * kThreads + threadIdx.x] = next_x[i];
-  };
+  constexpr int kWeightLoads = WR * (KS + 1);
 
   const int steps = a.col_tiles / KS * a.parts;
   const int row_in = wm * WT * 32 + (lane & 31), turn = turn_of<KS>(lane & 31), half = lane >> 5;
   constexpr int kRounds = 4 * KS, kProducts = WT * WR, kPairs = 4 * WR;
   i32x4 xs[2][WT], ws[2][WR];
   auto read = [&](int buffer, int j) {  // the rows' share in round j of a step's products
-    const i32x4* in = lds[buffer] + row_in * kPieces + (((j >> 2) * 8 + half * 4 + (j & 3)) ^ turn);
+    const i32x4* in = (buffer ? lds1 : lds0) + row_in * kPieces + (((j >> 2) * 8 + half * 4 + (j & 3)) ^ turn);
 #pragma unroll
     for (int t = 0; t < WT; ++t) xs[j & 1][t] = in[t * 32 * kPieces];
   };
@@ -292,13 +347,17 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
   };
   // The weights' pairs of the next round are made between the products of this one: a conversion takes the vector unit for 16 cycles, a
   // product the matrix unit for 32.  A step's last round runs behind the barrier, while the next step's first reads are under
-  // way; the next step's numbers go to LDS in the last but one, and those of the step after it are asked for.  All reads
-  // of a buffer have ended when its step's barrier is passed, so two buffers are enough.
+  // way.  All reads of a buffer have ended when its step's barrier is passed: the rows of the step after the next are asked for there,
+  // and have a step to arrive.
   auto multiply = [&](int set) {
 #pragma unroll
     for (int j = 0; j < kRounds; ++j) {
       const bool last = j + 1 == kRounds;
-      if (last) __syncthreads();
+      if (last) {
+        fetch_weights(set);
+        barrier_but<kWeightLoads>();  // the rows of the next step are there: only weights were asked for after them
+        fetch_rows(set);
+      }
       read(last ? set ^ 1 : set, last ? 0 : j + 1);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -309,17 +368,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
         for (int c = i * kPairs / kProducts; c < (i + 1) * kPairs / kProducts; ++c) convert(last ? set ^ 1 : set, last ? 0 : j + 1, c);
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (j + 2 == kRounds) {
-        keep(set ^ 1);
-        fetch(set);
-        __builtin_amdgcn_sched_barrier(0);
-      }
     }
   };
-  fetch(0);
-  keep(0);
-  fetch(1);
-  __syncthreads();
+  fetch_weights(0);
+  fetch_rows(0);
+  barrier_but<0>();
+  fetch_rows(1);
+  fetch_weights(1);
   read(0, 0);
 #pragma unroll
   for (int c = 0; c < kPairs; ++c) convert(0, 0, c);
@@ -328,7 +383,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
     multiply(1);
   }
   if (steps & 1) multiply(0);
-  put_tile<WT, WR, OUT, GATED>(a, acc, row_in, half, first, count, (block * WN + wn) * WR);
+  put_tile<WT, OUT, GATED>(a, acc, wm * WT * 32, first, count, (block * WN + wn) * WR, stage[wave]);
 }
 
 // The same for rows that are in MX4 as well, in the weights' layout (csrc/mx4.h): products of 4-bit numbers with both blocks' scales
@@ -337,7 +392,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
 template <int WT, int WR, int WM, int WN, int OUT>
 __global__ __launch_bounds__(64 * WM * WN) void rounded_kernel(Product a) {
   constexpr int kTiles = WT * WM, kThreads = 64 * WM * WN, kLoads = kTiles * 128 / kThreads;
-  __shared__ i32x4 lds[2][kTiles * 128];
+  __shared__ i32x4 lds0[kTiles * 128], lds1[kTiles * 128], stage[WM * WN][256];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, wn = wave / WM;
   int block, tile;
@@ -369,72 +424,68 @@ __global__ __launch_bounds__(64 * WM * WN) void rounded_kernel(Product a) {
 #pragma unroll
     for (int r = 0; r < WR; ++r) acc[t][r] = f32x16{};
 
-  i32x4 next_x[kLoads], next_w[WR][2], w[WR][2];
-  int next_xs[WT], x_s[WT], next_ws[WR], ws[WR];
-  auto fetch = [&](int step) {
+  const int steps = a.col_tiles >> 1;
+  i32x4 w[2][WR][2], xs[2][WT];
+  int w_scale[2][WR], x_scale[2][WT];
+  int row_step = 0, weight_step = 0;
+  // past the last step that one again
+  auto fetch_rows = [&](int set) {
+    const int64_t at = (int64_t)min(row_step++, steps - 1) * 128;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) next_x[i] = from[i][(int64_t)step * 128];
+    for (int i = 0; i < kLoads; ++i) to_lds(from[i] + at, (set ? lds1 : lds0) + i * kThreads + wave * 64);
+  };
+  auto fetch_weights = [&](int set) {
+    const int64_t at = (int64_t)min(weight_step++, steps - 1) * 64;
 #pragma unroll
     for (int r = 0; r < WR; ++r) {
-      next_w[r][0] = codes[r][(int64_t)step * 128];
-      next_w[r][1] = codes[r][(int64_t)step * 128 + 64];
-      next_ws[r] = scales[r][(int64_t)step * 64];
+      w[set][r][0] = codes[r][at * 2];
+      w[set][r][1] = codes[r][at * 2 + 64];
+      w_scale[set][r] = scales[r][at];
     }
 #pragma unroll
-    for (int t = 0; t < WT; ++t) next_xs[t] = x_scales[t][(int64_t)step * 64];
+    for (int t = 0; t < WT; ++t) x_scale[set][t] = x_scales[t][at];
   };
-  auto keep = [&](int buffer) {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) lds[buffer][i * kThreads + threadIdx.x] = next_x[i];
-#pragma unroll
-    for (int r = 0; r < WR; ++r) w[r][0] = next_w[r][0], w[r][1] = next_w[r][1], ws[r] = next_ws[r];
-#pragma unroll
-    for (int t = 0; t < WT; ++t) x_s[t] = next_xs[t];
-  };
+  constexpr int kWeightLoads = WR * 3 + WT;
   auto wide = [](i32x4 v) { return i32x8{v.x, v.y, v.z, v.w, 0, 0, 0, 0}; };
-
-  const int steps = a.col_tiles >> 1;
-  i32x4 xs[2][WT], w1[WR];
-  int xs1[WT], ws1[WR];
   auto read = [&](int buffer, int j) {
-    const i32x4* in = lds[buffer] + wm * WT * 128 + lane + j * 64;
+    const i32x4* in = (buffer ? lds1 : lds0) + wm * WT * 128 + lane + j * 64;
 #pragma unroll
     for (int t = 0; t < WT; ++t) xs[j][t] = in[t * 128];
   };
-  // the order of things as in tile_kernel, with two rounds of products a step
-  fetch(0);
-  keep(0);
-  if (steps > 1) fetch(1);
-  __syncthreads();
+  // as in tile_kernel, with two rounds of products a step
+  auto multiply = [&](int set) {
+    read(set, 1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int t = 0; t < WT; ++t)
+#pragma unroll
+      for (int r = 0; r < WR; ++r)
+        acc[t][r] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(w[set][r][0]), wide(xs[0][t]), acc[t][r], 4, 4, 0, w_scale[set][r], 0, x_scale[set][t]);
+    __builtin_amdgcn_sched_barrier(0);
+    barrier_but<kWeightLoads>();
+    fetch_rows(set);
+    read(set ^ 1, 0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int t = 0; t < WT; ++t)
+#pragma unroll
+      for (int r = 0; r < WR; ++r)
+        acc[t][r] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(w[set][r][1]), wide(xs[1][t]), acc[t][r], 4, 4, 1, w_scale[set][r], 1, x_scale[set][t]);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_weights(set);
+  };
+  fetch_rows(0);
+  fetch_weights(0);
+  barrier_but<0>();
+  fetch_rows(1);
+  fetch_weights(1);
   read(0, 0);
-  for (int step = 0; step < steps; ++step) {
-    const bool more = step + 1 < steps;
-    read(step & 1, 1);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int t = 0; t < WT; ++t)
-#pragma unroll
-      for (int r = 0; r < WR; ++r)
-        acc[t][r] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(w[r][0]), wide(xs[0][t]), acc[t][r], 4, 4, 0, ws[r], 0, x_s[t]);
-#pragma unroll
-    for (int r = 0; r < WR; ++r) w1[r] = w[r][1], ws1[r] = ws[r];
-#pragma unroll
-    for (int t = 0; t < WT; ++t) xs1[t] = x_s[t];
-    if (more) {
-      keep((step + 1) & 1);
-      if (step + 2 < steps) fetch(step + 2);
-      __syncthreads();
-      read((step + 1) & 1, 0);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int t = 0; t < WT; ++t)
-#pragma unroll
-      for (int r = 0; r < WR; ++r)
-        acc[t][r] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(w1[r]), wide(xs[1][t]), acc[t][r], 4, 4, 1, ws1[r], 1, xs1[t]);
-    __builtin_amdgcn_sched_barrier(0);
+  for (int step = 0; step + 1 < steps; step += 2) {
+    multiply(0);
+    multiply(1);
   }
-  put_tile<WT, WR, OUT, false>(a, acc, wm * WT * 32 + (lane & 31), lane >> 5, first, count, (block * WN + wn) * WR);
+  if (steps & 1) multiply(0);
+  put_tile<WT, OUT, false>(a, acc, wm * WT * 32, first, count, (block * WN + wn) * WR, stage[wave]);
 }
 
 // ---- few rows: weights streamed once -----------------------------------------------------------------------------------
@@ -700,6 +751,7 @@ int tile_rows(Product& a, int rows_a_group, hipStream_t stream) {
 void set_weights(Product* a, const tetris_mx4* w) {
   a->codes = reinterpret_cast<const i32x4*>(w->codes);
   a->scales = w->scales;
+  a->zeros = w->zeros;
   a->row_tiles = w->row_tiles;
   a->col_tiles = w->col_tiles;
   a->n = w->n;
@@ -856,7 +908,7 @@ extern "C" int tetris_mx4_linear(tetris_mx4* w, const void* d_x, int type, int m
   if ((rc = ready_rows(&a, d_x, type, m, w->k, ldx, mx4_input, stream_it, d, &as, s))) return rc;
   a.y = d_y;
   a.ldy = ldy;
-  a.vec_out = ldy % 4 == 0 && (reinterpret_cast<size_t>(d_y) & (4 * elem_size(type) - 1)) == 0;
+  a.vec_out = ldy * elem_size(type) % 16 == 0 && (reinterpret_cast<size_t>(d_y) & 15) == 0;
   a.bias = d_bias;
   return launch_product(a, kLinear, as, type, m, stream_it, s);
 }

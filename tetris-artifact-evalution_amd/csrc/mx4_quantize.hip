@@ -370,7 +370,9 @@ int lay_out(tetris_mx4* w, const uint8_t* d_codes, const uint8_t* d_scales, hipS
   w->col_tiles = (int)(round_up(w->k, kMxPad) / 64);
   const int64_t tiles = (int64_t)w->experts * w->row_tiles * w->col_tiles;
   TETRIS_HIP(hipMalloc(&w->codes, (size_t)tiles * 1024));
-  TETRIS_HIP(hipMalloc(&w->scales, (size_t)tiles * 64));
+  TETRIS_HIP(hipMalloc(&w->scales, (size_t)tiles * 64 + 64));
+  w->zeros = w->scales + tiles * 64;
+  TETRIS_HIP(hipMemsetAsync(w->zeros, 0, 64, stream));
   const int64_t total = tiles * 64;
   hipLaunchKernelGGL(layout_kernel, dim3(blocks_for(total)), dim3(256), 0, stream, reinterpret_cast<const int4*>(d_codes), d_scales, w->n,
                      w->k, w->gated ? 1 : 0, w->row_tiles, w->col_tiles, total, reinterpret_cast<int4*>(w->codes), w->scales);
