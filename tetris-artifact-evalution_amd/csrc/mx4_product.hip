@@ -35,6 +35,7 @@ struct Product {
   // order[p].  NULL: one group, position = row.
   const int* offsets;
   const int* order;
+  const int* index;      // of up to 64 slots, in place of offsets and order
   int experts;
   int from_div;          // > 0: position p reads row order[p] / from_div; 0: row p
   int to_slot;           // position p writes row order[p], else row p
@@ -77,6 +78,34 @@ __device__ inline bool find_tile(const Product& a, int tile, int size, int* expe
     before += __builtin_amdgcn_readlane(sum, 63);
   }
   return false;
+}
+
+// The same for tiles of sixteen rows, and the lane's row of the tile (that of lane % 16; the last one past the end).  Up to 64 slots
+// need no sorting: workgroup `tile` looks for the slots that name the same expert as slot `tile`, and goes on if there are a multiple of sixteen
+// of them before it.
+__device__ inline bool find_rows(const Product& a, int tile, int* expert, int* first, int* count, int* from, int* to) {
+  const int lane = threadIdx.x & 63, r16 = lane & 15;
+  if (a.index) {
+    const int mine = lane < a.rows ? a.index[lane] : -1;
+    const int e = __builtin_amdgcn_readlane(mine, tile);
+    if (e < 0 || e >= a.experts) return false;
+    const unsigned long long same = __ballot(mine == e);
+    const int rank = __builtin_popcountll(same & ((1ull << lane) - 1)), before = __builtin_amdgcn_readlane(rank, tile);
+    if (before & 15) return false;
+    *expert = e;
+    *first = 0;
+    *count = min(16, __builtin_popcountll(same) - before);
+    const int place = rank - before;
+    const int slot = __builtin_amdgcn_ds_permute((mine == e && place >= 0 && place < 16 ? place : 63) * 4, lane);
+    *to = __shfl(slot, min(r16, *count - 1));
+    *from = *to / a.from_div;
+    return true;
+  }
+  if (!find_tile(a, tile, 16, expert, first, count)) return false;
+  const int p = *first + min(r16, *count - 1);
+  *from = a.from_div ? a.order[p] / a.from_div : p;
+  *to = a.to_slot ? a.order[p] : p;
+  return true;
 }
 
 // Eight codes and their scale's exponent bits to bf16.
@@ -490,136 +519,226 @@ __global__ __launch_bounds__(64 * WM * WN) void rounded_kernel(Product a) {
 
 // ---- few rows: weights streamed once -----------------------------------------------------------------------------------
 //
-// A workgroup computes 16 RT features for up to 16 TT rows; its waves take turns at stretches of 128 columns and add their sums
-// in LDS at the end, in the order of the waves.  Bound by the weights' bytes: a lane loads 16 bytes of codes, whose
-// 32 weights feed four 16 x 16 x 32 products, and the rows' numbers come from the caches, split into parts in registers.
+// A workgroup computes 16 RT features for up to 16 rows; its waves take turns at stretches of 128 columns and add their sums
+// in LDS at the end, in the order of the waves.  Bound by the weights' bytes and, for small matrices, by the latency of one pass through the
+// memory: a lane loads 16 bytes of codes, whose 32 weights feed four 16 x 16 x 32 products, and the rows' numbers come from the
+// caches, split into parts in registers.
+
 template <int TYPE>
-__device__ inline void parts8(const typename Elem<TYPE>::type* p, bool in, bf16x8 (&out)[TYPE == TETRIS_F32 ? 3 : TYPE == TETRIS_F16 ? 2 : 1]) {
-  if constexpr (TYPE == TETRIS_BF16) {
-    out[0] = __builtin_bit_cast(bf16x8, in ? *reinterpret_cast<const i32x4*>(p) : i32x4{0, 0, 0, 0});
-  } else {
-    constexpr int P = TYPE == TETRIS_F32 ? 3 : 2;
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (in) {
-      if constexpr (TYPE == TETRIS_F32) {
-        const f32x4 u = reinterpret_cast<const f32x4*>(p)[0], t = reinterpret_cast<const f32x4*>(p)[1];
+constexpr int kPartsOf = TYPE == TETRIS_F32 ? 3 : TYPE == TETRIS_F16 ? 2 : 1;
+
+// Eight numbers of a row, as they lie, and as parts.
+template <int TYPE>
+struct Eight {
+  i32x4 raw[TYPE == TETRIS_F32 ? 2 : 1];
+  __device__ inline void load(const typename Elem<TYPE>::type* p, bool in) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = u[i], v[4 + i] = t[i];
+    for (int i = 0; i < (TYPE == TETRIS_F32 ? 2 : 1); ++i) raw[i] = in ? reinterpret_cast<const i32x4*>(p)[i] : i32x4{0, 0, 0, 0};
+  }
+  // Parts by truncation.  What is left of an infinity is NaN here, where it has to be nothing: lanes that hold one take the longer way.
+  __device__ inline void split(bf16x8 (&out)[kPartsOf<TYPE>]) const {
+    if constexpr (TYPE == TETRIS_BF16) {
+      out[0] = __builtin_bit_cast(bf16x8, raw[0]);
+    } else {
+      float v[8];
+      if constexpr (TYPE == TETRIS_F32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __int_as_float(raw[i >> 2][i & 3]);
       } else {
         typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-        const half8 u = *reinterpret_cast<const half8*>(p);
+        const half8 u = __builtin_bit_cast(half8, raw[0]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = (float)u[i];
       }
-    }
+      float most = fabsf(v[0]);
 #pragma unroll
-    for (int q = 0; q < P; ++q) {
-      i32x4 o;
+      for (int i = 1; i < 8; ++i) most = fmaxf(most, fabsf(v[i]));
+      i32x4 o[kPartsOf<TYPE>];
+      if (most == __builtin_inff()) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const unsigned lo = leading(v[2 * i]), hi = leading(v[2 * i + 1]);
-        o[i] = (int)(lo | hi << 16);
+        for (int q = 0; q < kPartsOf<TYPE>; ++q)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const unsigned lo = leading(v[2 * i]), hi = leading(v[2 * i + 1]);
+            o[q][i] = (int)(lo | hi << 16);
+          }
+      } else {
+#pragma unroll
+        for (int q = 0; q < kPartsOf<TYPE>; ++q)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const unsigned lo = __float_as_uint(v[2 * i]), hi = __float_as_uint(v[2 * i + 1]);
+            o[q][i] = (int)__builtin_amdgcn_perm(hi, lo, 0x07060302);  // the upper halves
+            v[2 * i] -= __uint_as_float(lo & 0xffff0000u);
+            v[2 * i + 1] -= __uint_as_float(hi & 0xffff0000u);
+          }
       }
-      out[q] = __builtin_bit_cast(bf16x8, o);
+#pragma unroll
+      for (int q = 0; q < kPartsOf<TYPE>; ++q) out[q] = __builtin_bit_cast(bf16x8, o[q]);
     }
   }
+};
+
+// The products of U stretches of 128 columns, c, c + step, ...: all of their loads first.
+template <int TYPE, int RT, int U>
+__device__ inline void stretch(const typename Elem<TYPE>::type* from, bool have, const i32x4* const (&codes)[RT], const uint8_t* const (&scales)[RT],
+                               int c, int step, int end, int column, int k8, f32x4 (&acc)[RT]) {
+  i32x4 w[U][RT];
+  unsigned s[U][RT];
+  Eight<TYPE> x[U][4];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int at = min(c + u * step, end - 1);
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      w[u][r] = codes[r][(int64_t)at * 128];
+      s[u][r] = scales[r][(int64_t)at * 128];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[u][j].load(from + at * 128 + j * 8, have && c + u * step < end && at * 128 + column + j * 8 < k8);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      bf16x8 xs[kPartsOf<TYPE>];
+      x[u][j].split(xs);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const bf16x8 ws = weights8(w[u][r][j], __uint_as_float(s[u][r] << 23));
+#pragma unroll
+        for (int q = 0; q < kPartsOf<TYPE>; ++q) acc[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ws, xs[q], acc[r], 0, 0, 0);
+      }
+    }
 }
 
-template <int TYPE, int TT, int RT, int OUT, bool GATED>
-__global__ __launch_bounds__(TT == 1 ? 1024 : 512) void stream_kernel(Product a) {
+// All stretches c, c + step, ... before end, U at a time while there are as many.
+template <int TYPE, int RT, int U>
+__device__ inline void stretches(const typename Elem<TYPE>::type* from, bool have, const i32x4* const (&codes)[RT], const uint8_t* const (&scales)[RT],
+                                 int c, int step, int end, int column, int k8, f32x4 (&acc)[RT]) {
+  for (; c + (U - 1) * step < end; c += U * step) stretch<TYPE, RT, U>(from, have, codes, scales, c, step, end, column, k8, acc);
+  if constexpr (U > 1) stretches<TYPE, RT, U / 2>(from, have, codes, scales, c, step, end, column, k8, acc);
+}
+
+// Where a lane's codes and scales of 16-row half `half` of an expert's matrix begin.
+__device__ inline void half_of(const Product& a, int expert, int half, int lane, const i32x4** codes, const uint8_t** scales) {
+  const int r16 = lane & 15, g = lane >> 4;
+  const int64_t t = ((int64_t)expert * a.row_tiles + (half >> 1)) * a.col_tiles;
+  const int l = (g & 1) * 32 + (half & 1) * 16 + r16;
+  *codes = a.codes + (t + (g >> 1)) * 64 + l;
+  *scales = a.scales + t * 64 + l * 2 + (g >> 1);
+}
+
+template <int TYPE, int RT, int OUT, bool GATED>
+__global__ __launch_bounds__(1024) void stream_kernel(Product a) {
   using T = typename Elem<TYPE>::type;
-  constexpr int P = TYPE == TETRIS_F32 ? 3 : TYPE == TETRIS_F16 ? 2 : 1;
-  extern __shared__ float sums[];  // [wave][RT][TT][4][64]
+  extern __shared__ float sums[];  // [wave][RT][4][64]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int halves = a.row_tiles * 2, blocks = (halves + RT - 1) / RT;
   const int tile = blockIdx.x / blocks, block = blockIdx.x - tile * blocks;
-  int expert, first, count;
-  if (!find_tile(a, tile, 16 * TT, &expert, &first, &count)) return;
+  int expert, first, count, my_row, my_slot;  // of the lane's row of the tile
+  if (!find_rows(a, tile, &expert, &first, &count, &my_row, &my_slot)) return;
 
   const int r16 = lane & 15, g = lane >> 4;
-  const T* from[TT];
-  bool have[TT];
-#pragma unroll
-  for (int t = 0; t < TT; ++t) {
-    have[t] = t * 16 + r16 < count;
-    const int p = first + min(t * 16 + r16, count - 1);
-    const int64_t row = a.from_div ? a.order[p] / a.from_div : p;
-    from[t] = static_cast<const T*>(a.x) + row * a.ldx + 32 * g;
-  }
+  const T* from = static_cast<const T*>(a.x) + (int64_t)my_row * a.ldx + 32 * g;
   const i32x4* codes[RT];
   const uint8_t* scales[RT];
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int h = min(block * RT + r, halves - 1);
-    const int64_t t = ((int64_t)expert * a.row_tiles + (h >> 1)) * a.col_tiles;
-    const int l = (g & 1) * 32 + (h & 1) * 16 + r16;
-    codes[r] = a.codes + (t + (g >> 1)) * 64 + l;
-    scales[r] = a.scales + t * 64 + l * 2 + (g >> 1);
-  }
-  f32x4 acc[RT][TT];
+  for (int r = 0; r < RT; ++r) half_of(a, expert, min(block * RT + r, halves - 1), lane, &codes[r], &scales[r]);
+  f32x4 acc[RT];
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int t = 0; t < TT; ++t) acc[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-
+  for (int r = 0; r < RT; ++r) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int chunks = a.col_tiles >> 1;
-  for (int c = wave; c < chunks; c += waves) {
-    i32x4 w[RT];
-    float s[RT];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      w[r] = codes[r][(int64_t)c * 128];
-      s[r] = __uint_as_float((unsigned)scales[r][(int64_t)c * 128] << 23);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      bf16x8 ws[RT];
-#pragma unroll
-      for (int r = 0; r < RT; ++r) ws[r] = weights8(w[r][j], s[r]);
-#pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        bf16x8 xs[P];
-        parts8<TYPE>(from[t] + c * 128 + j * 8, have[t] && c * 128 + 32 * g + j * 8 < a.k8, xs);
-#pragma unroll
-        for (int q = 0; q < P; ++q)
-#pragma unroll
-          for (int r = 0; r < RT; ++r) acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ws[r], xs[q], acc[r][t], 0, 0, 0);
-      }
-    }
-  }
+  stretches<TYPE, RT, TYPE == TETRIS_F32 ? 1 : 2>(from, r16 < count, codes, scales, wave, waves, chunks, 32 * g, a.k8, acc);
 #pragma unroll
   for (int r = 0; r < RT; ++r)
 #pragma unroll
-    for (int t = 0; t < TT; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sums[(((wave * RT + r) * TT + t) * 4 + i) * 64 + lane] = acc[r][t][i];
+    for (int i = 0; i < 4; ++i) sums[((wave * RT + r) * 4 + i) * 64 + lane] = acc[r][i];
   __syncthreads();
 
   const int n = GATED ? a.n / 2 : a.n;
   auto sum = [&](int r, int row, int f) {
-    const int at = ((r * TT + (row >> 4)) * 4 + (f & 3)) * 64 + (f >> 2) * 16 + (row & 15);
+    const int at = (r * 4 + (f & 3)) * 64 + (f >> 2) * 16 + row;
     float v = 0.f;
-    for (int w = 0; w < waves; ++w) v += sums[w * (RT * TT * 256) + at];
+    for (int w = 0; w < waves; ++w) v += sums[w * (RT * 256) + at];
     return v;
   };
-  if constexpr (GATED) {
-    static_assert(RT == 2, "a gate's rows and what they gate");
-    for (int i = threadIdx.x; i < TT * 256; i += blockDim.x) {
-      const int row = i >> 4, f = i & 15;
-      if (row >= count) break;
-      const float v = silu(sum(0, row, f)) * sum(1, row, f);
-      const int64_t to = a.to_slot ? a.order[first + row] : first + row;
-      store1<OUT>(a, to * a.ldy + block * 16 + f, block * 16 + f < n ? v : 0.f);
+  constexpr int kWidth = GATED ? 16 : 16 * RT;
+  for (int i = threadIdx.x; i < 16 * kWidth; i += blockDim.x) {  // (whole waves: the rows' numbers are passed between lanes)
+    const int row = i / kWidth, f = i % kWidth, feature = block * kWidth + f;
+    const int to = __shfl(my_slot, row);
+    if (row >= count) continue;
+    if constexpr (GATED) {
+      static_assert(RT == 2, "a gate's rows and what they gate");
+      store1<OUT>(a, (int64_t)to * a.ldy + feature, feature < n ? silu(sum(0, row, f)) * sum(1, row, f) : 0.f);
+    } else if (feature < n) {
+      store1<OUT>(a, (int64_t)to * a.ldy + feature, sum(f >> 4, row, f & 15) + (a.bias ? a.bias[feature] : 0.f));
     }
-  } else {
-    for (int i = threadIdx.x; i < RT * TT * 256; i += blockDim.x) {
-      const int row = i / (16 * RT), f = i - row * (16 * RT), feature = block * RT * 16 + f;
-      if (row >= count) break;
-      if (feature >= n) continue;
-      const float v = sum(f >> 4, row, f & 15) + (a.bias ? a.bias[feature] : 0.f);
-      const int64_t to = a.to_slot ? a.order[first + row] : first + row;
-      store1<OUT>(a, to * a.ldy + feature, v);
+  }
+}
+
+// The second product of the experts for up to 64 slots in all, and the weighted sum of each token's.  A workgroup has 16 features and goes
+// through every expert that is named; its waves share (expert, stretch of columns) pairs evenly, in runs of neighbouring ones.  A wave's sums for one
+// expert are kept at place (number of the expert + number of the wave): along the runs each step raises one of the two, so
+// no two share a place.  Each output is then added up by one thread, slots in their order, waves in theirs.
+template <int TYPE, int OUT>
+__global__ __launch_bounds__(1024) void down_kernel(Product a, const float* __restrict__ weight, int top) {
+  using T = typename Elem<TYPE>::type;
+  extern __shared__ float sums[];  // [places][4][64]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int r16 = lane & 15, g = lane >> 4, block = blockIdx.x;
+  const int mine = lane < a.rows ? a.index[lane] : -1;
+  const bool named = mine >= 0 && mine < a.experts;
+  const float my_weight = lane < a.rows ? weight[lane] : 0.f;
+  // tiles of up to sixteen slots of one expert; a lane knows its slot's tile and place in it
+  int tiles = 0, my_tile = -1, my_column = 0;
+  unsigned long long left = __ballot(named);
+  int expert_of = 0;  // lane t: the expert of tile t
+  while (left) {
+    const int e = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
+    const unsigned long long same = __ballot(named && mine == e);
+    left &= ~same;
+    const int rank = __builtin_popcountll(same & ((1ull << lane) - 1)), all = __builtin_popcountll(same);
+    if (named && mine == e) my_tile = tiles + (rank >> 4), my_column = rank & 15;
+    if (lane >= tiles && lane < tiles + (all + 15) / 16) expert_of = e;
+    tiles += (all + 15) / 16;
+  }
+  const int chunks = a.col_tiles >> 1, items = tiles * chunks, each = (items + waves - 1) / waves;
+  const int begin = min(wave * each, items), end = min(begin + each, items);
+  for (int at = begin; at < end;) {
+    const int tile = at / chunks, c0 = at - tile * chunks, c1 = min(chunks, c0 + end - at);
+    const int expert = __builtin_amdgcn_readlane(expert_of, tile);
+    const unsigned long long in = __ballot(my_tile == tile);
+    const int count = __builtin_popcountll(in);
+    // lane with column q of the tile -> every lane with r16 == q
+    const int slot = __builtin_amdgcn_ds_permute((my_tile == tile ? my_column : 63) * 4, lane);
+    const int row = __shfl(slot, min(r16, count - 1));
+    const T* from = static_cast<const T*>(a.x) + (int64_t)row * a.ldx + 32 * g;
+    const i32x4* codes[1];
+    const uint8_t* scales[1];
+    half_of(a, expert, block, lane, &codes[0], &scales[0]);
+    f32x4 acc[1] = {f32x4{0.f, 0.f, 0.f, 0.f}};
+    stretches<TYPE, 1, 2>(from, r16 < count, codes, scales, c0, 1, c1, 32 * g, a.k8, acc);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sums[((tile + wave) * 4 + i) * 64 + lane] = acc[0][i];
+    at += c1 - c0;
+  }
+  __syncthreads();
+  const int tokens = a.rows / top;
+  for (int i = threadIdx.x; i < ((tokens * 16 + 63) & ~63); i += blockDim.x) {
+    const int token = i >> 4, f = i & 15, feature = block * 16 + f;
+    float y = 0.f;
+    for (int j = 0; j < top; ++j) {
+      const int slot = token * top + j;
+      const int tile = __shfl(my_tile, slot & 63), column = __shfl(my_column, slot & 63);
+      const float by = __shfl(my_weight, slot & 63);
+      if (token >= tokens || tile < 0) continue;
+      float v = 0.f;
+      for (int w = tile * chunks / each; w <= ((tile + 1) * chunks - 1) / each; ++w)
+        v += sums[((tile + w) * 4 + (f & 3)) * 64 + (f >> 2) * 16 + column];
+      y = fmaf(by, v, y);
     }
+    if (token < tokens && feature < a.n) store1<OUT>(a, (int64_t)token * a.ldy + feature, y);
   }
 }
 
@@ -698,6 +817,13 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ 
 
 constexpr int kStreamRows = 16;  // up to so many rows of a matrix are streamed
 
+// Waves that share a row of `chunks` stretches of 128 columns.
+int stream_waves(int chunks, int64_t workgroups) {
+  int waves = workgroups <= 512 ? 16 : 4;
+  while (waves > 1 && waves > chunks) waves >>= 1;
+  return waves;
+}
+
 template <int WT, int WR, int WM, int WN, int KS, int OUT, bool GATED>
 int launch_tile(Product& a, hipStream_t stream) {
   const int size = 32 * WT * WM, row_blocks = ceil_div(a.row_tiles, WR * WN);
@@ -719,25 +845,33 @@ int launch_rounded(Product& a, hipStream_t stream) {
   return TETRIS_OK;
 }
 
-template <int TYPE, int TT, int RT, int OUT, bool GATED>
+template <int TYPE, int RT, int OUT, bool GATED>
 int launch_stream(Product& a, hipStream_t stream) {
-  const int size = 16 * TT, blocks = ceil_div(a.row_tiles * 2, RT);
-  a.max_tiles = a.offsets ? std::min(a.rows, a.rows / size + std::min(a.experts, a.rows)) : ceil_div(a.rows, size);
+  const int blocks = ceil_div(a.row_tiles * 2, RT);
+  a.max_tiles = a.index ? a.rows : a.offsets ? std::min(a.rows, a.rows / 16 + std::min(a.experts, a.rows)) : ceil_div(a.rows, 16);
   const int64_t grid = (int64_t)blocks * a.max_tiles;
   if (grid > 0x7fffffff / 2) return fail(TETRIS_EINVAL, "%d rows by %d features are too many for one launch", a.rows, a.n);
-  const int chunks = a.col_tiles / 2;
-  int waves = 8;
-  while (waves > 1 && waves > chunks) waves >>= 1;
-  hipLaunchKernelGGL((stream_kernel<TYPE, TT, RT, OUT, GATED>), dim3((unsigned)grid), dim3(64 * waves), (size_t)waves * RT * TT * 1024, stream, a);
+  const int waves = stream_waves(a.col_tiles / 2, grid);
+  hipLaunchKernelGGL((stream_kernel<TYPE, RT, OUT, GATED>), dim3((unsigned)grid), dim3(64 * waves), (size_t)waves * RT * 1024, stream, a);
   TETRIS_HIP(hipGetLastError());
   return TETRIS_OK;
 }
 
-// The rows of `a` are of TYPE and streamed; rows_a_group: as many as a group has on average.
+// The rows of `a` are of TYPE and streamed.
 template <int TYPE, int OUT, bool GATED>
-int stream_rows(Product& a, int rows_a_group, hipStream_t stream) {
-  if (rows_a_group <= 16) return launch_stream<TYPE, 1, GATED ? 2 : 1, OUT, GATED>(a, stream);
-  return launch_stream<TYPE, 2, 2, OUT, GATED>(a, stream);
+int stream_rows(Product& a, hipStream_t stream) {
+  return launch_stream<TYPE, GATED ? 2 : 1, OUT, GATED>(a, stream);
+}
+
+template <int TYPE>
+int launch_down(Product& a, const float* weight, int top, hipStream_t stream) {
+  const int waves = 16;
+  const size_t lds = (size_t)(std::min(a.rows, a.rows / 16 + a.experts) + waves) * 1024;  // at most 80 KiB
+  static const hipError_t room = hipFuncSetAttribute(reinterpret_cast<const void*>(down_kernel<TYPE, TYPE>), hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
+  TETRIS_HIP(room);
+  hipLaunchKernelGGL((down_kernel<TYPE, TYPE>), dim3(ceil_div(a.n, 16)), dim3(64 * waves), lds, stream, a, weight, top);
+  TETRIS_HIP(hipGetLastError());
+  return TETRIS_OK;
 }
 
 template <int OUT, bool GATED>
@@ -841,15 +975,15 @@ enum Role { kLinear, kUp, kDown };
 int launch_product(Product& a, Role role, int as, int type, int rows_a_group, bool stream, hipStream_t s) {
   if (stream) {
     if (as == TETRIS_F32)
-      return role == kUp ? stream_rows<TETRIS_F32, kOutF32, true>(a, rows_a_group, s) : stream_rows<TETRIS_F32, kOutF32, false>(a, rows_a_group, s);
+      return role == kUp ? stream_rows<TETRIS_F32, kOutF32, true>(a, s) : stream_rows<TETRIS_F32, kOutF32, false>(a, s);
     if (as == TETRIS_F16)
-      return role == kUp     ? stream_rows<TETRIS_F16, kOutF16, true>(a, rows_a_group, s)
-             : role == kDown ? stream_rows<TETRIS_F16, kOutF32, false>(a, rows_a_group, s)
-                             : stream_rows<TETRIS_F16, kOutF16, false>(a, rows_a_group, s);
-    if (role == kUp) return stream_rows<TETRIS_BF16, kOutBF16, true>(a, rows_a_group, s);
-    if (role == kDown || type == TETRIS_F32) return stream_rows<TETRIS_BF16, kOutF32, false>(a, rows_a_group, s);
-    if (type == TETRIS_F16) return stream_rows<TETRIS_BF16, kOutF16, false>(a, rows_a_group, s);
-    return stream_rows<TETRIS_BF16, kOutBF16, false>(a, rows_a_group, s);
+      return role == kUp     ? stream_rows<TETRIS_F16, kOutF16, true>(a, s)
+             : role == kDown ? stream_rows<TETRIS_F16, kOutF32, false>(a, s)
+                             : stream_rows<TETRIS_F16, kOutF16, false>(a, s);
+    if (role == kUp) return stream_rows<TETRIS_BF16, kOutBF16, true>(a, s);
+    if (role == kDown || type == TETRIS_F32) return stream_rows<TETRIS_BF16, kOutF32, false>(a, s);
+    if (type == TETRIS_F16) return stream_rows<TETRIS_BF16, kOutF16, false>(a, s);
+    return stream_rows<TETRIS_BF16, kOutBF16, false>(a, s);
   }
   if (a.x_scales) {
     if (type == TETRIS_F32) return launch_rounded<4, 2, 2, 4, kOutF32>(a, s);
@@ -950,7 +1084,7 @@ extern "C" int tetris_experts_prepare(tetris_mx4* up, tetris_mx4* down, int toke
   const int rc = experts_check(up, down, tokens, top, type);
   if (rc || tokens == 0) return rc;
   uint8_t* d;
-  return workspace(up, static_cast<hipStream_t>(stream), expert_space(up, down, tokens, top, type, streams(rows_a_group(up, tokens, top))).all, &d);
+  return workspace(up, static_cast<hipStream_t>(stream), expert_space(up, down, tokens, top, type, tokens * top <= 64 || streams(rows_a_group(up, tokens, top))).all, &d);
 }
 
 extern "C" int tetris_experts(tetris_mx4* up, tetris_mx4* down, const void* d_x, int type, int tokens, int64_t ldx, int top,
@@ -964,23 +1098,30 @@ extern "C" int tetris_experts(tetris_mx4* up, tetris_mx4* down, const void* d_x,
   if ((reinterpret_cast<size_t>(d_index) | reinterpret_cast<size_t>(d_weight)) & 3) return fail(TETRIS_EINVAL, "index or weights not aligned to their elements");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int slots = tokens * top, each = rows_a_group(up, tokens, top);
-  const bool stream_it = streams(each);
+  const bool stream_it = slots <= 64 || streams(each);
   const ExpertSpace e = expert_space(up, down, tokens, top, type, stream_it);
   uint8_t* d;
   if ((rc = workspace(up, s, e.all, &d))) return rc;
   int* offsets = reinterpret_cast<int*>(d + e.offsets);
   int* order = reinterpret_cast<int*>(d + e.order);
-  const int threads = std::min(1024, (int)round_up(slots, 64));
-  hipLaunchKernelGGL(plan_kernel, dim3(up->experts), dim3(threads), 0, s, d_index, slots, up->experts, offsets, order);
-  TETRIS_HIP(hipGetLastError());
+  const bool few = slots <= 64;  // no sorting, two launches
+  if (!few) {
+    const int threads = std::min(1024, (int)round_up(slots, 64));
+    hipLaunchKernelGGL(plan_kernel, dim3(up->experts), dim3(threads), 0, s, d_index, slots, up->experts, offsets, order);
+    TETRIS_HIP(hipGetLastError());
+  }
 
   Product a{};
   set_weights(&a, up);
   int as;
   if ((rc = ready_rows(&a, d_x, type, tokens, up->k, ldx, false, stream_it, d + e.ready, &as, s))) return rc;
   a.rows = slots;
-  a.offsets = offsets;
-  a.order = order;
+  if (few) {
+    a.index = d_index;
+  } else {
+    a.offsets = offsets;
+    a.order = order;
+  }
   a.experts = up->experts;
   a.from_div = top;
   a.y = d + e.hidden;
@@ -996,9 +1137,17 @@ extern "C" int tetris_experts(tetris_mx4* up, tetris_mx4* down, const void* d_x,
   b.parts = stream_it ? 1 : parts_of(type);
   b.k8 = (int)round_up(down->k, 8);
   b.rows = slots;
+  b.experts = up->experts;
+  if (few) {
+    b.index = d_index;
+    b.y = d_y;
+    b.ldy = ldy;
+    return type == TETRIS_F32   ? launch_down<TETRIS_F32>(b, d_weight, top, s)
+           : type == TETRIS_F16 ? launch_down<TETRIS_F16>(b, d_weight, top, s)
+                                : launch_down<TETRIS_BF16>(b, d_weight, top, s);
+  }
   b.offsets = offsets;
   b.order = order;
-  b.experts = up->experts;
   b.to_slot = 1;
   b.y = d + e.rows;
   b.ldy = round_up(down->n, 4);
