@@ -299,11 +299,11 @@ __device__ inline void barrier_but() {
 template <int KS>
 __device__ inline int turn_of(int row) { return KS == 1 ? (row >> 1) & 7 : row & 15; }
 
-template <int WT, int WR, int WM, int WN, int KS, int OUT, bool GATED>
+template <int WT, int WR, int WM, int WN, int KS, int PI, int OUT, bool GATED>
 __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
   constexpr int kRows = 32 * WT * WM, kThreads = 64 * WM * WN, kPieces = 8 * KS, kLoads = kRows * kPieces / kThreads;
   static_assert(kThreads / kPieces % 16 == 0, "a thread's pieces lie in the same columns");
-  __shared__ i32x4 lds0[kRows * kPieces], lds1[kRows * kPieces], stage[WM * WN][256];
+  __shared__ i32x4 lds0[PI * kRows * kPieces], lds1[PI * kRows * kPieces], stage[WM * WN][256];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, wn = wave / WM;
   int block, tile;
@@ -341,10 +341,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
   // past the last step that one again
   auto fetch_rows = [&](int set) {  // straight to LDS; zeros past a row's end
     const int at = min(x_col, a.col_tiles - KS) * 64 + column;
-    const int64_t from_row = x_part * a.part + at;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) to_lds(at < a.k8 ? from[i] + from_row : static_cast<const __bf16*>(a.zeros), (set ? lds1 : lds0) + i * kThreads + wave * 64);
-    if (++x_part == a.parts) x_part = 0, x_col += KS;
+    for (int p = 0; p < PI; ++p) {
+      const int64_t from_row = (x_part + p) * a.part + at;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        to_lds(at < a.k8 ? from[i] + from_row : static_cast<const __bf16*>(a.zeros), (set ? lds1 : lds0) + (p * kLoads + i) * kThreads + wave * 64);
+    }
+    x_part += PI;
+    if (x_part == a.parts) x_part = 0, x_col += KS;
   };
   auto fetch_weights = [&](int set) {
     const int c0 = min(w_col, a.col_tiles - KS);
@@ -357,18 +362,20 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
       else
         s[set][r] = *reinterpret_cast<const unsigned short*>(scales[r] + (int64_t)c0 * 64);
     }
-    if (++w_step == a.parts) w_step = 0, w_col += KS;
+    w_step += PI;
+    if (w_step == a.parts) w_step = 0, w_col += KS;
   };
   constexpr int kWeightLoads = WR * (KS + 1);
 
-  const int steps = a.col_tiles / KS * a.parts;
+  const int steps = a.col_tiles / KS * (a.parts / PI);
   const int row_in = wm * WT * 32 + (lane & 31), turn = turn_of<KS>(lane & 31), half = lane >> 5;
-  constexpr int kRounds = 4 * KS, kProducts = WT * WR, kPairs = 4 * WR;
+  constexpr int kRounds = 4 * KS * PI, kProducts = WT * WR, kPairs = 4 * WR;
   i32x4 xs[2][WT], ws[2][WR];
-  auto read = [&](int buffer, int j) {  // the rows' share in round j of a step's products
-    const i32x4* in = (buffer ? lds1 : lds0) + row_in * kPieces + (((j >> 2) * 8 + half * 4 + (j & 3)) ^ turn);
+  auto read = [&](int buffer, int round) {  // the rows' share in a round of a step's products: PI parts of the same columns after another
+    const int j = round / PI, p = round % PI;
+    const i32x4* in = (buffer ? lds1 : lds0) + (p * kRows + row_in) * kPieces + (((j >> 2) * 8 + half * 4 + (j & 3)) ^ turn);
 #pragma unroll
-    for (int t = 0; t < WT; ++t) xs[j & 1][t] = in[t * 32 * kPieces];
+    for (int t = 0; t < WT; ++t) xs[round & 1][t] = in[t * 32 * kPieces];
   };
   auto convert = [&](int set, int j, int i) {  // (the sign bit of a scale is not looked at)
     const float scale = __uint_as_float((s[set][i >> 2] >> (8 * (j >> 2))) << 23);
@@ -380,21 +387,24 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
   // and have a step to arrive.
   auto multiply = [&](int set) {
 #pragma unroll
-    for (int j = 0; j < kRounds; ++j) {
-      const bool last = j + 1 == kRounds;
+    for (int round = 0; round < kRounds; ++round) {
+      const bool last = round + 1 == kRounds;
+      const int j = round / PI;
       if (last) {
         fetch_weights(set);
         barrier_but<kWeightLoads>();  // the rows of the next step are there: only weights were asked for after them
         fetch_rows(set);
       }
-      read(last ? set ^ 1 : set, last ? 0 : j + 1);
+      read(last ? set ^ 1 : set, last ? 0 : round + 1);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < kProducts; ++i) {
         const int t = i / WR, r = i % WR;
-        acc[t][r] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ws[j & 1][r]), __builtin_bit_cast(bf16x8, xs[j & 1][t]), acc[t][r], 0, 0, 0);
+        acc[t][r] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ws[j & 1][r]), __builtin_bit_cast(bf16x8, xs[round & 1][t]), acc[t][r], 0, 0, 0);
+        if (round % PI == PI - 1) {
 #pragma unroll
-        for (int c = i * kPairs / kProducts; c < (i + 1) * kPairs / kProducts; ++c) convert(last ? set ^ 1 : set, last ? 0 : j + 1, c);
+          for (int c = i * kPairs / kProducts; c < (i + 1) * kPairs / kProducts; ++c) convert(last ? set ^ 1 : set, last ? 0 : j + 1, c);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -824,13 +834,13 @@ int stream_waves(int chunks, int64_t workgroups) {
   return waves;
 }
 
-template <int WT, int WR, int WM, int WN, int KS, int OUT, bool GATED>
+template <int WT, int WR, int WM, int WN, int KS, int PI, int OUT, bool GATED>
 int launch_tile(Product& a, hipStream_t stream) {
   const int size = 32 * WT * WM, row_blocks = ceil_div(a.row_tiles, WR * WN);
   a.max_tiles = a.offsets ? std::min(a.rows, a.rows / size + std::min(a.experts, a.rows)) : ceil_div(a.rows, size);
   const int64_t blocks = round_up((int64_t)row_blocks * a.max_tiles, 256);
   if (blocks > 0x7fffffff / 2) return fail(TETRIS_EINVAL, "%d rows by %d features are too many for one launch", a.rows, a.n);
-  hipLaunchKernelGGL((tile_kernel<WT, WR, WM, WN, KS, OUT, GATED>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream, a);
+  hipLaunchKernelGGL((tile_kernel<WT, WR, WM, WN, KS, PI, OUT, GATED>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream, a);
   TETRIS_HIP(hipGetLastError());
   return TETRIS_OK;
 }
@@ -874,12 +884,13 @@ int launch_down(Product& a, const float* weight, int top, hipStream_t stream) {
   return TETRIS_OK;
 }
 
-template <int OUT, bool GATED>
+// P: the rows' parts.
+template <int OUT, bool GATED, int P>
 int tile_rows(Product& a, int rows_a_group, hipStream_t stream) {
-  if (rows_a_group <= 40) return launch_tile<1, 2, 1, 4, 2, OUT, GATED>(a, stream);
-  if (rows_a_group <= 80) return launch_tile<2, 2, 1, 4, 2, OUT, GATED>(a, stream);
-  if (rows_a_group <= 300) return launch_tile<4, 2, 1, 4, 2, OUT, GATED>(a, stream);
-  return launch_tile<4, 2, 2, 4, 1, OUT, GATED>(a, stream);
+  if (rows_a_group <= 40) return launch_tile<1, 2, 1, 4, 2, P, OUT, GATED>(a, stream);
+  if (rows_a_group <= 80) return launch_tile<2, 2, 1, 4, P == 3 ? 1 : 2, P, OUT, GATED>(a, stream);
+  if (rows_a_group <= 300) return launch_tile<4, 2, 1, 4, 1, 1, OUT, GATED>(a, stream);
+  return launch_tile<4, 2, 2, 4, 1, 1, OUT, GATED>(a, stream);
 }
 
 void set_weights(Product* a, const tetris_mx4* w) {
@@ -990,14 +1001,14 @@ int launch_product(Product& a, Role role, int as, int type, int rows_a_group, bo
     if (type == TETRIS_F16) return launch_rounded<4, 2, 2, 4, kOutF16>(a, s);
     return launch_rounded<4, 2, 2, 4, kOutBF16>(a, s);
   }
-  if (role == kUp) {
-    if (type == TETRIS_F32) return tile_rows<kOutParts3, true>(a, rows_a_group, s);
-    if (type == TETRIS_F16) return tile_rows<kOutParts2, true>(a, rows_a_group, s);
-    return tile_rows<kOutBF16, true>(a, rows_a_group, s);
-  }
-  if (role == kDown || type == TETRIS_F32) return tile_rows<kOutF32, false>(a, rows_a_group, s);
-  if (type == TETRIS_F16) return tile_rows<kOutF16, false>(a, rows_a_group, s);
-  return tile_rows<kOutBF16, false>(a, rows_a_group, s);
+  if (type == TETRIS_F32) return role == kUp ? tile_rows<kOutParts3, true, 3>(a, rows_a_group, s) : tile_rows<kOutF32, false, 3>(a, rows_a_group, s);
+  if (type == TETRIS_F16)
+    return role == kUp     ? tile_rows<kOutParts2, true, 2>(a, rows_a_group, s)
+           : role == kDown ? tile_rows<kOutF32, false, 2>(a, rows_a_group, s)
+                           : tile_rows<kOutF16, false, 2>(a, rows_a_group, s);
+  return role == kUp     ? tile_rows<kOutBF16, true, 1>(a, rows_a_group, s)
+         : role == kDown ? tile_rows<kOutF32, false, 1>(a, rows_a_group, s)
+                         : tile_rows<kOutBF16, false, 1>(a, rows_a_group, s);
 }
 
 int check_rows(const void* x, int type, int rows, int64_t ld, int k, const char* what) {
