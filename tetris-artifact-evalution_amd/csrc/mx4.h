@@ -47,6 +47,7 @@ int stage_rows(const void* d_x, int type, int64_t rows, int cols, int64_t ld, in
 struct tetris_mx4 {
   int experts = 0, n = 0, k = 0;
   bool gated = false;
+  bool half = false;                 // every weight is exact in f16
   int row_tiles = 0, col_tiles = 0;  // of one matrix
   uint8_t* codes = nullptr;
   uint8_t* scales = nullptr;  // zeros behind them

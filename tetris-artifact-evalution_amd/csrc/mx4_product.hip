@@ -14,6 +14,7 @@ namespace tetris {
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -118,14 +119,32 @@ __device__ inline bf16x8 weights8(int codes, float scale) {
   return __builtin_bit_cast(bf16x8, v);
 }
 
-// the same for the i-th pair
+// The i-th pair of eight codes to bf16, or to f16.
+template <bool HALF>
 __device__ inline int pair_of(int codes, float scale, int i) {
-  switch (i) {  // (a constant where this is used)
-    case 0: return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)codes, scale, 0));
-    case 1: return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)codes, scale, 1));
-    case 2: return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)codes, scale, 2));
-    default: return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((unsigned)codes, scale, 3));
+  const unsigned c = (unsigned)codes;
+  if constexpr (HALF) {
+    switch (i) {  // (a constant where this is used)
+      case 0: return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 0));
+      case 1: return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 1));
+      case 2: return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 2));
+      default: return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, scale, 3));
+    }
+  } else {
+    switch (i) {
+      case 0: return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 0));
+      case 1: return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 1));
+      case 2: return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 2));
+      default: return __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 3));
+    }
   }
+}
+template <bool HALF>
+__device__ inline f32x16 product32(i32x4 w, i32x4 x, f32x16 acc) {
+  if constexpr (HALF)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, w), __builtin_bit_cast(f16x8, x), acc, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, x), acc, 0, 0, 0);
 }
 
 __device__ inline float silu(float v) { return v / (1.f + expf(-v)); }
@@ -299,7 +318,7 @@ __device__ inline void barrier_but() {
 template <int KS>
 __device__ inline int turn_of(int row) { return KS == 1 ? (row >> 1) & 7 : row & 15; }
 
-template <int WT, int WR, int WM, int WN, int KS, int PI, int OUT, bool GATED>
+template <int WT, int WR, int WM, int WN, int KS, int PI, bool HALF, int OUT, bool GATED>
 __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
   constexpr int kRows = 32 * WT * WM, kThreads = 64 * WM * WN, kPieces = 8 * KS, kLoads = kRows * kPieces / kThreads;
   static_assert(kThreads / kPieces % 16 == 0, "a thread's pieces lie in the same columns");
@@ -379,7 +398,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
   };
   auto convert = [&](int set, int j, int i) {  // (the sign bit of a scale is not looked at)
     const float scale = __uint_as_float((s[set][i >> 2] >> (8 * (j >> 2))) << 23);
-    ws[j & 1][i >> 2][i & 3] = pair_of(w[set][i >> 2][j >> 2][j & 3], scale, i & 3);
+    ws[j & 1][i >> 2][i & 3] = pair_of<HALF>(w[set][i >> 2][j >> 2][j & 3], scale, i & 3);
   };
   // The weights' pairs of the next round are made between the products of this one: a conversion takes the vector unit for 16 cycles, a
   // product the matrix unit for 32.  A step's last round runs behind the barrier, while the next step's first reads are under
@@ -400,7 +419,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
 #pragma unroll
       for (int i = 0; i < kProducts; ++i) {
         const int t = i / WR, r = i % WR;
-        acc[t][r] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ws[j & 1][r]), __builtin_bit_cast(bf16x8, xs[round & 1][t]), acc[t][r], 0, 0, 0);
+        acc[t][r] = product32<HALF>(ws[j & 1][r], xs[round & 1][t], acc[t][r]);
         if (round % PI == PI - 1) {
 #pragma unroll
           for (int c = i * kPairs / kProducts; c < (i + 1) * kPairs / kProducts; ++c) convert(last ? set ^ 1 : set, last ? 0 : j + 1, c);
@@ -834,13 +853,13 @@ int stream_waves(int chunks, int64_t workgroups) {
   return waves;
 }
 
-template <int WT, int WR, int WM, int WN, int KS, int PI, int OUT, bool GATED>
+template <int WT, int WR, int WM, int WN, int KS, int PI, bool HALF, int OUT, bool GATED>
 int launch_tile(Product& a, hipStream_t stream) {
   const int size = 32 * WT * WM, row_blocks = ceil_div(a.row_tiles, WR * WN);
   a.max_tiles = a.offsets ? std::min(a.rows, a.rows / size + std::min(a.experts, a.rows)) : ceil_div(a.rows, size);
   const int64_t blocks = round_up((int64_t)row_blocks * a.max_tiles, 256);
   if (blocks > 0x7fffffff / 2) return fail(TETRIS_EINVAL, "%d rows by %d features are too many for one launch", a.rows, a.n);
-  hipLaunchKernelGGL((tile_kernel<WT, WR, WM, WN, KS, PI, OUT, GATED>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream, a);
+  hipLaunchKernelGGL((tile_kernel<WT, WR, WM, WN, KS, PI, HALF, OUT, GATED>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream, a);
   TETRIS_HIP(hipGetLastError());
   return TETRIS_OK;
 }
@@ -884,13 +903,13 @@ int launch_down(Product& a, const float* weight, int top, hipStream_t stream) {
   return TETRIS_OK;
 }
 
-// P: the rows' parts.
-template <int OUT, bool GATED, int P>
+// P: the rows' parts.  HALF: rows and weights in f16.
+template <int OUT, bool GATED, int P, bool HALF = false>
 int tile_rows(Product& a, int rows_a_group, hipStream_t stream) {
-  if (rows_a_group <= 40) return launch_tile<1, 2, 1, 4, 2, P, OUT, GATED>(a, stream);
-  if (rows_a_group <= 80) return launch_tile<2, 2, 1, 4, P == 3 ? 1 : 2, P, OUT, GATED>(a, stream);
-  if (rows_a_group <= 300) return launch_tile<4, 2, 1, 4, 1, 1, OUT, GATED>(a, stream);
-  return launch_tile<4, 2, 2, 4, 1, 1, OUT, GATED>(a, stream);
+  if (rows_a_group <= 40) return launch_tile<1, 2, 1, 4, 2, P, HALF, OUT, GATED>(a, stream);
+  if (rows_a_group <= 80) return launch_tile<2, 2, 1, 4, P == 3 ? 1 : 2, P, HALF, OUT, GATED>(a, stream);
+  if (rows_a_group <= 300) return launch_tile<4, 2, 1, 4, 1, 1, HALF, OUT, GATED>(a, stream);
+  return launch_tile<4, 2, 2, 4, 1, 1, HALF, OUT, GATED>(a, stream);
 }
 
 void set_weights(Product* a, const tetris_mx4* w) {
@@ -937,15 +956,18 @@ int workspace(tetris_mx4* w, hipStream_t stream, size_t need, uint8_t** out) {
 
 bool streams(int rows) { return rows <= kStreamRows; }
 
+// Whether rows of `type` are multiplied in f16: where the weights are exact in it.  Others of f16 are taken in two bf16 parts.
+bool in_half(int type, const tetris_mx4* w) { return type == TETRIS_F16 && w->half; }
+
 // bytes that rows made ready for a product take at most
-size_t staged_bytes(int rows, int k, int type, bool rounded, bool stream) {
+size_t staged_bytes(int rows, int k, int type, bool rounded, bool stream, bool half) {
   const size_t padded = (size_t)rows * round_up(k, kMxPad);
   if (rounded) return stream ? padded * 2 : (size_t)round_up(rows, 32) * round_up(k, kMxPad) / 32 * 17;
-  return padded * (stream ? elem_size(type) : 2 * parts_of(type));
+  return padded * (stream || half ? elem_size(type) : 2 * parts_of(type));
 }
 
 // Points `a` at rows x of `type`, made ready in d_ready where they have to be.  *as: the type the product reads.
-int ready_rows(Product* a, const void* x, int type, int rows, int k, int64_t ld, bool rounded, bool stream, uint8_t* d_ready, int* as,
+int ready_rows(Product* a, const void* x, int type, int rows, int k, int64_t ld, bool rounded, bool stream, bool half, uint8_t* d_ready, int* as,
                hipStream_t s) {
   const int64_t padded = round_up(k, kMxPad);
   a->rows = rows;
@@ -962,7 +984,8 @@ int ready_rows(Product* a, const void* x, int type, int rows, int k, int64_t ld,
     a->x_scales = scales;
     return mx4_quantize_to(kMxTiles, x, type, rows, k, ld, d_ready, scales, s);
   }
-  if (lies_well(x, ld, k, type) && (stream || type == TETRIS_BF16)) {
+  const bool as_is = stream || half || type == TETRIS_BF16;
+  if (lies_well(x, ld, k, type) && as_is) {
     a->x = x;
     a->ldx = ld;
     a->k8 = k;
@@ -971,7 +994,7 @@ int ready_rows(Product* a, const void* x, int type, int rows, int k, int64_t ld,
   a->x = d_ready;
   a->ldx = padded;
   a->k8 = (int)padded;
-  if (stream || type == TETRIS_BF16) return stage_rows(x, type, rows, k, ld, 0, d_ready, s);
+  if (as_is) return stage_rows(x, type, rows, k, ld, 0, d_ready, s);
   a->parts = parts_of(type);
   a->part = rows * padded;
   *as = TETRIS_BF16;
@@ -1002,6 +1025,10 @@ int launch_product(Product& a, Role role, int as, int type, int rows_a_group, bo
     return launch_rounded<4, 2, 2, 4, kOutBF16>(a, s);
   }
   if (type == TETRIS_F32) return role == kUp ? tile_rows<kOutParts3, true, 3>(a, rows_a_group, s) : tile_rows<kOutF32, false, 3>(a, rows_a_group, s);
+  if (as == TETRIS_F16)
+    return role == kUp     ? tile_rows<kOutF16, true, 1, true>(a, rows_a_group, s)
+           : role == kDown ? tile_rows<kOutF32, false, 1, true>(a, rows_a_group, s)
+                           : tile_rows<kOutF16, false, 1, true>(a, rows_a_group, s);
   if (type == TETRIS_F16)
     return role == kUp     ? tile_rows<kOutParts2, true, 2>(a, rows_a_group, s)
            : role == kDown ? tile_rows<kOutF32, false, 2>(a, rows_a_group, s)
@@ -1028,7 +1055,7 @@ extern "C" int tetris_mx4_prepare(tetris_mx4* w, int m, int type, int mx4_input,
   if (bad_type(type)) return fail(TETRIS_EINVAL, "type %d is not TETRIS_F32, TETRIS_F16 or TETRIS_BF16", type);
   if (m < 0) return fail(TETRIS_EINVAL, "%d rows", m);
   uint8_t* d;
-  return workspace(w, static_cast<hipStream_t>(stream), staged_bytes(m, w->k, type, mx4_input, streams(m)), &d);
+  return workspace(w, static_cast<hipStream_t>(stream), staged_bytes(m, w->k, type, mx4_input, streams(m), in_half(type, w)), &d);
 }
 
 extern "C" int tetris_mx4_linear(tetris_mx4* w, const void* d_x, int type, int m, int64_t ldx, void* d_y, int64_t ldy,
@@ -1044,13 +1071,14 @@ extern "C" int tetris_mx4_linear(tetris_mx4* w, const void* d_x, int type, int m
   if (reinterpret_cast<size_t>(d_bias) & 3) return fail(TETRIS_EINVAL, "bias not aligned to its elements");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool stream_it = streams(m);
-  const bool as_it_lies = !mx4_input && lies_well(d_x, ldx, w->k, type) && (stream_it || type == TETRIS_BF16);
+  const bool half = in_half(type, w);
+  const bool as_it_lies = !mx4_input && lies_well(d_x, ldx, w->k, type) && (stream_it || half || type == TETRIS_BF16);
   uint8_t* d = nullptr;
-  if (!as_it_lies && (rc = workspace(w, s, staged_bytes(m, w->k, type, mx4_input, stream_it), &d))) return rc;
+  if (!as_it_lies && (rc = workspace(w, s, staged_bytes(m, w->k, type, mx4_input, stream_it, half), &d))) return rc;
   Product a{};
   set_weights(&a, w);
   int as;
-  if ((rc = ready_rows(&a, d_x, type, m, w->k, ldx, mx4_input, stream_it, d, &as, s))) return rc;
+  if ((rc = ready_rows(&a, d_x, type, m, w->k, ldx, mx4_input, stream_it, half, d, &as, s))) return rc;
   a.y = d_y;
   a.ldy = ldy;
   a.vec_out = ldy * elem_size(type) % 16 == 0 && (reinterpret_cast<size_t>(d_y) & 15) == 0;
@@ -1066,13 +1094,14 @@ struct ExpertSpace {
 
 ExpertSpace expert_space(const tetris_mx4* up, const tetris_mx4* down, int tokens, int top, int type, bool stream) {
   const size_t slots = (size_t)tokens * top;
+  const bool half = in_half(type, up) && in_half(type, down);
   ExpertSpace e;
   e.offsets = 0;
   e.order = up256(e.offsets + 4 * ((size_t)up->experts + 1));
   e.hidden = up256(e.order + 4 * slots);
-  e.rows = up256(e.hidden + slots * round_up(down->k, kMxPad) * (stream ? elem_size(type) : 2 * parts_of(type)));
+  e.rows = up256(e.hidden + slots * round_up(down->k, kMxPad) * (stream || half ? elem_size(type) : 2 * parts_of(type)));
   e.ready = up256(e.rows + slots * round_up(down->n, 4) * 4);
-  e.all = e.ready + staged_bytes(tokens, up->k, type, false, stream);
+  e.all = e.ready + staged_bytes(tokens, up->k, type, false, stream, half);
   return e;
 }
 
@@ -1110,6 +1139,7 @@ extern "C" int tetris_experts(tetris_mx4* up, tetris_mx4* down, const void* d_x,
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int slots = tokens * top, each = rows_a_group(up, tokens, top);
   const bool stream_it = slots <= 64 || streams(each);
+  const bool half = in_half(type, up) && in_half(type, down);
   const ExpertSpace e = expert_space(up, down, tokens, top, type, stream_it);
   uint8_t* d;
   if ((rc = workspace(up, s, e.all, &d))) return rc;
@@ -1125,7 +1155,7 @@ extern "C" int tetris_experts(tetris_mx4* up, tetris_mx4* down, const void* d_x,
   Product a{};
   set_weights(&a, up);
   int as;
-  if ((rc = ready_rows(&a, d_x, type, tokens, up->k, ldx, false, stream_it, d + e.ready, &as, s))) return rc;
+  if ((rc = ready_rows(&a, d_x, type, tokens, up->k, ldx, false, stream_it, half, d + e.ready, &as, s))) return rc;
   a.rows = slots;
   if (few) {
     a.index = d_index;
@@ -1145,7 +1175,7 @@ extern "C" int tetris_experts(tetris_mx4* up, tetris_mx4* down, const void* d_x,
   b.x = d + e.hidden;
   b.ldx = a.ldy;
   b.part = a.y_part;
-  b.parts = stream_it ? 1 : parts_of(type);
+  b.parts = stream_it || half ? 1 : parts_of(type);
   b.k8 = (int)round_up(down->k, 8);
   b.rows = slots;
   b.experts = up->experts;
@@ -1163,7 +1193,7 @@ extern "C" int tetris_experts(tetris_mx4* up, tetris_mx4* down, const void* d_x,
   b.y = d + e.rows;
   b.ldy = round_up(down->n, 4);
   b.vec_out = 1;
-  if ((rc = launch_product(b, kDown, stream_it ? type : (int)TETRIS_BF16, type, each, stream_it, s))) return rc;
+  if ((rc = launch_product(b, kDown, stream_it || half ? type : (int)TETRIS_BF16, type, each, stream_it, s))) return rc;
 
   const int vec = ldy % 4 == 0 && (reinterpret_cast<size_t>(d_y) & (4 * elem_size(type) - 1)) == 0;
   const float* rows = reinterpret_cast<const float*>(d + e.rows);

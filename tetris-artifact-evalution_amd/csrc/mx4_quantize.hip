@@ -197,11 +197,13 @@ __global__ __launch_bounds__(256) void stage_kernel(const typename Elem<TYPE>::t
   }
 }
 
-// MX4 rows to the layout of csrc/mx4.h: one thread moves one block (16 bytes and a scale).
+// MX4 rows to the layout of csrc/mx4.h: one thread moves one block (16 bytes and a scale).  range: the least and the largest scale of
+// blocks that hold a number other than zero (kept by minimum and maximum, so the order of the atomics does not show).
 __global__ __launch_bounds__(256) void layout_kernel(const int4* __restrict__ codes, const uint8_t* __restrict__ scales, int n, int k,
                                                      int gated, int row_tiles, int col_tiles, int64_t total,
-                                                     int4* __restrict__ out, uint8_t* __restrict__ out_scales) {
+                                                     int4* __restrict__ out, uint8_t* __restrict__ out_scales, int* __restrict__ range) {
   const int blocks = (k + 31) / 32;
+  int least = 255, most = 0;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
     const int lane = (int)(i & 63);
     const int64_t tile = i >> 6, row_tile = tile / col_tiles, matrix = row_tile / row_tiles;
@@ -227,7 +229,20 @@ __global__ __launch_bounds__(256) void layout_kernel(const int4* __restrict__ co
       }
     }
     out[i] = c;
+    if (in && ((c.x | c.y | c.z | c.w) & 0x77777777) && scales[from] != 255) {
+      least = min(least, (int)scales[from]);
+      most = max(most, (int)scales[from]);
+    }
     out_scales[((row_tile * (col_tiles >> 1) + (col_tile >> 1)) * 64 + lane) * 2 + (col_tile & 1)] = in ? scales[from] : 127;
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    least = min(least, __shfl_xor(least, d));
+    most = max(most, __shfl_xor(most, d));
+  }
+  if ((threadIdx.x & 63) == 0) {
+    atomicMin(&range[0], least);
+    atomicMax(&range[1], most);
   }
 }
 
@@ -370,14 +385,20 @@ int lay_out(tetris_mx4* w, const uint8_t* d_codes, const uint8_t* d_scales, hipS
   w->col_tiles = (int)(round_up(w->k, kMxPad) / 64);
   const int64_t tiles = (int64_t)w->experts * w->row_tiles * w->col_tiles;
   TETRIS_HIP(hipMalloc(&w->codes, (size_t)tiles * 1024));
-  TETRIS_HIP(hipMalloc(&w->scales, (size_t)tiles * 64 + 64));
+  TETRIS_HIP(hipMalloc(&w->scales, (size_t)tiles * 64 + 128));
   w->zeros = w->scales + tiles * 64;
   TETRIS_HIP(hipMemsetAsync(w->zeros, 0, 64, stream));
   const int64_t total = tiles * 64;
+  int range[2] = {255, 0};
+  int* d_range = reinterpret_cast<int*>(w->zeros + 64);
+  TETRIS_HIP(hipMemcpyAsync(d_range, range, sizeof range, hipMemcpyHostToDevice, stream));
   hipLaunchKernelGGL(layout_kernel, dim3(blocks_for(total)), dim3(256), 0, stream, reinterpret_cast<const int4*>(d_codes), d_scales, w->n,
-                     w->k, w->gated ? 1 : 0, w->row_tiles, w->col_tiles, total, reinterpret_cast<int4*>(w->codes), w->scales);
+                     w->k, w->gated ? 1 : 0, w->row_tiles, w->col_tiles, total, reinterpret_cast<int4*>(w->codes), w->scales, d_range);
   TETRIS_HIP(hipGetLastError());
+  TETRIS_HIP(hipMemcpyAsync(range, d_range, sizeof range, hipMemcpyDeviceToHost, stream));
   TETRIS_HIP(hipStreamSynchronize(stream));
+  // f16 holds multiples of 2^-24 up to 65504: half a unit of the least scale, six of the largest
+  w->half = range[0] >= 127 - 23 && range[1] <= 127 + 13;
   return TETRIS_OK;
 }
 
