@@ -357,9 +357,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
   i32x4 w[2][WR][KS];
   unsigned s[2][WR];
   int w_step = 0, x_col = 0, x_part = 0, w_col = 0;
-  // past the last step that one again
-  auto fetch_rows = [&](int set) {  // straight to LDS; zeros past a row's end
-    const int at = min(x_col, a.col_tiles - KS) * 64 + column;
+  auto fetch_rows = [&](int set) {  // straight to LDS; zeros past a row's end, nothing past the last step
+    if (x_col >= a.col_tiles) return;
+    const int at = x_col * 64 + column;
 #pragma unroll
     for (int p = 0; p < PI; ++p) {
       const int64_t from_row = (x_part + p) * a.part + at;
@@ -370,7 +370,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
     x_part += PI;
     if (x_part == a.parts) x_part = 0, x_col += KS;
   };
-  auto fetch_weights = [&](int set) {
+  auto fetch_weights = [&](int set) {  // past the last step that one's again
     const int c0 = min(w_col, a.col_tiles - KS);
 #pragma unroll
     for (int r = 0; r < WR; ++r) {
@@ -387,6 +387,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
   constexpr int kWeightLoads = WR * (KS + 1);
 
   const int steps = a.col_tiles / KS * (a.parts / PI);
+  if (wm * WT * 32 >= count) {  // none of the wave's rows is there: it only helps to load
+    fetch_rows(0);
+    barrier_but<0>();
+    fetch_rows(1);
+    for (int step = 0; step < steps; ++step) {
+      barrier_but<0>();
+      fetch_rows(step & 1);
+    }
+    return;
+  }
   const int row_in = wm * WT * 32 + (lane & 31), turn = turn_of<KS>(lane & 31), half = lane >> 5;
   constexpr int kRounds = 4 * KS * PI, kProducts = WT * WR, kPairs = 4 * WR;
   i32x4 xs[2][WT], ws[2][WR];
@@ -486,13 +496,12 @@ __global__ __launch_bounds__(64 * WM * WN) void rounded_kernel(Product a) {
   i32x4 w[2][WR][2], xs[2][WT];
   int w_scale[2][WR], x_scale[2][WT];
   int row_step = 0, weight_step = 0;
-  // past the last step that one again
-  auto fetch_rows = [&](int set) {
+  auto fetch_rows = [&](int set) {  // past the last step that one again, into a buffer that nobody reads (a branch here costs registers)
     const int64_t at = (int64_t)min(row_step++, steps - 1) * 128;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) to_lds(from[i] + at, (set ? lds1 : lds0) + i * kThreads + wave * 64);
   };
-  auto fetch_weights = [&](int set) {
+  auto fetch_weights = [&](int set) {  // past the last step that one's again
     const int64_t at = (int64_t)min(weight_step++, steps - 1) * 64;
 #pragma unroll
     for (int r = 0; r < WR; ++r) {
@@ -544,6 +553,7 @@ __global__ __launch_bounds__(64 * WM * WN) void rounded_kernel(Product a) {
   }
   if (steps & 1) multiply(0);
   put_tile<WT, OUT, false>(a, acc, wm * WT * 32, first, count, (block * WN + wn) * WR, stage[wave]);
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): nothing may be on its way to LDS when the workgroup gives it back
 }
 
 // ---- few rows: weights streamed once -----------------------------------------------------------------------------------
