@@ -16,6 +16,8 @@
 namespace tetris {
 
 constexpr int kMxPad = 128;  // columns of a laid-out matrix and of staged rows are padded to this
+constexpr int kMxSide = 1 << 21;           // most rows and columns of a matrix, and most elements from one row to the next of rows read as they lie
+constexpr int64_t kMxReach = 0x7fff0000;   // bytes that a kernel's 32-bit offsets reach
 
 template <int TYPE>
 struct Elem;
@@ -50,8 +52,7 @@ struct tetris_mx4 {
   bool half = false;                 // every weight is exact in f16
   int row_tiles = 0, col_tiles = 0;  // of one matrix
   uint8_t* codes = nullptr;
-  uint8_t* scales = nullptr;  // zeros behind them
-  uint8_t* zeros = nullptr;
+  uint8_t* scales = nullptr;
   std::mutex mu;
   struct Space { void* ptr = nullptr; size_t bytes = 0; };
   std::map<hipStream_t, Space> space;

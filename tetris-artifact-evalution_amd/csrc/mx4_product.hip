@@ -25,7 +25,6 @@ enum { kOutF32 = TETRIS_F32, kOutF16 = TETRIS_F16, kOutBF16 = TETRIS_BF16, kOutP
 
 struct Product {
   const uint8_t* x_scales;  // of rows in MX4
-  const void* zeros;     // sixteen bytes of them
   const void* x;         // rows of ldx elements that start on 16 bytes; elements k .. k8 - 1 of a row are zero
   int64_t ldx, part;     // part: elements between the parts' arrays
   int parts, k8, rows;   // rows of all groups together
@@ -294,10 +293,20 @@ __device__ inline bool place_tile(const Product& a, int row_tiles_each, int* blo
   return true;
 }
 
-// Sixteen bytes a lane from memory to LDS, to `to` (the same for the whole wave) + lane.
-__device__ inline void to_lds(const void* from, i32x4* to) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+// Memory as the buffer loads see it: a base and offsets below 2^31 bytes; at kNowhere they read zeros.  (Loads by pointer that write LDS
+// make the compiler wait for every LDS read under way, these do not; and their addresses cost no vector instructions.)
+constexpr int kNowhere = 0x7fffffff;
+__device__ inline __amdgpu_buffer_rsrc_t buffer(const void* base) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, kNowhere, 0x00020000);
 }
+// Sixteen bytes a lane to LDS, to `to` (the same for the whole wave) + lane.
+__device__ inline void to_lds(__amdgpu_buffer_rsrc_t from, int at, int offset, i32x4* to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)to, 16, at, offset, 0, 0);
+}
+
+// Nothing may be on its way to LDS when a workgroup gives it back.
+__device__ inline void loads_have_ended() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
+
 // A barrier behind which the LDS of the whole workgroup may be read and written over: this wave's reads of it have ended, and all its loads
 // have arrived but the N issued last.  (__syncthreads would wait for those as well.)
 template <int N>
@@ -318,11 +327,13 @@ __device__ inline void barrier_but() {
 template <int KS>
 __device__ inline int turn_of(int row) { return KS == 1 ? (row >> 1) & 7 : row & 15; }
 
-template <int WT, int WR, int WM, int WN, int KS, int PI, bool HALF, int OUT, bool GATED>
+template <int WT, int WR, int WM, int WN, int KS, int PI, int D, bool HALF, int OUT, bool GATED>
 __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
   constexpr int kRows = 32 * WT * WM, kThreads = 64 * WM * WN, kPieces = 8 * KS, kLoads = kRows * kPieces / kThreads;
   static_assert(kThreads / kPieces % 16 == 0, "a thread's pieces lie in the same columns");
-  __shared__ i32x4 lds0[PI * kRows * kPieces], lds1[PI * kRows * kPieces], stage[WM * WN][256];
+  constexpr int kBuffer = PI * kRows * kPieces;
+  __shared__ i32x4 lds0[kBuffer], lds1[kBuffer], lds2[kBuffer], lds3[D > 3 ? kBuffer : 1], stage[WM * WN][256];
+  auto buffer_of = [&](int i) -> i32x4* { return i == 0 ? lds0 : i == 1 ? lds1 : i == 2 ? lds2 : lds3; };  // (i is a constant where this is used)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, wn = wave / WM;
   int block, tile;
@@ -331,20 +342,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
   if (!find_tile(a, tile, kRows, &expert, &first, &count)) return;
 
   const int column = ((threadIdx.x % kPieces) ^ turn_of<KS>(threadIdx.x / kPieces)) * 8;
-  const __bf16* from[kLoads];
+  const __amdgpu_buffer_rsrc_t rows = buffer(static_cast<const __bf16*>(a.x) + (a.from_div ? 0 : first * a.ldx));
+  int from[kLoads];  // bytes
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
-    const int p = first + min((int)(i * kThreads + threadIdx.x) / kPieces, count - 1);
-    const int64_t row = a.from_div ? a.order[p] / a.from_div : p;
-    from[i] = static_cast<const __bf16*>(a.x) + row * a.ldx;
+    const int p = min((int)(i * kThreads + threadIdx.x) / kPieces, count - 1);
+    from[i] = (a.from_div ? a.order[first + p] / a.from_div : p) * (int)a.ldx * 2 + column * 2;
   }
-  const i32x4* codes[WR];
-  const uint8_t* scales[WR];
+  __amdgpu_buffer_rsrc_t codes[WR], scales[WR];
 #pragma unroll
   for (int r = 0; r < WR; ++r) {
     const int64_t t = (int64_t)expert * a.row_tiles + min((block * WN + wn) * WR + r, a.row_tiles - 1);
-    codes[r] = a.codes + t * a.col_tiles * 64 + lane;
-    scales[r] = a.scales + t * a.col_tiles * 64 + lane * 2;
+    codes[r] = buffer(a.codes + t * a.col_tiles * 64);
+    scales[r] = buffer(a.scales + t * a.col_tiles * 64);
   }
 
   f32x16 acc[WT][WR];
@@ -353,20 +363,17 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
 #pragma unroll
     for (int r = 0; r < WR; ++r) acc[t][r] = f32x16{};
 
-  // Steps alternate between two LDS buffers and two sets of registers for weights, so that nothing is copied.
-  i32x4 w[2][WR][KS];
-  unsigned s[2][WR];
+  // Steps go round D LDS buffers and D sets of registers for weights, so that nothing is copied.
+  i32x4 w[D][WR][KS];
+  unsigned s[D][WR];
   int w_step = 0, x_col = 0, x_part = 0, w_col = 0;
-  auto fetch_rows = [&](int set) {  // straight to LDS; zeros past a row's end, nothing past the last step
-    if (x_col >= a.col_tiles) return;
-    const int at = x_col * 64 + column;
+  auto fetch_rows = [&](int set) {  // straight to LDS; zeros past a row's end, and past the last step, where nobody reads them (the barriers count them)
+    const bool in = x_col * 64 + column < a.k8;
 #pragma unroll
-    for (int p = 0; p < PI; ++p) {
-      const int64_t from_row = (x_part + p) * a.part + at;
+    for (int p = 0; p < PI; ++p)
 #pragma unroll
       for (int i = 0; i < kLoads; ++i)
-        to_lds(at < a.k8 ? from[i] + from_row : static_cast<const __bf16*>(a.zeros), (set ? lds1 : lds0) + (p * kLoads + i) * kThreads + wave * 64);
-    }
+        to_lds(rows, in ? from[i] : kNowhere, (x_part + p) * (int)a.part * 2 + x_col * 128, buffer_of(set) + (p * kLoads + i) * kThreads + wave * 64);
     x_part += PI;
     if (x_part == a.parts) x_part = 0, x_col += KS;
   };
@@ -375,26 +382,31 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
 #pragma unroll
     for (int r = 0; r < WR; ++r) {
 #pragma unroll
-      for (int c = 0; c < KS; ++c) w[set][r][c] = codes[r][(int64_t)(c0 + c) * 64];
+      for (int c = 0; c < KS; ++c) w[set][r][c] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(codes[r], lane * 16, (c0 + c) * 1024, 0));
       if constexpr (KS == 1)
-        s[set][r] = scales[r][(int64_t)(c0 >> 1) * 128 + (c0 & 1)];
+        s[set][r] = __builtin_amdgcn_raw_buffer_load_b8(scales[r], lane * 2, (c0 >> 1) * 128 + (c0 & 1), 0);
       else
-        s[set][r] = *reinterpret_cast<const unsigned short*>(scales[r] + (int64_t)c0 * 64);
+        s[set][r] = __builtin_amdgcn_raw_buffer_load_b16(scales[r], lane * 2, c0 * 64, 0);
     }
     w_step += PI;
     if (w_step == a.parts) w_step = 0, w_col += KS;
   };
-  constexpr int kWeightLoads = WR * (KS + 1);
+  constexpr int kWeightLoads = WR * (KS + 1), kRowLoads = PI * kLoads;
 
   const int steps = a.col_tiles / KS * (a.parts / PI);
   if (wm * WT * 32 >= count) {  // none of the wave's rows is there: it only helps to load
-    fetch_rows(0);
-    barrier_but<0>();
-    fetch_rows(1);
-    for (int step = 0; step < steps; ++step) {
-      barrier_but<0>();
-      fetch_rows(step & 1);
+#pragma unroll
+    for (int i = 0; i < D; ++i) fetch_rows(i);
+    barrier_but<(D - 1) * kRowLoads>();
+    for (int step = 0; step < steps; step += D) {
+#pragma unroll
+      for (int i = 0; i < D; ++i) {
+        if (step + i >= steps) break;
+        barrier_but<(D - 2) * kRowLoads>();
+        fetch_rows(i);
+      }
     }
+    loads_have_ended();
     return;
   }
   const int row_in = wm * WT * 32 + (lane & 31), turn = turn_of<KS>(lane & 31), half = lane >> 5;
@@ -402,7 +414,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
   i32x4 xs[2][WT], ws[2][WR];
   auto read = [&](int buffer, int round) {  // the rows' share in a round of a step's products: PI parts of the same columns after another
     const int j = round / PI, p = round % PI;
-    const i32x4* in = (buffer ? lds1 : lds0) + (p * kRows + row_in) * kPieces + (((j >> 2) * 8 + half * 4 + (j & 3)) ^ turn);
+    const i32x4* in = buffer_of(buffer) + (p * kRows + row_in) * kPieces + (((j >> 2) * 8 + half * 4 + (j & 3)) ^ turn);
 #pragma unroll
     for (int t = 0; t < WT; ++t) xs[round & 1][t] = in[t * 32 * kPieces];
   };
@@ -410,21 +422,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
     const float scale = __uint_as_float((s[set][i >> 2] >> (8 * (j >> 2))) << 23);
     ws[j & 1][i >> 2][i & 3] = pair_of<HALF>(w[set][i >> 2][j >> 2][j & 3], scale, i & 3);
   };
-  // The weights' pairs of the next round are made between the products of this one: a conversion takes the vector unit for 16 cycles, a
-  // product the matrix unit for 32.  A step's last round runs behind the barrier, while the next step's first reads are under
-  // way.  All reads of a buffer have ended when its step's barrier is passed: the rows of the step after the next are asked for there,
-  // and have a step to arrive.
+  // The weights' pairs of the next round are made between the products of this one.  A step's last round runs behind the barrier, while the
+  // next step's first reads are under way.  All reads of a buffer have ended when its step's barrier is passed: the rows of D steps
+  // on are asked for there, and with the weights of that step have D - 1 steps to arrive.  (One step is not enough: memory takes
+  // 0.8 us, a step of 32 rows 0.25.)  Loads arrive in the order of their issue, so the barrier lets those of the last steps be.
   auto multiply = [&](int set) {
+    const int next = set + 1 == D ? 0 : set + 1;
 #pragma unroll
     for (int round = 0; round < kRounds; ++round) {
       const bool last = round + 1 == kRounds;
       const int j = round / PI;
       if (last) {
         fetch_weights(set);
-        barrier_but<kWeightLoads>();  // the rows of the next step are there: only weights were asked for after them
+        barrier_but<(D - 2) * kRowLoads + (D - 1) * kWeightLoads>();  // the rows of the next step are there
         fetch_rows(set);
       }
-      read(last ? set ^ 1 : set, last ? 0 : round + 1);
+      read(last ? next : set, last ? 0 : round + 1);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < kProducts; ++i) {
@@ -432,35 +445,41 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
         acc[t][r] = product32<HALF>(ws[j & 1][r], xs[round & 1][t], acc[t][r]);
         if (round % PI == PI - 1) {
 #pragma unroll
-          for (int c = i * kPairs / kProducts; c < (i + 1) * kPairs / kProducts; ++c) convert(last ? set ^ 1 : set, last ? 0 : j + 1, c);
+          for (int c = i * kPairs / kProducts; c < (i + 1) * kPairs / kProducts; ++c) convert(last ? next : set, last ? 0 : j + 1, c);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
   };
-  fetch_weights(0);
-  fetch_rows(0);
-  barrier_but<0>();
-  fetch_rows(1);
-  fetch_weights(1);
+#pragma unroll
+  for (int i = 0; i < D; ++i) {
+    fetch_weights(i);
+    fetch_rows(i);
+  }
+  barrier_but<(D - 1) * (kRowLoads + kWeightLoads)>();
   read(0, 0);
 #pragma unroll
   for (int c = 0; c < kPairs; ++c) convert(0, 0, c);
-  for (int step = 0; step + 1 < steps; step += 2) {
-    multiply(0);
-    multiply(1);
+  int step = 0;
+  for (; step + D <= steps; step += D) {
+#pragma unroll
+    for (int i = 0; i < D; ++i) multiply(i);
   }
-  if (steps & 1) multiply(0);
+#pragma unroll
+  for (int i = 0; i < D - 1; ++i)
+    if (step + i < steps) multiply(i);
   put_tile<WT, OUT, GATED>(a, acc, wm * WT * 32, first, count, (block * WN + wn) * WR, stage[wave]);
+  loads_have_ended();
 }
 
 // The same for rows that are in MX4 as well, in the weights' layout (csrc/mx4.h): products of 4-bit numbers with both blocks' scales
 // applied by the matrix cores, four times the rate of bf16.  Rows come in steps of 128 columns through LDS, as they lie; a wave's
 // reads of it are one contiguous kilobyte.
-template <int WT, int WR, int WM, int WN, int OUT>
+template <int WT, int WR, int WM, int WN, int D, int OUT>
 __global__ __launch_bounds__(64 * WM * WN) void rounded_kernel(Product a) {
   constexpr int kTiles = WT * WM, kThreads = 64 * WM * WN, kLoads = kTiles * 128 / kThreads;
-  __shared__ i32x4 lds0[kTiles * 128], lds1[kTiles * 128], stage[WM * WN][256];
+  __shared__ i32x4 lds0[kTiles * 128], lds1[kTiles * 128], lds2[D > 2 ? kTiles * 128 : 1], stage[WM * WN][256];
+  auto buffer_of = [&](int i) -> i32x4* { return i == 0 ? lds0 : i == 1 ? lds1 : lds2; };  // (i is a constant where this is used)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, wn = wave / WM;
   int block, tile;
@@ -468,23 +487,21 @@ __global__ __launch_bounds__(64 * WM * WN) void rounded_kernel(Product a) {
   const int first = tile * kTiles * 32, count = min(kTiles * 32, a.rows - first);
   const int last = (a.rows - 1) >> 5, tile0 = first >> 5;
 
-  const i32x4* from[kLoads];
+  const __amdgpu_buffer_rsrc_t rows = buffer(static_cast<const i32x4*>(a.x) + (int64_t)tile0 * a.col_tiles * 64);
+  int from[kLoads];  // bytes
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
     const int q = i * kThreads + threadIdx.x;
-    from[i] = static_cast<const i32x4*>(a.x) + (int64_t)min(tile0 + (q >> 7), last) * a.col_tiles * 64 + (q & 127);
+    from[i] = min(q >> 7, last - tile0) * a.col_tiles * 1024 + (q & 127) * 16;
   }
-  const unsigned short* x_scales[WT];
+  __amdgpu_buffer_rsrc_t codes[WR], scales[WR], x_scales[WT];
 #pragma unroll
-  for (int t = 0; t < WT; ++t)
-    x_scales[t] = reinterpret_cast<const unsigned short*>(a.x_scales) + (int64_t)min(tile0 + wm * WT + t, last) * a.col_tiles * 32 + lane;
-  const i32x4* codes[WR];
-  const unsigned short* scales[WR];
+  for (int t = 0; t < WT; ++t) x_scales[t] = buffer(a.x_scales + (int64_t)min(tile0 + wm * WT + t, last) * a.col_tiles * 64);
 #pragma unroll
   for (int r = 0; r < WR; ++r) {
     const int64_t t = min((block * WN + wn) * WR + r, a.row_tiles - 1);
-    codes[r] = a.codes + t * a.col_tiles * 64 + lane;
-    scales[r] = reinterpret_cast<const unsigned short*>(a.scales) + t * a.col_tiles * 32 + lane;
+    codes[r] = buffer(a.codes + t * a.col_tiles * 64);
+    scales[r] = buffer(a.scales + t * a.col_tiles * 64);
   }
   f32x16 acc[WT][WR];
 #pragma unroll
@@ -493,34 +510,35 @@ __global__ __launch_bounds__(64 * WM * WN) void rounded_kernel(Product a) {
     for (int r = 0; r < WR; ++r) acc[t][r] = f32x16{};
 
   const int steps = a.col_tiles >> 1;
-  i32x4 w[2][WR][2], xs[2][WT];
-  int w_scale[2][WR], x_scale[2][WT];
+  i32x4 w[D][WR][2], xs[2][WT];
+  int w_scale[D][WR], x_scale[D][WT];
   int row_step = 0, weight_step = 0;
-  auto fetch_rows = [&](int set) {  // past the last step that one again, into a buffer that nobody reads (a branch here costs registers)
-    const int64_t at = (int64_t)min(row_step++, steps - 1) * 128;
+  auto fetch_rows = [&](int set) {  // past the last step that one again, into a buffer that nobody reads
+    const int at = min(row_step++, steps - 1) * 2048;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) to_lds(from[i] + at, (set ? lds1 : lds0) + i * kThreads + wave * 64);
+    for (int i = 0; i < kLoads; ++i) to_lds(rows, from[i], at, buffer_of(set) + i * kThreads + wave * 64);
   };
   auto fetch_weights = [&](int set) {  // past the last step that one's again
-    const int64_t at = (int64_t)min(weight_step++, steps - 1) * 64;
+    const int at = min(weight_step++, steps - 1) * 2048;
 #pragma unroll
     for (int r = 0; r < WR; ++r) {
-      w[set][r][0] = codes[r][at * 2];
-      w[set][r][1] = codes[r][at * 2 + 64];
-      w_scale[set][r] = scales[r][at];
+      w[set][r][0] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(codes[r], lane * 16, at, 0));
+      w[set][r][1] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(codes[r], lane * 16, at + 1024, 0));
+      w_scale[set][r] = __builtin_amdgcn_raw_buffer_load_b16(scales[r], lane * 2, at >> 4, 0);
     }
 #pragma unroll
-    for (int t = 0; t < WT; ++t) x_scale[set][t] = x_scales[t][at];
+    for (int t = 0; t < WT; ++t) x_scale[set][t] = __builtin_amdgcn_raw_buffer_load_b16(x_scales[t], lane * 2, at >> 4, 0);
   };
   constexpr int kWeightLoads = WR * 3 + WT;
   auto wide = [](i32x4 v) { return i32x8{v.x, v.y, v.z, v.w, 0, 0, 0, 0}; };
   auto read = [&](int buffer, int j) {
-    const i32x4* in = (buffer ? lds1 : lds0) + wm * WT * 128 + lane + j * 64;
+    const i32x4* in = buffer_of(buffer) + wm * WT * 128 + lane + j * 64;
 #pragma unroll
     for (int t = 0; t < WT; ++t) xs[j][t] = in[t * 128];
   };
   // as in tile_kernel, with two rounds of products a step
   auto multiply = [&](int set) {
+    const int next = set + 1 == D ? 0 : set + 1;
     read(set, 1);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -529,9 +547,9 @@ __global__ __launch_bounds__(64 * WM * WN) void rounded_kernel(Product a) {
       for (int r = 0; r < WR; ++r)
         acc[t][r] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(w[set][r][0]), wide(xs[0][t]), acc[t][r], 4, 4, 0, w_scale[set][r], 0, x_scale[set][t]);
     __builtin_amdgcn_sched_barrier(0);
-    barrier_but<kWeightLoads>();
+    barrier_but<(D - 2) * kLoads + (D - 1) * kWeightLoads>();
     fetch_rows(set);
-    read(set ^ 1, 0);
+    read(next, 0);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int t = 0; t < WT; ++t)
@@ -541,19 +559,23 @@ __global__ __launch_bounds__(64 * WM * WN) void rounded_kernel(Product a) {
     __builtin_amdgcn_sched_barrier(0);
     fetch_weights(set);
   };
-  fetch_rows(0);
-  fetch_weights(0);
-  barrier_but<0>();
-  fetch_rows(1);
-  fetch_weights(1);
-  read(0, 0);
-  for (int step = 0; step + 1 < steps; step += 2) {
-    multiply(0);
-    multiply(1);
+#pragma unroll
+  for (int i = 0; i < D; ++i) {
+    fetch_rows(i);
+    fetch_weights(i);
   }
-  if (steps & 1) multiply(0);
+  barrier_but<(D - 1) * kLoads + D * kWeightLoads>();
+  read(0, 0);
+  int step = 0;
+  for (; step + D <= steps; step += D) {
+#pragma unroll
+    for (int i = 0; i < D; ++i) multiply(i);
+  }
+#pragma unroll
+  for (int i = 0; i < D - 1; ++i)
+    if (step + i < steps) multiply(i);
   put_tile<WT, OUT, false>(a, acc, wm * WT * 32, first, count, (block * WN + wn) * WR, stage[wave]);
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): nothing may be on its way to LDS when the workgroup gives it back
+  loads_have_ended();
 }
 
 // ---- few rows: weights streamed once -----------------------------------------------------------------------------------
@@ -863,23 +885,23 @@ int stream_waves(int chunks, int64_t workgroups) {
   return waves;
 }
 
-template <int WT, int WR, int WM, int WN, int KS, int PI, bool HALF, int OUT, bool GATED>
+template <int WT, int WR, int WM, int WN, int KS, int PI, int D, bool HALF, int OUT, bool GATED>
 int launch_tile(Product& a, hipStream_t stream) {
   const int size = 32 * WT * WM, row_blocks = ceil_div(a.row_tiles, WR * WN);
   a.max_tiles = a.offsets ? std::min(a.rows, a.rows / size + std::min(a.experts, a.rows)) : ceil_div(a.rows, size);
   const int64_t blocks = round_up((int64_t)row_blocks * a.max_tiles, 256);
   if (blocks > 0x7fffffff / 2) return fail(TETRIS_EINVAL, "%d rows by %d features are too many for one launch", a.rows, a.n);
-  hipLaunchKernelGGL((tile_kernel<WT, WR, WM, WN, KS, PI, HALF, OUT, GATED>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream, a);
+  hipLaunchKernelGGL((tile_kernel<WT, WR, WM, WN, KS, PI, D, HALF, OUT, GATED>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream, a);
   TETRIS_HIP(hipGetLastError());
   return TETRIS_OK;
 }
 
-template <int WT, int WR, int WM, int WN, int OUT>
+template <int WT, int WR, int WM, int WN, int D, int OUT>
 int launch_rounded(Product& a, hipStream_t stream) {
   a.max_tiles = ceil_div(a.rows, 32 * WT * WM);
   const int64_t blocks = round_up((int64_t)ceil_div(a.row_tiles, WR * WN) * a.max_tiles, 256);
   if (blocks > 0x7fffffff / 2) return fail(TETRIS_EINVAL, "%d rows by %d features are too many for one launch", a.rows, a.n);
-  hipLaunchKernelGGL((rounded_kernel<WT, WR, WM, WN, OUT>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream, a);
+  hipLaunchKernelGGL((rounded_kernel<WT, WR, WM, WN, D, OUT>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream, a);
   TETRIS_HIP(hipGetLastError());
   return TETRIS_OK;
 }
@@ -916,16 +938,15 @@ int launch_down(Product& a, const float* weight, int top, hipStream_t stream) {
 // P: the rows' parts.  HALF: rows and weights in f16.
 template <int OUT, bool GATED, int P, bool HALF = false>
 int tile_rows(Product& a, int rows_a_group, hipStream_t stream) {
-  if (rows_a_group <= 40) return launch_tile<1, 2, 1, 4, 2, P, HALF, OUT, GATED>(a, stream);
-  if (rows_a_group <= 80) return launch_tile<2, 2, 1, 4, P == 3 ? 1 : 2, P, HALF, OUT, GATED>(a, stream);
-  if (rows_a_group <= 300) return launch_tile<4, 2, 1, 4, 1, 1, HALF, OUT, GATED>(a, stream);
-  return launch_tile<4, 2, 2, 4, 1, 1, HALF, OUT, GATED>(a, stream);
+  if (rows_a_group <= 40) return launch_tile<1, 2, 1, 4, P == 3 ? 1 : 2, P, 4, HALF, OUT, GATED>(a, stream);
+  if (rows_a_group <= 80) return launch_tile<2, 2, 1, 4, P == 2 ? 1 : 2, P == 2 ? 2 : 1, P == 1 ? 4 : 3, HALF, OUT, GATED>(a, stream);
+  if (rows_a_group <= 300) return launch_tile<4, 2, 1, 4, 1, 1, 3, HALF, OUT, GATED>(a, stream);
+  return launch_tile<4, 2, 2, 4, 1, 1, 3, HALF, OUT, GATED>(a, stream);
 }
 
 void set_weights(Product* a, const tetris_mx4* w) {
   a->codes = reinterpret_cast<const i32x4*>(w->codes);
   a->scales = w->scales;
-  a->zeros = w->zeros;
   a->row_tiles = w->row_tiles;
   a->col_tiles = w->col_tiles;
   a->n = w->n;
@@ -933,7 +954,7 @@ void set_weights(Product* a, const tetris_mx4* w) {
 
 // Whether the kernels can read rows as they lie.
 bool lies_well(const void* x, int64_t ld, int k, int type) {
-  return (reinterpret_cast<size_t>(x) & 15) == 0 && (ld * elem_size(type)) % 16 == 0 && k % 8 == 0;
+  return (reinterpret_cast<size_t>(x) & 15) == 0 && (ld * elem_size(type)) % 16 == 0 && k % 8 == 0 && ld <= kMxSide;
 }
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
@@ -1030,9 +1051,9 @@ int launch_product(Product& a, Role role, int as, int type, int rows_a_group, bo
     return stream_rows<TETRIS_BF16, kOutBF16, false>(a, s);
   }
   if (a.x_scales) {
-    if (type == TETRIS_F32) return launch_rounded<4, 2, 2, 4, kOutF32>(a, s);
-    if (type == TETRIS_F16) return launch_rounded<4, 2, 2, 4, kOutF16>(a, s);
-    return launch_rounded<4, 2, 2, 4, kOutBF16>(a, s);
+    if (type == TETRIS_F32) return launch_rounded<4, 2, 2, 4, 2, kOutF32>(a, s);
+    if (type == TETRIS_F16) return launch_rounded<4, 2, 2, 4, 2, kOutF16>(a, s);
+    return launch_rounded<4, 2, 2, 4, 2, kOutBF16>(a, s);
   }
   if (type == TETRIS_F32) return role == kUp ? tile_rows<kOutParts3, true, 3>(a, rows_a_group, s) : tile_rows<kOutF32, false, 3>(a, rows_a_group, s);
   if (as == TETRIS_F16)
@@ -1060,12 +1081,40 @@ int check_rows(const void* x, int type, int rows, int64_t ld, int k, const char*
 
 using namespace tetris;
 
+namespace {
+
+// rows of a linear product that a launch takes: those made ready in parts lie within a kernel's reach
+int rows_at_once(const tetris_mx4* w, int m, int type, bool rounded) {
+  if (rounded || streams(m) || parts_of(type) == 1 || in_half(type, w)) return m;
+  return (int)std::min<int64_t>(m, kMxReach / (2 * parts_of(type) * round_up(w->k, kMxPad)));
+}
+
+int linear_rows(tetris_mx4* w, const void* d_x, int type, int m, int64_t ldx, void* d_y, int64_t ldy, const float* d_bias, bool rounded, hipStream_t s) {
+  const bool stream_it = streams(m), half = in_half(type, w);
+  const bool as_it_lies = !rounded && lies_well(d_x, ldx, w->k, type) && (stream_it || half || type == TETRIS_BF16);
+  uint8_t* d = nullptr;
+  int rc;
+  if (!as_it_lies && (rc = workspace(w, s, staged_bytes(m, w->k, type, rounded, stream_it, half), &d))) return rc;
+  Product a{};
+  set_weights(&a, w);
+  int as;
+  if ((rc = ready_rows(&a, d_x, type, m, w->k, ldx, rounded, stream_it, half, d, &as, s))) return rc;
+  a.y = d_y;
+  a.ldy = ldy;
+  a.vec_out = ldy * elem_size(type) % 16 == 0 && (reinterpret_cast<size_t>(d_y) & 15) == 0;
+  a.bias = d_bias;
+  return launch_product(a, kLinear, as, type, m, stream_it, s);
+}
+
+}  // namespace
+
 extern "C" int tetris_mx4_prepare(tetris_mx4* w, int m, int type, int mx4_input, void* stream) {
   if (!w) return fail(TETRIS_EINVAL, "null argument");
   if (bad_type(type)) return fail(TETRIS_EINVAL, "type %d is not TETRIS_F32, TETRIS_F16 or TETRIS_BF16", type);
   if (m < 0) return fail(TETRIS_EINVAL, "%d rows", m);
   uint8_t* d;
-  return workspace(w, static_cast<hipStream_t>(stream), staged_bytes(m, w->k, type, mx4_input, streams(m), in_half(type, w)), &d);
+  const int rows = rows_at_once(w, m, type, mx4_input);
+  return workspace(w, static_cast<hipStream_t>(stream), staged_bytes(rows, w->k, type, mx4_input, streams(m), in_half(type, w)), &d);
 }
 
 extern "C" int tetris_mx4_linear(tetris_mx4* w, const void* d_x, int type, int m, int64_t ldx, void* d_y, int64_t ldy,
@@ -1079,21 +1128,13 @@ extern "C" int tetris_mx4_linear(tetris_mx4* w, const void* d_x, int type, int m
   if (!rc) rc = check_rows(d_y, type, m, ldy, w->n, "output");
   if (rc) return rc;
   if (reinterpret_cast<size_t>(d_bias) & 3) return fail(TETRIS_EINVAL, "bias not aligned to its elements");
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool stream_it = streams(m);
-  const bool half = in_half(type, w);
-  const bool as_it_lies = !mx4_input && lies_well(d_x, ldx, w->k, type) && (stream_it || half || type == TETRIS_BF16);
-  uint8_t* d = nullptr;
-  if (!as_it_lies && (rc = workspace(w, s, staged_bytes(m, w->k, type, mx4_input, stream_it, half), &d))) return rc;
-  Product a{};
-  set_weights(&a, w);
-  int as;
-  if ((rc = ready_rows(&a, d_x, type, m, w->k, ldx, mx4_input, stream_it, half, d, &as, s))) return rc;
-  a.y = d_y;
-  a.ldy = ldy;
-  a.vec_out = ldy * elem_size(type) % 16 == 0 && (reinterpret_cast<size_t>(d_y) & 15) == 0;
-  a.bias = d_bias;
-  return launch_product(a, kLinear, as, type, m, stream_it, s);
+  const int each = rows_at_once(w, m, type, mx4_input);
+  for (int64_t from = 0; from < m; from += each) {
+    rc = linear_rows(w, static_cast<const char*>(d_x) + from * ldx * elem_size(type), type, (int)std::min<int64_t>(each, m - from), ldx,
+                     static_cast<char*>(d_y) + from * ldy * elem_size(type), ldy, d_bias, mx4_input != 0, static_cast<hipStream_t>(stream));
+    if (rc) return rc;
+  }
+  return TETRIS_OK;
 }
 
 namespace {
@@ -1130,25 +1171,35 @@ int rows_a_group(const tetris_mx4* up, int tokens, int top) { return (int)(((int
 
 }  // namespace
 
+namespace {
+
+// tokens that one pass takes: their rows, and those between the products, lie within a kernel's reach
+int tokens_at_once(const tetris_mx4* up, const tetris_mx4* down, int tokens, int top, int type, int64_t ldx) {
+  const bool half = in_half(type, up) && in_half(type, down);
+  const int64_t bytes = half ? 2 : 2 * parts_of(type);
+  const int64_t most = std::max({std::min<int64_t>(ldx, kMxSide) * elem_size(type), round_up(up->k, kMxPad) * bytes, top * round_up(down->k, kMxPad) * bytes});
+  return (int)std::min<int64_t>(tokens, std::max<int64_t>(1, kMxReach / most));
+}
+
+bool streams_slots(const tetris_mx4* up, int tokens, int top) { return (int64_t)tokens * top <= 64 || streams(rows_a_group(up, tokens, top)); }
+
+}  // namespace
+
 extern "C" int tetris_experts_prepare(tetris_mx4* up, tetris_mx4* down, int tokens, int top, int type, void* stream) {
   const int rc = experts_check(up, down, tokens, top, type);
   if (rc || tokens == 0) return rc;
   uint8_t* d;
-  return workspace(up, static_cast<hipStream_t>(stream), expert_space(up, down, tokens, top, type, tokens * top <= 64 || streams(rows_a_group(up, tokens, top))).all, &d);
+  const int once = tokens_at_once(up, down, tokens, top, type, up->k);
+  return workspace(up, static_cast<hipStream_t>(stream), expert_space(up, down, once, top, type, streams_slots(up, once, top)).all, &d);
 }
 
-extern "C" int tetris_experts(tetris_mx4* up, tetris_mx4* down, const void* d_x, int type, int tokens, int64_t ldx, int top,
-                              const int32_t* d_index, const float* d_weight, void* d_y, int64_t ldy, void* stream) {
-  int rc = experts_check(up, down, tokens, top, type);
-  if (rc) return rc;
-  if (tokens == 0) return TETRIS_OK;
-  if ((rc = check_rows(d_x, type, tokens, ldx, up->k, "input"))) return rc;
-  if ((rc = check_rows(d_y, type, tokens, ldy, down->n, "output"))) return rc;
-  if (!d_index || !d_weight) return fail(TETRIS_EINVAL, "null argument");
-  if ((reinterpret_cast<size_t>(d_index) | reinterpret_cast<size_t>(d_weight)) & 3) return fail(TETRIS_EINVAL, "index or weights not aligned to their elements");
-  hipStream_t s = static_cast<hipStream_t>(stream);
+namespace {
+
+int expert_tokens(tetris_mx4* up, tetris_mx4* down, const void* d_x, int type, int tokens, int64_t ldx, int top, const int32_t* d_index,
+                  const float* d_weight, void* d_y, int64_t ldy, hipStream_t s) {
+  int rc;
   const int slots = tokens * top, each = rows_a_group(up, tokens, top);
-  const bool stream_it = slots <= 64 || streams(each);
+  const bool stream_it = streams_slots(up, tokens, top);
   const bool half = in_half(type, up) && in_half(type, down);
   const ExpertSpace e = expert_space(up, down, tokens, top, type, stream_it);
   uint8_t* d;
@@ -1218,5 +1269,25 @@ extern "C" int tetris_experts(tetris_mx4* up, tetris_mx4* down, const void* d_x,
     hipLaunchKernelGGL(combine_kernel<TETRIS_BF16>, grid, dim3(256), 0, s, rows, b.ldy, d_index, d_weight, tokens, top, up->experts, down->n,
                        static_cast<__bf16*>(d_y), ldy, vec);
   TETRIS_HIP(hipGetLastError());
+  return TETRIS_OK;
+}
+
+}  // namespace
+
+extern "C" int tetris_experts(tetris_mx4* up, tetris_mx4* down, const void* d_x, int type, int tokens, int64_t ldx, int top,
+                              const int32_t* d_index, const float* d_weight, void* d_y, int64_t ldy, void* stream) {
+  int rc = experts_check(up, down, tokens, top, type);
+  if (rc) return rc;
+  if (tokens == 0) return TETRIS_OK;
+  if ((rc = check_rows(d_x, type, tokens, ldx, up->k, "input"))) return rc;
+  if ((rc = check_rows(d_y, type, tokens, ldy, down->n, "output"))) return rc;
+  if (!d_index || !d_weight) return fail(TETRIS_EINVAL, "null argument");
+  if ((reinterpret_cast<size_t>(d_index) | reinterpret_cast<size_t>(d_weight)) & 3) return fail(TETRIS_EINVAL, "index or weights not aligned to their elements");
+  const int each = tokens_at_once(up, down, tokens, top, type, ldx);
+  for (int64_t from = 0; from < tokens; from += each) {
+    rc = expert_tokens(up, down, static_cast<const char*>(d_x) + from * ldx * elem_size(type), type, (int)std::min<int64_t>(each, tokens - from), ldx, top,
+                       d_index + from * top, d_weight + from * top, static_cast<char*>(d_y) + from * ldy * elem_size(type), ldy, static_cast<hipStream_t>(stream));
+    if (rc) return rc;
+  }
   return TETRIS_OK;
 }

@@ -374,8 +374,8 @@ namespace {
 int create_check(int experts, int n, int k, int gated, tetris_mx4** out) {
   if (!out) return fail(TETRIS_EINVAL, "null argument");
   *out = nullptr;
-  if (experts <= 0 || experts > 1024 || n <= 0 || n > (1 << 24) || k <= 0 || k > (1 << 24))
-    return fail(TETRIS_EINVAL, "bad weights: %d matrices of %d x %d (at most 1024, sides up to 2^24)", experts, n, k);
+  if (experts <= 0 || experts > 1024 || n <= 0 || n > kMxSide || k <= 0 || k > kMxSide)
+    return fail(TETRIS_EINVAL, "bad weights: %d matrices of %d x %d (at most 1024, sides up to 2^21)", experts, n, k);
   if (gated && (n & 1)) return fail(TETRIS_EINVAL, "a gated matrix has an even number of rows, got %d", n);
   return TETRIS_OK;
 }
@@ -385,12 +385,10 @@ int lay_out(tetris_mx4* w, const uint8_t* d_codes, const uint8_t* d_scales, hipS
   w->col_tiles = (int)(round_up(w->k, kMxPad) / 64);
   const int64_t tiles = (int64_t)w->experts * w->row_tiles * w->col_tiles;
   TETRIS_HIP(hipMalloc(&w->codes, (size_t)tiles * 1024));
-  TETRIS_HIP(hipMalloc(&w->scales, (size_t)tiles * 64 + 128));
-  w->zeros = w->scales + tiles * 64;
-  TETRIS_HIP(hipMemsetAsync(w->zeros, 0, 64, stream));
+  TETRIS_HIP(hipMalloc(&w->scales, (size_t)tiles * 64 + sizeof(int[2])));
   const int64_t total = tiles * 64;
   int range[2] = {255, 0};
-  int* d_range = reinterpret_cast<int*>(w->zeros + 64);
+  int* d_range = reinterpret_cast<int*>(w->scales + tiles * 64);
   TETRIS_HIP(hipMemcpyAsync(d_range, range, sizeof range, hipMemcpyHostToDevice, stream));
   hipLaunchKernelGGL(layout_kernel, dim3(blocks_for(total)), dim3(256), 0, stream, reinterpret_cast<const int4*>(d_codes), d_scales, w->n,
                      w->k, w->gated ? 1 : 0, w->row_tiles, w->col_tiles, total, reinterpret_cast<int4*>(w->codes), w->scales, d_range);
