@@ -876,8 +876,6 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ 
 
 // ---- launches ------------------------------------------------------------------------------------------------------------
 
-constexpr int kStreamRows = 16;  // up to so many rows of a matrix are streamed
-
 // Waves that share a row of `chunks` stretches of 128 columns.
 int stream_waves(int chunks, int64_t workgroups) {
   int waves = workgroups <= 512 ? 16 : 4;
@@ -935,13 +933,33 @@ int launch_down(Product& a, const float* weight, int top, hipStream_t stream) {
   return TETRIS_OK;
 }
 
+// Tiles of `size` rows that the groups make: one half more each than their mean number of rows fills.
+double tiles_of(const Product& a, int size) {
+  if (!a.offsets && !a.index) return ceil_div(a.rows, size);
+  const double named = std::min(a.experts, a.rows), mean = a.rows / named;
+  return mean <= size / 2 ? named : named * (mean / size + 0.5);
+}
+// What a product takes in tiles of `size` rows, in units of what a workgroup of 32 rows takes; a workgroup has 256 features, and each of the 256 compute
+// units needs one at a time to be full.  Measured, 4096 columns of bf16: 18, 27 and 51 us a workgroup of 32, 64 and 128 rows.
+double tile_cost(const Product& a, int size) {
+  const double each = size == 32 ? 1.0 : size == 64 ? 1.55 : 2.9;
+  return each * std::max(1.0, tiles_of(a, size) * ceil_div(a.row_tiles, 8) / 256);
+}
+// The same for streaming, whose workgroups have up to 16 rows and 16 features (a gated product 32, for a third more): 4 us, and for each 256 of them 1.2 us
+// with one row to 3.8 with sixteen.
+double stream_cost(const Product& a, bool gated) {
+  const bool groups = a.offsets || a.index;
+  const double rows = std::min(16.0, groups ? (double)a.rows / std::min(a.experts, a.rows) : (double)a.rows);
+  return 0.2 + (0.06 + 0.0095 * rows) * (gated ? 0.65 : 1.0) * tiles_of(a, 16) * a.row_tiles * 2 / 256;
+}
+
 // P: the rows' parts.  HALF: rows and weights in f16.
 template <int OUT, bool GATED, int P, bool HALF = false>
-int tile_rows(Product& a, int rows_a_group, hipStream_t stream) {
-  if (rows_a_group <= 40) return launch_tile<1, 2, 1, 4, P == 3 ? 1 : 2, P, 4, HALF, OUT, GATED>(a, stream);
-  if (rows_a_group <= 80) return launch_tile<2, 2, 1, 4, P == 2 ? 1 : 2, P == 2 ? 2 : 1, P == 1 ? 4 : 3, HALF, OUT, GATED>(a, stream);
-  if (rows_a_group <= 300) return launch_tile<4, 2, 1, 4, 1, 1, 3, HALF, OUT, GATED>(a, stream);
-  return launch_tile<4, 2, 2, 4, 1, 1, 3, HALF, OUT, GATED>(a, stream);
+int tile_rows(Product& a, hipStream_t stream) {
+  const double small = tile_cost(a, 32), middle = tile_cost(a, 64), large = tile_cost(a, 128);
+  if (small <= middle && small <= large) return launch_tile<1, 2, 1, 4, P == 3 ? 1 : 2, P, 4, HALF, OUT, GATED>(a, stream);
+  if (middle < large) return launch_tile<2, 2, 1, 4, P == 2 ? 1 : 2, P == 2 ? 2 : 1, P == 1 ? 4 : 3, HALF, OUT, GATED>(a, stream);
+  return launch_tile<4, 2, 1, 4, 1, 1, 3, HALF, OUT, GATED>(a, stream);
 }
 
 void set_weights(Product* a, const tetris_mx4* w) {
@@ -985,7 +1003,26 @@ int workspace(tetris_mx4* w, hipStream_t stream, size_t need, uint8_t** out) {
   }
 }
 
-bool streams(int rows) { return rows <= kStreamRows; }
+// Whether a product's rows are streamed.  Decided by its sizes alone, so that a workspace can be made ahead.
+bool streams(const tetris_mx4* w, int rows) {
+  Product a{};
+  a.rows = rows;
+  a.row_tiles = w->row_tiles;
+  return rows <= 1024 && stream_cost(a, false) < tile_cost(a, 32);
+}
+// The experts': of the first product, for both; up to 64 slots always are.
+bool streams_slots(const tetris_mx4* up, int tokens, int top) {
+  const int64_t slots = (int64_t)tokens * top;
+  if (slots <= 64) return true;
+  if (slots > 1024) return false;
+  Product a{};
+  a.rows = (int)slots;
+  a.experts = up->experts;
+  a.row_tiles = up->row_tiles;
+  static const int some = 0;
+  a.offsets = &some;
+  return stream_cost(a, true) < tile_cost(a, 32);
+}
 
 // Whether rows of `type` are multiplied in f16: where the weights are exact in it.  Others of f16 are taken in two bf16 parts.
 bool in_half(int type, const tetris_mx4* w) { return type == TETRIS_F16 && w->half; }
@@ -1037,7 +1074,7 @@ int ready_rows(Product* a, const void* x, int type, int rows, int k, int64_t ld,
 enum Role { kLinear, kUp, kDown };
 
 // `as`: the type of the rows; `type`: that of the operator.
-int launch_product(Product& a, Role role, int as, int type, int rows_a_group, bool stream, hipStream_t s) {
+int launch_product(Product& a, Role role, int as, int type, bool stream, hipStream_t s) {
   if (stream) {
     if (as == TETRIS_F32)
       return role == kUp ? stream_rows<TETRIS_F32, kOutF32, true>(a, s) : stream_rows<TETRIS_F32, kOutF32, false>(a, s);
@@ -1055,18 +1092,18 @@ int launch_product(Product& a, Role role, int as, int type, int rows_a_group, bo
     if (type == TETRIS_F16) return launch_rounded<4, 2, 2, 4, 2, kOutF16>(a, s);
     return launch_rounded<4, 2, 2, 4, 2, kOutBF16>(a, s);
   }
-  if (type == TETRIS_F32) return role == kUp ? tile_rows<kOutParts3, true, 3>(a, rows_a_group, s) : tile_rows<kOutF32, false, 3>(a, rows_a_group, s);
+  if (type == TETRIS_F32) return role == kUp ? tile_rows<kOutParts3, true, 3>(a, s) : tile_rows<kOutF32, false, 3>(a, s);
   if (as == TETRIS_F16)
-    return role == kUp     ? tile_rows<kOutF16, true, 1, true>(a, rows_a_group, s)
-           : role == kDown ? tile_rows<kOutF32, false, 1, true>(a, rows_a_group, s)
-                           : tile_rows<kOutF16, false, 1, true>(a, rows_a_group, s);
+    return role == kUp     ? tile_rows<kOutF16, true, 1, true>(a, s)
+           : role == kDown ? tile_rows<kOutF32, false, 1, true>(a, s)
+                           : tile_rows<kOutF16, false, 1, true>(a, s);
   if (type == TETRIS_F16)
-    return role == kUp     ? tile_rows<kOutParts2, true, 2>(a, rows_a_group, s)
-           : role == kDown ? tile_rows<kOutF32, false, 2>(a, rows_a_group, s)
-                           : tile_rows<kOutF16, false, 2>(a, rows_a_group, s);
-  return role == kUp     ? tile_rows<kOutBF16, true, 1>(a, rows_a_group, s)
-         : role == kDown ? tile_rows<kOutF32, false, 1>(a, rows_a_group, s)
-                         : tile_rows<kOutBF16, false, 1>(a, rows_a_group, s);
+    return role == kUp     ? tile_rows<kOutParts2, true, 2>(a, s)
+           : role == kDown ? tile_rows<kOutF32, false, 2>(a, s)
+                           : tile_rows<kOutF16, false, 2>(a, s);
+  return role == kUp     ? tile_rows<kOutBF16, true, 1>(a, s)
+         : role == kDown ? tile_rows<kOutF32, false, 1>(a, s)
+                         : tile_rows<kOutBF16, false, 1>(a, s);
 }
 
 int check_rows(const void* x, int type, int rows, int64_t ld, int k, const char* what) {
@@ -1085,12 +1122,12 @@ namespace {
 
 // rows of a linear product that a launch takes: those made ready in parts lie within a kernel's reach
 int rows_at_once(const tetris_mx4* w, int m, int type, bool rounded) {
-  if (rounded || streams(m) || parts_of(type) == 1 || in_half(type, w)) return m;
+  if (rounded || streams(w, m) || parts_of(type) == 1 || in_half(type, w)) return m;
   return (int)std::min<int64_t>(m, kMxReach / (2 * parts_of(type) * round_up(w->k, kMxPad)));
 }
 
 int linear_rows(tetris_mx4* w, const void* d_x, int type, int m, int64_t ldx, void* d_y, int64_t ldy, const float* d_bias, bool rounded, hipStream_t s) {
-  const bool stream_it = streams(m), half = in_half(type, w);
+  const bool stream_it = streams(w, m), half = in_half(type, w);
   const bool as_it_lies = !rounded && lies_well(d_x, ldx, w->k, type) && (stream_it || half || type == TETRIS_BF16);
   uint8_t* d = nullptr;
   int rc;
@@ -1103,7 +1140,7 @@ int linear_rows(tetris_mx4* w, const void* d_x, int type, int m, int64_t ldx, vo
   a.ldy = ldy;
   a.vec_out = ldy * elem_size(type) % 16 == 0 && (reinterpret_cast<size_t>(d_y) & 15) == 0;
   a.bias = d_bias;
-  return launch_product(a, kLinear, as, type, m, stream_it, s);
+  return launch_product(a, kLinear, as, type, stream_it, s);
 }
 
 }  // namespace
@@ -1114,7 +1151,7 @@ extern "C" int tetris_mx4_prepare(tetris_mx4* w, int m, int type, int mx4_input,
   if (m < 0) return fail(TETRIS_EINVAL, "%d rows", m);
   uint8_t* d;
   const int rows = rows_at_once(w, m, type, mx4_input);
-  return workspace(w, static_cast<hipStream_t>(stream), staged_bytes(rows, w->k, type, mx4_input, streams(m), in_half(type, w)), &d);
+  return workspace(w, static_cast<hipStream_t>(stream), staged_bytes(rows, w->k, type, mx4_input, streams(w, m), in_half(type, w)), &d);
 }
 
 extern "C" int tetris_mx4_linear(tetris_mx4* w, const void* d_x, int type, int m, int64_t ldx, void* d_y, int64_t ldy,
@@ -1166,8 +1203,6 @@ int experts_check(const tetris_mx4* up, const tetris_mx4* down, int tokens, int 
   return TETRIS_OK;
 }
 
-// rows of a group, were all groups alike
-int rows_a_group(const tetris_mx4* up, int tokens, int top) { return (int)(((int64_t)tokens * top + up->experts - 1) / up->experts); }
 
 }  // namespace
 
@@ -1180,8 +1215,6 @@ int tokens_at_once(const tetris_mx4* up, const tetris_mx4* down, int tokens, int
   const int64_t most = std::max({std::min<int64_t>(ldx, kMxSide) * elem_size(type), round_up(up->k, kMxPad) * bytes, top * round_up(down->k, kMxPad) * bytes});
   return (int)std::min<int64_t>(tokens, std::max<int64_t>(1, kMxReach / most));
 }
-
-bool streams_slots(const tetris_mx4* up, int tokens, int top) { return (int64_t)tokens * top <= 64 || streams(rows_a_group(up, tokens, top)); }
 
 }  // namespace
 
@@ -1198,7 +1231,7 @@ namespace {
 int expert_tokens(tetris_mx4* up, tetris_mx4* down, const void* d_x, int type, int tokens, int64_t ldx, int top, const int32_t* d_index,
                   const float* d_weight, void* d_y, int64_t ldy, hipStream_t s) {
   int rc;
-  const int slots = tokens * top, each = rows_a_group(up, tokens, top);
+  const int slots = tokens * top;
   const bool stream_it = streams_slots(up, tokens, top);
   const bool half = in_half(type, up) && in_half(type, down);
   const ExpertSpace e = expert_space(up, down, tokens, top, type, stream_it);
@@ -1229,7 +1262,7 @@ int expert_tokens(tetris_mx4* up, tetris_mx4* down, const void* d_x, int type, i
   a.y = d + e.hidden;
   a.ldy = round_up(down->k, kMxPad);
   a.y_part = slots * a.ldy;
-  if ((rc = launch_product(a, kUp, as, type, each, stream_it, s))) return rc;
+  if ((rc = launch_product(a, kUp, as, type, stream_it, s))) return rc;
 
   Product b{};
   set_weights(&b, down);
@@ -1254,7 +1287,7 @@ int expert_tokens(tetris_mx4* up, tetris_mx4* down, const void* d_x, int type, i
   b.y = d + e.rows;
   b.ldy = round_up(down->n, 4);
   b.vec_out = 1;
-  if ((rc = launch_product(b, kDown, stream_it || half ? type : (int)TETRIS_BF16, type, each, stream_it, s))) return rc;
+  if ((rc = launch_product(b, kDown, stream_it || half ? type : (int)TETRIS_BF16, type, stream_it, s))) return rc;
 
   const int vec = ldy % 4 == 0 && (reinterpret_cast<size_t>(d_y) & (4 * elem_size(type) - 1)) == 0;
   const float* rows = reinterpret_cast<const float*>(d + e.rows);
