@@ -1,6 +1,7 @@
-// Routing of tokens to experts: scores, groups, choice and weights, and the gradient of the weights.  One wave a token; the
-// logits are read once and stay in registers, expert e with lane e / V, place e % V of the lane's V.  Bound by the instructions of
-// the choice -- `top` rounds of a maximum over the wave -- and, for few tokens, by the launch.
+// Routing of tokens to experts: scores, groups, choice and weights, and the gradient of the weights.  L lanes of a wave have a token (sixteen up
+// to 256 experts, else the whole wave); the logits are read once and stay in registers, expert e with lane e / V of them.  Bound by the instructions of the
+// choice -- `top` rounds of a maximum over a token's lanes -- and, for few tokens, by the launch: 16384 tokens of 256 experts, eight groups of which
+// four stay, eight chosen, 14.4 us; a wave a token, logits loaded one by one, 25.2 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -17,6 +18,8 @@ struct Route {
   int tokens, experts, top, score, groups, top_groups, group_by, renorm;
   float scale;
   const float* bias;
+  int whole; // rows and bias lie on 16 bytes, and every lane has V experts
+  int span;  // lanes that a group fills, of sixteen; 0: groups begin or end inside a lane's experts
 };
 
 // Numbers to integers of the same order; NaN as -inf.  Zero is below all of them.
@@ -31,26 +34,47 @@ template <int CTRL>
 __device__ inline unsigned dpp(unsigned v) {
   return (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
 }
-// the largest of the wave's values, in every lane
-__device__ inline unsigned wave_max(unsigned v) {
-  v = max(v, dpp<0x111>(v));  // row_shr 1, 2, 4, 8: lane 15 of a row of sixteen has the row's
-  v = max(v, dpp<0x112>(v));
-  v = max(v, dpp<0x114>(v));
-  v = max(v, dpp<0x118>(v));
-  v = max(v, dpp<0x142>(v));  // row_bcast 15, 31: lane 63 has the wave's
-  v = max(v, dpp<0x143>(v));
-  return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
-}
-__device__ inline float wave_sum(float v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+// f over the values of a token's L lanes, in all of them.  Sixteen lanes: rotations by 8, 4, 2 and 1 of a row.
+template <int L, typename F>
+__device__ inline unsigned lanes(unsigned v, F f) {
+  v = f(v, dpp<0x128>(v));
+  v = f(v, dpp<0x124>(v));
+  v = f(v, dpp<0x122>(v));
+  v = f(v, dpp<0x121>(v));
+  if constexpr (L == 64) {
+    v = f(v, (unsigned)__shfl_xor((int)v, 16));
+    v = f(v, (unsigned)__shfl_xor((int)v, 32));
+  }
   return v;
+}
+template <int L>
+__device__ inline unsigned lanes_max(unsigned v) { return lanes<L>(v, [](unsigned a, unsigned b) { return max(a, b); }); }
+template <int L>
+__device__ inline unsigned lanes_min(unsigned v) { return lanes<L>(v, [](unsigned a, unsigned b) { return min(a, b); }); }
+template <int L>
+__device__ inline float lanes_sum(float v) {
+  return __uint_as_float(lanes<L>(__float_as_uint(v), [](unsigned a, unsigned b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
+}
+
+// V numbers from p on, which lie on 16 bytes
+template <typename T, int V>
+__device__ inline void load_whole(const T* p, float (&x)[V]) {
+  constexpr int N = V * (int)sizeof(T) / 16;
+  int4 raw[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) raw[i] = reinterpret_cast<const int4*>(p)[i];
+#pragma unroll
+  for (int v = 0; v < V; ++v) x[v] = (float)reinterpret_cast<const T*>(raw)[v];
 }
 
 // the lane's V logits; those past the last expert -inf
 template <int TYPE, int V>
 __device__ inline void load_logits(const Route& a, int token, int lane, float (&x)[V]) {
-  const auto* row = static_cast<const typename Elem<TYPE>::type*>(a.logits) + token * a.ld;
+  using T = typename Elem<TYPE>::type;
+  const T* row = static_cast<const T*>(a.logits) + token * a.ld;
+  if constexpr (V * sizeof(T) >= 16) {
+    if (a.whole) return load_whole<T, V>(row + lane * V, x);
+  }
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int e = lane * V + v;
@@ -58,113 +82,179 @@ __device__ inline void load_logits(const Route& a, int token, int lane, float (&
   }
 }
 
+// What a token's scores need besides the logit: softmax's largest logit and the sum of the exponentials.
+struct Norm { float top, sum; };
+__device__ inline float exponential(float x, float top) {
+  return top == -__builtin_inff() && !(x != x) ? 0.f : x == top ? 1.f : expf(x - top);
+}
+__device__ inline float score_of(const Route& a, float x, Norm n) {
+  if (a.score == TETRIS_SCORE_SIGMOID) return 1.f / (1.f + expf(-x));
+  return n.sum == 0.f ? 0.f : exponential(x, n.top) / n.sum;
+}
+
 // x to scores
-template <int V>
-__device__ inline void scores(const Route& a, const float (&x)[V], float (&s)[V]) {
-  const float inf = __builtin_inff();
+template <int L, int V>
+__device__ inline Norm scores(const Route& a, const float (&x)[V], float (&s)[V]) {
   if (a.score == TETRIS_SCORE_SIGMOID) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) s[v] = 1.f / (1.f + expf(-x[v]));
-    return;
+    for (int v = 0; v < V; ++v) s[v] = score_of(a, x[v], Norm{});
+    return {};
   }
   unsigned key = 0x007fffffu;
 #pragma unroll
   for (int v = 0; v < V; ++v) key = max(key, key_of(x[v]));
-  key = wave_max(key);
-  const float top = __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
-  float sum = 0.f;
+  key = lanes_max<L>(key);
+  Norm n{__uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key), 0.f};
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    s[v] = top == -inf && !(x[v] != x[v]) ? 0.f : x[v] == top ? 1.f : expf(x[v] - top);
-    sum += s[v];
+    s[v] = exponential(x[v], n.top);
+    n.sum += s[v];
   }
-  sum = wave_sum(sum);
+  n.sum = lanes_sum<L>(n.sum);
 #pragma unroll
-  for (int v = 0; v < V; ++v) s[v] = sum == 0.f ? 0.f : s[v] / sum;
+  for (int v = 0; v < V; ++v) s[v] = n.sum == 0.f ? 0.f : s[v] / n.sum;
+  return n;
 }
 
-// ranks -> keys of the experts that may be chosen, zero for the others
-template <int V>
-__device__ inline void keys_of(const Route& a, int lane, float* shared, const float (&rank)[V], const float (&two)[V], unsigned (&key)[V]) {
+// Keys of the experts that may be chosen, zero for the others.  `by_expert`: LDS of the token, a float for each expert; `lane`: among the token's.
+template <int L, int V>
+__device__ inline void keys_of(const Route& a, int lane, float* by_expert, const float (&rank)[V], const float (&two)[V], unsigned (&key)[V]) {
 #pragma unroll
   for (int v = 0; v < V; ++v) key[v] = lane * V + v < a.experts ? key_of(rank[v]) : 0u;
-  if (a.groups == 1 || a.top_groups == a.groups) return;
+  if (a.top_groups == a.groups) return;
   const float inf = __builtin_inff();
   const int size = a.experts / a.groups;
+  if (L == 16 && a.span) {  // a group is the experts of 1, 2, 4, 8 or 16 neighbouring lanes
+    float first = -inf, second = -inf;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float u = a.group_by == TETRIS_GROUP_TWO ? two[v] : rank[v];
+      u = u != u || lane * V + v >= a.experts ? -inf : u;
+      second = fmaxf(second, fminf(first, u));
+      first = fmaxf(first, u);
+    }
+    auto join = [&](float f, float o) {
+      second = fmaxf(fmaxf(second, o), fminf(first, f));
+      first = fmaxf(first, f);
+    };
+    auto of = [](float v, auto ctrl) { return __uint_as_float(dpp<decltype(ctrl)::value>(__float_as_uint(v))); };
+#define TETRIS_JOIN(CTRL) join(of(first, std::integral_constant<int, CTRL>{}), of(second, std::integral_constant<int, CTRL>{}))
+    if (a.span > 1) TETRIS_JOIN(0xb1);   // lane ^ 1
+    if (a.span > 2) TETRIS_JOIN(0x4e);   // lane ^ 2
+    if (a.span > 4) TETRIS_JOIN(0x141);  // the other four of eight
+    if (a.span > 8) TETRIS_JOIN(0x140);  // the other eight of sixteen
+#undef TETRIS_JOIN
+    const int shift = 31 - __builtin_clz(a.span), g = lane >> shift;
+    const unsigned mine = g < a.groups ? key_of(a.group_by == TETRIS_GROUP_TWO ? first + second : first) : 0u;
+    unsigned other = mine;
+    int before = 0;  // lanes of groups that come first, a.span of each
+#pragma unroll
+    for (int k = 1; k < 16; ++k) {
+      other = dpp<0x121>(other);  // that of lane - k
+      before += other > mine || (other == mine && (((lane - k) & 15) >> shift) < g);
+    }
+    const bool stays = before < a.top_groups * a.span;
+#pragma unroll
+    for (int v = 0; v < V; ++v) key[v] = stays ? key[v] : 0u;
+    return;
+  }
 #pragma unroll
   for (int v = 0; v < V; ++v)
-    if (lane * V + v < a.experts) shared[lane * V + v] = a.group_by == TETRIS_GROUP_TWO ? two[v] : rank[v];
+    if (lane * V + v < a.experts) by_expert[lane * V + v] = a.group_by == TETRIS_GROUP_TWO ? two[v] : rank[v];
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  unsigned mine = 0;
-  if (lane < a.groups) {
+  // lane l has groups l, l + L, ...; it begins with the l-th of a group's experts, so that lanes read different banks
+  unsigned mine[64 / L];
+#pragma unroll
+  for (int t = 0; t < 64 / L; ++t) {
+    const int g = lane + t * L;
     float first = -inf, second = -inf;
-    for (int i = 0; i < size; ++i) {
-      float v = shared[lane * size + i];
-      v = v != v ? -inf : v;
-      second = fmaxf(second, fminf(first, v));
-      first = fmaxf(first, v);
+    if (g < a.groups) {
+      int i = g % size;
+      for (int n = 0; n < size; ++n) {
+        float v = by_expert[g * size + i];
+        v = v != v ? -inf : v;
+        second = fmaxf(second, fminf(first, v));
+        first = fmaxf(first, v);
+        if (++i == size) i = 0;
+      }
     }
-    mine = key_of(a.group_by == TETRIS_GROUP_TWO ? first + second : first);
+    mine[t] = g < a.groups ? key_of(a.group_by == TETRIS_GROUP_TWO ? first + second : first) : 0u;
   }
-  int before = 0;
-  for (int g = 0; g < a.groups; ++g) {
-    const unsigned other = (unsigned)__builtin_amdgcn_readlane((int)mine, g);
-    before += other > mine || (other == mine && g < lane);
+  unsigned long long stay = 0;
+  const int shift = (threadIdx.x & 63) & ~(L - 1);
+#pragma unroll
+  for (int t = 0; t < 64 / L; ++t) {
+    if (t * L >= a.groups) break;
+    int before = 0;
+    for (int g = 0; g < a.groups; ++g) {
+      unsigned other = 0;
+#pragma unroll
+      for (int q = 0; q < 64 / L; ++q) {
+        const unsigned o = (unsigned)__shfl((int)mine[q], g % L, L);
+        if (g / L == q) other = o;
+        if ((q + 1) * L >= a.groups) break;
+      }
+      before += other > mine[t] || (other == mine[t] && g < lane + t * L);
+    }
+    const unsigned long long in = __ballot(lane + t * L < a.groups && before < a.top_groups) >> shift;
+    stay |= (L == 64 ? in : in & 0xffff) << (t * L % 64);
   }
-  const unsigned long long stay = __ballot(lane < a.groups && before < a.top_groups);
+  int g = lane * V / size, i = lane * V - g * size;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int e = lane * V + v;
-    if (e < a.experts && !((stay >> (e / size)) & 1)) key[v] = 0;
+    if (!((stay >> (g & 63)) & 1)) key[v] = 0;
+    if (++i == size) i = 0, ++g;
   }
 }
 
-template <int TYPE, int V>
+template <int TYPE, int L, int V>
 __global__ __launch_bounds__(256) void route_kernel(Route a, int* __restrict__ index, float* __restrict__ weight) {
-  __shared__ float shared[4][64 * V];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int token = blockIdx.x * 4 + wave;
-  if (token >= a.tokens) return;
+  __shared__ float shared[256 / L][L * V];
+  const int lane = threadIdx.x & (L - 1), mine = threadIdx.x / L;
+  const int token = blockIdx.x * (256 / L) + mine, read = min(token, a.tokens - 1);  // (lanes without a token follow the last one's)
   float x[V], s[V], rank[V], two[V];
   unsigned key[V];
-  load_logits<TYPE, V>(a, token, lane, x);
-  scores<V>(a, x, s);
+  load_logits<TYPE, V>(a, read, lane, x);
+  const Norm norm = scores<L, V>(a, x, s);
+  float bias[V];
+  bool read_whole = false;
+  if constexpr (V >= 4) {
+    read_whole = a.bias && a.whole;
+    if (read_whole) load_whole<float, V>(a.bias + lane * V, bias);
+  }
+  if (!read_whole) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) bias[v] = a.bias && lane * V + v < a.experts ? a.bias[lane * V + v] : 0.f;
+  }
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const float b = a.bias && lane * V + v < a.experts ? a.bias[lane * V + v] : 0.f;
-    two[v] = s[v] + b;
+    two[v] = s[v] + bias[v];
     rank[v] = a.bias ? two[v] : x[v];
   }
-  keys_of<V>(a, lane, shared[wave], rank, two, key);
+  keys_of<L, V>(a, lane, shared[mine], rank, two, key);
 
-  // the best that is left, `top` times; lane r keeps the r-th
-  int my_index = 0;
-  float my_score = 0.f, sum = 0.f;
+  // the best that is left, `top` times, the lowest index of equal ones; lane r keeps the r-th
+  unsigned my_index = 0;
   for (int r = 0; r < a.top; ++r) {
     unsigned best = 0;
 #pragma unroll
     for (int v = 0; v < V; ++v) best = max(best, key[v]);
-    const unsigned all = wave_max(best);
-    const int owner = __builtin_ctzll(__ballot(best == all));
-    int place = 0;
-    float score = 0.f;
-    bool found = false;
+    best = lanes_max<L>(best);
+    unsigned e = ~0u;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const bool this_one = !found && key[v] == all;
-      if (this_one) place = v, score = s[v];
-      found |= this_one;
-      if (this_one && lane == owner) key[v] = 0;
-    }
-    place = __builtin_amdgcn_readlane(place, owner);
-    score = __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(score), owner));
-    sum += score;
-    if (lane == r) my_index = owner * V + place, my_score = score;
+    for (int v = V - 1; v >= 0; --v) e = key[v] == best ? (unsigned)(lane * V + v) : e;
+    e = lanes_min<L>(e);
+#pragma unroll
+    for (int v = 0; v < V; ++v) key[v] = e == (unsigned)(lane * V + v) ? 0u : key[v];
+    if (lane == r) my_index = e;
   }
-  if (lane < a.top) {
-    const float w = !a.renorm ? my_score : sum == 0.f ? 0.f : my_score / sum;
-    index[(int64_t)token * a.top + lane] = my_index;
-    weight[(int64_t)token * a.top + lane] = w * a.scale;
+  // its score from its logit again, rather than from the lane that has it
+  const auto* row = static_cast<const typename Elem<TYPE>::type*>(a.logits) + read * a.ld;
+  const float score = lane < a.top ? score_of(a, (float)row[my_index], norm) : 0.f;
+  const float sum = a.renorm ? lanes_sum<L>(score) : 1.f;
+  if (lane < a.top && token < a.tokens) {
+    index[(int64_t)token * a.top + lane] = (int)my_index;
+    weight[(int64_t)token * a.top + lane] = sum == 0.f ? 0.f : (a.renorm ? score / sum : score) * a.scale;
   }
 }
 
@@ -180,7 +270,7 @@ __global__ __launch_bounds__(256) void route_backward_kernel(Route a, const int*
   if (token >= a.tokens) return;
   float x[V], s[V], d[V];
   load_logits<TYPE, V>(a, token, lane, x);
-  scores<V>(a, x, s);
+  scores<64, V>(a, x, s);
   float* mine = shared[wave];
 #pragma unroll
   for (int v = 0; v < V; ++v) mine[lane * V + v] = s[v], d[v] = 0.f;
@@ -193,11 +283,11 @@ __global__ __launch_bounds__(256) void route_backward_kernel(Route a, const int*
     if (e >= 0) dw = a.scale * dweight[(int64_t)token * a.top + lane], score = mine[e];
   }
   if (a.renorm) {
-    const float sum = wave_sum(score);
-    const float mean = sum == 0.f ? 0.f : wave_sum(dw * score) / sum;
+    const float sum = lanes_sum<64>(score);
+    const float mean = sum == 0.f ? 0.f : lanes_sum<64>(dw * score) / sum;
     dw = sum == 0.f || e < 0 ? 0.f : (dw - mean) / sum;
   }
-  const float all = a.score == TETRIS_SCORE_SOFTMAX && !a.renorm ? wave_sum(dw * score) : 0.f;
+  const float all = a.score == TETRIS_SCORE_SOFTMAX && !a.renorm ? lanes_sum<64>(dw * score) : 0.f;
   for (int j = 0; j < a.top; ++j) {
     const int ej = __builtin_amdgcn_readlane(e, j);
     const float dj = __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(dw), j));
@@ -213,9 +303,23 @@ __global__ __launch_bounds__(256) void route_backward_kernel(Route a, const int*
   }
 }
 
-template <int TYPE, int V>
-void launch_route(const Route& a, int* index, float* weight, hipStream_t s) {
-  hipLaunchKernelGGL((route_kernel<TYPE, V>), dim3((a.tokens + 3) / 4), dim3(256), 0, s, a, index, weight);
+template <int TYPE, int L, int V>
+void launch_route(Route a, int* index, float* weight, hipStream_t s) {
+  const int size = a.experts / a.groups, lanes_each = size / V;
+  a.whole = a.experts == L * V && (reinterpret_cast<size_t>(a.logits) & 15) == 0 && a.ld * elem_size(TYPE) % 16 == 0 && (reinterpret_cast<size_t>(a.bias) & 15) == 0;
+  a.span = L == 16 && size % V == 0 && (lanes_each & (lanes_each - 1)) == 0 ? lanes_each : 0;
+  hipLaunchKernelGGL((route_kernel<TYPE, L, V>), dim3(ceil_div(a.tokens, 256 / L)), dim3(256), 0, s, a, index, weight);
+}
+template <int TYPE>
+void route_any(const Route& a, int* index, float* weight, hipStream_t s) {
+  if (a.experts <= 256 && a.top <= 16) {
+    if (a.experts <= 16) launch_route<TYPE, 16, 1>(a, index, weight, s);
+    else if (a.experts <= 64) launch_route<TYPE, 16, 4>(a, index, weight, s);
+    else if (a.experts <= 128) launch_route<TYPE, 16, 8>(a, index, weight, s);
+    else launch_route<TYPE, 16, 16>(a, index, weight, s);
+  } else if (a.experts <= 256) launch_route<TYPE, 64, 4>(a, index, weight, s);
+  else if (a.experts <= 512) launch_route<TYPE, 64, 8>(a, index, weight, s);
+  else launch_route<TYPE, 64, 16>(a, index, weight, s);
 }
 template <int TYPE, int V>
 void launch_backward(const Route& a, const int* index, const float* dweight, void* out, int64_t ld, hipStream_t s) {
@@ -257,7 +361,7 @@ int check(const tetris_router* r, int type, int tokens, int64_t ld) {
 }
 
 Route route_of(const tetris_router* r, const void* logits, int tokens, int64_t ld, const float* bias) {
-  return {logits, ld, tokens, r->experts, r->top, r->score, r->groups, r->top_groups, r->group_by, r->renorm, r->scale, bias};
+  return {logits, ld, tokens, r->experts, r->top, r->score, r->groups, r->top_groups, r->group_by, r->renorm, r->scale, bias, 0, 0};
 }
 
 }  // namespace
@@ -273,9 +377,7 @@ extern "C" int tetris_route(const tetris_router* r, const void* d_logits, int ty
   if (reinterpret_cast<size_t>(d_logits) % elem_size(type)) return fail(TETRIS_EINVAL, "logits not aligned to their elements");
   const Route a = route_of(r, d_logits, tokens, ld, d_bias);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  by_type(type, [&](auto t) {
-    by_width<decltype(t)::value>(r->experts, [&](auto v) { launch_route<decltype(t)::value, decltype(v)::value>(a, d_index, d_weight, s); });
-  });
+  by_type(type, [&](auto t) { route_any<decltype(t)::value>(a, d_index, d_weight, s); });
   TETRIS_HIP(hipGetLastError());
   return TETRIS_OK;
 }
