@@ -112,7 +112,9 @@ def test_dequantise_every_code_at_every_scale():
 # ---- products ----
 
 SIZES = [(1, 32, 32), (1, 4096, 80), (2, 33, 17), (5, 1001, 100), (16, 128, 48), (17, 264, 64), (40, 96, 33), (64, 512, 1000), (65, 128, 31),
-         (100, 77, 257), (129, 200, 300), (257, 1032, 70), (300, 64, 520)]
+         (100, 77, 257), (129, 200, 300), (257, 1032, 70), (300, 64, 520),
+         # more rows than are streamed: tiles of 32 rows, of 64, and of 128
+         (1030, 1001, 70), (1100, 96, 33), (1500, 200, 2100), (3999, 100, 4091)]
 
 
 @pytest.mark.parametrize("kind", TYPES)
@@ -135,7 +137,7 @@ def test_linear(kind, m, k, n):
 
 
 @pytest.mark.parametrize("kind", TYPES)
-@pytest.mark.parametrize("m,k,n", [(1, 64, 32), (3, 1001, 65), (64, 256, 100), (65, 128, 300), (130, 96, 40), (300, 520, 257), (513, 1024, 600)])
+@pytest.mark.parametrize("m,k,n", [(1, 64, 32), (3, 1001, 65), (64, 256, 100), (65, 128, 300), (130, 96, 40), (300, 520, 257), (513, 1024, 600), (1025, 96, 40), (1300, 520, 257)])
 def test_linear_of_rounded_rows(kind, m, k, n):
     rng = np.random.default_rng(m + k + n)
     codes, scales, w = random_weights(rng, n, k)
@@ -150,7 +152,7 @@ def test_linear_of_rounded_rows(kind, m, k, n):
 
 
 @pytest.mark.parametrize("rounded", [False, True])
-@pytest.mark.parametrize("m", [3, 200])
+@pytest.mark.parametrize("m", [3, 200, 1100])
 def test_linear_where_numbers_are_no_numbers(m, rounded):
     rng = np.random.default_rng(m)
     k, n = 96, 40
@@ -179,7 +181,7 @@ def test_linear_at_the_ends_of_the_scales():
         w = rounded_to(P.values(code, scales, k), "f32")  # 6 * 2^127 is infinite in 32 bits
         d = torch.from_numpy(P.packed(code)).cuda(), torch.from_numpy(scales).cuda()
         W = T.MX4Weights(d[0].data_ptr(), d[1].data_ptr(), n, k)
-        for m in (2, 150):
+        for m in (2, 150, 1100):
             x = rounded_to(rng.normal(size=(m, k)) * size, "bf16")
             with np.errstate(invalid="ignore"):
                 want, _, far = P.product(x, w, "f32")
@@ -189,6 +191,65 @@ def test_linear_at_the_ends_of_the_scales():
                 got, fine = numbers(y), np.isfinite(want)
                 assert np.array_equal(got[~fine], want[~fine], equal_nan=True) and (fine.all() or scale == 254)
                 within(got[fine], want[fine], (far + P.ROUNDING[kind] * np.abs(want))[fine])
+
+
+@pytest.mark.parametrize("least,most", [(104, 140), (103, 140), (104, 141), (90, 150)])
+def test_f16_rows_and_weights_at_the_ends_of_f16(least, most):
+    """Scales 2^-23 .. 2^13 make weights that are exact in f16; others are multiplied in parts."""
+    rng = np.random.default_rng(least + most)
+    k, n = 128, 48
+    code = rng.integers(0, 16, (n, 4, 32)).astype(np.uint8)
+    scales = rng.integers(least, most + 1, (n, 4)).astype(np.uint8)
+    scales[0, 0], scales[1, 1] = least, most
+    scales[2, 2], code[2, 2] = 0, 8  # zeros need no scale
+    d = torch.from_numpy(P.packed(code)).cuda(), torch.from_numpy(scales).cuda()
+    W = T.MX4Weights(d[0].data_ptr(), d[1].data_ptr(), n, k)
+    for m in (5, 1100):
+        x = rounded_to(rng.normal(size=(m, k)) * 2.0 ** -12, "f16")  # f16's subnormal numbers among them
+        want, _, far = P.product(x, P.values(code, scales, k), "f16")
+        y = torch.zeros(m, n, dtype=torch.float16, device="cuda")
+        W.linear(on_gpu(x, "f16").data_ptr(), y.data_ptr(), m, T.F16)
+        fine = np.abs(want) + far < 65504
+        within(numbers(y)[fine], want[fine], far[fine])
+        assert fine.mean() > 0.3
+
+
+@pytest.mark.parametrize("kind,m,k", [("bf16", 2200000, 1024), ("f32", 360000, 1024), ("f16", 600000, 1000)])
+def test_rows_beyond_32_bit_offsets(kind, m, k):
+    """Rows of 4.5 GB as they lie, and of 1.5 GB and 1.2 GB whose parts and copies pass 2^31 bytes."""
+    rng = np.random.default_rng(m)
+    n = 40
+    code = rng.integers(0, 16, (n, -(-k // 32), 32)).astype(np.uint8)
+    code.reshape(n, -1)[:, k:] = 0
+    scales = rng.integers(90, 160, code.shape[:2]).astype(np.uint8)  # beyond f16
+    d = torch.from_numpy(P.packed(code)).cuda(), torch.from_numpy(scales).cuda()
+    W = T.MX4Weights(d[0].data_ptr(), d[1].data_ptr(), n, k)
+    x = torch.empty(m, k, dtype=TYPES[kind][1], device="cuda").normal_() * 2.0 ** -9
+    y = torch.empty(m, n, dtype=torch.float32 if kind == "f32" else TYPES[kind][1], device="cuda")
+    W.linear(x.data_ptr(), y.data_ptr(), m, TYPES[kind][0])
+    rows = np.unique(np.concatenate([rng.integers(0, m, 60), [0, m - 1, m // 2], (2**31 // (2 * k) + np.arange(-2, 3)) % m]))
+    at = torch.from_numpy(rows).cuda()
+    want, _, far = P.product(numbers(x[at]), P.values(code, scales, k), kind)
+    got, fine = numbers(y[at]), np.abs(want) + far < (65504 if kind == "f16" else np.inf)
+    within(got[fine], want[fine], far[fine])
+
+
+def test_experts_of_rows_beyond_32_bit_offsets():
+    rng = np.random.default_rng(17)
+    tokens, count, width, hidden = 1150000, 3, 1024, 32
+    up, down = random_weights(rng, count * 2 * hidden, width), random_weights(rng, count * width, hidden)
+    layer = T.ExpertLayer(T.MX4Weights(up[0].data_ptr(), up[1].data_ptr(), 2 * hidden, width, experts=count, gated=True),
+                          T.MX4Weights(down[0].data_ptr(), down[1].data_ptr(), width, hidden, experts=count))
+    x = torch.empty(tokens, width, dtype=torch.bfloat16, device="cuda").normal_() * 0.01
+    index = torch.randint(0, count, (tokens, 1), dtype=torch.int32, device="cuda")
+    weight = torch.rand(tokens, 1, device="cuda")
+    y = torch.empty_like(x)
+    layer.run(x.data_ptr(), index.data_ptr(), weight.data_ptr(), y.data_ptr(), tokens, 1, T.BF16)
+    rows = np.unique(np.concatenate([rng.integers(0, tokens, 60), [0, tokens - 1], 2**31 // (2 * width) + np.arange(-3, 3)]))
+    at = torch.from_numpy(rows).cuda()
+    want, far = P.experts(numbers(x[at]), up[2].reshape(count, 2 * hidden, width), down[2].reshape(count, width, hidden), index[at].cpu().numpy(),
+                          numbers(weight[at]), "bf16")
+    within(numbers(y[at]), want, far)
 
 
 def test_weights_from_numbers_are_those_from_their_codes():
@@ -245,7 +306,9 @@ def run_experts(layer, x, index, weight, kind, ldx=None, offset=0, stream=0):
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("tokens,count,top,width,hidden", [
     (1, 4, 2, 64, 32), (1, 1, 1, 33, 5), (3, 8, 3, 100, 48), (20, 70, 4, 128, 40), (17, 3, 3, 256, 72), (64, 8, 2, 264, 100), (50, 60, 8, 96, 31),
-    (200, 4, 2, 128, 96), (260, 2, 1, 72, 130), (300, 3, 2, 520, 64)])
+    (200, 4, 2, 128, 96), (260, 2, 1, 72, 130), (300, 3, 2, 520, 64),
+    # more slots than are streamed, in tiles of 32 rows; of 64 and of 128 in the first product, and in the second
+    (600, 3, 2, 520, 64), (1100, 2, 1, 72, 130), (1200, 2, 2, 72, 1040), (3000, 2, 2, 72, 1040), (1200, 2, 2, 2100, 48), (3000, 2, 2, 2100, 48)])
 def test_experts(kind, tokens, count, top, width, hidden):
     rng = np.random.default_rng(tokens + count + width)
     layer, x, index, weight, want, far = expert_case(rng, tokens, count, top, width, hidden, kind)
@@ -264,7 +327,7 @@ def test_experts_of_uneven_load(kind, tokens):
     within(run_experts(layer, x, index, weight, kind), want, far)
 
 
-@pytest.mark.parametrize("tokens", [6, 400])
+@pytest.mark.parametrize("tokens", [6, 200, 400])
 def test_experts_that_are_none(tokens):
     rng = np.random.default_rng(tokens)
     pick = rng.integers(-2, 6, (tokens, 3))
@@ -535,3 +598,14 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     within(numbers(ys[0]), want, far)
     assert torch.equal(ys[0], ys[1])
+
+
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("tokens", [3, 100])
+def test_block_of_experts_end_to_end(tokens, graph):
+    from tetris_amd import expert_block
+
+    args = ["--tokens", str(tokens), "--width", "256", "--hidden", "96", "--experts", "12", "--top", "3", "--classes", "50", "--steps", "3"]
+    out = expert_block.main(args + (["--graph"] if graph else []))
+    # roundings to bf16: what lies between the products and the output of the block, those of the scores; 2^-8 bounds each
+    assert out["block_error"] <= 3 * 2.0 ** -8 and out["scores_error"] <= 2.0 ** -8
