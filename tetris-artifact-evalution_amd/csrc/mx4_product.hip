@@ -470,9 +470,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
 // reads of it are one contiguous kilobyte.
 template <int WT, int WR, int WM, int WN, int OUT>
 __global__ __launch_bounds__(64 * WM * WN) void rounded_kernel(Product a) {
+  constexpr int D = 3;  // LDS buffers and sets of registers; with two of them 8192^3 takes 2 % longer
   constexpr int kTiles = WT * WM, kThreads = 64 * WM * WN, kLoads = kTiles * 128 / kThreads;
-  __shared__ i32x4 lds0[kTiles * 128], lds1[kTiles * 128], stage[WM * WN][256];
-  auto buffer_of = [&](int i) -> i32x4* { return i ? lds1 : lds0; };
+  __shared__ i32x4 lds0[kTiles * 128], lds1[kTiles * 128], lds2[kTiles * 128], stage[WM * WN][256];
+  auto buffer_of = [&](int i) -> i32x4* { return i == 0 ? lds0 : i == 1 ? lds1 : lds2; };  // (i is a constant where this is used)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, wn = wave / WM;
   int block, tile;
@@ -503,8 +504,8 @@ __global__ __launch_bounds__(64 * WM * WN) void rounded_kernel(Product a) {
     for (int r = 0; r < WR; ++r) acc[t][r] = f32x16{};
 
   const int steps = a.col_tiles >> 1;
-  i32x4 w[2][WR][2], xs[2][WT];
-  int w_scale[2][WR], x_scale[2][WT];
+  i32x4 w[D][WR][2], xs[2][WT];
+  int w_scale[D][WR], x_scale[D][WT];
   int row_step = 0, weight_step = 0;
   auto fetch_rows = [&](int set) {  // past the last step that one again, into a buffer that nobody reads
     const int at = min(row_step++, steps - 1) * 2048;
@@ -531,7 +532,7 @@ __global__ __launch_bounds__(64 * WM * WN) void rounded_kernel(Product a) {
   };
   // as in tile_kernel, with two rounds of products a step
   auto multiply = [&](int set) {
-    const int next = set ^ 1;
+    const int next = set + 1 == D ? 0 : set + 1;
     read(set, 1);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -540,7 +541,7 @@ __global__ __launch_bounds__(64 * WM * WN) void rounded_kernel(Product a) {
       for (int r = 0; r < WR; ++r)
         acc[t][r] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(w[set][r][0]), wide(xs[0][t]), acc[t][r], 4, 4, 0, w_scale[set][r], 0, x_scale[set][t]);
     __builtin_amdgcn_sched_barrier(0);
-    barrier_but<kWeightLoads>();
+    barrier_but<(D - 2) * kLoads + (D - 1) * kWeightLoads>();
     fetch_rows(set);
     read(next, 0);
     __builtin_amdgcn_sched_barrier(0);
@@ -552,17 +553,21 @@ __global__ __launch_bounds__(64 * WM * WN) void rounded_kernel(Product a) {
     __builtin_amdgcn_sched_barrier(0);
     fetch_weights(set);
   };
-  fetch_rows(0);
-  fetch_weights(0);
-  fetch_rows(1);
-  fetch_weights(1);
-  barrier_but<kLoads + 2 * kWeightLoads>();
-  read(0, 0);
-  for (int step = 0; step + 1 < steps; step += 2) {
-    multiply(0);
-    multiply(1);
+#pragma unroll
+  for (int i = 0; i < D; ++i) {
+    fetch_rows(i);
+    fetch_weights(i);
   }
-  if (steps & 1) multiply(0);
+  barrier_but<(D - 1) * kLoads + D * kWeightLoads>();
+  read(0, 0);
+  int step = 0;
+  for (; step + D <= steps; step += D) {
+#pragma unroll
+    for (int i = 0; i < D; ++i) multiply(i);
+  }
+#pragma unroll
+  for (int i = 0; i < D - 1; ++i)
+    if (step + i < steps) multiply(i);
   put_tile<WT, OUT, false>(a, acc, wm * WT * 32, first, count, (block * WN + wn) * WR, stage[wave]);
   loads_have_ended();
 }
