@@ -261,6 +261,7 @@ __global__ __launch_bounds__(256) void route_kernel(Route a, int* __restrict__ i
 // With s the scores, c the chosen, S the sum of theirs and d_j = scale dweight_j (renorm: (d_j - sum_l d_l s_l / S) / S):
 //   sigmoid  dlogit_i = s_i (1 - s_i) d_i for the chosen, else 0
 //   softmax  dlogit_i = s_i (d_i - sum_j s_j d_j), with d_i = 0 for those not chosen; with renorm that sum is zero
+// A wave a token.  8192 tokens of 128 experts in bf16: 6.2 us (4.7 MB); the launch and one wave's chain of instructions, not memory.
 template <int TYPE, int V>
 __global__ __launch_bounds__(256) void route_backward_kernel(Route a, const int* __restrict__ index, const float* __restrict__ dweight,
                                                              typename Elem<TYPE>::type* __restrict__ out, int64_t ld_out) {
