@@ -6,7 +6,8 @@
  * `type` names the elements of activations, logits and outputs: TETRIS_F32, TETRIS_F16 or TETRIS_BF16.  A leading
  * dimension (`ld`) is the distance of two rows in elements.  Rows and bases need no alignment beyond their element's;
  * rows that start on 16 bytes and widths that are multiples of eight are read without a copy.
- * A call with no rows does nothing and succeeds.
+ * Outputs may not overlap inputs.  A call with no rows does nothing and succeeds.  Launches of one handle on one stream come from one
+ * thread at a time (they share that stream's workspace).
  */
 #ifndef TETRIS_MX4_H_
 #define TETRIS_MX4_H_
@@ -42,7 +43,7 @@ int tetris_mx4_dequantize(const uint8_t* d_codes, const uint8_t* d_scales, int64
  * Weights in MX4, laid out once for the kernels: `experts` matrices of n rows and k columns.
  * tetris_mx4_create takes MX4 rows (experts * n of them, as tetris_mx4_quantize writes them), tetris_mx4_create_values
  * numbers of any type, which it quantises.  gated: the first n / 2 rows of a matrix are a gate's and the others the rows
- * it gates (tetris_experts); n is then even.  Both wait for `stream`: the arrays may be freed afterwards, and the handle
+ * it gates (tetris_experts); n is then even.  At most 1024 matrices, sides up to 2^21.  Both wait for `stream`: the arrays may be freed afterwards, and the handle
  * used on any stream.
  * ---------------------------------------------------------------------------------------------- */
 typedef struct tetris_mx4 tetris_mx4;
@@ -56,7 +57,7 @@ void tetris_mx4_destroy(tetris_mx4* w); /* no launch that uses it may be under w
  * y[i] = x[i] W^T + bias for m rows x[i] of k and y[i] of n elements of `type`; d_bias: n floats or NULL.  W is one
  * matrix, not gated.  Products are exact and summed in 32 bits.  mx4_input: the rows of x are rounded to MX4 (as
  * tetris_mx4_quantize does) before the product, on the fly; large m then runs on the matrix cores' 4-bit products.
- * Workspace is the handle's, one per stream it is launched on; tetris_mx4_prepare makes it ahead (of a graph capture,
+ * Workspace is the handle's, one per stream it is launched on; tetris_mx4_prepare makes it ahead, for up to m rows (of a graph capture,
  * under which a launch that would have to allocate is refused with TETRIS_EINVAL).
  * ---------------------------------------------------------------------------------------------- */
 int tetris_mx4_prepare(tetris_mx4* w, int m, int type, int mx4_input, void* stream);

@@ -584,6 +584,50 @@ def test_graph_of_a_routed_layer(tokens):
         assert torch.equal(y, first[0]) and torch.equal(index, first[1]) and torch.equal(weight, first[2])
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rounded", [False, True])
+def test_workspace_made_for_more_rows_is_enough_for_fewer(kind, rounded):
+    rng = np.random.default_rng(9)
+    k, n = 200, 40
+    codes, scales, w = random_weights(rng, n, k)
+    s = torch.cuda.Stream()
+    for most in (2000, 1000):
+        W = T.MX4Weights(codes.data_ptr(), scales.data_ptr(), n, k)
+        W.prepare(most, TYPES[kind][0], mx4_input=rounded, stream=s.cuda_stream)
+        for m in (most, 1025, 1000, 700, 17, 1):
+            if m > most:
+                continue
+            x = rounded_to(rng.normal(size=(m, k)), kind)
+            dx = on_gpu(x, kind, k + 1, 1)  # lies badly: is copied or split
+            y = torch.zeros(m, n, dtype=TYPES[kind][1], device="cuda")
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=s):
+                W.linear(dx.data_ptr(), y.data_ptr(), m, TYPES[kind][0], ldx=k + 1, mx4_input=rounded, stream=s.cuda_stream)
+            graph.replay()
+            torch.cuda.synchronize()
+            want, _, far = P.product(P.values(*P.quantise(x), k) if rounded else x, w, kind)
+            within(numbers(y), want, far)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_experts_workspace_made_for_more_tokens_is_enough_for_fewer(kind):
+    rng = np.random.default_rng(10)
+    layer, x, index, weight, want, far = expert_case(rng, 900, 4, 2, 72, 40, kind)
+    s = torch.cuda.Stream()
+    layer.prepare(900, 2, TYPES[kind][0], stream=s.cuda_stream)
+    for tokens in (900, 500, 100, 20, 1):
+        dx, y = on_gpu(x[:tokens], kind, 73, 1), torch.zeros(tokens, 72, dtype=TYPES[kind][1], device="cuda")
+        di, dw = torch.from_numpy(index[:tokens].astype(np.int32)).cuda(), torch.from_numpy(weight[:tokens]).cuda()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            layer.run(dx.data_ptr(), di.data_ptr(), dw.data_ptr(), y.data_ptr(), tokens, 2, TYPES[kind][0], ldx=73, stream=s.cuda_stream)
+        graph.replay()
+        torch.cuda.synchronize()
+        within(numbers(y), want[:tokens], far[:tokens])
+
+
 def test_two_streams_at_once():
     rng = np.random.default_rng(5)
     tokens = 150

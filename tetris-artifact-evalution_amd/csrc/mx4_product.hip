@@ -1002,18 +1002,20 @@ int workspace(tetris_mx4* w, hipStream_t stream, size_t need, uint8_t** out) {
   }
 }
 
+constexpr int kStreamMost = 1024;  // more rows are not streamed, whatever the matrix
+
 // Whether a product's rows are streamed.  Decided by its sizes alone, so that a workspace can be made ahead.
 bool streams(const tetris_mx4* w, int rows) {
   Product a{};
   a.rows = rows;
   a.row_tiles = w->row_tiles;
-  return rows <= 1024 && stream_cost(a, false) < tile_cost(a, 32);
+  return rows <= kStreamMost && stream_cost(a, false) < tile_cost(a, 32);
 }
 // The experts': of the first product, for both; up to 64 slots always are.
 bool streams_slots(const tetris_mx4* up, int tokens, int top) {
   const int64_t slots = (int64_t)tokens * top;
   if (slots <= 64) return true;
-  if (slots > 1024) return false;
+  if (slots > kStreamMost) return false;
   Product a{};
   a.rows = (int)slots;
   a.experts = up->experts;
@@ -1150,7 +1152,10 @@ extern "C" int tetris_mx4_prepare(tetris_mx4* w, int m, int type, int mx4_input,
   if (m < 0) return fail(TETRIS_EINVAL, "%d rows", m);
   uint8_t* d;
   const int rows = rows_at_once(w, m, type, mx4_input);
-  return workspace(w, static_cast<hipStream_t>(stream), staged_bytes(rows, w->k, type, mx4_input, streams(w, m), in_half(type, w)), &d);
+  const bool half = in_half(type, w);
+  // fewer rows may be streamed where these are not, and rounded ones then take more room each
+  const size_t need = std::max(staged_bytes(rows, w->k, type, mx4_input, streams(w, m), half), staged_bytes(std::min(m, kStreamMost), w->k, type, mx4_input, true, half));
+  return workspace(w, static_cast<hipStream_t>(stream), need, &d);
 }
 
 extern "C" int tetris_mx4_linear(tetris_mx4* w, const void* d_x, int type, int m, int64_t ldx, void* d_y, int64_t ldy,
