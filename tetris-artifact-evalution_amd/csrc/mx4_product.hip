@@ -320,7 +320,7 @@ __device__ inline void barrier_but() {
 
 // ---- many rows: tiles through LDS ---------------------------------------------------------------------------------
 //
-// A workgroup computes 32 WT WM rows by 32 WR WN features (KS: column tiles a step, PI: parts of the rows taken in one step, each with the weights made once).
+// A workgroup computes 32 WT rows by 32 WR WN features (KS: column tiles a step, PI: parts of the rows taken in one step, each with the weights made once).
 // Bound by the matrix cores: 4096 x 4096 x 8192 of bf16 in 193 us (1.42 PFLOP/s), their pipes 80 % busy at the clock that power leaves; by the
 // weights' bytes where groups are small: 2.9 TB/s on 200 tokens of 8 of 64 experts of 2048 x 1000.  Rows come in steps of 64 KS columns, 128 KS bytes of each
 // row in one stretch, through registers into one of two LDS buffers while the other is multiplied; weights come straight
@@ -329,32 +329,24 @@ __device__ inline void barrier_but() {
 template <int KS>
 __device__ inline int turn_of(int row) { return KS == 1 ? (row >> 1) & 7 : row & 15; }
 
-template <int WT, int WR, int WM, int WN, int KS, int PI, bool HALF, int OUT, bool GATED>
-__global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
-  constexpr int kRows = 32 * WT * WM, kThreads = 64 * WM * WN, kPieces = 8 * KS, kLoads = kRows * kPieces / kThreads;
+template <int WT, int WR, int WN, int KS, int PI, bool HALF, int OUT, bool GATED>
+__global__ __launch_bounds__(64 * WN, 2) void tile_kernel(Product a) {
+  constexpr int kRows = 32 * WT, kThreads = 64 * WN, kPieces = 8 * KS, kLoads = kRows * kPieces / kThreads;
   static_assert(kThreads / kPieces % 16 == 0, "a thread's pieces lie in the same columns");
   constexpr int kBuffer = PI * kRows * kPieces;
-  __shared__ i32x4 lds0[kBuffer], lds1[kBuffer], stage[WM * WN][256];  // (two arrays, so that the compiler can tell a load to one from reads of the other)
+  __shared__ i32x4 lds0[kBuffer], lds1[kBuffer], stage[WN][256];  // (two arrays, so that the compiler can tell a load to one from reads of the other)
   auto buffer_of = [&](int i) -> i32x4* { return i ? lds1 : lds0; };
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave % WM, wn = wave / WM;
   int block, tile;
   if (!place_tile(a, WR * WN, &block, &tile)) return;
   int expert, first, count;
   if (!find_tile(a, tile, kRows, &expert, &first, &count)) return;
 
   const int column = ((threadIdx.x % kPieces) ^ turn_of<KS>(threadIdx.x / kPieces)) * 8;
-  const __amdgpu_buffer_rsrc_t rows = buffer(static_cast<const __bf16*>(a.x) + (a.from_div ? 0 : first * a.ldx));
-  int from[kLoads];  // bytes
-#pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int p = min((int)(i * kThreads + threadIdx.x) / kPieces, count - 1);
-    from[i] = (a.from_div ? a.order[first + p] / a.from_div : p) * (int)a.ldx * 2 + column * 2;
-  }
   __amdgpu_buffer_rsrc_t codes[WR], scales[WR];
 #pragma unroll
   for (int r = 0; r < WR; ++r) {
-    const int64_t t = (int64_t)expert * a.row_tiles + min((block * WN + wn) * WR + r, a.row_tiles - 1);
+    const int64_t t = (int64_t)expert * a.row_tiles + min((block * WN + wave) * WR + r, a.row_tiles - 1);
     codes[r] = buffer(a.codes + t * a.col_tiles * 64);
     scales[r] = buffer(a.scales + t * a.col_tiles * 64);
   }
@@ -369,16 +361,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
   i32x4 w[2][WR][KS];
   unsigned s[2][WR];
   int w_step = 0, x_col = 0, x_part = 0, w_col = 0;
-  auto fetch_rows = [&](int set) {  // straight to LDS; zeros past a row's end, and past the last step, where nobody reads them (the barriers count them)
-    const bool in = x_col * 64 + column < a.k8;
-#pragma unroll
-    for (int p = 0; p < PI; ++p)
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-        to_lds(rows, in ? from[i] : kNowhere, (x_part + p) * (int)a.part * 2 + x_col * 128, buffer_of(set) + (p * kLoads + i) * kThreads + wave * 64);
-    x_part += PI;
-    if (x_part == a.parts) x_part = 0, x_col += KS;
-  };
   auto fetch_weights = [&](int set) {  // past the last step that one's again
     const int c0 = min(w_col, a.col_tiles - KS);
 #pragma unroll
@@ -393,21 +375,30 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
     w_step += PI;
     if (w_step == a.parts) w_step = 0, w_col += KS;
   };
+  fetch_weights(0);  // on their way while the tile's rows are looked up
+  fetch_weights(1);
+
+  const __amdgpu_buffer_rsrc_t rows = buffer(static_cast<const __bf16*>(a.x) + (a.from_div ? 0 : first * a.ldx));
+  int from[kLoads];  // bytes
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int p = min((int)(i * kThreads + threadIdx.x) / kPieces, count - 1);
+    from[i] = (a.from_div ? a.order[first + p] / a.from_div : p) * (int)a.ldx * 2 + column * 2;
+  }
+  auto fetch_rows = [&](int set) {  // straight to LDS; zeros past a row's end, and past the last step, where nobody reads them (the barriers count them)
+    const bool in = x_col * 64 + column < a.k8;
+#pragma unroll
+    for (int p = 0; p < PI; ++p)
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        to_lds(rows, in ? from[i] : kNowhere, (x_part + p) * (int)a.part * 2 + x_col * 128, buffer_of(set) + (p * kLoads + i) * kThreads + wave * 64);
+    x_part += PI;
+    if (x_part == a.parts) x_part = 0, x_col += KS;
+  };
   constexpr int kWeightLoads = WR * (KS + 1), kRowLoads = PI * kLoads;
 
   const int steps = a.col_tiles / KS * (a.parts / PI);
-  if (wm * WT * 32 >= count) {  // none of the wave's rows is there: it only helps to load
-    fetch_rows(0);
-    fetch_rows(1);
-    barrier_but<kRowLoads>();
-    for (int step = 0; step < steps; ++step) {
-      barrier_but<0>();
-      fetch_rows(step & 1);
-    }
-    loads_have_ended();
-    return;
-  }
-  const int row_in = wm * WT * 32 + (lane & 31), turn = turn_of<KS>(lane & 31), half = lane >> 5;
+  const int row_in = lane & 31, turn = turn_of<KS>(row_in), half = lane >> 5;
   constexpr int kRounds = 4 * KS * PI, kProducts = WT * WR, kPairs = 4 * WR;
   i32x4 xs[2][WT], ws[2][WR];
   auto read = [&](int buffer, int round) {  // the rows' share in a round of a step's products: PI parts of the same columns after another
@@ -450,11 +441,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
       }
     }
   };
-  fetch_weights(0);
   fetch_rows(0);
-  fetch_weights(1);
   fetch_rows(1);
-  barrier_but<kRowLoads + kWeightLoads>();
+  barrier_but<kRowLoads>();
   read(0, 0);
 #pragma unroll
   for (int c = 0; c < kPairs; ++c) convert(0, 0, c);
@@ -463,7 +452,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Product a) {
     multiply(1);
   }
   if (steps & 1) multiply(0);
-  put_tile<WT, OUT, GATED>(a, acc, wm * WT * 32, first, count, (block * WN + wn) * WR, stage[wave]);
+  put_tile<WT, OUT, GATED>(a, acc, 0, first, count, (block * WN + wave) * WR, stage[wave]);
   loads_have_ended();
 }
 
@@ -855,13 +844,22 @@ __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ 
     const int64_t t = i / quads;
     const int c = (int)(i - t * quads) * 4;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int j = 0; j < top; ++j) {
-      const int e = index[t * top + j];
-      if (e < 0 || e >= experts) continue;
-      const f32x4 r = *reinterpret_cast<const f32x4*>(rows + (t * top + j) * ld_rows + c);
-      const float w = weight[t * top + j];
+    for (int j0 = 0; j0 < top; j0 += 4) {  // four rows under way; those of no expert were never written and count for nothing
+      f32x4 r[4];
+      float w[4];
+      bool in[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v[q] = fmaf(w, r[q], v[q]);
+      for (int q = 0; q < 4; ++q) {
+        const int64_t slot = t * top + min(j0 + q, top - 1);
+        const int e = index[slot];
+        in[q] = j0 + q < top && e >= 0 && e < experts;
+        w[q] = weight[slot];
+        r[q] = *reinterpret_cast<const f32x4*>(rows + slot * ld_rows + c);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = in[q] ? fmaf(w[q], r[q][i], v[i]) : v[i];
     }
     T* out = y + t * ldy + c;
     if (vec && c + 4 <= width) {
@@ -882,13 +880,13 @@ int stream_waves(int chunks, int64_t workgroups) {
   return waves;
 }
 
-template <int WT, int WR, int WM, int WN, int KS, int PI, bool HALF, int OUT, bool GATED>
+template <int WT, int WR, int WN, int KS, int PI, bool HALF, int OUT, bool GATED>
 int launch_tile(Product& a, hipStream_t stream) {
-  const int size = 32 * WT * WM, row_blocks = ceil_div(a.row_tiles, WR * WN);
+  const int size = 32 * WT, row_blocks = ceil_div(a.row_tiles, WR * WN);
   a.max_tiles = a.offsets ? std::min(a.rows, a.rows / size + std::min(a.experts, a.rows)) : ceil_div(a.rows, size);
   const int64_t blocks = round_up((int64_t)row_blocks * a.max_tiles, 256);
   if (blocks > 0x7fffffff / 2) return fail(TETRIS_EINVAL, "%d rows by %d features are too many for one launch", a.rows, a.n);
-  hipLaunchKernelGGL((tile_kernel<WT, WR, WM, WN, KS, PI, HALF, OUT, GATED>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream, a);
+  hipLaunchKernelGGL((tile_kernel<WT, WR, WN, KS, PI, HALF, OUT, GATED>), dim3((unsigned)blocks), dim3(64 * WN), 0, stream, a);
   TETRIS_HIP(hipGetLastError());
   return TETRIS_OK;
 }
@@ -956,9 +954,9 @@ double stream_cost(const Product& a, bool gated) {
 template <int OUT, bool GATED, int P, bool HALF = false>
 int tile_rows(Product& a, hipStream_t stream) {
   const double small = tile_cost(a, 32), middle = tile_cost(a, 64), large = tile_cost(a, 128);
-  if (small <= middle && small <= large) return launch_tile<1, 2, 1, 4, P == 3 ? 1 : 2, P, HALF, OUT, GATED>(a, stream);
-  if (middle < large) return launch_tile<2, 2, 1, 4, P == 2 ? 1 : 2, P == 2 ? 2 : 1, HALF, OUT, GATED>(a, stream);
-  return launch_tile<4, 2, 1, 4, 1, 1, HALF, OUT, GATED>(a, stream);
+  if (small <= middle && small <= large) return launch_tile<1, 2, 4, P == 3 ? 1 : 2, P, HALF, OUT, GATED>(a, stream);
+  if (middle < large) return launch_tile<2, 2, 4, P == 2 ? 1 : 2, P == 2 ? 2 : 1, HALF, OUT, GATED>(a, stream);
+  return launch_tile<4, 2, 4, 1, 1, HALF, OUT, GATED>(a, stream);
 }
 
 void set_weights(Product* a, const tetris_mx4* w) {
