@@ -24,7 +24,8 @@ enum { TETRIS_F32 = 0, TETRIS_F16 = 1, TETRIS_BF16 = 2 };
  * MX4 rows.  A row of `cols` values is ceil(cols / 32) blocks; a block is 16 bytes of codes (element 2i in the low half
  * of byte i) and one scale byte.  Value = code * 2^(scale - 127); codes 0..7 are 0, 0.5, 1, 1.5, 2, 3, 4, 6, 8..15 the
  * same negated; scale 255 makes the block NaN; what
- * lies beyond 32 bits' range (scales 253 and 254 have such codes; no quantised number has them) counts as infinite.  Elements past `cols` in the last block are zero codes.
+ * lies beyond 32 bits' range (scales 253 and 254 have such codes; no quantised number has them) counts as infinite, and a sum with
+ * one may be NaN in place of an infinity (rows are multiplied in parts, some of them zero).  Elements past `cols` in the last block are zero codes.
  *
  * tetris_mx4_quantize: the scale of a block is 2^(floor(log2 a) - 2), a its largest magnitude, and at least 2^-127; an
  * element goes to the nearest value, to the even code where two are as near, and to 6 beyond 6; a block that holds an
@@ -96,7 +97,7 @@ int tetris_route_backward(const tetris_router* r, const void* d_logits, int type
  * The experts' products: y[t] = sum over j of d_weight[t][j] * down_e(silu(gate_e x[t]) * up_e x[t]), e = d_index[t][j].
  * `up` is gated, experts x 2 hidden x width; `down` experts x width x hidden.  Entries of d_index outside the experts
  * add nothing (a token of nothing but such entries gets zeros).  Sums are of 32 bits and in the order of j; between the
- * products numbers are held in `type`'s precision or better.  Workspace: up's, as for tetris_mx4_linear;
+ * products numbers are held in `type`'s precision or better; of TETRIS_F16, those beyond its range may become infinities.  Workspace: up's, as for tetris_mx4_linear;
  * tetris_experts_prepare makes it ahead.
  * ---------------------------------------------------------------------------------------------- */
 int tetris_experts_prepare(tetris_mx4* up, tetris_mx4* down, int tokens, int top, int type, void* stream);

@@ -57,9 +57,11 @@ def product(x, w, kind, bias=None):
     return y, sums, sums + ROUNDING[kind] * (np.abs(y) + sums) + LEAST[kind]
 
 
-def experts(x, up, down, index, weight, kind):
-    """The experts' products and their bound; up [E, 2F, D], down [E, D, F]."""
+def experts(x, up, down, index, weight, kind, between=None):
+    """The experts' products and their bound; up [E, 2F, D], down [E, D, F].  between: how far (relative, absolute) the numbers between the products
+    may be off, if not by the rounding to `kind`."""
     f = down.shape[2]
+    rel, least = between or (ROUNDING[kind], LEAST[kind])
     y, far = np.zeros((x.shape[0], down.shape[1])), np.zeros((x.shape[0], down.shape[1]))
     with np.errstate(over="ignore"):
         for e in range(up.shape[0]):
@@ -72,7 +74,7 @@ def experts(x, up, down, index, weight, kind):
             eg = 1.1 * eg + np.abs(act) * (2.0 ** -21 + 2.0 ** -23 * np.abs(gate))  # silu's slope is below 1.1; exp of a rounded argument
             h = act * more
             eh = eg * np.abs(more) + np.abs(act) * eu + eg * eu
-            eh = eh + (ROUNDING[kind] + 2.0 ** -23) * (np.abs(h) + eh) + LEAST[kind]
+            eh = eh + (rel + 2.0 ** -23) * (np.abs(h) + eh) + least
             z, sums, _ = product(h, down[e], "f32")
             ez = sums + eh @ np.abs(down[e]).T * 1.01
             w = weight[t, j][:, None]

@@ -281,15 +281,15 @@ def test_codes_past_the_last_column_count_for_nothing():
 # ---- experts ----
 
 
-def expert_case(rng, tokens, count, top, width, hidden, kind, pick=None):
+def expert_case(rng, tokens, count, top, width, hidden, kind, pick=None, size=1.0, share=1.0, between=None):
     up = random_weights(rng, count * 2 * hidden, width)
     down = random_weights(rng, count * width, hidden)
-    x = rounded_to(rng.normal(size=(tokens, width)) * width ** -0.5 / 3, kind)
+    x = rounded_to(rng.normal(size=(tokens, width)) * width ** -0.5 / 3 * size, kind)
     index = np.stack([rng.permutation(count)[:top] for _ in range(tokens)]) if pick is None else pick
-    weight = rng.uniform(0.1, 1.0, (tokens, top)).astype(np.float32)
+    weight = (rng.uniform(0.1, 1.0, (tokens, top)) * share).astype(np.float32)
     layer = T.ExpertLayer(T.MX4Weights(up[0].data_ptr(), up[1].data_ptr(), 2 * hidden, width, experts=count, gated=True),
                           T.MX4Weights(down[0].data_ptr(), down[1].data_ptr(), width, hidden, experts=count))
-    want, far = P.experts(x, up[2].reshape(count, 2 * hidden, width), down[2].reshape(count, width, hidden), index, weight.astype(np.float64), kind)
+    want, far = P.experts(x, up[2].reshape(count, 2 * hidden, width), down[2].reshape(count, width, hidden), index, weight.astype(np.float64), kind, between)
     return layer, x, index, weight, want, far
 
 
@@ -336,6 +336,44 @@ def test_experts_that_are_none(tokens):
     got = run_experts(layer, x, index, weight, "bf16")
     within(got, want, far)
     assert (got[:2] == 0).all()
+
+
+# Two truncated bf16 parts: the second has 8 of the bits that the first, of 8, leaves.
+PAIR = 2.0 ** -14, 2.0 ** -125
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("tokens,count,top,width,hidden", [(1, 1, 1, 64, 8), (1, 16, 5, 130, 64), (9, 3, 1, 64, 40), (64, 2, 1, 72, 200), (21, 3, 3, 48, 130), (8, 64, 8, 256, 31), (1, 64, 64, 40, 24)])
+def test_few_slots_keep_more_than_their_type_between_the_products(kind, tokens, count, top, width, hidden):
+    rng = np.random.default_rng(tokens + 5 * hidden)
+    layer, x, index, weight, want, far = expert_case(rng, tokens, count, top, width, hidden, kind, between=PAIR)
+    within(run_experts(layer, x, index, weight, kind), want, far)
+    within(run_experts(layer, x, index, weight, kind, width + 3, 1), want, far)
+
+
+def test_few_slots_of_f16_go_beyond_its_range_between_the_products():
+    rng = np.random.default_rng(23)
+    layer, x, index, weight, want, far = expert_case(rng, 6, 4, 2, 96, 64, "f16", size=4000.0, share=1e-7, between=PAIR)
+    assert 1.0 < np.abs(want).max() < 60000.0
+    within(run_experts(layer, x, index, weight, "f16"), want, far)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_experts_workspace_made_for_more_slots_than_are_few(kind):
+    rng = np.random.default_rng(12)
+    layer, x, index, weight, want, far = expert_case(rng, 66, 3, 1, 64, 256, kind)
+    s = torch.cuda.Stream()
+    layer.prepare(66, 1, TYPES[kind][0], stream=s.cuda_stream)
+    for tokens in (66, 65, 64, 63):
+        dx, y = on_gpu(x[:tokens], kind), torch.zeros(tokens, 64, dtype=TYPES[kind][1], device="cuda")
+        di, dw = torch.from_numpy(index[:tokens].astype(np.int32)).cuda(), torch.from_numpy(weight[:tokens]).cuda()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):  # a workspace that had to grow would be refused
+            layer.run(dx.data_ptr(), di.data_ptr(), dw.data_ptr(), y.data_ptr(), tokens, 1, TYPES[kind][0], stream=s.cuda_stream)
+        graph.replay()
+        torch.cuda.synchronize()
+        within(numbers(y), want[:tokens], far[:tokens])
 
 
 def test_experts_keep_tokens_apart():

@@ -728,9 +728,17 @@ __global__ __launch_bounds__(1024) void stream_kernel(Product a) {
 // The second product of the experts for up to 64 slots in all, and the weighted sum of each token's.  A workgroup has 16 features and goes
 // through every expert that is named; its waves share (expert, stretch of columns) pairs evenly, in runs of neighbouring ones.  A wave's sums for one
 // expert are kept at place (number of the expert + number of the wave): along the runs each step raises one of the two, so
-// no two share a place.  Bound by latency: the slots, then weights, then the sums; 10.8 us for four tokens of 4 of 64 experts of 1024 x 2048 (8.3 MB).  Each output is then added up by one thread, slots in their order, waves in theirs.
-template <int TYPE, int OUT>
+// no two share a place.  Bound by latency: the slots, then weights, then the sums; 10.9 us for four tokens of 4 of 64 experts of 1024 x 2048
+// (8.3 MB).  Each output is then added up by one thread, slots in their order, waves in theirs.
+//
+// Rows of an operator of 16 bits come as two bf16 parts, in two arrays: eight slots' leading parts are columns 0 to 7 of the products, what they leave is
+// columns 8 to 15, as few experts have more than eight of 64 slots.  So the numbers between the two products are off by 2^-14 at most, at the price of one
+// part (19.8 us for both products above; 19.4 with one, rounded to bf16; 22.4 with two parts in a lane, 28.0 with 32 bits split here).  With them rounded
+// to bf16, one token of 5 experts of 64 numbers each was off by 0.0026; 0.0017 is the rounding of the output itself.
+template <int OUT>
 __global__ __launch_bounds__(1024) void down_kernel(Product a, const float* __restrict__ weight, int top) {
+  constexpr int TYPE = OUT == kOutF32 ? TETRIS_F32 : TETRIS_BF16;
+  constexpr int kSlots = OUT == kOutF32 ? 16 : 8;  // in a tile
   using T = typename Elem<TYPE>::type;
   extern __shared__ float sums[];  // [places][4][64]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
@@ -738,7 +746,7 @@ __global__ __launch_bounds__(1024) void down_kernel(Product a, const float* __re
   const int mine = lane < a.rows ? a.index[lane] : -1;
   const bool named = mine >= 0 && mine < a.experts;
   const float my_weight = lane < a.rows ? weight[lane] : 0.f;
-  // tiles of up to sixteen slots of one expert; a lane knows its slot's tile and place in it
+  // tiles of up to kSlots slots of one expert; a lane knows its slot's tile and place in it
   int tiles = 0, my_tile = -1, my_column = 0;
   unsigned long long left = __ballot(named);
   int expert_of = 0;  // lane t: the expert of tile t
@@ -747,9 +755,9 @@ __global__ __launch_bounds__(1024) void down_kernel(Product a, const float* __re
     const unsigned long long same = __ballot(named && mine == e);
     left &= ~same;
     const int rank = __builtin_popcountll(same & ((1ull << lane) - 1)), all = __builtin_popcountll(same);
-    if (named && mine == e) my_tile = tiles + (rank >> 4), my_column = rank & 15;
-    if (lane >= tiles && lane < tiles + (all + 15) / 16) expert_of = e;
-    tiles += (all + 15) / 16;
+    if (named && mine == e) my_tile = tiles + rank / kSlots, my_column = rank % kSlots;
+    if (lane >= tiles && lane < tiles + (all + kSlots - 1) / kSlots) expert_of = e;
+    tiles += (all + kSlots - 1) / kSlots;
   }
   const int chunks = a.col_tiles >> 1, items = tiles * chunks, each = (items + waves - 1) / waves;
   const int begin = min(wave * each, items), end = min(begin + each, items);
@@ -758,15 +766,15 @@ __global__ __launch_bounds__(1024) void down_kernel(Product a, const float* __re
     const int expert = __builtin_amdgcn_readlane(expert_of, tile);
     const unsigned long long in = __ballot(my_tile == tile);
     const int count = __builtin_popcountll(in);
-    // lane with column q of the tile -> every lane with r16 == q
+    // lane with column q of the tile -> every lane with r16 % kSlots == q
     const int slot = __builtin_amdgcn_ds_permute((my_tile == tile ? my_column : 63) * 4, lane);
-    const int row = __shfl(slot, min(r16, count - 1));
-    const T* from = static_cast<const T*>(a.x) + (int64_t)row * a.ldx + 32 * g;
+    const int row = __shfl(slot, min(r16 % kSlots, count - 1));
+    const T* from = static_cast<const T*>(a.x) + (r16 / kSlots) * a.part + (int64_t)row * a.ldx + 32 * g;
     const i32x4* codes[1];
     const uint8_t* scales[1];
     half_of(a, expert, block, lane, &codes[0], &scales[0]);
     f32x4 acc[1] = {f32x4{0.f, 0.f, 0.f, 0.f}};
-    stretches<TYPE, 1, 2>(from, r16 < count, codes, scales, c0, 1, c1, 32 * g, a.k8, acc);
+    stretches<TYPE, 1, 2>(from, r16 % kSlots < count, codes, scales, c0, 1, c1, 32 * g, a.k8, acc);
 #pragma unroll
     for (int i = 0; i < 4; ++i) sums[((tile + wave) * 4 + i) * 64 + lane] = acc[0][i];
     at += c1 - c0;
@@ -783,7 +791,8 @@ __global__ __launch_bounds__(1024) void down_kernel(Product a, const float* __re
       if (token >= tokens || tile < 0) continue;
       float v = 0.f;
       for (int w = tile * chunks / each; w <= ((tile + 1) * chunks - 1) / each; ++w)
-        v += sums[((tile + w) * 4 + (f & 3)) * 64 + (f >> 2) * 16 + column];
+#pragma unroll
+        for (int p = 0; p < 16; p += kSlots) v += sums[((tile + w) * 4 + (f & 3)) * 64 + (f >> 2) * 16 + p + column];
       y = fmaf(by, v, y);
     }
     if (token < tokens && feature < a.n) store1<OUT>(a, (int64_t)token * a.ldy + feature, y);
@@ -922,10 +931,10 @@ int stream_rows(Product& a, hipStream_t stream) {
 template <int TYPE>
 int launch_down(Product& a, const float* weight, int top, hipStream_t stream) {
   const int waves = 16;
-  const size_t lds = (size_t)(std::min(a.rows, a.rows / 16 + a.experts) + waves) * 1024;  // at most 80 KiB
-  static const hipError_t room = hipFuncSetAttribute(reinterpret_cast<const void*>(down_kernel<TYPE, TYPE>), hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
+  const size_t lds = (size_t)(std::min(a.rows, a.rows / (TYPE == TETRIS_F32 ? 16 : 8) + a.experts) + waves) * 1024;  // at most 80 KiB
+  static const hipError_t room = hipFuncSetAttribute(reinterpret_cast<const void*>(down_kernel<TYPE>), hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
   TETRIS_HIP(room);
-  hipLaunchKernelGGL((down_kernel<TYPE, TYPE>), dim3(ceil_div(a.n, 16)), dim3(64 * waves), lds, stream, a, weight, top);
+  hipLaunchKernelGGL((down_kernel<TYPE>), dim3(ceil_div(a.n, 16)), dim3(64 * waves), lds, stream, a, weight, top);
   TETRIS_HIP(hipGetLastError());
   return TETRIS_OK;
 }
@@ -1000,6 +1009,7 @@ int workspace(tetris_mx4* w, hipStream_t stream, size_t need, uint8_t** out) {
   }
 }
 
+constexpr int kFewSlots = 64;      // the experts' slots that down_kernel takes, a lane each
 constexpr int kStreamMost = 1024;  // more rows are not streamed, whatever the matrix
 
 // Whether a product's rows are streamed.  Decided by its sizes alone, so that a workspace can be made ahead.
@@ -1012,7 +1022,7 @@ bool streams(const tetris_mx4* w, int rows) {
 // The experts': of the first product, for both; up to 64 slots always are.
 bool streams_slots(const tetris_mx4* up, int tokens, int top) {
   const int64_t slots = (int64_t)tokens * top;
-  if (slots <= 64) return true;
+  if (slots <= kFewSlots) return true;
   if (slots > kStreamMost) return false;
   Product a{};
   a.rows = (int)slots;
@@ -1077,6 +1087,8 @@ int launch_product(Product& a, Role role, int as, int type, bool stream, hipStre
   if (stream) {
     if (as == TETRIS_F32)
       return role == kUp ? stream_rows<TETRIS_F32, kOutF32, true>(a, s) : stream_rows<TETRIS_F32, kOutF32, false>(a, s);
+    if (role == kUp && a.index && type != TETRIS_F32)
+      return as == TETRIS_F16 ? stream_rows<TETRIS_F16, kOutParts2, true>(a, s) : stream_rows<TETRIS_BF16, kOutParts2, true>(a, s);
     if (as == TETRIS_F16)
       return role == kUp     ? stream_rows<TETRIS_F16, kOutF16, true>(a, s)
              : role == kDown ? stream_rows<TETRIS_F16, kOutF32, false>(a, s)
@@ -1185,11 +1197,12 @@ struct ExpertSpace {
 ExpertSpace expert_space(const tetris_mx4* up, const tetris_mx4* down, int tokens, int top, int type, bool stream) {
   const size_t slots = (size_t)tokens * top;
   const bool half = in_half(type, up) && in_half(type, down);
+  const int between = slots <= kFewSlots ? 4 : stream || half ? elem_size(type) : 2 * parts_of(type);
   ExpertSpace e;
   e.offsets = 0;
   e.order = up256(e.offsets + 4 * ((size_t)up->experts + 1));
   e.hidden = up256(e.order + 4 * slots);
-  e.rows = up256(e.hidden + slots * round_up(down->k, kMxPad) * (stream || half ? elem_size(type) : 2 * parts_of(type)));
+  e.rows = up256(e.hidden + slots * round_up(down->k, kMxPad) * between);
   e.ready = up256(e.rows + slots * round_up(down->n, 4) * 4);
   e.all = e.ready + staged_bytes(tokens, up->k, type, false, stream, half);
   return e;
@@ -1224,8 +1237,10 @@ extern "C" int tetris_experts_prepare(tetris_mx4* up, tetris_mx4* down, int toke
   const int rc = experts_check(up, down, tokens, top, type);
   if (rc || tokens == 0) return rc;
   uint8_t* d;
-  const int once = tokens_at_once(up, down, tokens, top, type, up->k);
-  return workspace(up, static_cast<hipStream_t>(stream), expert_space(up, down, once, top, type, streams_slots(up, once, top)).all, &d);
+  const int once = tokens_at_once(up, down, tokens, top, type, up->k), few = std::min(once, kFewSlots / top);
+  size_t need = expert_space(up, down, once, top, type, streams_slots(up, once, top)).all;
+  if (few) need = std::max(need, expert_space(up, down, few, top, type, true).all);  // a few tokens' numbers between the products take more
+  return workspace(up, static_cast<hipStream_t>(stream), need, &d);
 }
 
 namespace {
@@ -1241,7 +1256,7 @@ int expert_tokens(tetris_mx4* up, tetris_mx4* down, const void* d_x, int type, i
   if ((rc = workspace(up, s, e.all, &d))) return rc;
   int* offsets = reinterpret_cast<int*>(d + e.offsets);
   int* order = reinterpret_cast<int*>(d + e.order);
-  const bool few = slots <= 64;  // no sorting, two launches
+  const bool few = slots <= kFewSlots;  // no sorting, two launches
   if (!few) {
     const int threads = std::min(1024, (int)round_up(slots, 64));
     hipLaunchKernelGGL(plan_kernel, dim3(up->experts), dim3(threads), 0, s, d_index, slots, up->experts, offsets, order);
@@ -1263,7 +1278,7 @@ int expert_tokens(tetris_mx4* up, tetris_mx4* down, const void* d_x, int type, i
   a.from_div = top;
   a.y = d + e.hidden;
   a.ldy = round_up(down->k, kMxPad);
-  a.y_part = slots * a.ldy;
+  a.y_part = (int64_t)slots * a.ldy;
   if ((rc = launch_product(a, kUp, as, type, stream_it, s))) return rc;
 
   Product b{};
