@@ -728,12 +728,12 @@ __global__ __launch_bounds__(1024) void stream_kernel(Product a) {
 // The second product of the experts for up to 64 slots in all, and the weighted sum of each token's.  A workgroup has 16 features and goes
 // through every expert that is named; its waves share (expert, stretch of columns) pairs evenly, in runs of neighbouring ones.  A wave's sums for one
 // expert are kept at place (number of the expert + number of the wave): along the runs each step raises one of the two, so
-// no two share a place.  Bound by latency: the slots, then weights, then the sums; 10.9 us for four tokens of 4 of 64 experts of 1024 x 2048
+// no two share a place.  Bound by latency: the slots, then weights, then the sums; 10.0 us for four tokens of 4 of 64 experts of 1024 x 2048
 // (8.3 MB).  Each output is then added up by one thread, slots in their order, waves in theirs.
 //
 // Rows of an operator of 16 bits come as two bf16 parts, in two arrays: eight slots' leading parts are columns 0 to 7 of the products, what they leave is
 // columns 8 to 15, as few experts have more than eight of 64 slots.  So the numbers between the two products are off by 2^-14 at most, at the price of one
-// part (19.8 us for both products above; 19.4 with one, rounded to bf16; 22.4 with two parts in a lane, 28.0 with 32 bits split here).  With them rounded
+// part (for both products, before slots were found by bits, 19.8 us; 19.4 with one, rounded to bf16; 22.4 with two parts in a lane, 28.0 with 32 bits split here).  With them rounded
 // to bf16, one token of 5 experts of 64 numbers each was off by 0.0026; 0.0017 is the rounding of the output itself.
 template <int OUT>
 __global__ __launch_bounds__(1024) void down_kernel(Product a, const float* __restrict__ weight, int top) {
@@ -746,19 +746,24 @@ __global__ __launch_bounds__(1024) void down_kernel(Product a, const float* __re
   const int mine = lane < a.rows ? a.index[lane] : -1;
   const bool named = mine >= 0 && mine < a.experts;
   const float my_weight = lane < a.rows ? weight[lane] : 0.f;
-  // tiles of up to kSlots slots of one expert; a lane knows its slot's tile and place in it
-  int tiles = 0, my_tile = -1, my_column = 0;
-  unsigned long long left = __ballot(named);
-  int expert_of = 0;  // lane t: the expert of tile t
-  while (left) {
-    const int e = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
-    const unsigned long long same = __ballot(named && mine == e);
-    left &= ~same;
-    const int rank = __builtin_popcountll(same & ((1ull << lane) - 1)), all = __builtin_popcountll(same);
-    if (named && mine == e) my_tile = tiles + rank / kSlots, my_column = rank % kSlots;
-    if (lane >= tiles && lane < tiles + (all + kSlots - 1) / kSlots) expert_of = e;
-    tiles += (all + kSlots - 1) / kSlots;
+  // Tiles of up to kSlots slots of one expert, numbered by their first slots; a lane knows its slot's tile and place in it.  Which slots name the same expert
+  // is found a bit of its number at a time (a loop over the experts named took 1.1 us more of sixteen slots of as many experts).
+  unsigned long long same = __ballot(named);
+  for (int bit = 0; (1 << bit) < a.experts; ++bit) {
+    const bool set = mine >> bit & 1;
+    const unsigned long long those = __ballot(set);
+    same &= set ? those : ~those;
   }
+  const int rank = __builtin_popcountll(same & ((1ull << lane) - 1)), my_column = rank % kSlots;
+  const unsigned long long starts = __ballot(named && my_column == 0);
+  const int tiles = __builtin_popcountll(starts);
+  const int number = __builtin_popcountll(starts & ((1ull << lane) - 1));  // of the tile that starts here
+  unsigned long long from_mine = same;
+  for (int i = rank - my_column; i > 0; --i) from_mine &= from_mine - 1;
+  const int its = __shfl(number, __builtin_ctzll(from_mine | 1ull << 63));
+  const int my_tile = named ? its : -1;
+  // lane t: the expert of tile t (lane 63 takes what starts no tile, unless every lane starts one)
+  const int expert_of = __builtin_amdgcn_ds_permute((named && my_column == 0 ? number : 63) * 4, mine);
   const int chunks = a.col_tiles >> 1, items = tiles * chunks, each = (items + waves - 1) / waves;
   const int begin = min(wave * each, items), end = min(begin + each, items);
   for (int at = begin; at < end;) {
