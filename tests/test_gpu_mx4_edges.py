@@ -1,0 +1,54 @@
+"""The operators on MX4 weights (include/tetris_mx4.h) at the edges of what they accept, against their definitions in 64 bits
+(tests/mx4_plain.py)."""
+import numpy as np
+import pytest
+
+import mx4_plain as P
+
+T = pytest.importorskip("tetris_amd")
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from test_gpu_mx4 import PAIR, TYPES, numbers, on_gpu, rounded_to, within  # noqa: E402
+
+
+def weights(rng, rows, cols, least=124, most=130):
+    """MX4 rows with scales of `least` to `most`: (codes on the GPU, scales on the GPU, float64 values)."""
+    blocks = -(-cols // 32)
+    code = rng.integers(0, 16, (rows, blocks, 32), dtype=np.uint8)
+    code.reshape(rows, -1)[:, cols:] = 0
+    scales = rng.integers(least, most + 1, (rows, blocks), dtype=np.uint8)
+    return torch.from_numpy(P.packed(code)).cuda(), torch.from_numpy(scales).cuda(), P.values(code, scales, cols)
+
+
+@pytest.mark.parametrize("kind,top", [("f32", 700), ("f32", 1024), ("f16", 1024), ("bf16", 1024)])
+def test_one_token_of_more_slots_than_32_bit_offsets_reach(kind, top):
+    """Between the products the numbers' parts of one such token take more than 2 GiB.  All but 200 of the hidden numbers are zero, which keeps the bound narrow."""
+    rng = np.random.default_rng(top)
+    width, hidden = 8, 1 << 20
+    live = np.sort(rng.permutation(hidden)[:200])
+    live[-1] = hidden - 1
+    few_codes, few_scales, few_up = weights(rng, 400, width, 90, 130)  # not exact in f16
+    at = torch.from_numpy(np.concatenate([live, hidden + live])).cuda()
+    codes = torch.zeros(2 * hidden, 16, dtype=torch.uint8, device="cuda")
+    scales = torch.full((2 * hidden, 1), 127, dtype=torch.uint8, device="cuda")
+    codes[at], scales[at] = few_codes, few_scales
+    down_codes, down_scales, down = weights(rng, width, hidden)
+    layer = T.ExpertLayer(T.MX4Weights(codes.data_ptr(), scales.data_ptr(), 2 * hidden, width, gated=True),
+                          T.MX4Weights(down_codes.data_ptr(), down_scales.data_ptr(), width, hidden))
+    x = rounded_to(rng.normal(size=(1, width)), kind)
+    index = np.zeros((1, top), np.int32)
+    index[0, 5::7] = -1
+    weight = (rng.uniform(0.1, 1.0, (1, top)) * 1e-3).astype(np.float32)
+    dx, di, dw = on_gpu(x, kind), torch.from_numpy(index).cuda(), torch.from_numpy(weight).cuda()
+    y = torch.full((1, width), float("nan"), dtype=TYPES[kind][1], device="cuda")
+    print("one token,", kind, top, flush=True)
+    layer.run(dx.data_ptr(), di.data_ptr(), dw.data_ptr(), y.data_ptr(), 1, top, TYPES[kind][0])
+    torch.cuda.synchronize()
+    # every slot names the one expert: its outputs times the sum of the weights
+    between = PAIR if kind == "f16" else (P.ROUNDING[kind], P.LEAST[kind])
+    one, off = P.experts(x, few_up[None], down[None][:, :, live], np.zeros((1, 1), int), np.ones((1, 1)), "f32", between)
+    total = weight[index == 0].astype(np.float64).sum()
+    want = total * one
+    far = total * (off + 2.0 ** -22 * top * np.abs(one))
+    within(numbers(y), want, far + P.ROUNDING[kind] * (np.abs(want) + far) + P.LEAST[kind])

@@ -1228,12 +1228,17 @@ int experts_check(const tetris_mx4* up, const tetris_mx4* down, int tokens, int 
 
 namespace {
 
-// tokens that one pass takes: their rows, and those between the products, lie within a kernel's reach
+// slots whose numbers between the products, all parts of them, lie within a kernel's reach; 341 at least
+int64_t slots_at_once(const tetris_mx4* up, const tetris_mx4* down, int type) {
+  const bool half = in_half(type, up) && in_half(type, down);
+  return kMxReach / (round_up(down->k, kMxPad) * (half ? 2 : 2 * parts_of(type)));
+}
+
+// tokens that one pass takes: their rows, and those between the products, lie within a kernel's reach (unless one token has too many)
 int tokens_at_once(const tetris_mx4* up, const tetris_mx4* down, int tokens, int top, int type, int64_t ldx) {
   const bool half = in_half(type, up) && in_half(type, down);
-  const int64_t bytes = half ? 2 : 2 * parts_of(type);
-  const int64_t most = std::max({std::min<int64_t>(ldx, kMxSide) * elem_size(type), round_up(up->k, kMxPad) * bytes, top * round_up(down->k, kMxPad) * bytes});
-  return (int)std::min<int64_t>(tokens, std::max<int64_t>(1, kMxReach / most));
+  const int64_t row = std::max<int64_t>(std::min<int64_t>(ldx, kMxSide) * elem_size(type), round_up(up->k, kMxPad) * (half ? 2 : 2 * parts_of(type)));
+  return (int)std::min<int64_t>(tokens, std::max<int64_t>(1, std::min(kMxReach / row, slots_at_once(up, down, type) / top)));
 }
 
 }  // namespace
@@ -1250,35 +1255,25 @@ extern "C" int tetris_experts_prepare(tetris_mx4* up, tetris_mx4* down, int toke
 
 namespace {
 
-int expert_tokens(tetris_mx4* up, tetris_mx4* down, const void* d_x, int type, int tokens, int64_t ldx, int top, const int32_t* d_index,
-                  const float* d_weight, void* d_y, int64_t ldy, hipStream_t s) {
+// Both products of the slots of `tokens` rows, sorted by expert first: slot i's numbers of 32 bits to row i of `out`.
+int expert_products(tetris_mx4* up, tetris_mx4* down, const void* d_x, int type, int tokens, int64_t ldx, int top, const int32_t* d_index,
+                    bool stream_it, const ExpertSpace& e, uint8_t* d, float* out, int64_t ld_out, hipStream_t s) {
   int rc;
   const int slots = tokens * top;
-  const bool stream_it = streams_slots(up, tokens, top);
   const bool half = in_half(type, up) && in_half(type, down);
-  const ExpertSpace e = expert_space(up, down, tokens, top, type, stream_it);
-  uint8_t* d;
-  if ((rc = workspace(up, s, e.all, &d))) return rc;
   int* offsets = reinterpret_cast<int*>(d + e.offsets);
   int* order = reinterpret_cast<int*>(d + e.order);
-  const bool few = slots <= kFewSlots;  // no sorting, two launches
-  if (!few) {
-    const int threads = std::min(1024, (int)round_up(slots, 64));
-    hipLaunchKernelGGL(plan_kernel, dim3(up->experts), dim3(threads), 0, s, d_index, slots, up->experts, offsets, order);
-    TETRIS_HIP(hipGetLastError());
-  }
+  const int threads = std::min(1024, (int)round_up(slots, 64));
+  hipLaunchKernelGGL(plan_kernel, dim3(up->experts), dim3(threads), 0, s, d_index, slots, up->experts, offsets, order);
+  TETRIS_HIP(hipGetLastError());
 
   Product a{};
   set_weights(&a, up);
   int as;
   if ((rc = ready_rows(&a, d_x, type, tokens, up->k, ldx, false, stream_it, half, d + e.ready, &as, s))) return rc;
   a.rows = slots;
-  if (few) {
-    a.index = d_index;
-  } else {
-    a.offsets = offsets;
-    a.order = order;
-  }
+  a.offsets = offsets;
+  a.order = order;
   a.experts = up->experts;
   a.from_div = top;
   a.y = d + e.hidden;
@@ -1295,33 +1290,79 @@ int expert_tokens(tetris_mx4* up, tetris_mx4* down, const void* d_x, int type, i
   b.k8 = (int)round_up(down->k, 8);
   b.rows = slots;
   b.experts = up->experts;
-  if (few) {
-    b.index = d_index;
-    b.y = d_y;
-    b.ldy = ldy;
-    return type == TETRIS_F32   ? launch_down<TETRIS_F32>(b, d_weight, top, s)
-           : type == TETRIS_F16 ? launch_down<TETRIS_F16>(b, d_weight, top, s)
-                                : launch_down<TETRIS_BF16>(b, d_weight, top, s);
-  }
   b.offsets = offsets;
   b.order = order;
   b.to_slot = 1;
-  b.y = d + e.rows;
-  b.ldy = round_up(down->n, 4);
+  b.y = out;
+  b.ldy = ld_out;
   b.vec_out = 1;
-  if ((rc = launch_product(b, kDown, stream_it || half ? type : (int)TETRIS_BF16, type, stream_it, s))) return rc;
+  return launch_product(b, kDown, stream_it || half ? type : (int)TETRIS_BF16, type, stream_it, s);
+}
+
+// The same for up to 64 slots: no sorting, two launches, the weighted sum in the second.
+int few_slots(tetris_mx4* up, tetris_mx4* down, const void* d_x, int type, int tokens, int64_t ldx, int top, const int32_t* d_index,
+              const float* d_weight, void* d_y, int64_t ldy, const ExpertSpace& e, uint8_t* d, hipStream_t s) {
+  int rc;
+  const int slots = tokens * top;
+  Product a{};
+  set_weights(&a, up);
+  int as;
+  if ((rc = ready_rows(&a, d_x, type, tokens, up->k, ldx, false, true, false, d + e.ready, &as, s))) return rc;
+  a.rows = slots;
+  a.index = d_index;
+  a.experts = up->experts;
+  a.from_div = top;
+  a.y = d + e.hidden;
+  a.ldy = round_up(down->k, kMxPad);
+  a.y_part = (int64_t)slots * a.ldy;
+  if ((rc = launch_product(a, kUp, as, type, true, s))) return rc;
+
+  Product b{};
+  set_weights(&b, down);
+  b.x = d + e.hidden;
+  b.ldx = a.ldy;
+  b.part = a.y_part;
+  b.parts = 1;
+  b.k8 = (int)round_up(down->k, 8);
+  b.rows = slots;
+  b.experts = up->experts;
+  b.index = d_index;
+  b.y = d_y;
+  b.ldy = ldy;
+  return type == TETRIS_F32   ? launch_down<TETRIS_F32>(b, d_weight, top, s)
+         : type == TETRIS_F16 ? launch_down<TETRIS_F16>(b, d_weight, top, s)
+                              : launch_down<TETRIS_BF16>(b, d_weight, top, s);
+}
+
+int expert_tokens(tetris_mx4* up, tetris_mx4* down, const void* d_x, int type, int tokens, int64_t ldx, int top, const int32_t* d_index,
+                  const float* d_weight, void* d_y, int64_t ldy, hipStream_t s) {
+  int rc;
+  const int slots = tokens * top;
+  const bool stream_it = streams_slots(up, tokens, top);
+  const ExpertSpace e = expert_space(up, down, tokens, top, type, stream_it);
+  uint8_t* d;
+  if ((rc = workspace(up, s, e.all, &d))) return rc;
+  if (slots <= kFewSlots) return few_slots(up, down, d_x, type, tokens, ldx, top, d_index, d_weight, d_y, ldy, e, d, s);
+
+  float* rows = reinterpret_cast<float*>(d + e.rows);
+  const int64_t ld_rows = round_up(down->n, 4);
+  // One token may still have more slots than tile_kernel's 32-bit offsets reach between the products: they are taken in several passes.
+  const int each = tokens == 1 && !stream_it ? (int)std::min<int64_t>(top, slots_at_once(up, down, type)) : top;
+  for (int from = 0; from < top; from += each) {
+    rc = expert_products(up, down, d_x, type, tokens, ldx, std::min(each, top - from), d_index + from, stream_it, e, d, rows + from * ld_rows, ld_rows, s);
+    if (rc) return rc;
+  }
 
   const int vec = ldy % 4 == 0 && (reinterpret_cast<size_t>(d_y) & (4 * elem_size(type) - 1)) == 0;
-  const float* rows = reinterpret_cast<const float*>(d + e.rows);
   const dim3 grid((unsigned)std::min<int64_t>(((int64_t)tokens * ceil_div(down->n, 4) + 255) / 256, 256 * 64));
   if (type == TETRIS_F32)
-    hipLaunchKernelGGL(combine_kernel<TETRIS_F32>, grid, dim3(256), 0, s, rows, b.ldy, d_index, d_weight, tokens, top, up->experts, down->n,
+    hipLaunchKernelGGL(combine_kernel<TETRIS_F32>, grid, dim3(256), 0, s, rows, ld_rows, d_index, d_weight, tokens, top, up->experts, down->n,
                        static_cast<float*>(d_y), ldy, vec);
   else if (type == TETRIS_F16)
-    hipLaunchKernelGGL(combine_kernel<TETRIS_F16>, grid, dim3(256), 0, s, rows, b.ldy, d_index, d_weight, tokens, top, up->experts, down->n,
+    hipLaunchKernelGGL(combine_kernel<TETRIS_F16>, grid, dim3(256), 0, s, rows, ld_rows, d_index, d_weight, tokens, top, up->experts, down->n,
                        static_cast<_Float16*>(d_y), ldy, vec);
   else
-    hipLaunchKernelGGL(combine_kernel<TETRIS_BF16>, grid, dim3(256), 0, s, rows, b.ldy, d_index, d_weight, tokens, top, up->experts, down->n,
+    hipLaunchKernelGGL(combine_kernel<TETRIS_BF16>, grid, dim3(256), 0, s, rows, ld_rows, d_index, d_weight, tokens, top, up->experts, down->n,
                        static_cast<__bf16*>(d_y), ldy, vec);
   TETRIS_HIP(hipGetLastError());
   return TETRIS_OK;
