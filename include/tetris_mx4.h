@@ -97,7 +97,7 @@ int tetris_route_backward(const tetris_router* r, const void* d_logits, int type
  * The experts' products: y[t] = sum over j of d_weight[t][j] * down_e(silu(gate_e x[t]) * up_e x[t]), e = d_index[t][j].
  * `up` is gated, experts x 2 hidden x width; `down` experts x width x hidden.  Entries of d_index outside the experts
  * add nothing (a token of nothing but such entries gets zeros).  Sums are of 32 bits and in the order of j; between the
- * products numbers are held in `type`'s precision or better; of TETRIS_F16, those beyond its range may become infinities.  Workspace: up's, as for tetris_mx4_linear;
+ * products numbers are held in `type`'s precision or better, with the range of 32 bits.  Workspace: up's, as for tetris_mx4_linear;
  * tetris_experts_prepare makes it ahead.
  * ---------------------------------------------------------------------------------------------- */
 int tetris_experts_prepare(tetris_mx4* up, tetris_mx4* down, int tokens, int top, int type, void* stream);

@@ -9,7 +9,7 @@ T = pytest.importorskip("tetris_amd")
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_mx4 import PAIR, TYPES, numbers, on_gpu, rounded_to, within  # noqa: E402
+from test_gpu_mx4 import PAIR, TYPES, expert_case, numbers, on_gpu, rounded_to, run_experts, within  # noqa: E402
 
 
 def weights(rng, rows, cols, least=124, most=130):
@@ -52,3 +52,13 @@ def test_one_token_of_more_slots_than_32_bit_offsets_reach(kind, top):
     want = total * one
     far = total * (off + 2.0 ** -22 * top * np.abs(one))
     within(numbers(y), want, far + P.ROUNDING[kind] * (np.abs(want) + far) + P.LEAST[kind])
+
+
+@pytest.mark.parametrize("tokens,count,top,width,hidden", [(40, 4, 2, 96, 64), (200, 4, 2, 128, 96), (600, 3, 2, 520, 64), (1200, 2, 2, 72, 1040), (3000, 2, 2, 72, 1040), (1200, 2, 2, 2100, 48)])
+def test_f16_goes_beyond_its_range_between_the_products(tokens, count, top, width, hidden):
+    """More slots than are few: streamed, and in tiles of 32, 64 and 128 rows."""
+    rng = np.random.default_rng(tokens + hidden)
+    layer, x, index, weight, want, far = expert_case(rng, tokens, count, top, width, hidden, "f16", size=4000.0, share=1e-8, between=PAIR)
+    assert 1.0 < np.abs(want).max() < 60000.0
+    within(run_experts(layer, x, index, weight, "f16"), want, far)
+    within(run_experts(layer, x, index, weight, "f16", width + 3, 1), want, far)

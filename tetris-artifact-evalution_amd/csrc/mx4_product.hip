@@ -1084,7 +1084,10 @@ int ready_rows(Product* a, const void* x, int type, int rows, int k, int64_t ld,
 }
 
 // Which of the three products it is: numbers of a type; the gated product of the experts, which writes what the next
-// reads; and that one, which writes numbers of 32 bits.
+// reads; and that one, which writes numbers of 32 bits.  Beyond 64 slots what lies between those two is, of f32, all of its 24 bits; of f16, whose range a product
+// of two sums may leave, two bf16 parts, or 32 bits where rows are streamed (in f16 200 tokens of 8 of 64 experts take 77 us instead of 84, 4096 of 4 of 16 322
+// instead of 405, but a number above 65504 there makes the output infinite or NaN); of bf16, which has the range, bf16: one rounding of 2^-9, where the output's is
+// one as well (in two parts 4096 tokens of 4 of 32 experts take 983 us instead of 777).
 enum Role { kLinear, kUp, kDown };
 
 // `as`: the type of the rows; `type`: that of the operator.
@@ -1095,9 +1098,7 @@ int launch_product(Product& a, Role role, int as, int type, bool stream, hipStre
     if (role == kUp && a.index && type != TETRIS_F32)
       return as == TETRIS_F16 ? stream_rows<TETRIS_F16, kOutParts2, true>(a, s) : stream_rows<TETRIS_BF16, kOutParts2, true>(a, s);
     if (as == TETRIS_F16)
-      return role == kUp     ? stream_rows<TETRIS_F16, kOutF16, true>(a, s)
-             : role == kDown ? stream_rows<TETRIS_F16, kOutF32, false>(a, s)
-                             : stream_rows<TETRIS_F16, kOutF16, false>(a, s);
+      return role == kUp ? stream_rows<TETRIS_F16, kOutF32, true>(a, s) : stream_rows<TETRIS_F16, kOutF16, false>(a, s);
     if (role == kUp) return stream_rows<TETRIS_BF16, kOutBF16, true>(a, s);
     if (role == kDown || type == TETRIS_F32) return stream_rows<TETRIS_BF16, kOutF32, false>(a, s);
     if (type == TETRIS_F16) return stream_rows<TETRIS_BF16, kOutF16, false>(a, s);
@@ -1109,10 +1110,7 @@ int launch_product(Product& a, Role role, int as, int type, bool stream, hipStre
     return launch_rounded<4, 2, 2, 4, kOutBF16>(a, s);
   }
   if (type == TETRIS_F32) return role == kUp ? tile_rows<kOutParts3, true, 3>(a, s) : tile_rows<kOutF32, false, 3>(a, s);
-  if (as == TETRIS_F16)
-    return role == kUp     ? tile_rows<kOutF16, true, 1, true>(a, s)
-           : role == kDown ? tile_rows<kOutF32, false, 1, true>(a, s)
-                           : tile_rows<kOutF16, false, 1, true>(a, s);
+  if (as == TETRIS_F16) return role == kUp ? tile_rows<kOutParts2, true, 1, true>(a, s) : tile_rows<kOutF16, false, 1, true>(a, s);
   if (type == TETRIS_F16)
     return role == kUp     ? tile_rows<kOutParts2, true, 2>(a, s)
            : role == kDown ? tile_rows<kOutF32, false, 2>(a, s)
@@ -1201,15 +1199,14 @@ struct ExpertSpace {
 
 ExpertSpace expert_space(const tetris_mx4* up, const tetris_mx4* down, int tokens, int top, int type, bool stream) {
   const size_t slots = (size_t)tokens * top;
-  const bool half = in_half(type, up) && in_half(type, down);
-  const int between = slots <= kFewSlots ? 4 : stream || half ? elem_size(type) : 2 * parts_of(type);
+  const int between = slots <= kFewSlots || (stream && type == TETRIS_F16) ? 4 : stream ? elem_size(type) : 2 * parts_of(type);
   ExpertSpace e;
   e.offsets = 0;
   e.order = up256(e.offsets + 4 * ((size_t)up->experts + 1));
   e.hidden = up256(e.order + 4 * slots);
   e.rows = up256(e.hidden + slots * round_up(down->k, kMxPad) * between);
   e.ready = up256(e.rows + slots * round_up(down->n, 4) * 4);
-  e.all = e.ready + staged_bytes(tokens, up->k, type, false, stream, half);
+  e.all = e.ready + staged_bytes(tokens, up->k, type, false, stream, in_half(type, up));
   return e;
 }
 
@@ -1229,16 +1226,13 @@ int experts_check(const tetris_mx4* up, const tetris_mx4* down, int tokens, int 
 namespace {
 
 // slots whose numbers between the products, all parts of them, lie within a kernel's reach; 341 at least
-int64_t slots_at_once(const tetris_mx4* up, const tetris_mx4* down, int type) {
-  const bool half = in_half(type, up) && in_half(type, down);
-  return kMxReach / (round_up(down->k, kMxPad) * (half ? 2 : 2 * parts_of(type)));
-}
+int64_t slots_at_once(const tetris_mx4* down, int type) { return kMxReach / (round_up(down->k, kMxPad) * 2 * parts_of(type)); }
 
 // tokens that one pass takes: their rows, and those between the products, lie within a kernel's reach (unless one token has too many)
 int tokens_at_once(const tetris_mx4* up, const tetris_mx4* down, int tokens, int top, int type, int64_t ldx) {
-  const bool half = in_half(type, up) && in_half(type, down);
+  const bool half = in_half(type, up);
   const int64_t row = std::max<int64_t>(std::min<int64_t>(ldx, kMxSide) * elem_size(type), round_up(up->k, kMxPad) * (half ? 2 : 2 * parts_of(type)));
-  return (int)std::min<int64_t>(tokens, std::max<int64_t>(1, std::min(kMxReach / row, slots_at_once(up, down, type) / top)));
+  return (int)std::min<int64_t>(tokens, std::max<int64_t>(1, std::min(kMxReach / row, slots_at_once(down, type) / top)));
 }
 
 }  // namespace
@@ -1260,7 +1254,7 @@ int expert_products(tetris_mx4* up, tetris_mx4* down, const void* d_x, int type,
                     bool stream_it, const ExpertSpace& e, uint8_t* d, float* out, int64_t ld_out, hipStream_t s) {
   int rc;
   const int slots = tokens * top;
-  const bool half = in_half(type, up) && in_half(type, down);
+  const bool half = in_half(type, up);
   int* offsets = reinterpret_cast<int*>(d + e.offsets);
   int* order = reinterpret_cast<int*>(d + e.order);
   const int threads = std::min(1024, (int)round_up(slots, 64));
@@ -1286,7 +1280,7 @@ int expert_products(tetris_mx4* up, tetris_mx4* down, const void* d_x, int type,
   b.x = d + e.hidden;
   b.ldx = a.ldy;
   b.part = a.y_part;
-  b.parts = stream_it || half ? 1 : parts_of(type);
+  b.parts = stream_it ? 1 : parts_of(type);
   b.k8 = (int)round_up(down->k, 8);
   b.rows = slots;
   b.experts = up->experts;
@@ -1296,7 +1290,8 @@ int expert_products(tetris_mx4* up, tetris_mx4* down, const void* d_x, int type,
   b.y = out;
   b.ldy = ld_out;
   b.vec_out = 1;
-  return launch_product(b, kDown, stream_it || half ? type : (int)TETRIS_BF16, type, stream_it, s);
+  const int between = !stream_it ? TETRIS_BF16 : type == TETRIS_F16 ? TETRIS_F32 : type;
+  return launch_product(b, kDown, between, type, stream_it, s);
 }
 
 // The same for up to 64 slots: no sorting, two launches, the weighted sum in the second.
@@ -1347,7 +1342,7 @@ int expert_tokens(tetris_mx4* up, tetris_mx4* down, const void* d_x, int type, i
   float* rows = reinterpret_cast<float*>(d + e.rows);
   const int64_t ld_rows = round_up(down->n, 4);
   // One token may still have more slots than tile_kernel's 32-bit offsets reach between the products: they are taken in several passes.
-  const int each = tokens == 1 && !stream_it ? (int)std::min<int64_t>(top, slots_at_once(up, down, type)) : top;
+  const int each = tokens == 1 && !stream_it ? (int)std::min<int64_t>(top, slots_at_once(down, type)) : top;
   for (int from = 0; from < top; from += each) {
     rc = expert_products(up, down, d_x, type, tokens, ldx, std::min(each, top - from), d_index + from, stream_it, e, d, rows + from * ld_rows, ld_rows, s);
     if (rc) return rc;
