@@ -62,3 +62,38 @@ def test_f16_goes_beyond_its_range_between_the_products(tokens, count, top, widt
     assert 1.0 < np.abs(want).max() < 60000.0
     within(run_experts(layer, x, index, weight, "f16"), want, far)
     within(run_experts(layer, x, index, weight, "f16", width + 3, 1), want, far)
+
+
+def sigmoid_gradient(x, index, dweight, renorm, scale):
+    """The gradient of the weights carried to the logits, and the size of the numbers that it is a difference of; 1 - s from the logit."""
+    s, rest = 1 / (1 + np.exp(-x)), 1 / (1 + np.exp(x))
+    c, d = np.take_along_axis(s, index, 1), scale * dweight
+    share, size = s, np.abs(d).max(1, keepdims=True)
+    if renorm:
+        total = c.sum(1, keepdims=True)
+        d = d - (d * (c / total)).sum(1, keepdims=True)
+        share = s / total
+    full = np.zeros_like(s)
+    np.put_along_axis(full, index, d, 1)
+    return share * rest * full, share * rest * size
+
+
+def run_backward(x, kind, index, dweight, **how):
+    di, dd = torch.from_numpy(index.astype(np.int32)).cuda(), torch.from_numpy(dweight).cuda()
+    y = torch.full(x.shape, 99.0, dtype=TYPES[kind][1], device="cuda")
+    T.Router(x.shape[1], index.shape[1], **how).backward(on_gpu(x, kind).data_ptr(), TYPES[kind][0], x.shape[0], di.data_ptr(), dd.data_ptr(), y.data_ptr())
+    return numbers(y)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("renorm", [False, True])
+@pytest.mark.parametrize("least,most", [(8, 30), (-30, -8), (-30, 30)])
+def test_sigmoid_gradient_of_large_logits(kind, renorm, least, most):
+    rng = np.random.default_rng(most - least + renorm)
+    tokens, experts, top = 20, 70, 6
+    x = rounded_to(rng.uniform(least, most, (tokens, experts)), kind)
+    index, _ = P.route(x, top, True)
+    dweight = rng.normal(size=(tokens, top)).astype(np.float32)
+    got = run_backward(x, kind, index, dweight, score=T.SCORE_SIGMOID, renorm=renorm, scale=1.5)
+    want, size = sigmoid_gradient(x, index, dweight.astype(np.float64), renorm, 1.5)
+    within(got, want, size * (top + 32) * 2.0 ** -22 + P.ROUNDING[kind] * np.abs(want) + P.LEAST[kind])

@@ -299,7 +299,8 @@ __global__ __launch_bounds__(256) void route_backward_kernel(Route a, const int*
   auto* row = out + token * ld_out;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const float g = a.score == TETRIS_SCORE_SIGMOID ? s[v] * (1.f - s[v]) * d[v] : s[v] * (d[v] - all);
+    // (1 - s from the logit: from s, which is 1 to 32 bits beyond a logit of 17, nothing would be left)
+    const float g = a.score == TETRIS_SCORE_SIGMOID ? s[v] * (1.f / (1.f + expf(x[v]))) * d[v] : s[v] * (d[v] - all);
     if (lane * V + v < a.experts) row[lane * V + v] = (typename Elem<TYPE>::type)g;
   }
 }
