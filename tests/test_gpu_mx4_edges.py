@@ -97,3 +97,21 @@ def test_sigmoid_gradient_of_large_logits(kind, renorm, least, most):
     got = run_backward(x, kind, index, dweight, score=T.SCORE_SIGMOID, renorm=renorm, scale=1.5)
     want, size = sigmoid_gradient(x, index, dweight.astype(np.float64), renorm, 1.5)
     within(got, want, size * (top + 32) * 2.0 ** -22 + P.ROUNDING[kind] * np.abs(want) + P.LEAST[kind])
+
+
+@pytest.mark.parametrize("score,about", [("softmax", -86), ("sigmoid", -86), ("softmax", -95)])
+def test_gradient_of_weights_of_small_scores(score, about):
+    """Scores of some 1e-38 and 1e-41, of which the weights are quotients: the softmax's are chosen against the largest logit, as by a bias."""
+    rng = np.random.default_rng(87)
+    tokens, experts, top = 9, 70, 4
+    x = rounded_to(rng.uniform(about - 0.5, about, (tokens, experts)), "f32")
+    index = np.stack([1 + rng.permutation(experts - 1)[:top] for _ in range(tokens)])
+    dweight = (rng.normal(size=(tokens, top)) * 100).astype(np.float32)
+    if score == "softmax":
+        x[:, 0] = 0.0
+    got = run_backward(x, "f32", index, dweight, score=T.SCORE_SOFTMAX if score == "softmax" else T.SCORE_SIGMOID, scale=1.5)
+    # the sum of the exponentials is 1 to 32 bits, and so is the sigmoid's complement: one formula is good for both
+    want, size = sigmoid_gradient(x, index, dweight.astype(np.float64), True, 1.5)
+    step = 2.0 ** -149 / np.exp(about - 0.5)  # of the scores, relative; a score, the sum and the mean are each off by up to two
+    within(got[:, 1:], want[:, 1:], (size * ((top + 32) * 2.0 ** -22 + 8 * step) + P.LEAST["f32"])[:, 1:])
+    assert (got[:, 0] == 0).all()

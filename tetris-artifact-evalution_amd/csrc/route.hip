@@ -258,9 +258,9 @@ __global__ __launch_bounds__(256) void route_kernel(Route a, int* __restrict__ i
   }
 }
 
-// With s the scores, c the chosen, S the sum of theirs and d_j = scale dweight_j (renorm: (d_j - sum_l d_l s_l / S) / S):
-//   sigmoid  dlogit_i = s_i (1 - s_i) d_i for the chosen, else 0
-//   softmax  dlogit_i = s_i (d_i - sum_j s_j d_j), with d_i = 0 for those not chosen; with renorm that sum is zero
+// With s the scores, c the chosen, S the sum of theirs, p = s and d_j = scale dweight_j (renorm: p = s / S and d_j less sum_l d_l p_l):
+//   sigmoid  dlogit_i = p_i (1 - s_i) d_i for the chosen, else 0
+//   softmax  dlogit_i = p_i (d_i - sum_j s_j d_j), with d_i = 0 for those not chosen; with renorm that sum is zero
 // A wave a token.  8192 tokens of 128 experts in bf16: 6.2 us (4.7 MB); the launch and one wave's chain of instructions, not memory.
 template <int TYPE, int V>
 __global__ __launch_bounds__(256) void route_backward_kernel(Route a, const int* __restrict__ index, const float* __restrict__ dweight,
@@ -283,10 +283,11 @@ __global__ __launch_bounds__(256) void route_backward_kernel(Route a, const int*
     if (e < 0 || e >= a.experts) e = -1;
     if (e >= 0) dw = a.scale * dweight[(int64_t)token * a.top + lane], score = mine[e];
   }
+  float sum = 1.f;  // what scores are divided by: they, not d, so that nothing overflows where all of them are small
   if (a.renorm) {
-    const float sum = lanes_sum<64>(score);
-    const float mean = sum == 0.f ? 0.f : lanes_sum<64>(dw * score) / sum;
-    dw = sum == 0.f || e < 0 ? 0.f : (dw - mean) / sum;
+    sum = lanes_sum<64>(score);
+    const float mean = sum == 0.f ? 0.f : lanes_sum<64>(dw * (score / sum));
+    dw = sum == 0.f || e < 0 ? 0.f : dw - mean;
   }
   const float all = a.score == TETRIS_SCORE_SOFTMAX && !a.renorm ? lanes_sum<64>(dw * score) : 0.f;
   for (int j = 0; j < a.top; ++j) {
@@ -300,7 +301,9 @@ __global__ __launch_bounds__(256) void route_backward_kernel(Route a, const int*
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     // (1 - s from the logit: from s, which is 1 to 32 bits beyond a logit of 17, nothing would be left)
-    const float g = a.score == TETRIS_SCORE_SIGMOID ? s[v] * (1.f / (1.f + expf(x[v]))) * d[v] : s[v] * (d[v] - all);
+    // (those not chosen may be any times `sum`, but not infinitely: they are multiplied by zero)
+    const float share = sum == 0.f ? 0.f : a.renorm ? fminf(s[v], sum) / sum : s[v];
+    const float g = a.score == TETRIS_SCORE_SIGMOID ? share * (1.f / (1.f + expf(x[v]))) * d[v] : share * (d[v] - all);
     if (lane * V + v < a.experts) row[lane * V + v] = (typename Elem<TYPE>::type)g;
   }
 }
