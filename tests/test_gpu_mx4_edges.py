@@ -115,3 +115,23 @@ def test_gradient_of_weights_of_small_scores(score, about):
     step = 2.0 ** -149 / np.exp(about - 0.5)  # of the scores, relative; a score, the sum and the mean are each off by up to two
     within(got[:, 1:], want[:, 1:], (size * ((top + 32) * 2.0 ** -22 + 8 * step) + P.LEAST["f32"])[:, 1:])
     assert (got[:, 0] == 0).all()
+
+
+def test_workspace_that_grows_step_by_step_stays_bounded():
+    """Batches of one more row each time, as a server without prepare() sees them."""
+    rng = np.random.default_rng(4)
+    k, n, most = 8192, 32, 300
+    codes, scales, w = weights(rng, n, k)
+    W = T.MX4Weights(codes.data_ptr(), scales.data_ptr(), n, k)
+    x = rounded_to(rng.normal(size=(most, k)), "f32")
+    dx, y = on_gpu(x, "f32", k + 1, 1), torch.zeros(most, n, device="cuda")  # lies badly: is copied
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    for m in range(1, most + 1):
+        W.linear(dx.data_ptr(), y.data_ptr(), m, T.F32, ldx=k + 1)
+    torch.cuda.synchronize()
+    held = before - torch.cuda.mem_get_info()[0]
+    # the last buffer is below twice what 300 rows take (4 bytes a number), those kept are no more than it; whole pages of 2 MiB, a dozen buffers
+    assert held <= 4 * most * k * 4 + 16 * 2 ** 21
+    want, _, far = P.product(x, w, "f32")
+    within(numbers(y), want, far)

@@ -989,7 +989,7 @@ bool lies_well(const void* x, int64_t ld, int k, int type) {
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 // The workspace of (handle, stream), at least `need` bytes.  A buffer that has to grow is replaced and kept until the handle goes: a
-// captured graph may hold its address.
+// captured graph may hold its address.  It at least doubles, so that those kept are together no larger than the last one.
 int workspace(tetris_mx4* w, hipStream_t stream, size_t need, uint8_t** out) {
   *out = nullptr;
   if (!need) return TETRIS_OK;
@@ -1002,10 +1002,15 @@ int workspace(tetris_mx4* w, hipStream_t stream, size_t need, uint8_t** out) {
         return fail(TETRIS_EINVAL, "this launch would allocate its workspace: prepare it before capturing");
       w->retired.reserve(w->retired.size() + 1);
       void* d = nullptr;
-      TETRIS_HIP(hipMalloc(&d, need));
+      size_t bytes = std::max(need, 2 * s.bytes);
+      if (bytes > need && hipMalloc(&d, bytes) != hipSuccess) {
+        (void)hipGetLastError();  // no room for twice as much
+        d = nullptr;
+      }
+      if (!d) TETRIS_HIP(hipMalloc(&d, bytes = need));
       if (s.ptr) w->retired.push_back(s.ptr);
       s.ptr = d;
-      s.bytes = need;
+      s.bytes = bytes;
     }
     *out = static_cast<uint8_t*>(s.ptr);
     return TETRIS_OK;
