@@ -7,7 +7,9 @@
  * dimension (`ld`) is the distance of two rows in elements.  Rows and bases need no alignment beyond their element's;
  * rows that start on 16 bytes and widths that are multiples of eight are read without a copy.
  * Outputs may not overlap inputs.  A call with no rows does nothing and succeeds.  Launches of one handle on one stream come from one
- * thread at a time (they share that stream's workspace).
+ * thread at a time (they share that stream's workspace; hipStreamPerThread is a stream of each thread).  A graph keeps the workspace of the stream
+ * that its launches were captured on: on whatever stream it is replayed, it may not overlap other launches of the handle on that stream, nor
+ * other graphs that were captured there with the handle.
  */
 #ifndef TETRIS_MX4_H_
 #define TETRIS_MX4_H_

@@ -1,5 +1,7 @@
 """The operators on MX4 weights (include/tetris_mx4.h) at the edges of what they accept, against their definitions in 64 bits
 (tests/mx4_plain.py)."""
+import threading
+
 import numpy as np
 import pytest
 
@@ -135,3 +137,38 @@ def test_workspace_that_grows_step_by_step_stays_bounded():
     assert held <= 4 * most * k * 4 + 16 * 2 ** 21
     want, _, far = P.product(x, w, "f32")
     within(numbers(y), want, far)
+
+
+def test_threads_on_their_own_default_streams_have_their_own_workspaces():
+    """hipStreamPerThread is one value that names a stream of each thread."""
+    per_thread = 2  # its value, from the HIP headers
+    rng = np.random.default_rng(6)
+    k, n, m = 8192, 64, 1000
+    codes, scales, w = weights(rng, n, k)
+    W = T.MX4Weights(codes.data_ptr(), scales.data_ptr(), n, k)
+    xs = [rounded_to(rng.normal(size=(m, k)), "f32") for _ in range(2)]
+    dxs, ys = [on_gpu(x, "f32", k + 1, 1) for x in xs], [torch.zeros(m, n, device="cuda") for _ in xs]
+    torch.cuda.synchronize()
+    before, failures = torch.cuda.mem_get_info()[0], []
+    ready = threading.Barrier(len(xs))
+
+    def run(dx, y):
+        try:
+            W.prepare(m, T.F32, stream=per_thread)
+            ready.wait(30)
+            for _ in range(20):
+                W.linear(dx.data_ptr(), y.data_ptr(), m, T.F32, ldx=k + 1, stream=per_thread)
+            torch.cuda.synchronize()
+        except Exception as e:  # shown by the test's own thread
+            failures.append(e)
+
+    threads = [threading.Thread(target=run, args=a) for a in zip(dxs, ys)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
+    assert before - torch.cuda.mem_get_info()[0] >= 2 * m * k * 4
+    for x, y in zip(xs, ys):
+        want, _, far = P.product(x, w, "f32")
+        within(numbers(y), want, far)

@@ -55,7 +55,7 @@ struct tetris_mx4 {
   uint8_t* scales = nullptr;
   std::mutex mu;
   struct Space { void* ptr = nullptr; size_t bytes = 0; };
-  std::map<hipStream_t, Space> space;
+  std::map<std::pair<hipStream_t, uint64_t>, Space> space;  // the number: of the thread, for hipStreamPerThread, which is one value for many streams
   std::vector<void*> retired;  // replaced by larger ones; a captured graph may hold their addresses
 };
 

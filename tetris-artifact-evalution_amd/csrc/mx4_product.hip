@@ -5,6 +5,7 @@
 // significand in parts of 8), so every product is exact in every type.  Codes become bf16 pairs with one instruction a pair, which
 // also multiplies by the scale, in the registers of the wave that uses them: what comes from memory is 17 bytes for 32 weights.
 #include <algorithm>
+#include <atomic>
 #include <new>
 #include <type_traits>
 
@@ -988,6 +989,13 @@ bool lies_well(const void* x, int64_t ld, int k, int type) {
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
+// A number of the calling thread, never given to another one.
+uint64_t thread_number() {
+  static std::atomic<uint64_t> threads{0};
+  static thread_local const uint64_t mine = ++threads;
+  return mine;
+}
+
 // The workspace of (handle, stream), at least `need` bytes.  A buffer that has to grow is replaced and kept until the handle goes: a
 // captured graph may hold its address.  It at least doubles, so that those kept are together no larger than the last one.
 int workspace(tetris_mx4* w, hipStream_t stream, size_t need, uint8_t** out) {
@@ -995,7 +1003,7 @@ int workspace(tetris_mx4* w, hipStream_t stream, size_t need, uint8_t** out) {
   if (!need) return TETRIS_OK;
   try {
     std::lock_guard<std::mutex> lock(w->mu);
-    tetris_mx4::Space& s = w->space[stream];
+    tetris_mx4::Space& s = w->space[{stream, stream == hipStreamPerThread ? thread_number() : 0}];
     if (s.bytes < need) {
       hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
       if (hipStreamIsCapturing(stream, &cap) == hipSuccess && cap != hipStreamCaptureStatusNone)
