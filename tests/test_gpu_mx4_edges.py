@@ -172,3 +172,26 @@ def test_threads_on_their_own_default_streams_have_their_own_workspaces():
     for x, y in zip(xs, ys):
         want, _, far = P.product(x, w, "f32")
         within(numbers(y), want, far)
+
+
+def test_workspace_of_very_many_tokens_stays_bounded():
+    """In one pass their numbers before the weighted sum would take 8.6 GB."""
+    rng = np.random.default_rng(8)
+    tokens, count, top, width, hidden = 260000, 2, 2, 4096, 32
+    up, down = weights(rng, count * 2 * hidden, width), weights(rng, count * width, hidden)
+    layer = T.ExpertLayer(T.MX4Weights(up[0].data_ptr(), up[1].data_ptr(), 2 * hidden, width, experts=count, gated=True),
+                          T.MX4Weights(down[0].data_ptr(), down[1].data_ptr(), width, hidden, experts=count))
+    x = torch.empty(tokens, width, dtype=torch.bfloat16, device="cuda").normal_() * 0.01
+    index = torch.randint(-1, count, (tokens, top), dtype=torch.int32, device="cuda")
+    weight, y = torch.rand(tokens, top, device="cuda"), torch.empty_like(x)
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info()[0]
+    layer.run(x.data_ptr(), index.data_ptr(), weight.data_ptr(), y.data_ptr(), tokens, top, T.BF16)
+    torch.cuda.synchronize()
+    # 2 GiB of them, and what lies between the products, a sixteenth of that
+    assert before - torch.cuda.mem_get_info()[0] <= 2.25 * 2 ** 30
+    rows = np.unique(np.concatenate([rng.integers(0, tokens, 60), [0, tokens - 1], (2 ** 31 // (top * width * 4) + np.arange(-12, 3)) % tokens]))
+    at = torch.from_numpy(rows).cuda()
+    want, far = P.experts(numbers(x[at]), up[2].reshape(count, 2 * hidden, width), down[2].reshape(count, width, hidden), index[at].cpu().numpy(),
+                          numbers(weight[at]), "bf16")
+    within(numbers(y[at]), want, far)

@@ -1054,6 +1054,11 @@ bool streams_slots(const tetris_mx4* up, int tokens, int top) {
 // Whether rows of `type` are multiplied in f16: where the weights are exact in it.  Others of f16 are taken in two bf16 parts.
 bool in_half(int type, const tetris_mx4* w) { return type == TETRIS_F16 && w->half; }
 
+// Whether a product reads them so.
+bool as_they_lie(const void* x, int type, int k, int64_t ld, bool rounded, bool stream, bool half) {
+  return !rounded && (stream || half || type == TETRIS_BF16) && lies_well(x, ld, k, type);
+}
+
 // bytes that rows made ready for a product take at most
 size_t staged_bytes(int rows, int k, int type, bool rounded, bool stream, bool half) {
   const size_t padded = (size_t)rows * round_up(k, kMxPad);
@@ -1079,8 +1084,7 @@ int ready_rows(Product* a, const void* x, int type, int rows, int k, int64_t ld,
     a->x_scales = scales;
     return mx4_quantize_to(kMxTiles, x, type, rows, k, ld, d_ready, scales, s);
   }
-  const bool as_is = stream || half || type == TETRIS_BF16;
-  if (lies_well(x, ld, k, type) && as_is) {
+  if (as_they_lie(x, type, k, ld, rounded, stream, half)) {
     a->x = x;
     a->ldx = ld;
     a->k8 = k;
@@ -1089,7 +1093,7 @@ int ready_rows(Product* a, const void* x, int type, int rows, int k, int64_t ld,
   a->x = d_ready;
   a->ldx = padded;
   a->k8 = (int)padded;
-  if (as_is) return stage_rows(x, type, rows, k, ld, 0, d_ready, s);
+  if (stream || half || type == TETRIS_BF16) return stage_rows(x, type, rows, k, ld, 0, d_ready, s);
   a->parts = parts_of(type);
   a->part = rows * padded;
   *as = TETRIS_BF16;
@@ -1155,10 +1159,9 @@ int rows_at_once(const tetris_mx4* w, int m, int type, bool rounded) {
 
 int linear_rows(tetris_mx4* w, const void* d_x, int type, int m, int64_t ldx, void* d_y, int64_t ldy, const float* d_bias, bool rounded, hipStream_t s) {
   const bool stream_it = streams(w, m), half = in_half(type, w);
-  const bool as_it_lies = !rounded && lies_well(d_x, ldx, w->k, type) && (stream_it || half || type == TETRIS_BF16);
   uint8_t* d = nullptr;
   int rc;
-  if (!as_it_lies && (rc = workspace(w, s, staged_bytes(m, w->k, type, rounded, stream_it, half), &d))) return rc;
+  if (!as_they_lie(d_x, type, w->k, ldx, rounded, stream_it, half) && (rc = workspace(w, s, staged_bytes(m, w->k, type, rounded, stream_it, half), &d))) return rc;
   Product a{};
   set_weights(&a, w);
   int as;
@@ -1241,11 +1244,13 @@ namespace {
 // slots whose numbers between the products, all parts of them, lie within a kernel's reach; 341 at least
 int64_t slots_at_once(const tetris_mx4* down, int type) { return kMxReach / (round_up(down->k, kMxPad) * 2 * parts_of(type)); }
 
-// tokens that one pass takes: their rows, and those between the products, lie within a kernel's reach (unless one token has too many)
+// tokens that one pass takes: their rows, and those between the products, lie within a kernel's reach (unless one token has too many), and the
+// rows before the weighted sum, 4 bytes a number, take no more memory than that
 int tokens_at_once(const tetris_mx4* up, const tetris_mx4* down, int tokens, int top, int type, int64_t ldx) {
   const bool half = in_half(type, up);
   const int64_t row = std::max<int64_t>(std::min<int64_t>(ldx, kMxSide) * elem_size(type), round_up(up->k, kMxPad) * (half ? 2 : 2 * parts_of(type)));
-  return (int)std::min<int64_t>(tokens, std::max<int64_t>(1, std::min(kMxReach / row, slots_at_once(down, type) / top)));
+  const int64_t sums = top * round_up(down->n, 4) * 4;
+  return (int)std::min<int64_t>(tokens, std::max<int64_t>(1, std::min({kMxReach / row, slots_at_once(down, type) / top, kMxReach / sums})));
 }
 
 }  // namespace
@@ -1349,7 +1354,7 @@ int expert_tokens(tetris_mx4* up, tetris_mx4* down, const void* d_x, int type, i
   const bool stream_it = streams_slots(up, tokens, top);
   const ExpertSpace e = expert_space(up, down, tokens, top, type, stream_it);
   uint8_t* d;
-  if ((rc = workspace(up, s, e.all, &d))) return rc;
+  if ((rc = workspace(up, s, as_they_lie(d_x, type, up->k, ldx, false, stream_it, in_half(type, up)) ? e.ready : e.all, &d))) return rc;
   if (slots <= kFewSlots) return few_slots(up, down, d_x, type, tokens, ldx, top, d_index, d_weight, d_y, ldy, e, d, s);
 
   float* rows = reinterpret_cast<float*>(d + e.rows);
