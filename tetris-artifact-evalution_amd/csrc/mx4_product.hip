@@ -308,6 +308,13 @@ __device__ inline void to_lds(__amdgpu_buffer_rsrc_t from, int at, int offset, i
 // Nothing may be on its way to LDS when a workgroup gives it back.
 __device__ inline void loads_have_ended() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
 
+// What is loaded before it is asked for before what is loaded behind it: the counts below rest on the order of the issue, which nothing else holds where
+// loads do not depend on each other.
+__device__ inline void in_order() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // A barrier behind which the LDS of the whole workgroup may be read and written over: this wave's reads of it have ended, and all its loads
 // have arrived but the N issued last.  (__syncthreads would wait for those as well.)
 template <int N>
@@ -378,6 +385,7 @@ __global__ __launch_bounds__(64 * WN, 2) void tile_kernel(Product a) {
   };
   fetch_weights(0);  // on their way while the tile's rows are looked up
   fetch_weights(1);
+  in_order();
 
   const __amdgpu_buffer_rsrc_t rows = buffer(static_cast<const __bf16*>(a.x) + (a.from_div ? 0 : first * a.ldx));
   int from[kLoads];  // bytes
@@ -443,7 +451,9 @@ __global__ __launch_bounds__(64 * WN, 2) void tile_kernel(Product a) {
     }
   };
   fetch_rows(0);
+  in_order();
   fetch_rows(1);
+  in_order();
   barrier_but<kRowLoads>();
   read(0, 0);
 #pragma unroll
@@ -549,7 +559,9 @@ __global__ __launch_bounds__(64 * WM * WN) void rounded_kernel(Product a) {
 #pragma unroll
   for (int i = 0; i < D; ++i) {
     fetch_rows(i);
+    in_order();
     fetch_weights(i);
+    in_order();
   }
   barrier_but<(D - 1) * kLoads + D * kWeightLoads>();
   read(0, 0);
