@@ -11,7 +11,7 @@ T = pytest.importorskip("tetris_amd")
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_mx4 import PAIR, TYPES, expert_case, numbers, on_gpu, rounded_to, run_experts, within  # noqa: E402
+from test_gpu_mx4 import PAIR, SCORE, TYPES, expert_case, numbers, on_gpu, rounded_to, run_experts, run_route, within  # noqa: E402
 
 
 def weights(rng, rows, cols, least=124, most=130):
@@ -195,3 +195,94 @@ def test_workspace_of_very_many_tokens_stays_bounded():
     want, far = P.experts(numbers(x[at]), up[2].reshape(count, 2 * hidden, width), down[2].reshape(count, width, hidden), index[at].cpu().numpy(),
                           numbers(weight[at]), "bf16")
     within(numbers(y[at]), want, far)
+
+
+def scaled_experts(rng, tokens, count, top, width, hidden, up_scales, down_scales):
+    """As expert_case of f16, with the ranges of the scales."""
+    up, down = weights(rng, count * 2 * hidden, width, *up_scales), weights(rng, count * width, hidden, *down_scales)
+    x = rounded_to(rng.normal(size=(tokens, width)) * width ** -0.5 / 3, "f16")
+    index = np.stack([rng.permutation(count)[:top] for _ in range(tokens)])
+    weight = rng.uniform(0.1, 1.0, (tokens, top)).astype(np.float32)
+    layer = T.ExpertLayer(T.MX4Weights(up[0].data_ptr(), up[1].data_ptr(), 2 * hidden, width, experts=count, gated=True),
+                          T.MX4Weights(down[0].data_ptr(), down[1].data_ptr(), width, hidden, experts=count))
+    want, far = P.experts(x, up[2].reshape(count, 2 * hidden, width), down[2].reshape(count, width, hidden), index, weight.astype(np.float64), "f16", PAIR)
+    assert np.abs(want).max() < 60000
+    return layer, x, index, weight, want, far
+
+
+FITS, BEYOND = (124, 130), (90, 130)  # scales of weights that are exact in f16, and of some that are not
+
+
+@pytest.mark.parametrize("up_scales,down_scales", [(BEYOND, FITS), (FITS, BEYOND), (BEYOND, BEYOND)])
+@pytest.mark.parametrize("tokens,count,top,width,hidden", [(20, 8, 2, 96, 40), (60, 3, 2, 136, 64), (600, 3, 2, 520, 64), (1100, 2, 1, 72, 130), (1200, 2, 2, 72, 1040), (3000, 2, 2, 72, 1040),
+                                                          (1200, 2, 2, 2100, 48)])
+def test_experts_of_f16_whose_weights_are_not_exact_in_it(tokens, count, top, width, hidden, up_scales, down_scales):
+    rng = np.random.default_rng(tokens + width)
+    layer, x, index, weight, want, far = scaled_experts(rng, tokens, count, top, width, hidden, up_scales, down_scales)
+    within(run_experts(layer, x, index, weight, "f16"), want, far)
+    within(run_experts(layer, x, index, weight, "f16", width + 1, 1), want, far)
+
+
+@pytest.mark.parametrize("up_scales,down_scales", [(BEYOND, FITS), (FITS, BEYOND), (FITS, FITS)])
+def test_experts_workspace_of_f16_in_parts_is_enough_for_fewer(up_scales, down_scales):
+    rng = np.random.default_rng(13)
+    layer, x, index, weight, want, far = scaled_experts(rng, 900, 4, 2, 72, 40, up_scales, down_scales)
+    s = torch.cuda.Stream()
+    layer.prepare(900, 2, T.F16, stream=s.cuda_stream)
+    for tokens in (900, 500, 100, 33, 32, 1):
+        dx, y = on_gpu(x[:tokens], "f16", 73, 1), torch.zeros(tokens, 72, dtype=torch.float16, device="cuda")
+        di, dw = torch.from_numpy(index[:tokens].astype(np.int32)).cuda(), torch.from_numpy(weight[:tokens]).cuda()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):  # a workspace that had to grow would be refused
+            layer.run(dx.data_ptr(), di.data_ptr(), dw.data_ptr(), y.data_ptr(), tokens, 2, T.F16, ldx=73, stream=s.cuda_stream)
+        for _ in range(2):
+            y.zero_()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            within(numbers(y), want[:tokens], far[:tokens])
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rounded", [False, True])
+@pytest.mark.parametrize("m", [3, 200, 1100])
+def test_linear_beside_numbers_that_are_none(m, rounded, kind):
+    """A row with an infinity, one with a NaN and a feature with a NaN block; all other outputs are those of the definition."""
+    rng = np.random.default_rng(m)
+    k, n = 96, 40
+    code = rng.integers(1, 8, (n, 3, 32)).astype(np.uint8)  # positive weights
+    scales = np.full((n, 3), 127, np.uint8)
+    scales[7, 1] = 255
+    x = rounded_to(np.abs(rng.normal(size=(m, k))) + 0.1, kind)
+    x[1, 5], x[2, 40] = np.inf, np.nan
+    d = torch.from_numpy(P.packed(code)).cuda(), torch.from_numpy(scales).cuda()
+    W = T.MX4Weights(d[0].data_ptr(), d[1].data_ptr(), n, k)
+    dx, y = on_gpu(x, kind), torch.zeros(m, n, dtype=TYPES[kind][1], device="cuda")
+    W.linear(dx.data_ptr(), y.data_ptr(), m, TYPES[kind][0], mx4_input=rounded)
+    got = numbers(y)
+    assert np.isnan(got[:, 7]).all() and np.isnan(got[2]).all()
+    features, rows = np.delete(np.arange(n), 7), np.delete(np.arange(m), [1, 2])
+    assert (np.isnan(got[1, features]) if rounded else np.isposinf(got[1, features])).all()
+    read = P.values(*P.quantise(x[rows]), k) if rounded else x[rows]
+    want, _, far = P.product(read, P.values(code[features], scales[features], k), kind)
+    within(got[np.ix_(rows, features)], want, far)
+
+
+@pytest.mark.parametrize("experts,groups,top_groups,top", [(1024, 16, 4, 32), (1024, 64, 9, 8), (1000, 8, 3, 8), (512, 8, 4, 8)])
+@pytest.mark.parametrize("two", [False, True])
+def test_route_of_groups_of_many_experts(experts, groups, top_groups, top, two):
+    """Ranks that are multiples of 2^-11 and so apart in 32 bits; what pairs of them add up to is where groups could be equal, which is ruled out."""
+    rng = np.random.default_rng(experts + groups)
+    tokens, size = 5, experts // groups
+    x = np.float32(rng.uniform(-3, 3, experts)).astype(np.float64)
+    s = P.scores(x[None], True)[0]
+    steps = rng.permutation(4096)[:experts]
+    bias = (steps * 2.0 ** -11 - s).astype(np.float32)
+    best = np.sort(steps.reshape(groups, size), 1)[:, ::-1]
+    assert np.unique(best[:, 0] + (best[:, 1] if two else 0)).size == groups
+    rows = np.stack([x] * tokens)
+    index, weight = run_route(rows, "f32", top, bias, score=T.SCORE_SIGMOID, groups=groups, top_groups=top_groups, group_by=T.GROUP_TWO if two else T.GROUP_MAX)
+    want_index, want = P.route(rows, top, True, bias, groups, top_groups, two)
+    assert np.array_equal(index, want_index)
+    within(weight, want, SCORE * np.abs(want))
