@@ -329,9 +329,9 @@ __device__ inline void barrier_but() {
 // ---- many rows: tiles through LDS ---------------------------------------------------------------------------------
 //
 // A workgroup computes 32 WT rows by 32 WR WN features (KS: column tiles a step, PI: parts of the rows taken in one step, each with the weights made once).
-// Bound by the matrix cores: 4096 x 4096 x 8192 of bf16 in 193 us (1.42 PFLOP/s), their pipes 80 % busy at the clock that power leaves; by the
-// weights' bytes where groups are small: 2.9 TB/s on 200 tokens of 8 of 64 experts of 2048 x 1000.  Rows come in steps of 64 KS columns, 128 KS bytes of each
-// row in one stretch, through registers into one of two LDS buffers while the other is multiplied; weights come straight
+// Bound by the matrix cores: 4096 x 4096 x 8192 of bf16 in 193 us (1.42 PFLOP/s), their pipes 83 % busy at the clock that power leaves; by the
+// weights' bytes where groups are small: 4.2 TB/s in the first product of 200 tokens of 8 of 64 experts of 2048 x 1000.  Rows come in steps of 64 KS columns, 128 KS bytes of each
+// row in one stretch, straight to one of two LDS buffers while the other is multiplied; weights come straight
 // from memory to the registers that use them, a step ahead, once for all parts of the rows.  A row's 16-byte pieces are permuted in LDS
 // (by turn_of, exclusive or) so that the sixteen lanes that an LDS read serves at once touch all 64 banks.
 template <int KS>
@@ -468,8 +468,9 @@ __global__ __launch_bounds__(64 * WN, 2) void tile_kernel(Product a) {
 }
 
 // The same for rows that are in MX4 as well, in the weights' layout (csrc/mx4.h): products of 4-bit numbers with both blocks' scales
-// applied by the matrix cores, four times the rate of bf16.  8192^3 in 258 us behind 41 for the rows' quantisation (4.3 PFLOP/s), pipes 54 % busy: for each 128
-// columns a CU loads 48 KiB, some 750 cycles, beside 1024 of products.  Rows come in steps of 128 columns through LDS, as they lie; a wave's
+// applied by the matrix cores, four times the rate of bf16.  8192^3 in 262 us behind 41 for the rows' quantisation (4.2 PFLOP/s), pipes 57 % busy: for each 128
+// columns a CU loads 48 KiB, some 750 cycles, beside 1024 of products; and every third step waits for all loads under way, as the scales, loaded in 16 bits,
+// are widened to 32 behind the last of them.  Rows come in steps of 128 columns through LDS, as they lie; a wave's
 // reads of it are one contiguous kilobyte.
 template <int WT, int WR, int WM, int WN, int OUT>
 __global__ __launch_bounds__(64 * WM * WN) void rounded_kernel(Product a) {
@@ -741,8 +742,8 @@ __global__ __launch_bounds__(1024) void stream_kernel(Product a) {
 // The second product of the experts for up to 64 slots in all, and the weighted sum of each token's.  A workgroup has 16 features and goes
 // through every expert that is named; its waves share (expert, stretch of columns) pairs evenly, in runs of neighbouring ones.  A wave's sums for one
 // expert are kept at place (number of the expert + number of the wave): along the runs each step raises one of the two, so
-// no two share a place.  Bound by latency: the slots, then weights, then the sums; 10.0 us for four tokens of 4 of 64 experts of 1024 x 2048
-// (8.3 MB).  Each output is then added up by one thread, slots in their order, waves in theirs.
+// no two share a place.  Bound by latency: the slots, then weights, then the sums; 9.7 us for four tokens of 4 of 64 experts of 1024 x 2048
+// (16 MB of codes and scales).  Each output is then added up by one thread, slots in their order, waves in theirs.
 //
 // Rows of an operator of 16 bits come as two bf16 parts, in two arrays: eight slots' leading parts are columns 0 to 7 of the products, what they leave is
 // columns 8 to 15, as few experts have more than eight of 64 slots.  So the numbers between the two products are off by 2^-14 at most, at the price of one
@@ -859,7 +860,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(const int* __restrict__ inde
 }
 
 // y[t] = sum over j of weight[t][j] rows[t top + j], four columns a thread; bound by the rows' bytes: 4096 tokens of
-// four rows of 4096 in 54.5 us (302 MB, 5.5 TB/s).
+// four rows of 4096 in 46.4 us (302 MB, 6.5 TB/s, half of the rows still in the last-level cache).
 template <int TYPE>
 __global__ __launch_bounds__(256) void combine_kernel(const float* __restrict__ rows, int64_t ld_rows, const int* __restrict__ index,
                                                       const float* __restrict__ weight, int tokens, int top, int experts, int width,
@@ -928,8 +929,10 @@ int launch_rounded(Product& a, hipStream_t stream) {
   return TETRIS_OK;
 }
 
-template <int TYPE, int RT, int OUT, bool GATED>
+// The rows of `a` are of TYPE.
+template <int TYPE, int OUT, bool GATED>
 int launch_stream(Product& a, hipStream_t stream) {
+  constexpr int RT = GATED ? 2 : 1;
   const int blocks = ceil_div(a.row_tiles * 2, RT);
   a.max_tiles = a.index ? a.rows : a.offsets ? std::min(a.rows, a.rows / 16 + std::min(a.experts, a.rows)) : ceil_div(a.rows, 16);
   const int64_t grid = (int64_t)blocks * a.max_tiles;
@@ -938,12 +941,6 @@ int launch_stream(Product& a, hipStream_t stream) {
   hipLaunchKernelGGL((stream_kernel<TYPE, RT, OUT, GATED>), dim3((unsigned)grid), dim3(64 * waves), (size_t)waves * RT * 1024, stream, a);
   TETRIS_HIP(hipGetLastError());
   return TETRIS_OK;
-}
-
-// The rows of `a` are of TYPE and streamed.
-template <int TYPE, int OUT, bool GATED>
-int stream_rows(Product& a, hipStream_t stream) {
-  return launch_stream<TYPE, GATED ? 2 : 1, OUT, GATED>(a, stream);
 }
 
 template <int TYPE>
@@ -1123,15 +1120,15 @@ enum Role { kLinear, kUp, kDown };
 int launch_product(Product& a, Role role, int as, int type, bool stream, hipStream_t s) {
   if (stream) {
     if (as == TETRIS_F32)
-      return role == kUp ? stream_rows<TETRIS_F32, kOutF32, true>(a, s) : stream_rows<TETRIS_F32, kOutF32, false>(a, s);
+      return role == kUp ? launch_stream<TETRIS_F32, kOutF32, true>(a, s) : launch_stream<TETRIS_F32, kOutF32, false>(a, s);
     if (role == kUp && a.index && type != TETRIS_F32)
-      return as == TETRIS_F16 ? stream_rows<TETRIS_F16, kOutParts2, true>(a, s) : stream_rows<TETRIS_BF16, kOutParts2, true>(a, s);
+      return as == TETRIS_F16 ? launch_stream<TETRIS_F16, kOutParts2, true>(a, s) : launch_stream<TETRIS_BF16, kOutParts2, true>(a, s);
     if (as == TETRIS_F16)
-      return role == kUp ? stream_rows<TETRIS_F16, kOutF32, true>(a, s) : stream_rows<TETRIS_F16, kOutF16, false>(a, s);
-    if (role == kUp) return stream_rows<TETRIS_BF16, kOutBF16, true>(a, s);
-    if (role == kDown || type == TETRIS_F32) return stream_rows<TETRIS_BF16, kOutF32, false>(a, s);
-    if (type == TETRIS_F16) return stream_rows<TETRIS_BF16, kOutF16, false>(a, s);
-    return stream_rows<TETRIS_BF16, kOutBF16, false>(a, s);
+      return role == kUp ? launch_stream<TETRIS_F16, kOutF32, true>(a, s) : launch_stream<TETRIS_F16, kOutF16, false>(a, s);
+    if (role == kUp) return launch_stream<TETRIS_BF16, kOutBF16, true>(a, s);
+    if (role == kDown || type == TETRIS_F32) return launch_stream<TETRIS_BF16, kOutF32, false>(a, s);
+    if (type == TETRIS_F16) return launch_stream<TETRIS_BF16, kOutF16, false>(a, s);
+    return launch_stream<TETRIS_BF16, kOutBF16, false>(a, s);
   }
   if (a.x_scales) {
     if (type == TETRIS_F32) return launch_rounded<4, 2, 2, 4, kOutF32>(a, s);

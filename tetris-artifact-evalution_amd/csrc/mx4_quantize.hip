@@ -7,7 +7,6 @@
 namespace tetris {
 namespace {
 
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // Eight elements of a row from element `at`, those from `cols` on zero.  VEC: the row starts on 16 bytes and `at` is a
@@ -58,7 +57,7 @@ __device__ inline unsigned quad_max(unsigned v) {
 
 // A piece of eight elements a lane, four lanes a block: loads and stores of a wave are contiguous (1 or 2 KiB in, 256 bytes
 // of codes out).  The scale's exponent is the largest magnitude's, less two (6 = 1.5 * 2^2 is the largest code); the
-// instruction that makes codes divides by the scale, rounds to nearest even and saturates.  8192 x 8200 of f32 in 54 us (304 MB, 5.6 TB/s), 8192 x 8192
+// instruction that makes codes divides by the scale, rounds to nearest even and saturates.  8192 x 8200 of f32 in 57 us (304 MB, 5.4 TB/s, half of them found in the last-level cache), 8192 x 8192
 // of bf16 to the products' layout in 42 (4.1 TB/s: 16 bytes of a line at a time).
 template <int TYPE, int KIND, bool VEC>
 __global__ __launch_bounds__(256) void quantize_kernel(const typename Elem<TYPE>::type* __restrict__ x, int64_t rows, int cols,
