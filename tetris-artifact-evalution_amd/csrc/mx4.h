@@ -12,6 +12,7 @@
 
 #include "common.h"
 #include "tetris_mx4.h"
+#include "workspace.h"
 
 namespace tetris {
 
@@ -53,10 +54,7 @@ struct tetris_mx4 {
   int row_tiles = 0, col_tiles = 0;  // of one matrix
   uint8_t* codes = nullptr;
   uint8_t* scales = nullptr;
-  std::mutex mu;
-  struct Space { void* ptr = nullptr; size_t bytes = 0; };
-  std::map<std::pair<hipStream_t, uint64_t>, Space> space;  // the number: of the thread, for hipStreamPerThread, which is one value for many streams
-  std::vector<void*> retired;  // replaced by larger ones; a captured graph may hold their addresses
+  tetris::Workspaces space;
 };
 
 #endif  // TETRIS_CSRC_MX4_H_

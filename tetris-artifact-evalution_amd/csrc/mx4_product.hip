@@ -998,44 +998,6 @@ bool lies_well(const void* x, int64_t ld, int k, int type) {
 
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
-// A number of the calling thread, never given to another one.
-uint64_t thread_number() {
-  static std::atomic<uint64_t> threads{0};
-  static thread_local const uint64_t mine = ++threads;
-  return mine;
-}
-
-// The workspace of (handle, stream), at least `need` bytes.  A buffer that has to grow is replaced and kept until the handle goes: a
-// captured graph may hold its address.  It at least doubles, so that those kept are together no larger than the last one.
-int workspace(tetris_mx4* w, hipStream_t stream, size_t need, uint8_t** out) {
-  *out = nullptr;
-  if (!need) return TETRIS_OK;
-  try {
-    std::lock_guard<std::mutex> lock(w->mu);
-    tetris_mx4::Space& s = w->space[{stream, stream == hipStreamPerThread ? thread_number() : 0}];
-    if (s.bytes < need) {
-      hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-      if (hipStreamIsCapturing(stream, &cap) == hipSuccess && cap != hipStreamCaptureStatusNone)
-        return fail(TETRIS_EINVAL, "this launch would allocate its workspace: prepare it before capturing");
-      w->retired.reserve(w->retired.size() + 1);
-      void* d = nullptr;
-      size_t bytes = std::max(need, 2 * s.bytes);
-      if (bytes > need && hipMalloc(&d, bytes) != hipSuccess) {
-        (void)hipGetLastError();  // no room for twice as much
-        d = nullptr;
-      }
-      if (!d) TETRIS_HIP(hipMalloc(&d, bytes = need));
-      if (s.ptr) w->retired.push_back(s.ptr);
-      s.ptr = d;
-      s.bytes = bytes;
-    }
-    *out = static_cast<uint8_t*>(s.ptr);
-    return TETRIS_OK;
-  } catch (const std::exception& e) {
-    return fail(TETRIS_EINVAL, "%s", e.what());
-  }
-}
-
 constexpr int kFewSlots = 64;      // the experts' slots that down_kernel takes, a lane each
 constexpr int kStreamMost = 1024;  // more rows are not streamed, whatever the matrix
 
@@ -1170,7 +1132,7 @@ int linear_rows(tetris_mx4* w, const void* d_x, int type, int m, int64_t ldx, vo
   const bool stream_it = streams(w, m), half = in_half(type, w);
   uint8_t* d = nullptr;
   int rc;
-  if (!as_they_lie(d_x, type, w->k, ldx, rounded, stream_it, half) && (rc = workspace(w, s, staged_bytes(m, w->k, type, rounded, stream_it, half), &d))) return rc;
+  if (!as_they_lie(d_x, type, w->k, ldx, rounded, stream_it, half) && (rc = w->space.get(s, staged_bytes(m, w->k, type, rounded, stream_it, half), &d))) return rc;
   Product a{};
   set_weights(&a, w);
   int as;
@@ -1193,7 +1155,7 @@ extern "C" int tetris_mx4_prepare(tetris_mx4* w, int m, int type, int mx4_input,
   const bool half = in_half(type, w);
   // fewer rows may be streamed where these are not, and rounded ones then take more room each
   const size_t need = std::max(staged_bytes(rows, w->k, type, mx4_input, streams(w, m), half), staged_bytes(std::min(m, kStreamMost), w->k, type, mx4_input, true, half));
-  return workspace(w, static_cast<hipStream_t>(stream), need, &d);
+  return w->space.get(static_cast<hipStream_t>(stream), need, &d);
 }
 
 extern "C" int tetris_mx4_linear(tetris_mx4* w, const void* d_x, int type, int m, int64_t ldx, void* d_y, int64_t ldy,
@@ -1271,7 +1233,7 @@ extern "C" int tetris_experts_prepare(tetris_mx4* up, tetris_mx4* down, int toke
   const int once = tokens_at_once(up, down, tokens, top, type, up->k), few = std::min(once, kFewSlots / top);
   size_t need = expert_space(up, down, once, top, type, streams_slots(up, once, top)).all;
   if (few) need = std::max(need, expert_space(up, down, few, top, type, true).all);  // a few tokens' numbers between the products take more
-  return workspace(up, static_cast<hipStream_t>(stream), need, &d);
+  return up->space.get(static_cast<hipStream_t>(stream), need, &d);
 }
 
 namespace {
@@ -1363,7 +1325,7 @@ int expert_tokens(tetris_mx4* up, tetris_mx4* down, const void* d_x, int type, i
   const bool stream_it = streams_slots(up, tokens, top);
   const ExpertSpace e = expert_space(up, down, tokens, top, type, stream_it);
   uint8_t* d;
-  if ((rc = workspace(up, s, as_they_lie(d_x, type, up->k, ldx, false, stream_it, in_half(type, up)) ? e.ready : e.all, &d))) return rc;
+  if ((rc = up->space.get(s, as_they_lie(d_x, type, up->k, ldx, false, stream_it, in_half(type, up)) ? e.ready : e.all, &d))) return rc;
   if (slots <= kFewSlots) return few_slots(up, down, d_x, type, tokens, ldx, top, d_index, d_weight, d_y, ldy, e, d, s);
 
   float* rows = reinterpret_cast<float*>(d + e.rows);

@@ -3,57 +3,12 @@
 #include <algorithm>
 
 #include "mx4.h"
+#include "rows.h"
 
 namespace tetris {
 namespace {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-
-// Eight elements of a row from element `at`, those from `cols` on zero.  VEC: the row starts on 16 bytes and `at` is a
-// multiple of eight.
-template <typename T, bool VEC>
-__device__ inline void load8(const T* row, int at, int cols, float (&v)[8]) {
-  if (VEC && at + 8 <= cols) {
-    T t[8];
-    const int4* src = reinterpret_cast<const int4*>(row + at);
-    int4* dst = reinterpret_cast<int4*>(t);
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) dst[i] = src[i];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)t[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = at + i < cols ? (float)row[at + i] : 0.f;
-  }
-}
-
-// A lane's place in a matrix of `per_row` pieces of eight elements a row, the pieces numbered through: wave w of the grid takes
-// pieces 64 w .. 64 w + 63, so the division is the wave's, on the scalar unit, and a lane only steps over row ends.
-struct Place { int64_t row; int piece; };
-__device__ inline Place place_of(int64_t wave, unsigned per_row) {
-  const int64_t first = wave * 64;
-  Place p;
-  p.row = first / per_row;
-  unsigned piece = (unsigned)(first - p.row * per_row) + (threadIdx.x & 63);
-  if (piece >= per_row) {
-    const unsigned over = per_row >= 64 ? 1 : piece / per_row;
-    piece -= over * per_row;
-    p.row += over;
-  }
-  p.piece = (int)piece;
-  return p;
-}
-
-__device__ inline int64_t wave_of() {
-  return (int64_t)blockIdx.x * (blockDim.x >> 6) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-}
-
-// Largest magnitude of the four lanes that share a block, as bits: those of non-negative numbers order like the numbers, and
-// an infinity or a NaN comes out as 0x7f800000 or more.
-__device__ inline unsigned quad_max(unsigned v) {
-  v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, true));  // lanes 1 0 3 2
-  return max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, true));  // lanes 2 3 0 1
-}
 
 // A piece of eight elements a lane, four lanes a block: loads and stores of a wave are contiguous (1 or 2 KiB in, 256 bytes
 // of codes out).  The scale's exponent is the largest magnitude's, less two (6 = 1.5 * 2^2 is the largest code); the
@@ -365,9 +320,7 @@ extern "C" void tetris_mx4_destroy(tetris_mx4* w) {
   if (!w) return;
   if (w->codes) (void)hipFree(w->codes);
   if (w->scales) (void)hipFree(w->scales);
-  for (auto& s : w->space)
-    if (s.second.ptr) (void)hipFree(s.second.ptr);
-  for (void* p : w->retired) (void)hipFree(p);
+  w->space.release();
   delete w;
 }
 

@@ -1,0 +1,194 @@
+// Rotary positions: pairs of a head's elements turned by position * rate, each pair by the position of its section's axis.  A workgroup
+// makes the cosines and sines of a few tokens once, in LDS, and turns all heads of these tokens with them; one pass over memory.
+//
+// A pair's angle in turns is formed in 64 bits and its whole turns taken off, which leaves a far position's angle exact to about
+// 2^-49 of the position.  What is left goes to 32 bits as t + d with d below 2^-25 t, and cos(t + d) = cos t - d sin t, so that the cosine is
+// as near as one rounded from 64 bits.
+#include <cmath>
+
+#include "mx4.h"
+#include "tetris_attention.h"
+
+namespace tetris {
+namespace {
+
+constexpr int kRotaryHead = 1024;     // most elements of a head
+constexpr int kRotaryEntries = 1024;  // cosines and sines of a workgroup
+
+struct Rotary {
+  const void* x;
+  void* y;
+  const int* position;
+  int64_t ldx, ldy, ldp;
+  int tokens, heads, head, half;  // half: pairs of a head
+  int start[5];                   // first pair of each section, and the end
+  int halves, by_axis, backward;
+  int each;    // tokens of a workgroup
+  int splits;  // workgroups that share a token's heads
+  double turns;  // log2 of the base
+};
+
+template <typename T>
+__device__ inline void load_eight(const T* p, float (&v)[8]) {
+  int4 raw[sizeof(T) / 2];
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = reinterpret_cast<const int4*>(p)[i];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = (float)reinterpret_cast<const T*>(raw)[i];
+}
+template <typename T>
+__device__ inline void store_eight(T* p, const float (&v)[8]) {
+  T t[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] = (T)v[i];
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<int4*>(p)[i] = reinterpret_cast<const int4*>(t)[i];
+}
+
+// VEC: rows lie on 16 bytes, and a unit of work is eight elements, or eight pairs of halves.  Otherwise it is a pair, or an element past the pairs.
+template <int TYPE, bool VEC, bool HALVES>
+__global__ __launch_bounds__(256) void rotary_kernel(Rotary a) {
+  using T = typename Elem<TYPE>::type;
+  __shared__ float2 table[kRotaryEntries];  // cosine and sine of a token's pairs
+  const int group = blockIdx.x / a.splits, split = blockIdx.x - group * a.splits;
+  const int first = group * a.each, count = min(a.each, a.tokens - first);
+  for (int e = threadIdx.x; e < count * a.half; e += 256) {
+    const int token = e / a.half, pair = e - token * a.half;
+    int axis = 0;
+#pragma unroll
+    for (int k = 1; k < 4; ++k) axis += pair >= a.start[k] ? 1 : 0;
+    int from = 0, of = a.half;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (a.by_axis && axis == k) from = a.start[k], of = a.start[k + 1] - a.start[k];
+    const double rate = exp2(-(double)(pair - from) * a.turns / (double)of);
+    const int position = a.position[axis * a.ldp + first + token];
+    double t = (double)position * (rate * 0.15915494309189533577);  // 1 / (2 pi)
+    t = 2.0 * (t - rint(t));
+    const float near = (float)t, left = (float)((t - (double)near) * 3.14159265358979323846);
+    float s, c;
+    sincospif(near, &s, &c);
+    const float sine = fmaf(left, c, s);
+    table[e] = make_float2(fmaf(-left, s, c), a.backward ? -sine : sine);
+  }
+  __syncthreads();
+  const int dims = 2 * a.half, tail = a.head - dims;
+  const int turned = VEC ? (HALVES ? a.half / 8 : a.half / 4) : a.half, units = turned + (VEC ? tail / 8 : tail);  // of a head
+  const int h0 = (int)((int64_t)a.heads * split / a.splits), heads = (int)((int64_t)a.heads * (split + 1) / a.splits) - h0;
+  const int all = heads * units;
+  for (int token = 0; token < count; ++token) {
+    const T* x = static_cast<const T*>(a.x) + (int64_t)(first + token) * a.ldx;
+    T* y = static_cast<T*>(a.y) + (int64_t)(first + token) * a.ldy;
+    const float2* angle = table + token * a.half;
+    for (int w = threadIdx.x; w < all; w += 256) {
+      const int h = w / units, u = w - h * units;
+      const int64_t at = (int64_t)(h0 + h) * a.head;
+      if constexpr (VEC) {
+        float p[8], q[8];
+        if (u >= turned) {  // as they are
+          const int64_t from = at + dims + (u - turned) * 8;
+          int4 raw[sizeof(T) / 2];
+#pragma unroll
+          for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = reinterpret_cast<const int4*>(x + from)[i];
+#pragma unroll
+          for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<int4*>(y + from)[i] = raw[i];
+        } else if constexpr (HALVES) {
+          load_eight(x + at + u * 8, p);
+          load_eight(x + at + a.half + u * 8, q);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 cs = angle[u * 8 + i];
+            const float f = p[i] * cs.x - q[i] * cs.y;
+            q[i] = p[i] * cs.y + q[i] * cs.x;
+            p[i] = f;
+          }
+          store_eight(y + at + u * 8, p);
+          store_eight(y + at + a.half + u * 8, q);
+        } else {
+          load_eight(x + at + u * 8, p);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 cs = angle[u * 4 + i];
+            q[2 * i] = p[2 * i] * cs.x - p[2 * i + 1] * cs.y;
+            q[2 * i + 1] = p[2 * i] * cs.y + p[2 * i + 1] * cs.x;
+          }
+          store_eight(y + at + u * 8, q);
+        }
+      } else if (u >= turned) {
+        y[at + dims + u - turned] = x[at + dims + u - turned];
+      } else {
+        const int64_t i = at + (HALVES ? u : 2 * u), j = HALVES ? i + a.half : i + 1;
+        const float p = (float)x[i], q = (float)x[j];
+        const float2 cs = angle[u];
+        y[i] = (T)(p * cs.x - q * cs.y);
+        y[j] = (T)(p * cs.y + q * cs.x);
+      }
+    }
+  }
+}
+
+template <int TYPE>
+void launch(Rotary a, bool vec, int64_t groups, hipStream_t s) {
+  const dim3 grid((unsigned)groups), block(256);
+  if (vec && a.halves) hipLaunchKernelGGL((rotary_kernel<TYPE, true, true>), grid, block, 0, s, a);
+  else if (vec) hipLaunchKernelGGL((rotary_kernel<TYPE, true, false>), grid, block, 0, s, a);
+  else if (a.halves) hipLaunchKernelGGL((rotary_kernel<TYPE, false, true>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((rotary_kernel<TYPE, false, false>), grid, block, 0, s, a);
+}
+
+}  // namespace
+}  // namespace tetris
+
+using namespace tetris;
+
+extern "C" int tetris_rotate(const tetris_rotary* r, const void* d_x, int type, int tokens, int heads, int64_t ldx, const int32_t* d_position,
+                             int64_t ld_position, int backward, void* d_y, int64_t ldy, void* stream) {
+  if (!r) return fail(TETRIS_EINVAL, "null argument");
+  if (bad_type(type)) return fail(TETRIS_EINVAL, "type %d is not TETRIS_F32, TETRIS_F16 or TETRIS_BF16", type);
+  if (r->head <= 0 || r->head > kRotaryHead) return fail(TETRIS_EINVAL, "heads of %d elements (1 to %d)", r->head, kRotaryHead);
+  if (r->dims <= 0 || r->dims > r->head || (r->dims & 1)) return fail(TETRIS_EINVAL, "%d elements of %d to turn (an even number of them)", r->dims, r->head);
+  if (r->axes < 1 || r->axes > 4) return fail(TETRIS_EINVAL, "%d axes (1 to 4)", r->axes);
+  Rotary a{};
+  a.half = r->dims / 2;
+  for (int k = 0; k < 4; ++k) {
+    const int n = k < r->axes ? r->sections[k] : 0;
+    if (n < 0 || n > a.half) return fail(TETRIS_EINVAL, "a section of %d pairs", n);
+    a.start[k + 1] = a.start[k] + n;
+  }
+  if (a.start[4] != a.half) return fail(TETRIS_EINVAL, "sections of %d pairs together where %d are turned", a.start[4], a.half);
+  if (r->pairing != TETRIS_PAIR_HALVES && r->pairing != TETRIS_PAIR_NEIGHBOURS) return fail(TETRIS_EINVAL, "pairing %d", r->pairing);
+  if (r->rate != TETRIS_RATE_HEAD && r->rate != TETRIS_RATE_AXIS) return fail(TETRIS_EINVAL, "rate %d", r->rate);
+  if (!(r->base > 0.0) || !std::isfinite(r->base)) return fail(TETRIS_EINVAL, "base %g is not positive and finite", r->base);
+  if (tokens < 0 || heads < 0 || heads > (1 << 20)) return fail(TETRIS_EINVAL, "%d tokens of %d heads", tokens, heads);
+  const int64_t width = (int64_t)heads * r->head;
+  if (ldx < width || ldy < width) return fail(TETRIS_EINVAL, "leading dimension %lld below the %lld elements of a token", (long long)(ldx < ldy ? ldx : ldy), (long long)width);
+  if (r->axes > 1 && ld_position < tokens) return fail(TETRIS_EINVAL, "positions: leading dimension %lld below the %d tokens", (long long)ld_position, tokens);
+  if (tokens == 0 || heads == 0) return TETRIS_OK;
+  if (!d_x || !d_y || !d_position) return fail(TETRIS_EINVAL, "null argument");
+  if ((reinterpret_cast<size_t>(d_x) | reinterpret_cast<size_t>(d_y)) % elem_size(type)) return fail(TETRIS_EINVAL, "rows not aligned to their elements");
+  if (reinterpret_cast<size_t>(d_position) & 3) return fail(TETRIS_EINVAL, "positions not aligned to their elements");
+  if (d_x == d_y && ldx != ldy) return fail(TETRIS_EINVAL, "in place with another leading dimension");
+  a.x = d_x; a.y = d_y; a.position = d_position;
+  a.ldx = ldx; a.ldy = ldy; a.ldp = ld_position;
+  a.tokens = tokens; a.heads = heads; a.head = r->head;
+  a.halves = r->pairing == TETRIS_PAIR_HALVES;
+  a.by_axis = r->rate == TETRIS_RATE_AXIS;
+  a.backward = backward != 0;
+  a.turns = std::log2(r->base);
+  const int size = elem_size(type);
+  const bool vec = ((reinterpret_cast<size_t>(d_x) | reinterpret_cast<size_t>(d_y)) & 15) == 0 && ldx * size % 16 == 0 && ldy * size % 16 == 0 &&
+                   r->head % 8 == 0 && a.half % (a.halves ? 8 : 4) == 0;
+  // Few tokens: a workgroup each, or several that share its heads.  Many: as many as fill the table, so that every thread makes an angle or two.
+  a.each = 1;
+  while (a.each * 2 * a.half <= kRotaryEntries / 2 && (int64_t)(tokens / (a.each * 2)) >= 1024) a.each *= 2;
+  int64_t groups = ceil_div(tokens, a.each);
+  a.splits = 1;
+  while (a.splits * 2 <= heads && groups * a.splits < 512 && width / (a.splits * 2) >= 1024) a.splits *= 2;
+  if (groups * a.splits > 0x7fffffff) a.splits = 1;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (type == TETRIS_F32) launch<TETRIS_F32>(a, vec, groups * a.splits, s);
+  else if (type == TETRIS_F16) launch<TETRIS_F16>(a, vec, groups * a.splits, s);
+  else launch<TETRIS_BF16>(a, vec, groups * a.splits, s);
+  TETRIS_HIP(hipGetLastError());
+  return TETRIS_OK;
+}

@@ -523,3 +523,4 @@ def TensorEqual(x, y):
 
 from .mx4 import (BF16, F16, F32, GROUP_MAX, GROUP_TWO, SCORE_SIGMOID, SCORE_SOFTMAX, ExpertLayer, MX4Weights, Router,  # noqa: E402
                   mx4_code_bytes, mx4_dequantize, mx4_quantize, mx4_scale_bytes)
+from .attention import (PAIR_HALVES, PAIR_NEIGHBOURS, RATE_AXIS, RATE_HEAD, MX4Cache, Rotary, cache_page_bytes, rms_norm)  # noqa: E402
