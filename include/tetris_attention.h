@@ -67,7 +67,7 @@ int tetris_cache_read(tetris_cache* c, const int64_t* d_slot, int tokens, void* 
  * at place j % page.  Row i of n of a sequence of length L is at position p = L - n + i, sees tokens j with j <= p and, with a window,
  * j > p - window, and becomes  y = sum_j softmax_j(scale * q.k_j) v_j; a row that sees nothing becomes zeros.  Keys and values
  * that a row does not see do not touch it, whatever they are.
- * most_length and most_rows: no sequence is longer, nor has more rows; what is longer counts as most_length, rows beyond most_rows are left as they
+ * most_length (up to 2^28) and most_rows: no sequence is longer, nor has more rows; what is longer counts as most_length, rows beyond most_rows are left as they
  * are, as are those of no sequence.  d_table: a row of ceil(most_length / page) page numbers for each sequence, ld_table
  * apart; a number outside of the pool stands for a page that no row sees.  The lengths, tables and offsets are read on the device: a captured
  * launch serves whatever they hold when it is replayed.

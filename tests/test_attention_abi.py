@@ -84,7 +84,7 @@ def test_attend_refusals():
         return lambda: c.attend(q, y, dtype, heads, sequences, length, table, most_length, **how)
 
     for call in (attend(q=0), attend(y=0), attend(length=0), attend(table=0), attend(dtype=3), attend(heads=0), attend(heads=3), attend(heads=1026),
-                 attend(sequences=-1), attend(most_length=-1), attend(most_length=(1 << 30) + 1), attend(window=-1), attend(rows=-1, d_first=A),
+                 attend(sequences=-1), attend(most_length=-1), attend(most_length=(1 << 28) + 1, ld_table=1 << 30), attend(window=-1), attend(rows=-1, d_first=A),
                  attend(rows=5), attend(rows=1 << 29, d_first=A), attend(most_rows=-1), attend(ld_table=2), attend(ldq=255), attend(ldy=255),
                  attend(q=A + 2), attend(y=B + 2), attend(length=A + 1), attend(table=A + 2), attend(d_first=A + 2), attend(q=B)):
         refused(call)
