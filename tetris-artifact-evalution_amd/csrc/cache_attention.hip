@@ -33,11 +33,14 @@ struct Attend {
   const int* first;
   const int* length;
   const int* table;
-  float* part;  // of chunks: maximum and sum [chunk][row][head][2], then outputs [chunk][row][head][elements]
+  float* part;  // [2 workgroups][16 NT rows]: maximum and sum, then outputs (struct Slot)
+  int2* shares; // of a unit: the first workgroup that has some of it, and how many have
   int64_t page_bytes, ldt, ldq, ldy;
   int pages, page, granules, kv_heads, heads, group, sequences, rows, most_rows, most_length, window;
-  int blocks;  // of rows
-  int chunk, chunks;  // tokens of a workgroup; most of them in a sequence
+  int tiles;   // NT
+  int blocks;  // most blocks of 16 NT rows of a sequence and kv head
+  int workgroups;
+  int chunk, chunks;  // quanta of a workgroup, or zero for equal shares; most chunks of a unit
   int whole;   // rows of q lie on 16 bytes
   unsigned page_magic;  // to divide by granules (0 where that is one)
   float scale;  // to powers of two, not negative
@@ -338,36 +341,64 @@ struct Rows {
 struct Pages { int page[2]; };
 __device__ inline unsigned page_index(const Attend& a, unsigned granule) { return a.page_magic ? __umulhi(granule, a.page_magic) : granule; }
 
-// SHARED: the workgroup's waves take the steps of one block of rows in turn and join their outputs; else each has its own block.
-// (Two waves a SIMD at least: with 256 registers or fewer the products' sums stay in ordinary registers, not in those that have to be copied for the rest.)
-template <int TYPE, int D, int NT, bool SHARED>
-__global__ __launch_bounds__(256, 2) void attend_kernel(Attend a) {
+// How the work is dealt out.  A unit is a block of 16 NT rows of a sequence and kv head; it is as many quanta of four steps as its sequence
+// has tokens for (one at least: rows that see nothing become zeros).  What a workgroup does of a unit that it does not do all of it leaves to join_kernel.
+//   little work     a.chunk quanta of one unit each; chunks that a sequence is too short for end at once.  It begins without looking at the
+//                   other sequences: one token of 4000 tokens by 32 heads takes 10 us in place of 13.
+//   much work       the units' quanta, sequence after sequence, in equal shares, whatever the lengths are: 64 sequences of up to 8192 tokens, 3700 on
+//                   average, take 68 us in place of 86.
+constexpr int kQuantum = 4 * kStep;
+constexpr int kBegin = 3;  // quanta's time that a unit takes besides: queries, the first loads, joining the waves' outputs
+struct Units { int quanta, blocks; };
+__device__ inline Units units_of(const Attend& a, const Sequence& q) {
+  const int rows = min(q.rows, a.most_rows) * a.group, size = 16 * a.tiles;
+  return {max((q.length - q.base + kQuantum - 1) / kQuantum, 1), (rows + size - 1) / size};
+}
+__device__ inline int quanta_of(const Attend& a, int s) {
+  if (s >= a.sequences) return 0;
+  const Units u = units_of(a, sequence_of(a, s));
+  return (u.quanta + kBegin) * u.blocks * a.kv_heads;
+}
+
+// the sums of v over the lanes up to this one
+__device__ inline int sums_upto(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // from 1, 2, 4 and 8 lanes below in rows of sixteen
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // a row's last to the next row, the second row's to the upper half
+  return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+}
+
+// Where a workgroup leaves a unit's rows: its last unit, if that goes on behind it, has slot 2 w + 1, and one that began before it 2 w.
+struct Slot {
+  float* top;  // [rows][2]
+  float* out;  // [rows][elements]
+};
+__device__ inline Slot slot_of(const Attend& a, int slot, int head) {
+  const int rows = 16 * a.tiles;
+  return {a.part + (int64_t)slot * rows * 2, a.part + 4 * (int64_t)a.workgroups * rows + (int64_t)slot * rows * head};
+}
+
+// `count` quanta of a unit from its quantum `skip` on, by a workgroup; parts: how many workgroups have some of the unit.
+template <int TYPE, int D, int NT>
+__device__ inline void attend_unit(const Attend& a, const Sequence& seq, int quanta, int s, int kv, int block, int skip, int count, int parts) {
   using T = typename Elem<TYPE>::type;
-  constexpr int S = D / 16, W = 4;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, quad = lane >> 4;
-  int id = blockIdx.x;
-  const int chunk = id % a.chunks;
-  id /= a.chunks;
-  // (kv heads first: the blocks of rows of one kv head are a multiple of 8 workgroups apart where there are 8, 16, .. kv heads, on one of the eight
-  // dies, whose cache then holds this kv head's tokens; the last rows first, which see the most)
-  const int kv = id % a.kv_heads;
-  id /= a.kv_heads;
-  const int s = id % a.sequences, group = id / a.sequences;
-  const int block = SHARED ? group : ((a.blocks + W - 1) / W - 1 - group) * W + wave;
-  const Sequence seq = sequence_of(a, s);
+  constexpr int S = D / 16, W = 4, kStride = W * kStep;
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // (what is computed from it is computed here, and not kept in registers from one unit to the next)
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, quad = lane >> 4;
+  __shared__ float out[W][NT * 16][D + 1];
+  __shared__ float tops[W][NT * 16], sums[W][NT * 16];
   const int all = min(seq.rows, a.most_rows) * a.group, r0 = block * (16 * NT);
   const int left = all - r0;  // rows of this block and those behind it
-  if (SHARED && (left <= 0 || (chunk > 0 && seq.base + chunk * a.chunk >= seq.length))) return;
-  if (!SHARED && left <= 0) return;
 
   // the block's query tokens, and the tokens that some of its rows sees
   const int t0 = r0 / a.group, t1 = min(r0 + 16 * NT - 1, all - 1) / a.group;
   const int p0 = seq.length - seq.rows;  // position of row 0
-  int from = seq.base + chunk * a.chunk, to = min(from + a.chunk, min(p0 + t1, seq.length - 1) + 1);
+  int from = seq.base + skip * kQuantum;
+  const int to = min(from + count * kQuantum, min(p0 + t1, seq.length - 1) + 1);
   if (a.window) from = max(from, max(p0 + t0 - a.window + 1, 0) & ~(kStep - 1));
-
-  Rows<TYPE, D, NT> rows;
-  rows.begin(a, seq, kv, r0, all, lane);
 
   const int* table = a.table + s * a.ldt;
   const uint8_t* head = a.data + (int64_t)kv * a.granules * (17 * D);
@@ -375,11 +406,9 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(Attend a) {
     Pages p;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      p.page[u] = -1;
-      if (at + 16 * u < seq.length) {
-        const int page = table[page_index(a, (unsigned)at / 16 + u)];
-        if ((unsigned)page < (unsigned)a.pages) p.page[u] = page;
-      }
+      // (read wherever the table has an entry, so that it need not wait for the sequence's length)
+      const int page = table[page_index(a, (unsigned)min(at + 16 * u, a.most_length - 1) / 16)];
+      p.page[u] = at + 16 * u < seq.length && (unsigned)page < (unsigned)a.pages ? page : -1;
     }
     return p;
   };
@@ -390,155 +419,225 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(Attend a) {
       g[u].load(head + (int64_t)max(p.page[u], 0) * a.page_bytes + in_page * (17 * D), lane);
     }
   };
-  constexpr int kStride = SHARED ? W * kStep : kStep;
-  const int start = from + (SHARED ? wave * kStep : 0);
-  // First the steps whose tokens all rows of the block see, as long as their pages are in the pool: two in turn, so that one's loads are under way while
-  // the other is worked on, and the pages' numbers for the next while these loads are asked for.
-  int at = start;
-  if (a.window && at <= p0 + t1 - a.window) at += (p0 + t1 - a.window - at) / kStride * kStride + kStride;
-  const int first = at, end = min(to, p0 + t0 + 1) - kStep;  // the last of these steps begins there or before
-  if (at <= end) {
-    Granule<D> even[2], odd[2];
-    Pages pages = pages_of(at);
-    const int full[2] = {16, 16};
-    auto good = [](const Pages& p) { return p.page[0] >= 0 && p.page[1] >= 0; };
-    if (good(pages)) {
-      load(even, at, pages);
-      pages = pages_of(at + kStride);
-      for (;;) {
-        const bool more = at + kStride <= end && good(pages);
-        if (more) {
-          load(odd, at + kStride, pages);
-          pages = pages_of(at + 2 * kStride);
-        }
-        rows.template step<false>(a, even, at, full, lane);
-        at += kStride;
-        if (!more) break;
-        const bool again = at + kStride <= end && good(pages);
-        if (again) {
-          load(even, at + kStride, pages);
-          pages = pages_of(at + 2 * kStride);
-        }
-        rows.template step<false>(a, odd, at, full, lane);
-        at += kStride;
-        if (!again) break;
+  const int begin = from + wave * kStep;
+  // First the steps whose tokens all rows of the block see, as long as their pages are in the pool: two in turn, so that one's loads are under way
+  // while the other is worked on, and the pages' numbers for the next while these loads are asked for.  What comes behind them is loaded ahead as well.
+  int now = begin;
+  if (a.window && now <= p0 + t1 - a.window) now += (p0 + t1 - a.window - now) / kStride * kStride + kStride;
+  const int first = now, end = min(to, p0 + t0 + 1) - kStep;  // the last of these steps begins there or before
+  Granule<D> even[2], odd[2];
+  Pages pages = {-1, -1}, ahead;  // of the step at `now`, of the next
+  const int full[2] = {16, 16};
+  auto good = [](const Pages& p) { return p.page[0] >= 0 && p.page[1] >= 0; };
+  if (now < to) {
+    pages = pages_of(now);
+    load(even, now, pages);
+  }
+  Rows<TYPE, D, NT> rows;
+  rows.begin(a, seq, kv, r0, all, lane);
+  if (now <= end && good(pages)) {
+    ahead = pages_of(now + kStride);
+    for (;;) {
+      if (now + kStride < to) load(odd, now + kStride, ahead);
+      pages = ahead;
+      ahead = pages_of(now + 2 * kStride);
+      rows.template step<false>(a, even, now, full, lane);
+      now += kStride;
+      if (now > end || !good(pages)) {
+        even[0] = odd[0];
+        even[1] = odd[1];
+        break;
       }
+      if (now + kStride < to) load(even, now + kStride, ahead);
+      pages = ahead;
+      ahead = pages_of(now + 2 * kStride);
+      rows.template step<false>(a, odd, now, full, lane);
+      now += kStride;
+      if (now > end || !good(pages)) break;
     }
   }
   // Then the others: at the rows' newest tokens, where a window begins, and all that come behind a page that is not in the pool.
-  for (int rest = start; rest < to; rest += kStride) {
-    if (rest >= first && rest < at) {
-      rest = at - kStride;
-      continue;
+  bool loaded = now < to, wrapped = false;
+  for (;; now += kStride) {
+    if (!wrapped && now >= to) wrapped = true, now = begin;
+    if (wrapped && now >= min(first, to)) break;
+    if (!loaded) {
+      pages = pages_of(now);
+      load(even, now, pages);
     }
-    Granule<D> g[2];
-    const Pages pages = pages_of(rest);
-    load(g, rest, pages);
+    loaded = false;
     int upto[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) upto[u] = pages.page[u] < 0 ? 0 : min(seq.length - rest - 16 * u, 16);
-    rows.template step<true>(a, g, rest, upto, lane);
+    for (int u = 0; u < 2; ++u) upto[u] = pages.page[u] < 0 ? 0 : min(seq.length - now - 16 * u, 16);
+    rows.template step<true>(a, even, now, upto, lane);
   }
 
+  // the waves' outputs joined, to the output or to a slot
 #pragma unroll
-  for (int n = 0; n < NT; ++n) rows.l[n] = sum_of_row(rows.l[n]);
-
-  // outputs of row r of the block: of this workgroup's chunk or, if that is all, finished
-  auto finish = [&](int r, int element, float v, float top, float sum) {
-    const int t = (r0 + r) / a.group, h = kv * a.group + r0 + r - t * a.group;
-    if (SHARED && a.part) {
-      const int64_t row = (int64_t)(seq.begin + t) * a.heads + h, at = row * a.chunks + chunk;
-      a.part[2 * (int64_t)a.chunks * a.rows * a.heads + at * D + element] = v;
-      if (element == 0) a.part[2 * at] = top, a.part[2 * at + 1] = sum;
-    } else {
+  for (int n = 0; n < NT; ++n) {
+    const float sum = sum_of_row(rows.l[n]);
+    if (quad == 0) tops[wave][n * 16 + r16] = rows.m[n], sums[wave][n * 16 + r16] = sum;
+#pragma unroll
+    for (int j = 0; j < S; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out[wave][n * 16 + r16][element_of<D>(j, 4 * quad + i)] = rows.o[n][j][i];
+  }
+  __syncthreads();
+  const bool whole = count == quanta;
+  const Slot slot = slot_of(a, 2 * blockIdx.x + (skip == 0), D);
+  for (int e = threadIdx.x; e < min(left, 16 * NT) * D; e += 256) {
+    const int r = e / D, element = e - r * D;
+    float top = tops[0][r];
+#pragma unroll
+    for (int w = 1; w < W; ++w) top = fmaxf(top, tops[w][r]);
+    float v = 0.f, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float by = tops[w][r] == top ? 1.f : __builtin_amdgcn_exp2f(tops[w][r] - top);
+      v += out[w][r][element] * by;
+      sum += sums[w][r] * by;
+    }
+    if (whole) {
+      const int t = (r0 + r) / a.group, h = kv * a.group + r0 + r - t * a.group;
       static_cast<T*>(a.y)[(int64_t)(seq.begin + t) * a.ldy + (int64_t)h * D + element] = (T)(sum == 0.f ? 0.f : v / sum);
+    } else {
+      slot.out[r * D + element] = v;
+      if (element == 0) slot.top[2 * r] = top, slot.top[2 * r + 1] = sum;
     }
-  };
-  if constexpr (SHARED) {
-    __shared__ float out[W][NT * 16][D + 1];
-    __shared__ float tops[W][NT * 16], sums[W][NT * 16];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      if (quad == 0) tops[wave][n * 16 + r16] = rows.m[n], sums[wave][n * 16 + r16] = rows.l[n];
-#pragma unroll
-      for (int j = 0; j < S; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) out[wave][n * 16 + r16][element_of<D>(j, 4 * quad + i)] = rows.o[n][j][i];
+  }
+  if (skip == 0 && threadIdx.x == 0) a.shares[((int64_t)s * a.kv_heads + kv) * a.blocks + block] = make_int2(blockIdx.x, parts);
+}
+
+// Waves of a SIMD, and so workgroups of a compute unit, that the registers of a wave leave room for.
+constexpr int waves_of(int parts, int head, int tiles) { return parts * tiles * head <= 64 ? 4 : tiles * head <= 128 && parts * tiles * head <= 256 ? 3 : 2; }
+// (Two waves a SIMD at least: with 256 registers or fewer the products' sums stay in ordinary registers, not in those that have to be copied for the rest.)
+template <int TYPE, int D, int NT>
+__global__ __launch_bounds__(256, waves_of(kParts<TYPE>, D, NT)) void attend_chunks_kernel(Attend a) {
+  int id = blockIdx.x / a.chunks;
+  const int chunk = blockIdx.x - id * a.chunks, s = id / (a.kv_heads * a.blocks);
+  id -= s * (a.kv_heads * a.blocks);
+  const int kv = id / a.blocks, block = id - kv * a.blocks, skip = chunk * a.chunk;
+  const Sequence seq = sequence_of(a, s);
+  const Units units = units_of(a, seq);
+  if (block >= units.blocks || skip >= units.quanta) return;
+  attend_unit<TYPE, D, NT>(a, seq, units.quanta, s, kv, block, skip, min(a.chunk, units.quanta - skip), (units.quanta + a.chunk - 1) / a.chunk);
+}
+template <int TYPE, int D, int NT>
+__global__ __launch_bounds__(256, waves_of(kParts<TYPE>, D, NT)) void attend_shares_kernel(Attend a) {
+  const int lane = threadIdx.x & 63;
+  // this workgroup's share, and the sequence that it begins in
+  const int mine = sums_upto(quanta_of(a, lane));
+  int total = __builtin_amdgcn_readlane(mine, 63);
+  for (int s0 = 64; s0 < a.sequences; s0 += 64) total += __builtin_amdgcn_readlane(sums_upto(quanta_of(a, s0 + lane)), 63);
+  const int share = (total + a.workgroups - 1) / a.workgroups;
+  int at = blockIdx.x * share;
+  const int stop = min(at + share, total);
+  if (at >= stop) return;
+  int s = 0, start = 0;  // the sequence and its first quantum
+  for (int s0 = 0; s0 < a.sequences; s0 += 64) {
+    const int upto = s0 ? sums_upto(quanta_of(a, s0 + lane)) : mine;
+    const unsigned long long behind = __ballot(start + upto > at);
+    if (behind) {
+      const int l = __builtin_ctzll(behind);
+      s = s0 + l;
+      start += l ? __builtin_amdgcn_readlane(upto, l - 1) : 0;
+      break;
     }
-    __syncthreads();
-    for (int e = threadIdx.x; e < min(left, 16 * NT) * D; e += 256) {
-      const int r = e / D, element = e - r * D;
-      float top = tops[0][r];
-#pragma unroll
-      for (int w = 1; w < W; ++w) top = fmaxf(top, tops[w][r]);
-      float v = 0.f, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const float by = tops[w][r] == top ? 1.f : __builtin_amdgcn_exp2f(tops[w][r] - top);
-        v += out[w][r][element] * by;
-        sum += sums[w][r] * by;
+    start += __builtin_amdgcn_readlane(upto, 63);
+  }
+  while (at < stop) {
+    const Sequence seq = sequence_of(a, s);
+    const Units units = units_of(a, seq);
+    if (units.blocks) {
+      const int cost = units.quanta + kBegin, unit = (at - start) / cost, into = at - start - unit * cost, kv = unit / units.blocks;
+      const int mine = min(cost - into, stop - at), skip = max(into - kBegin, 0), count = max(into + mine - kBegin, 0) - skip;
+      if (count > 0) {
+        attend_unit<TYPE, D, NT>(a, seq, units.quanta, s, kv, unit - kv * units.blocks, skip, count, (at - into + cost - 1) / share - (int)blockIdx.x + 1);
+        __syncthreads();
       }
-      finish(r, element, v, top, sum);
+      at += mine;
     }
-  } else {
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-      if (n * 16 + r16 < left) {
-#pragma unroll
-        for (int j = 0; j < S; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) finish(n * 16 + r16, element_of<D>(j, 4 * quad + i), rows.o[n][j][i], rows.m[n], rows.l[n]);
-      }
+    if (at - start == (units.quanta + kBegin) * units.blocks * a.kv_heads) start = at, ++s;
   }
 }
 
-// Chunks' outputs joined: a workgroup has a row and head, a wave of it every fourth chunk.
-template <int TYPE>
-__global__ __launch_bounds__(256) void join_kernel(Attend a, int head) {
+// Units that several workgroups have parts of: a workgroup of W waves joins four rows, a wave of it every W-th part.  What the parts' weights are is known
+// only with the last of their maxima, so a wave joins its own parts first, and all loads of a part are under way together.
+template <int TYPE, int D, int W>
+__global__ __launch_bounds__(64 * W) void join_kernel(Attend a) {
   using T = typename Elem<TYPE>::type;
-  constexpr int W = 4;
-  __shared__ float out[W][kCacheHead];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int each = a.most_rows * a.heads, s = blockIdx.x / each, t = (blockIdx.x - s * each) / a.heads, h = blockIdx.x - s * each - t * a.heads;
+  constexpr int R = 4, V = (R * D + 255) / 256, K = 4;  // rows; fours of a lane; parts that are loaded together
+  __shared__ float4 out[W][V * 64];
+  __shared__ float tops[W][R], sums[W][R];
+  const int groups = 4 * a.tiles, g = blockIdx.x % groups;  // of a unit's rows
+  const int64_t unit = blockIdx.x / groups;
+  const int2 shares = a.shares[unit];
+  const int block = (int)(unit % a.blocks), kv = (int)(unit / a.blocks % a.kv_heads), s = (int)(unit / a.blocks / a.kv_heads);
   const Sequence seq = sequence_of(a, s);
-  if (t >= seq.rows) return;
-  const int64_t row = (int64_t)(seq.begin + t) * a.heads + h;
-  // (chunks past the sequence's newest token are not written)
-  const int chunks = min(a.chunks, (max(seq.length - seq.base, 0) + a.chunk - 1) / a.chunk);
-  const float2* tops = reinterpret_cast<const float2*>(a.part) + row * a.chunks;
-  const float* part = a.part + 2 * (int64_t)a.chunks * a.rows * a.heads + row * a.chunks * head;
-  float top = -__builtin_inff();
-  for (int c = lane; c < chunks; c += 64) top = fmaxf(top, tops[c].x);
+  const int all = min(seq.rows, a.most_rows) * a.group, r0 = block * 16 * a.tiles + g * R;
+  if (r0 >= all || shares.y == 1) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  float top[R], sum[R];
+  float4 v[V];
 #pragma unroll
-  for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-  float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int c0 = 0; c0 < chunks; c0 += 64) {
-    float by = 0.f;
-    if (c0 + lane < chunks) {
-      const float2 of = tops[c0 + lane];
-      by = of.x == top ? 1.f : __builtin_amdgcn_exp2f(of.x - top);
-      sum += of.y * by;
+  for (int r = 0; r < R; ++r) top[r] = -__builtin_inff(), sum[r] = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = wave; p0 < shares.y; p0 += W * K) {
+    float4 of[K][2], x[K][V];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int p = min(p0 + k * W, shares.y - 1);
+      const Slot slot = slot_of(a, 2 * (shares.x + p) + (p == 0), D);
+      of[k][0] = reinterpret_cast<const float4*>(slot.top + 2 * g * R)[0];
+      of[k][1] = reinterpret_cast<const float4*>(slot.top + 2 * g * R)[1];
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[k][i] = reinterpret_cast<const float4*>(slot.out + g * R * D)[min(lane + 64 * i, D - 1)];
     }
-    const int end = min(chunks - c0, 64);
-    for (int c = wave; c < end; c += W) {
-      const float w = __shfl(by, c);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < head) v[i] += part[(int64_t)(c0 + c) * head + lane + 64 * i] * w;
+    for (int k = 0; k < K; ++k) {
+      if (p0 + k * W >= shares.y) break;
+      const float m[R] = {of[k][0].x, of[k][0].z, of[k][1].x, of[k][1].z}, l[R] = {of[k][0].y, of[k][0].w, of[k][1].y, of[k][1].w};
+      float keep[R], take[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float most = fmaxf(top[r], m[r]);
+        keep[r] = top[r] == most ? 1.f : __builtin_amdgcn_exp2f(top[r] - most);
+        take[r] = m[r] == most ? 1.f : __builtin_amdgcn_exp2f(m[r] - most);
+        top[r] = most;
+        sum[r] = sum[r] * keep[r] + l[r] * take[r];
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int r = (lane + 64 * i) * 4 / D;
+        const float f = r == 0 ? keep[0] : r == 1 ? keep[1] : r == 2 ? keep[2] : keep[3];
+        const float t = r == 0 ? take[0] : r == 1 ? take[1] : r == 2 ? take[2] : take[3];
+        v[i].x = v[i].x * f + x[k][i].x * t;
+        v[i].y = v[i].y * f + x[k][i].y * t;
+        v[i].z = v[i].z * f + x[k][i].z * t;
+        v[i].w = v[i].w * f + x[k][i].w * t;
+      }
     }
   }
 #pragma unroll
-  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < head) out[wave][lane + 64 * i] = v[i];
+  for (int i = 0; i < V; ++i) out[wave][lane + 64 * i] = v[i];
+  if (lane < R) tops[wave][lane] = lane == 0 ? top[0] : lane == 1 ? top[1] : lane == 2 ? top[2] : top[3];
+  if (lane < R) sums[wave][lane] = lane == 0 ? sum[0] : lane == 1 ? sum[1] : lane == 2 ? sum[2] : sum[3];
   __syncthreads();
-  T* y = static_cast<T*>(a.y) + (int64_t)(seq.begin + t) * a.ldy + (int64_t)h * head;
-  if ((int)threadIdx.x < head) {
-    float all = out[0][threadIdx.x];
+  for (int e = threadIdx.x; e < R * D; e += 64 * W) {
+    const int r = e / D;
+    if (r0 + r >= all) break;
+    float most = tops[0][r], z = 0.f, y = 0.f;
 #pragma unroll
-    for (int w = 1; w < W; ++w) all += out[w][threadIdx.x];
-    y[threadIdx.x] = (T)(sum == 0.f ? 0.f : all / sum);
+    for (int w = 1; w < W; ++w) most = fmaxf(most, tops[w][r]);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float by = tops[w][r] == most ? 1.f : __builtin_amdgcn_exp2f(tops[w][r] - most);
+      z += sums[w][r] * by;
+      y += reinterpret_cast<const float*>(out[w])[e] * by;
+    }
+    const int t = (r0 + r) / a.group, h = kv * a.group + r0 + r - t * a.group;
+    static_cast<T*>(a.y)[(int64_t)(seq.begin + t) * a.ldy + (int64_t)h * D + e - r * D] = (T)(z == 0.f ? 0.f : y / z);
   }
 }
 
@@ -548,41 +647,48 @@ template <int TYPE, int D>
 constexpr int kMostTiles = most_tiles(kParts<TYPE>, D);
 
 // How a call is cut: by its sizes alone, so that its workspace can be made ahead.
-struct Cut { int tiles; bool shared; int blocks, chunk, chunks; size_t space; };
+struct Cut { int tiles, blocks, workgroups, chunk, chunks; int64_t units, most; size_t part, shares, space; };
 Cut cut_of(const tetris_cache* c, const tetris_attention* a, int type) {
   Cut k{};
-  const int group = a->heads / c->kv_heads;
-  const int64_t rows = (int64_t)std::min(a->most_rows, a->rows) * group, units = (int64_t)a->sequences * c->kv_heads;
-  k.tiles = most_tiles(parts_of(type), c->head);
-  const int64_t own = (rows + 64 * k.tiles - 1) / (64 * k.tiles);  // workgroups of four blocks
-  k.shared = rows <= 32 || units * own < 256;
-  if (rows <= 16) k.tiles = 1;
+  const int64_t rows = (int64_t)std::min(a->most_rows, a->rows) * (a->heads / c->kv_heads);
+  k.tiles = rows <= 16 ? 1 : most_tiles(parts_of(type), c->head);
   k.blocks = (int)((rows + 16 * k.tiles - 1) / (16 * k.tiles));
   const int64_t span = a->window ? std::min<int64_t>(a->most_length, (int64_t)a->window + a->most_rows + kStep) : a->most_length;
-  int64_t chunks = 1;
-  // about 1024 workgroups, of at least two steps a wave
-  if (k.shared) chunks = std::max<int64_t>(1, std::min<int64_t>(1024 / std::max<int64_t>(units * k.blocks, 1), (span + 8 * kStep - 1) / (8 * kStep)));
-  k.chunk = (int)(((span + chunks - 1) / chunks + 4 * kStep - 1) / (4 * kStep) * (4 * kStep));
-  if (k.chunk == 0) k.chunk = 4 * kStep;
-  k.chunks = (int)std::max<int64_t>(1, (span + k.chunk - 1) / k.chunk);
-  if (k.chunks > 1) k.space = (size_t)k.chunks * a->rows * a->heads * (c->head + 2) * sizeof(float);
+  const int64_t quanta = std::max<int64_t>((span + kQuantum - 1) / kQuantum, 1);
+  k.units = (int64_t)a->sequences * c->kv_heads * k.blocks;
+  k.most = k.units * (quanta + kBegin);
+  const int resident = 256 * waves_of(parts_of(type), c->head, k.tiles);
+  if (a->sequences > 1 && k.most >= 16 * (int64_t)resident) {
+    k.workgroups = resident;
+  } else {
+    const int64_t chunks = std::min<int64_t>(std::max<int64_t>(resident / std::max<int64_t>(k.units, 1), 1), quanta);
+    k.chunk = (int)((quanta + chunks - 1) / chunks);
+    k.chunks = (int)((quanta + k.chunk - 1) / k.chunk);
+    k.workgroups = (int)std::min<int64_t>(k.units * k.chunks, 0x7fffffff);
+  }
+  if (k.chunks != 1) k.part = (size_t)k.workgroups * 2 * 16 * k.tiles * (c->head + 2) * sizeof(float);
+  k.part = (k.part + 15) / 16 * 16;
+  k.shares = (size_t)k.units * sizeof(int2);
+  k.space = k.part + k.shares;
   return k;
 }
 
 template <int TYPE, int D>
 int launch(Attend a, const Cut& k, hipStream_t s) {
-  const int64_t groups = (int64_t)k.chunks * a.kv_heads * a.sequences * (k.shared ? k.blocks : ceil_div(k.blocks, 4));
-  const int64_t joined = k.chunks > 1 ? (int64_t)a.sequences * a.most_rows * a.heads : 0;
-  if (std::max(groups, joined) > 0x7fffffff) return fail(TETRIS_EUNSUPPORTED, "%lld workgroups are more than a launch has", (long long)std::max(groups, joined));
-  const dim3 grid((unsigned)groups), block(256);
-  if (!k.shared) hipLaunchKernelGGL((attend_kernel<TYPE, D, kMostTiles<TYPE, D>, false>), grid, block, 0, s, a);
-  else if (k.tiles == 1) hipLaunchKernelGGL((attend_kernel<TYPE, D, 1, true>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((attend_kernel<TYPE, D, kMostTiles<TYPE, D>, true>), grid, block, 0, s, a);
-  TETRIS_HIP(hipGetLastError());
-  if (joined) {
-    hipLaunchKernelGGL((join_kernel<TYPE>), dim3((unsigned)joined), block, 0, s, a, D);
-    TETRIS_HIP(hipGetLastError());
+  const dim3 grid((unsigned)k.workgroups), block(256);
+  if (k.chunk) {
+    if (k.tiles == 1) hipLaunchKernelGGL((attend_chunks_kernel<TYPE, D, 1>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((attend_chunks_kernel<TYPE, D, kMostTiles<TYPE, D>>), grid, block, 0, s, a);
+  } else {
+    if (k.tiles == 1) hipLaunchKernelGGL((attend_shares_kernel<TYPE, D, 1>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((attend_shares_kernel<TYPE, D, kMostTiles<TYPE, D>>), grid, block, 0, s, a);
   }
+  TETRIS_HIP(hipGetLastError());
+  if (k.chunks == 1) return TETRIS_OK;
+  const dim3 joins((unsigned)(k.units * 4 * k.tiles));
+  if (k.workgroups <= 4 * k.units) hipLaunchKernelGGL((join_kernel<TYPE, D, 4>), joins, block, 0, s, a);
+  else hipLaunchKernelGGL((join_kernel<TYPE, D, 16>), joins, dim3(1024), 0, s, a);
+  TETRIS_HIP(hipGetLastError());
   return TETRIS_OK;
 }
 template <int TYPE>
@@ -641,6 +747,8 @@ extern "C" int tetris_cache_attend(tetris_cache* c, const tetris_attention* a, c
   if (d_q == d_y) return fail(TETRIS_EINVAL, "the output is the input");
   if ((rc = check_cache(c))) return rc;
   const Cut k = cut_of(c, a, type);
+  if (k.most > 0x7fffffff || k.units * 4 * k.tiles > 0x7fffffff)
+    return fail(TETRIS_EUNSUPPORTED, "%d sequences of up to %d rows and %d tokens are more than a launch has", a->sequences, a->most_rows, a->most_length);
   uint8_t* d = nullptr;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if ((rc = c->space.get(s, k.space, &d))) return rc;
@@ -648,12 +756,13 @@ extern "C" int tetris_cache_attend(tetris_cache* c, const tetris_attention* a, c
   t.data = c->data; t.q = d_q; t.y = d_y;
   t.first = d_first; t.length = d_length; t.table = d_table;
   t.part = reinterpret_cast<float*>(d);
+  t.shares = reinterpret_cast<int2*>(d + k.part);
   t.page_bytes = c->page_bytes; t.ldt = ld_table; t.ldq = ldq; t.ldy = ldy;
   t.pages = c->pages; t.page = c->page; t.granules = c->page / kGranule;
   t.kv_heads = c->kv_heads; t.heads = a->heads; t.group = a->heads / c->kv_heads;
   t.sequences = a->sequences; t.rows = a->rows; t.most_rows = std::min(a->most_rows, a->rows); t.most_length = a->most_length;
   t.window = std::min(a->window, a->most_length);
-  t.blocks = k.blocks; t.chunk = k.chunk; t.chunks = k.chunks;
+  t.tiles = k.tiles; t.blocks = k.blocks; t.workgroups = k.workgroups; t.chunk = k.chunk; t.chunks = k.chunks;
   const int size = elem_size(type);
   t.whole = (reinterpret_cast<size_t>(d_q) & 15) == 0 && ldq * size % 16 == 0;
   t.scale = a->scale == 0.f ? 1.f : std::fabs(a->scale) * 1.44269504088896340736f;
