@@ -44,7 +44,9 @@ def attend(q, k, v, scale, kind, window=0, absent=()):
     y and its bound:
       a score       sums of `head` products, one rounding for each eight of each of up to three parts of q and 40 more, of the size that the
                     magnitudes bound; three roundings (scale, its conversion to powers of two, the product) and one of what is left of the maximum
-      a weight      the score's error, as relative; an exponential within 2^-22; in two parts of 8 bits, the last rounded: 2^-16
+      a weight      the score's error, as relative; an exponential within 2^-22; in two parts of 8 bits, the last rounded: 2^-16.  It is relative to
+                    the row's largest, and what is below 32 bits' normal numbers, of the exponential or of one of up to three parts, may become
+                    zero: 4 times 2^-126 and no more, as the arithmetic's own maximum is not above the row's
       the sums      one rounding for each eight weights of each part and 100 more
     """
     n, heads, head = q.shape
@@ -65,6 +67,6 @@ def attend(q, k, v, scale, kind, window=0, absent=()):
             z = w.sum()
             sums = (3 * see.sum() / 8 + 100) * 2 * ONE
             y[i, h] = w @ vv / z
-            e = ((w * (ew + sums)) @ np.abs(vv) + np.abs(y[i, h]) * (w * (ew + sums)).sum()) / z * 1.01
+            e = ((w * (ew + sums) + 2.0 ** -124) @ np.abs(vv) + np.abs(y[i, h]) * (w * (ew + sums)).sum()) / z * 1.01
             far[i, h] = e + ROUNDING[kind] * (np.abs(y[i, h]) + e) + LEAST[kind]
     return y, far

@@ -41,23 +41,34 @@ struct Attend {
   int blocks;  // most blocks of 16 NT rows of a sequence and kv head
   int workgroups;
   int chunk, chunks;  // quanta of a workgroup, or zero for equal shares; most chunks of a unit
-  int whole;   // rows of q lie on 16 bytes
+  int whole, y_whole;  // rows of q, of y lie on 16 bytes
   unsigned page_magic;  // to divide by granules (0 where that is one)
   float scale;  // to powers of two, not negative
   float sign;  // what q is multiplied by: scale's sign, or zero where scale is
 };
 
+// What nothing writes while a kernel runs, from an address that is the wave's: by the scalar unit, also behind barriers and stores, where the compiler
+// would not take it for unchanged.
+template <typename V>
+__device__ inline V fixed(const V* p) { return *(const __attribute__((address_space(4))) V*)(reinterpret_cast<uintptr_t>(p)); }
+
 // What a sequence is: its rows and tokens, whatever the arrays hold.
 struct Sequence { int begin, rows, length, base; };
-__device__ inline Sequence sequence_of(const Attend& a, int s) {
+__device__ inline Sequence sequence_from(const Attend& a, int s, int first, int behind, int length) {
   Sequence q;
-  q.begin = a.first ? min(max(a.first[s], 0), a.rows) : s;
-  const int end = a.first ? min(max(a.first[s + 1], q.begin), a.rows) : s + 1;
+  q.begin = a.first ? min(max(first, 0), a.rows) : s;
+  const int end = a.first ? min(max(behind, q.begin), a.rows) : s + 1;
   q.rows = end - q.begin;
-  q.length = min(max(a.length[s], 0), a.most_length);
+  q.length = min(max(length, 0), a.most_length);
   // the first token that any row sees, down to a whole step
   q.base = a.window ? max(q.length - q.rows - a.window + 1, 0) & ~(kStep - 1) : 0;
   return q;
+}
+__device__ inline Sequence sequence_of(const Attend& a, int s) {  // the wave's
+  return sequence_from(a, s, a.first ? fixed(a.first + s) : 0, a.first ? fixed(a.first + s + 1) : 0, fixed(a.length + s));
+}
+__device__ inline Sequence sequence_of_lane(const Attend& a, int s) {
+  return sequence_from(a, s, a.first ? a.first[s] : 0, a.first ? a.first[s + 1] : 0, a.length[s]);
 }
 
 template <int TYPE>
@@ -213,6 +224,80 @@ struct Rows {
     }
   }
 
+  // whether the lane's row sees token 4 (lane / 16) + i of granule u
+  __device__ inline bool sees(const Attend& a, int n, int u, int i, int at, const int (&upto)[2], int lane) const {
+    const int place = 4 * (lane >> 4) + i, j = at + 16 * u + place;
+    return place < upto[u] && j <= last[n] && (!a.window || j > last[n] - a.window);
+  }
+  // what the rows do not see of 32 tokens out of their scores
+  __device__ inline void mask(const Attend& a, f32x4 (&x)[NT][2], int at, const int (&upto)[2], int lane) const {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[n][u][i] = sees(a, n, u, i, at, upto, lane) ? x[n][u][i] : -__builtin_inff();
+  }
+  // ones for what they see, in the form of a product's second operand
+  __device__ inline i32x4 seen(const Attend& a, int n, int at, const int (&upto)[2], int lane) const {
+    i32x4 ones{};
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ones[2 * u + i / 2] |= sees(a, n, u, i, at, upto, lane) ? 0x3f80 << (16 * (i & 1)) : 0;
+    return ones;
+  }
+
+  // Scores of 32 tokens (lane 16 g + r has tokens 4 g .. 4 g + 3 of each granule for row r) to weights in parts, with the sums and the bounds m brought up to
+  // date.
+  __device__ inline void weights(const Attend& a, f32x4 (&x)[NT][2], i32x4 (&p)[PP][NT]) {
+    float top[NT];
+    bool above = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      top[n] = -__builtin_inff();
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top[n] = fmaxf(top[n], x[n][u][i]);
+      top[n] *= a.scale;
+      // Taken before the branch: where a branch comes between a matrix instruction and the first use of its result, the compiler has left out
+      // the wait that the instruction needs (tests/test_matrix_waits.py looks for that in the built library).
+      asm volatile("" : "+v"(top[n]));
+      above = above || top[n] > m[n] + kRoom;
+    }
+    if (__ballot(above)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float best = max_of_row(top[n]), higher = best > m[n] + kRoom ? best : m[n];  // (a row's own matter, whatever its neighbours do)
+        const float by = m[n] == higher ? 1.f : __builtin_amdgcn_exp2f(m[n] - higher);
+        m[n] = higher;
+        l[n] *= by;
+#pragma unroll
+        for (int j = 0; j < S; ++j) o[n][j] *= by;
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float base = m[n] == -__builtin_inff() ? 0.f : -m[n];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[n][u][i] = __builtin_amdgcn_exp2f(fmaf(x[n][u][i], a.scale, base));
+          l[n] += x[n][u][i];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          unsigned parts[PP];
+          split_pair<PP>(x[n][u][2 * i], x[n][u][2 * i + 1], parts);
+#pragma unroll
+          for (int k = 0; k < PP; ++k) p[k][n][2 * u + i] = (int)parts[k];
+        }
+      }
+    }
+  }
+
   // 32 tokens from `at` on, upto[u] of granule u's 16 in the sequence.  EDGE: some row does not see all of them.
   template <bool EDGE>
   __device__ inline void step(const Attend& a, Granule<D> (&g)[2], int at, const int (&upto)[2], int lane) {
@@ -232,7 +317,7 @@ struct Rows {
             if (!there) g[u].vs[c] = (g[u].vs[c] & ~(255u << (8 * i))) | 127u << (8 * i);  // whatever lies there, it counts as a number
           }
     }
-    i32x4 p[PP][NT], seen[NT];
+    i32x4 p[PP][NT];
     f32x4 x[NT][2];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -244,51 +329,8 @@ struct Rows {
 #pragma unroll
           for (int i = QP - 1; i >= 0; --i) x[n][u] = product(key, q[i][n][w], w == 0 && i == QP - 1 ? f32x4{0.f, 0.f, 0.f, 0.f} : x[n][u]);
       }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float top = -__builtin_inff();
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (EDGE) {
-            const int place = 4 * quad + i, j = at + 16 * u + place;
-            const bool see = place < upto[u] && j <= last[n] && (!a.window || j > last[n] - a.window);
-            x[n][u][i] = see ? x[n][u][i] : -__builtin_inff();
-            const int one = see ? 0x3f80 : 0, k = 2 * u + i / 2;
-            seen[n][k] = i & 1 ? seen[n][k] | one << 16 : one;
-          }
-          top = fmaxf(top, x[n][u][i]);
-        }
-      top *= a.scale;
-      // Taken before the branch: where a branch comes between a matrix instruction and the first use of its result, the compiler has left out
-      // the wait that the instruction needs (tests/test_matrix_waits.py looks for that in the built library).
-      asm volatile("" : "+v"(top));
-      if (__ballot(top > m[n] + kRoom)) {
-        const float best = max_of_row(top), higher = best > m[n] + kRoom ? best : m[n];  // (a row's own matter, whatever its neighbours do)
-        const float by = m[n] == higher ? 1.f : __builtin_amdgcn_exp2f(m[n] - higher);
-        m[n] = higher;
-        l[n] *= by;
-#pragma unroll
-        for (int j = 0; j < S; ++j) o[n][j] *= by;
-      }
-      const float base = m[n] == -__builtin_inff() ? 0.f : -m[n];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[n][u][i] = __builtin_amdgcn_exp2f(fmaf(x[n][u][i], a.scale, base));
-          l[n] += x[n][u][i];
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          unsigned parts[PP];
-          split_pair<PP>(x[n][u][2 * i], x[n][u][2 * i + 1], parts);
-#pragma unroll
-          for (int k = 0; k < PP; ++k) p[k][n][2 * u + i] = (int)parts[k];
-        }
-      }
-    }
+    if constexpr (EDGE) mask(a, x, at, upto, lane);
+    weights(a, x, p);
     if constexpr (EDGE) {
       if (__ballot(nan)) {
         // A NaN that some rows see and others do not: rows that see it get it by a product of their own (a one for each
@@ -303,7 +345,7 @@ struct Rows {
               is_nan[2 * u + i / 2] |= (g[u].vs[neighbours(D) ? 0 : c] >> (8 * i) & 255u) == 255u ? 0x3f80 << (16 * (i & 1)) : 0;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const f32x4 hit = product(is_nan, seen[n], f32x4{0.f, 0.f, 0.f, 0.f});
+            const f32x4 hit = product(is_nan, seen(a, n, at, upto, lane), f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const float add = hit[i] > 0.f ? __builtin_nanf("") : 0.f;
@@ -356,7 +398,7 @@ __device__ inline Units units_of(const Attend& a, const Sequence& q) {
 }
 __device__ inline int quanta_of(const Attend& a, int s) {
   if (s >= a.sequences) return 0;
-  const Units u = units_of(a, sequence_of(a, s));
+  const Units u = units_of(a, sequence_of_lane(a, s));
   return (u.quanta + kBegin) * u.blocks * a.kv_heads;
 }
 
@@ -407,7 +449,7 @@ __device__ inline void attend_unit(const Attend& a, const Sequence& seq, int qua
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       // (read wherever the table has an entry, so that it need not wait for the sequence's length)
-      const int page = table[page_index(a, (unsigned)min(at + 16 * u, a.most_length - 1) / 16)];
+      const int page = fixed(table + page_index(a, (unsigned)min(at + 16 * u, a.most_length - 1) / 16));
       p.page[u] = at + 16 * u < seq.length && (unsigned)page < (unsigned)a.pages ? page : -1;
     }
     return p;
@@ -561,6 +603,282 @@ __global__ __launch_bounds__(256, waves_of(kParts<TYPE>, D, NT)) void attend_sha
   }
 }
 
+// All waves' writes to LDS are done; loads from memory may be under way (__syncthreads would wait for them too).
+__device__ inline void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Many rows of a sequence: four waves, each with 16 NT rows of its own, share what is made of the keys and values of 64 tokens: each makes a quarter of it
+// bf16, in the form in which the products take it, and leaves it in LDS (8 KiB for 32 elements of a head, twice, so that one barrier a turn is enough).
+constexpr int kPromptWaves = 4, kTurn = 64;
+template <int D>
+struct Share {
+  static constexpr int N = D / 32, KS = neighbours(D) ? (D + 127) / 128 : N, VS = neighbours(D) ? 1 : N;
+  static constexpr int VU = (N + 1) / 2;  // bytes of a token's values
+  // the keys of granule `wave`; of the values of 32 tokens (the first or the last two granules, by the wave's lowest bit) every second byte from wave / 2 on
+  unsigned k[N], ks[KS], v[2][N], vs[2][VS];
+
+  __device__ inline void load(const uint8_t* g, const uint8_t* v0, const uint8_t* v1, int lane) {
+    const int r = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < N; ++i) k[i] = (reinterpret_cast<const unsigned*>(g) + i)[(unsigned)lane * N];
+#pragma unroll
+    for (int i = 0; i < KS; ++i) ks[i] = (g + 16 * D)[(unsigned)(r * N + (neighbours(D) ? q * D / 128 + i : (q * (D / 4) + 8 * i) / 32))];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint8_t* from = u ? v1 : v0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[u][i] = (reinterpret_cast<const unsigned*>(from + 8 * D) + i)[(unsigned)lane * N];
+#pragma unroll
+      for (int i = 0; i < VS; ++i) vs[u][i] = (reinterpret_cast<const unsigned*>(from + 16 * D + D / 2) + (neighbours(D) ? 0 : i))[(unsigned)(q * N + (neighbours(D) ? r * (D / 16) / 32 : 0))];
+    }
+  }
+  // To LDS.  Values that are NaN are zeros there, and so are those behind the newest token, whatever they are.  nans: whether 32 tokens have a NaN, and then
+  // which (nan_of[token][block]).
+  __device__ inline void store(i32x4* keys, i32x4* values, int* nans, uint8_t* nan_of, const int (&upto)[4], int wave, int lane) {
+    const int half = wave & 1, c0 = wave >> 1;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float s = __uint_as_float(ks[neighbours(D) ? i / 4 : i] << 23);
+      keys[(wave * N + i) * 64 + lane] = i32x4{(int)pair<0>(k[i], s), (int)pair<1>(k[i], s), (int)pair<2>(k[i], s), (int)pair<3>(k[i], s)};
+    }
+    const int there[2] = {half ? upto[2] : upto[0], half ? upto[3] : upto[1]};
+    bool full = false;  // some scale is 255
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int c = 0; c < VS; ++c) full = full || (((vs[u][c] & 0x7f7f7f7fu) + 0x01010101u) & vs[u][c] & 0x80808080u) != 0;
+    i32x4* to = values + half * 2 * N * 64 + lane;
+    if (there[0] == 16 && there[1] == 16 && !__ballot(full)) {
+      if (c0 == 0 && lane == 0) nans[half] = 0;
+      convert<false>(to, c0, {});
+      return;
+    }
+    bool nan = false;
+    unsigned gone[2] = {};  // what counts as zero: bit 4 c + i for token i and the c-th word of scales
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int c = 0; c < VS; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int token = 4 * (lane >> 4) + i;
+          const bool in = token < there[u], is = in && (vs[u][c] >> (8 * i) & 255u) == 255u;
+          nan = nan || is;
+          if (c0 == 0) nan_of[(half * 32 + u * 16 + token) * N + (neighbours(D) ? (lane & 15) * (D / 16) / 32 : c)] = is;
+          if (is || !in) gone[u] |= 1u << (4 * c + i);
+        }
+    const int any = __ballot(nan) != 0;
+    if (c0 == 0 && lane == 0) nans[half] = any;
+    convert<true>(to, c0, {gone[0], gone[1]});
+  }
+  template <bool SPECIAL>
+  __device__ inline void convert(i32x4* to, int c0, uint2 gone) {
+    unsigned codes[2][N];  // from byte c0 of the first token on
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < N; ++i) codes[u][i] = __builtin_amdgcn_alignbyte(i + 1 < N ? v[u][i + 1] : 0u, v[u][i], (unsigned)c0);
+#pragma unroll
+    for (int j = 0; j < VU; ++j) {
+      const int c = c0 + 2 * j;
+      if (c >= N) break;
+      i32x4 even, odd;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const unsigned scales = neighbours(D) ? vs[u][0] : c0 && 2 * j + 1 < VS ? vs[u][2 * j + 1 < VS ? 2 * j + 1 : 0] : vs[u][2 * j];
+        unsigned t[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int b = i * N + 2 * j;
+          const float scale = scale_of(scales, i);
+          t[i] = pair_at(codes[u][b / 4], scale, b % 4);
+          if (SPECIAL) t[i] = (u ? gone.y : gone.x) >> ((VS > 1 ? 4 * c : 0) + i) & 1u ? 0u : t[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          even[2 * u + i] = (int)__builtin_amdgcn_perm(t[2 * i + 1], t[2 * i], 0x05040100u);
+          odd[2 * u + i] = (int)__builtin_amdgcn_perm(t[2 * i + 1], t[2 * i], 0x07060302u);
+        }
+      }
+      to[2 * c * 64] = even;
+      to[(2 * c + 1) * 64] = odd;
+    }
+  }
+};
+
+template <int TYPE, int D, int NT>
+__global__ __launch_bounds__(64 * kPromptWaves, 2) void attend_prompt_kernel(Attend a) {
+  using T = typename Elem<TYPE>::type;
+  using R = Rows<TYPE, D, NT>;
+  constexpr int N = D / 32, S = D / 16, W = kPromptWaves, QP = R::QP, PP = R::PP;
+  __shared__ i32x4 keys[2][4 * N * 64], values[2][4 * N * 64];
+  __shared__ int nans[2][2];
+  __shared__ uint8_t nan_of[2][kTurn * N];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, quad = lane >> 4;
+  // (kv heads first: the workgroups of one kv head are a multiple of 8 apart where there are 8, 16, .. kv heads, on one of the eight dies, whose cache then
+  // holds this kv head's tokens; the last rows first, which see the most)
+  int id = blockIdx.x;
+  const int kv = id % a.kv_heads;
+  id /= a.kv_heads;
+  const int s = id % a.sequences, group = (a.blocks + W - 1) / W - 1 - id / a.sequences;
+  const Sequence seq = sequence_of(a, s);
+  const int all = min(seq.rows, a.most_rows) * a.group, w0 = group * W * (16 * NT), r0 = w0 + wave * (16 * NT);
+  if (w0 >= all) return;
+  const int p0 = seq.length - seq.rows;
+  // the tokens that some row of the workgroup sees, and of the wave
+  auto span = [&](int first, int count, int& from, int& to) {
+    const int t0 = first / a.group, t1 = min(first + count - 1, all - 1) / a.group;
+    from = a.window ? max(p0 + t0 - a.window + 1, 0) : 0;
+    to = first < all ? min(p0 + t1, seq.length - 1) + 1 : 0;
+  };
+  int from, to, mine_from, mine_to;
+  span(w0, W * 16 * NT, from, to);
+  span(r0, 16 * NT, mine_from, mine_to);
+  from &= ~(kTurn - 1);
+  const int t0 = r0 / a.group, t1 = min(r0 + 16 * NT - 1, all - 1) / a.group;
+
+  const int* table = a.table + s * a.ldt;
+  const uint8_t* head = a.data + (int64_t)kv * a.granules * (17 * D);
+  Share<D> share;
+  // The table's entries from `entry` on, a lane each.
+  const int entries = (int)page_index(a, (unsigned)max(a.most_length - 1, 0) / 16) + 1;
+  int entry = 0, page_of_lane = 0;
+  auto turn_table = [&](int to) {
+    entry = to;
+    page_of_lane = table[min(entry + lane, entries - 1)];
+  };
+  // Asks for the wave's share of 64 tokens; the granules that are there, a bit each.
+  auto ask = [&](int at) {
+    const unsigned g0 = (unsigned)at / 16;
+    int page[4], place[4], there = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int index = (int)page_index(a, g0 + u);
+      if (index >= entry + 64) turn_table(index);
+      const int p = __builtin_amdgcn_readlane(page_of_lane, index - entry);
+      const bool good = at + 16 * u < seq.length && (unsigned)p < (unsigned)a.pages;
+      there |= good << u;
+      page[u] = good ? p : 0;
+      place[u] = (int)(g0 + u) - index * a.granules;
+    }
+    auto granule = [&](int page, int place) { return head + (int64_t)page * a.page_bytes + place * (17 * D); };
+    const bool odd = wave & 1, high = wave & 2;
+    share.load(granule(high ? (odd ? page[3] : page[2]) : odd ? page[1] : page[0], high ? (odd ? place[3] : place[2]) : odd ? place[1] : place[0]),
+               granule(odd ? page[2] : page[0], odd ? place[2] : place[0]), granule(odd ? page[3] : page[1], odd ? place[3] : place[1]), lane);
+    return there;
+  };
+  int next = 0;
+  if (from < to) {
+    turn_table((int)page_index(a, (unsigned)from / 16));
+    next = ask(from);
+  }
+  R rows;
+  rows.begin(a, seq, kv, r0, all, lane);
+  unsigned lost[NT] = {};  // outputs that are NaN: bit i for elements of row 4 (lane / 16) + i of all products, or 4 c + i for those of products 2 c and 2 c + 1
+  int buffer = 0;
+  for (int at = from; at < to; at += kTurn, buffer ^= 1) {
+    const int granules = __builtin_amdgcn_readfirstlane(next), behind = seq.length - at;
+    int upto[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) upto[u] = granules >> u & 1 ? min(behind - 16 * u, 16) : 0;
+    share.store(keys[buffer], values[buffer], nans[buffer], nan_of[buffer], upto, wave, lane);
+    if (at + kTurn < to) next = ask(at + kTurn);
+    lds_barrier();
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+      const int begin = at + h * kStep;
+      if (begin >= mine_to || begin + kStep <= mine_from) continue;
+      const int there[2] = {h ? upto[2] : upto[0], h ? upto[3] : upto[1]};
+      const bool plain = there[0] == 16 && there[1] == 16 && begin + kStep - 1 <= p0 + t0 && (!a.window || begin > p0 + t1 - a.window);
+      f32x4 x[NT][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int w = 0; w < N; ++w) {
+          const i32x4 key = keys[buffer][((2 * h + u) * N + w) * 64 + lane];
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = QP - 1; i >= 0; --i) x[n][u] = product(key, rows.q[i][n][w], w == 0 && i == QP - 1 ? f32x4{0.f, 0.f, 0.f, 0.f} : x[n][u]);
+        }
+      // (used before the branch: see Rows::weights)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float v = x[n][u][i];
+            asm volatile("" : "+v"(v));
+            x[n][u][i] = v;
+          }
+      if (!plain) rows.mask(a, x, begin, there, lane);
+      i32x4 p[PP][NT];
+      rows.weights(a, x, p);
+      if (__builtin_amdgcn_readfirstlane(nans[buffer][h])) {
+        // A NaN that some rows see and others do not: those that see it are found by a product of a one for each NaN value by a one for each token
+        // that is seen.  The value itself is zero in LDS.
+#pragma unroll
+        for (int c = 0; c < (neighbours(D) ? 1 : N); ++c) {
+          i32x4 ones{};
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              ones[2 * u + i / 2] |= nan_of[buffer][(h * 32 + u * 16 + 4 * quad + i) * N + (neighbours(D) ? r16 * (D / 16) / 32 : c)] ? 0x3f80 << (16 * (i & 1)) : 0;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const f32x4 hit = product(ones, rows.seen(a, n, begin, there, lane), f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int i = 0; i < 4; ++i) lost[n] |= (hit[i] > 0.f ? 1u : 0u) << (4 * c + i);
+          }
+        }
+      }
+      const i32x4* value = values[buffer] + h * 2 * N * 64 + lane;
+#pragma unroll
+      for (int j = 0; j < S; ++j) {
+        const i32x4 v = value[j * 64];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int k = PP - 1; k >= 0; --k) rows.o[n][j] = product(v, p[k][n], rows.o[n][j]);
+      }
+    }
+  }
+
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const float sum = sum_of_row(rows.l[n]);
+    const int r = r0 + n * 16 + r16;
+    if (r >= all) continue;
+    const int t = r / a.group, h = kv * a.group + r - t * a.group;
+    T* y = static_cast<T*>(a.y) + (int64_t)(seq.begin + t) * a.ldy + (int64_t)h * D;
+    auto output = [&](int j, int i) {
+      const bool nan = lost[n] >> (neighbours(D) ? i : 4 * (j / 2) + i) & 1u;
+      return (T)(nan ? __builtin_nanf("") : sum == 0.f ? 0.f : rows.o[n][j][i] / sum);
+    };
+    if (neighbours(D) && S * sizeof(T) >= 16 && a.y_whole) {  // a lane's S elements of a row lie together
+      constexpr int V = S * (int)sizeof(T) / 16 ? S * (int)sizeof(T) / 16 : 1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        T v[V * 16 / sizeof(T)];
+#pragma unroll
+        for (int j = 0; j < S; ++j) v[j] = output(j, i);
+#pragma unroll
+        for (int k = 0; k < V; ++k) reinterpret_cast<int4*>(y + element_of<D>(0, 4 * quad + i))[k] = reinterpret_cast<const int4*>(v)[k];
+      }
+    } else if (!neighbours(D) && a.y_whole) {  // four of them
+      typedef T T4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+      for (int j = 0; j < S; ++j) *reinterpret_cast<T4*>(y + element_of<D>(j, 4 * quad)) = T4{output(j, 0), output(j, 1), output(j, 2), output(j, 3)};
+    } else {
+#pragma unroll
+      for (int j = 0; j < S; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[element_of<D>(j, 4 * quad + i)] = output(j, i);
+    }
+  }
+}
+
 // Units that several workgroups have parts of: a workgroup of W waves joins four rows, a wave of it every W-th part.  What the parts' weights are is known
 // only with the last of their maxima, so a wave joins its own parts first, and all loads of a part are under way together.
 template <int TYPE, int D, int W>
@@ -647,7 +965,7 @@ template <int TYPE, int D>
 constexpr int kMostTiles = most_tiles(kParts<TYPE>, D);
 
 // How a call is cut: by its sizes alone, so that its workspace can be made ahead.
-struct Cut { int tiles, blocks, workgroups, chunk, chunks; int64_t units, most; size_t part, shares, space; };
+struct Cut { bool prompt; int tiles, blocks, workgroups, chunk, chunks; int64_t units, most; size_t part, shares, space; };
 Cut cut_of(const tetris_cache* c, const tetris_attention* a, int type) {
   Cut k{};
   const int64_t rows = (int64_t)std::min(a->most_rows, a->rows) * (a->heads / c->kv_heads);
@@ -657,6 +975,14 @@ Cut cut_of(const tetris_cache* c, const tetris_attention* a, int type) {
   const int64_t quanta = std::max<int64_t>((span + kQuantum - 1) / kQuantum, 1);
   k.units = (int64_t)a->sequences * c->kv_heads * k.blocks;
   k.most = k.units * (quanta + kBegin);
+  const int64_t turns = (int64_t)a->sequences * c->kv_heads * ((k.blocks + kPromptWaves - 1) / kPromptWaves);
+  const int PR=getenv("PR")?atoi(getenv("PR")):64, PW=getenv("PW")?atoi(getenv("PW")):64;
+  k.prompt = rows > PR && turns >= PW;
+  if (k.prompt) {
+    k.tiles = most_tiles(parts_of(type), c->head);
+    k.workgroups = (int)std::min<int64_t>(turns, 0x7fffffff);
+    return k;
+  }
   const int resident = 256 * waves_of(parts_of(type), c->head, k.tiles);
   if (a->sequences > 1 && k.most >= 16 * (int64_t)resident) {
     k.workgroups = resident;
@@ -676,6 +1002,11 @@ Cut cut_of(const tetris_cache* c, const tetris_attention* a, int type) {
 template <int TYPE, int D>
 int launch(Attend a, const Cut& k, hipStream_t s) {
   const dim3 grid((unsigned)k.workgroups), block(256);
+  if (k.prompt) {
+    hipLaunchKernelGGL((attend_prompt_kernel<TYPE, D, kMostTiles<TYPE, D>>), grid, dim3(64 * kPromptWaves), 0, s, a);
+    TETRIS_HIP(hipGetLastError());
+    return TETRIS_OK;
+  }
   if (k.chunk) {
     if (k.tiles == 1) hipLaunchKernelGGL((attend_chunks_kernel<TYPE, D, 1>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((attend_chunks_kernel<TYPE, D, kMostTiles<TYPE, D>>), grid, block, 0, s, a);
@@ -765,6 +1096,7 @@ extern "C" int tetris_cache_attend(tetris_cache* c, const tetris_attention* a, c
   t.tiles = k.tiles; t.blocks = k.blocks; t.workgroups = k.workgroups; t.chunk = k.chunk; t.chunks = k.chunks;
   const int size = elem_size(type);
   t.whole = (reinterpret_cast<size_t>(d_q) & 15) == 0 && ldq * size % 16 == 0;
+  t.y_whole = (reinterpret_cast<size_t>(d_y) & 15) == 0 && ldy * size % 16 == 0;
   t.scale = a->scale == 0.f ? 1.f : std::fabs(a->scale) * 1.44269504088896340736f;
   t.sign = a->scale == 0.f ? 0.f : a->scale < 0.f ? -1.f : 1.f;
   t.page_magic = magic_reciprocal(t.granules);
