@@ -44,7 +44,8 @@ def attend(q, k, v, scale, kind, window=0, absent=()):
     y and its bound:
       a score       sums of `head` products, one rounding for each eight of each of up to three parts of q and 40 more, of the size that the
                     magnitudes bound; three roundings (scale, its conversion to powers of two, the product) and one of what is left of the maximum
-      a weight      the score's error, as relative; an exponential within 2^-22; in two parts of 8 bits, the last rounded: 2^-16.  It is relative to
+      a weight      the score's error, as relative; an exponential within 2^-22; f16: in two parts of 8 bits, the last rounded, 2^-16; bf16: so, or
+                    in one of 11 bits, 2^-12, and below 2^-21 of the row's largest within 2^-32 of that.  It is relative to
                     the row's largest, and what is below 32 bits' normal numbers, of the exponential or of one of up to three parts, may become
                     zero: 4 times 2^-126 and no more, as the arithmetic's own maximum is not above the row's
       the sums      one rounding for each eight weights of each part and 100 more
@@ -63,10 +64,11 @@ def attend(q, k, v, scale, kind, window=0, absent=()):
             s, size = kk @ q[i, h] * scale, np.abs(kk) @ np.abs(q[i, h]) * abs(scale)
             off = (3 * head / 8 + 40) * 2 * ONE * size + 4 * ONE * np.abs(s)
             w = np.exp(s - s.max())
-            ew = np.expm1(off + off.max()) + 2.0 ** -22 + (2.0 ** -16 if kind != "f32" else 0)
+            ew = np.expm1(off + off.max()) + 2.0 ** -22 + {"f32": 0.0, "f16": 2.0 ** -16, "bf16": 2.0 ** -12}[kind]
+            least = 2.0 ** -32 if kind == "bf16" else 2.0 ** -124
             z = w.sum()
             sums = (3 * see.sum() / 8 + 100) * 2 * ONE
             y[i, h] = w @ vv / z
-            e = ((w * (ew + sums) + 2.0 ** -124) @ np.abs(vv) + np.abs(y[i, h]) * (w * (ew + sums)).sum()) / z * 1.01
+            e = ((w * (ew + sums) + least) @ np.abs(vv) + np.abs(y[i, h]) * (w * (ew + sums)).sum()) / z * 1.01
             far[i, h] = e + ROUNDING[kind] * (np.abs(y[i, h]) + e) + LEAST[kind]
     return y, far

@@ -76,6 +76,9 @@ constexpr int kParts = TYPE == TETRIS_BF16 ? 1 : TYPE == TETRIS_F16 ? 2 : 3;
 template <int TYPE>
 constexpr int kWeightParts = TYPE == TETRIS_F32 ? 3 : 2;
 
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
 // the i-th pair of the codes in a word to bf16
 template <int I>
 __device__ inline unsigned pair(unsigned codes, float scale) {
@@ -89,9 +92,21 @@ __device__ inline unsigned pair_at(unsigned codes, float scale, int i) {  // (i 
     default: return pair<3>(codes, scale);
   }
 }
+__device__ inline unsigned half_at(unsigned codes, float scale, int i) {  // to f16
+  switch (i) {
+    case 0: return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 0));
+    case 1: return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 1));
+    case 2: return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 2));
+    default: return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 3));
+  }
+}
 __device__ inline float scale_of(unsigned word, int byte) { return __uint_as_float((word >> (8 * byte) & 255u) << 23); }
 __device__ inline f32x4 product(i32x4 a, i32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+__device__ inline f32x4 half_product(i32x4 a, i32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
 // the leading 16 bits of v, and what they leave of it; nothing of an infinity or NaN
@@ -180,6 +195,7 @@ struct Rows {
   static constexpr int QP = kParts<TYPE>, PP = kWeightParts<TYPE>, N = D / 32, S = D / 16;
   i32x4 q[QP][NT][N];
   f32x4 o[NT][S];
+  f32x4 sums[NT];  // of weights multiplied as f16, the whole row's in every element
   float m[NT], l[NT];
   int last[NT];  // the newest token that the lane's row sees
 
@@ -217,66 +233,54 @@ struct Rows {
             q[p][n][w][i] = (int)(low | leading(v[2 * i + 1]) << 16);
           }
       }
+    }
+    reset();
+  }
+  __device__ inline void reset() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
       m[n] = -__builtin_inff();
       l[n] = 0.f;
+      sums[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < S; ++j) o[n][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
   }
 
   // whether the lane's row sees token 4 (lane / 16) + i of granule u
-  __device__ inline bool sees(const Attend& a, int n, int u, int i, int at, const int (&upto)[2], int lane) const {
+  template <int G>
+  __device__ inline bool sees(const Attend& a, int n, int u, int i, int at, const int (&upto)[G], int lane) const {
     const int place = 4 * (lane >> 4) + i, j = at + 16 * u + place;
     return place < upto[u] && j <= last[n] && (!a.window || j > last[n] - a.window);
   }
-  // what the rows do not see of 32 tokens out of their scores
-  __device__ inline void mask(const Attend& a, f32x4 (&x)[NT][2], int at, const int (&upto)[2], int lane) const {
+  // what the rows do not see of G granules out of their scores
+  template <int G>
+  __device__ inline void mask(const Attend& a, f32x4 (&x)[NT][G], int at, const int (&upto)[G], int lane) const {
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < G; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[n][u][i] = sees(a, n, u, i, at, upto, lane) ? x[n][u][i] : -__builtin_inff();
   }
-  // ones for what they see, in the form of a product's second operand
-  __device__ inline i32x4 seen(const Attend& a, int n, int at, const int (&upto)[2], int lane) const {
+  // ones for what they see of granules 2 h and 2 h + 1, in the form of a product's second operand
+  template <int G>
+  __device__ inline i32x4 seen(const Attend& a, int n, int h, int at, const int (&upto)[G], int lane) const {
     i32x4 ones{};
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) ones[2 * u + i / 2] |= sees(a, n, u, i, at, upto, lane) ? 0x3f80 << (16 * (i & 1)) : 0;
+      for (int i = 0; i < 4; ++i) ones[2 * u + i / 2] |= sees(a, n, 2 * h + u, i, at, upto, lane) ? 0x3f80 << (16 * (i & 1)) : 0;
     return ones;
   }
 
   // Scores of 32 tokens (lane 16 g + r has tokens 4 g .. 4 g + 3 of each granule for row r) to weights in parts, with the sums and the bounds m brought up to
   // date.
   __device__ inline void weights(const Attend& a, f32x4 (&x)[NT][2], i32x4 (&p)[PP][NT]) {
-    float top[NT];
-    bool above = false;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      top[n] = -__builtin_inff();
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top[n] = fmaxf(top[n], x[n][u][i]);
-      top[n] *= a.scale;
-      // Taken before the branch: where a branch comes between a matrix instruction and the first use of its result, the compiler has left out
-      // the wait that the instruction needs (tests/test_matrix_waits.py looks for that in the built library).
-      asm volatile("" : "+v"(top[n]));
-      above = above || top[n] > m[n] + kRoom;
-    }
-    if (__ballot(above)) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const float best = max_of_row(top[n]), higher = best > m[n] + kRoom ? best : m[n];  // (a row's own matter, whatever its neighbours do)
-        const float by = m[n] == higher ? 1.f : __builtin_amdgcn_exp2f(m[n] - higher);
-        m[n] = higher;
-        l[n] *= by;
-#pragma unroll
-        for (int j = 0; j < S; ++j) o[n][j] *= by;
-      }
-    }
+    raise(a, x);
+    parts(a, x, p);
+  }
+  __device__ inline void parts(const Attend& a, f32x4 (&x)[NT][2], i32x4 (&p)[PP][NT]) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const float base = m[n] == -__builtin_inff() ? 0.f : -m[n];
@@ -294,6 +298,37 @@ struct Rows {
 #pragma unroll
           for (int k = 0; k < PP; ++k) p[k][n][2 * u + i] = (int)parts[k];
         }
+      }
+    }
+  }
+  // the bounds m up to these scores, and the sums and outputs to the bounds
+  template <int G>
+  __device__ inline void raise(const Attend& a, const f32x4 (&x)[NT][G]) {
+    float top[NT];
+    bool above = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      top[n] = -__builtin_inff();
+#pragma unroll
+      for (int u = 0; u < G; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top[n] = fmaxf(top[n], x[n][u][i]);
+      top[n] *= a.scale;
+      // Taken before the branch: where a branch comes between a matrix instruction and the first use of its result, the compiler has left out
+      // the wait that the instruction needs (tests/test_matrix_waits.py looks for that in the built library).
+      asm volatile("" : "+v"(top[n]));
+      above = above || top[n] > m[n] + kRoom;
+    }
+    if (__ballot(above)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float best = max_of_row(top[n]), higher = best > m[n] + kRoom ? best : m[n];  // (a row's own matter, whatever its neighbours do)
+        const float by = m[n] == higher ? 1.f : __builtin_amdgcn_exp2f(m[n] - higher);
+        m[n] = higher;
+        l[n] *= by;
+        sums[n] *= by;
+#pragma unroll
+        for (int j = 0; j < S; ++j) o[n][j] *= by;
       }
     }
   }
@@ -345,7 +380,7 @@ struct Rows {
               is_nan[2 * u + i / 2] |= (g[u].vs[neighbours(D) ? 0 : c] >> (8 * i) & 255u) == 255u ? 0x3f80 << (16 * (i & 1)) : 0;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const f32x4 hit = product(is_nan, seen(a, n, at, upto, lane), f32x4{0.f, 0.f, 0.f, 0.f});
+            const f32x4 hit = product(is_nan, seen(a, n, 0, at, upto, lane), f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const float add = hit[i] > 0.f ? __builtin_nanf("") : 0.f;
@@ -608,7 +643,23 @@ __device__ inline void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_b
 
 // Many rows of a sequence: four waves, each with 16 NT rows of its own, share what is made of the keys and values of 64 tokens: each makes a quarter of it
 // bf16, in the form in which the products take it, and leaves it in LDS (8 KiB for 32 elements of a head, twice, so that one barrier a turn is enough).
-constexpr int kPromptWaves = 4, kTurn = 64;
+//
+// A weight of bf16 operators enters the second product as f16, 2^7 as large as it is (2^15 at most), with values that are exact in f16: one
+// product in place of two, and one conversion of a pair of weights in place of six instructions.  It is within 2^-12 of itself, or 2^-32 of the row's
+// largest; a row's sum is of the weights as they are multiplied.  Where some
+// values are beyond f16's range a workgroup begins again with bf16, and weights in two parts.
+constexpr int kPromptWaves = 4, kTurn = 64, kShift = 7;
+constexpr int kNan = 1, kBf16 = 2;
+// Scales whose values are exact in f16: those are multiples of half the scale, and six times it at most; f16 has multiples of 2^-24 up to 65504.
+constexpr unsigned kHalfLeast = 127 - 23, kHalfMost = 127 + 13;
+__device__ inline bool has_nan(unsigned scales) { return (((scales & 0x7f7f7f7fu) + 0x01010101u) & scales & 0x80808080u) != 0; }
+// whether one of four scales is outside of [kHalfLeast, kHalfMost]: bytes less kHalfLeast, and those above 36, by their borrows and carries
+__device__ inline bool beyond_half(unsigned scales) {
+  const unsigned low = (scales | 0x80808080u) - kHalfLeast * 0x01010101u;  // bit 7 stays where the low seven bits are not below 104
+  const unsigned under = ~(low | scales) & 0x80808080u;                    // below 104
+  const unsigned over = scales & ((scales & 0x7f7f7f7fu) + (0x7fu - (kHalfMost - 128)) * 0x01010101u) & 0x80808080u;  // above 140: 128 and more than 12
+  return (under | over) != 0;
+}
 template <int D>
 struct Share {
   static constexpr int N = D / 32, KS = neighbours(D) ? (D + 127) / 128 : N, VS = neighbours(D) ? 1 : N;
@@ -631,9 +682,10 @@ struct Share {
       for (int i = 0; i < VS; ++i) vs[u][i] = (reinterpret_cast<const unsigned*>(from + 16 * D + D / 2) + (neighbours(D) ? 0 : i))[(unsigned)(q * N + (neighbours(D) ? r * (D / 16) / 32 : 0))];
     }
   }
-  // To LDS.  Values that are NaN are zeros there, and so are those behind the newest token, whatever they are.  nans: whether 32 tokens have a NaN, and then
-  // which (nan_of[token][block]).
-  __device__ inline void store(i32x4* keys, i32x4* values, int* nans, uint8_t* nan_of, const int (&upto)[4], int wave, int lane) {
+  // To LDS.  Values that are NaN are zeros there, and so are those behind the newest token, whatever they are.  forms: of 32 tokens, whether they have a NaN
+  // (kNan; which ones: nan_of[token][block]) and whether values that are to be f16 (HALF) are not exact in it (kBf16).
+  template <bool HALF>
+  __device__ inline void store(i32x4* keys, i32x4* values, int* forms, uint8_t* nan_of, const int (&upto)[4], int wave, int lane) {
     const int half = wave & 1, c0 = wave >> 1;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -641,18 +693,19 @@ struct Share {
       keys[(wave * N + i) * 64 + lane] = i32x4{(int)pair<0>(k[i], s), (int)pair<1>(k[i], s), (int)pair<2>(k[i], s), (int)pair<3>(k[i], s)};
     }
     const int there[2] = {half ? upto[2] : upto[0], half ? upto[3] : upto[1]};
-    bool full = false;  // some scale is 255
+    // whether some scale needs a closer look
+    bool odd = false;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int c = 0; c < VS; ++c) full = full || (((vs[u][c] & 0x7f7f7f7fu) + 0x01010101u) & vs[u][c] & 0x80808080u) != 0;
+      for (int c = 0; c < VS; ++c) odd = odd || (HALF ? beyond_half(vs[u][c]) : has_nan(vs[u][c]));
     i32x4* to = values + half * 2 * N * 64 + lane;
-    if (there[0] == 16 && there[1] == 16 && !__ballot(full)) {
-      if (c0 == 0 && lane == 0) nans[half] = 0;
-      convert<false>(to, c0, {});
+    if (there[0] == 16 && there[1] == 16 && !__ballot(odd)) {
+      if (c0 == 0 && lane == 0) forms[half] = 0;
+      convert<false, HALF>(to, c0, {});
       return;
     }
-    bool nan = false;
+    bool nan = false, wide = false;
     unsigned gone[2] = {};  // what counts as zero: bit 4 c + i for token i and the c-th word of scales
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -661,16 +714,21 @@ struct Share {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int token = 4 * (lane >> 4) + i;
-          const bool in = token < there[u], is = in && (vs[u][c] >> (8 * i) & 255u) == 255u;
+          const unsigned scale = vs[u][c] >> (8 * i) & 255u;
+          const bool in = token < there[u], is = in && scale == 255u;
           nan = nan || is;
+          unsigned code = 0;  // (zeros have the least scale)
+#pragma unroll
+          for (int b = i * N + c; b < i * N + c + (VS > 1 ? 1 : N); ++b) code |= v[u][b / 4] >> (8 * (b % 4)) & 0x77u;
+          wide = wide || (in && !is && code && (scale < kHalfLeast || scale > kHalfMost));
           if (c0 == 0) nan_of[(half * 32 + u * 16 + token) * N + (neighbours(D) ? (lane & 15) * (D / 16) / 32 : c)] = is;
           if (is || !in) gone[u] |= 1u << (4 * c + i);
         }
-    const int any = __ballot(nan) != 0;
-    if (c0 == 0 && lane == 0) nans[half] = any;
-    convert<true>(to, c0, {gone[0], gone[1]});
+    const bool any = __ballot(nan) != 0, bf16 = HALF && __ballot(wide) != 0;  // (then what is left here is not read)
+    if (c0 == 0 && lane == 0) forms[half] = (any ? kNan : 0) | (bf16 ? kBf16 : 0);
+    convert<true, HALF>(to, c0, {gone[0], gone[1]});
   }
-  template <bool SPECIAL>
+  template <bool SPECIAL, bool HALF>
   __device__ inline void convert(i32x4* to, int c0, uint2 gone) {
     unsigned codes[2][N];  // from byte c0 of the first token on
 #pragma unroll
@@ -690,7 +748,7 @@ struct Share {
         for (int i = 0; i < 4; ++i) {
           const int b = i * N + 2 * j;
           const float scale = scale_of(scales, i);
-          t[i] = pair_at(codes[u][b / 4], scale, b % 4);
+          t[i] = HALF ? half_at(codes[u][b / 4], scale, b % 4) : pair_at(codes[u][b / 4], scale, b % 4);
           if (SPECIAL) t[i] = (u ? gone.y : gone.x) >> ((VS > 1 ? 4 * c : 0) + i) & 1u ? 0u : t[i];
         }
 #pragma unroll
@@ -711,7 +769,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void attend_prompt_kernel(Att
   using R = Rows<TYPE, D, NT>;
   constexpr int N = D / 32, S = D / 16, W = kPromptWaves, QP = R::QP, PP = R::PP;
   __shared__ i32x4 keys[2][4 * N * 64], values[2][4 * N * 64];
-  __shared__ int nans[2][2];
+  __shared__ int forms[2][2];
   __shared__ uint8_t nan_of[2][kTurn * N];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, quad = lane >> 4;
   // (kv heads first: the workgroups of one kv head are a multiple of 8 apart where there are 8, 16, .. kv heads, on one of the eight dies, whose cache then
@@ -739,115 +797,168 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void attend_prompt_kernel(Att
   const int* table = a.table + s * a.ldt;
   const uint8_t* head = a.data + (int64_t)kv * a.granules * (17 * D);
   Share<D> share;
-  // The table's entries from `entry` on, a lane each.
-  const int entries = (int)page_index(a, (unsigned)max(a.most_length - 1, 0) / 16) + 1;
-  int entry = 0, page_of_lane = 0;
-  auto turn_table = [&](int to) {
-    entry = to;
-    page_of_lane = table[min(entry + lane, entries - 1)];
+  // Where 64 granules lie, a lane each, and which of them are there; and the pages of the 64 behind them, asked for early.
+  int batch = 0, page_ahead = 0, offset_low = 0, offset_high = 0;
+  unsigned long long there = 0;
+  const int granules = (a.most_length + 15) / 16;  // that the table has pages for
+  auto look_ahead = [&](int g) { page_ahead = table[page_index(a, (unsigned)min(g + lane, granules - 1))]; };
+  auto turn_table = [&](int g0) {
+    const int g = g0 + lane, index = (int)page_index(a, (unsigned)g);
+    const bool good = g < granules && 16 * g < seq.length && (unsigned)page_ahead < (unsigned)a.pages;
+    const int64_t offset = (good ? page_ahead : 0) * a.page_bytes + (g - index * a.granules) * (17 * D);
+    offset_low = (int)offset;
+    offset_high = (int)(offset >> 32);
+    there = __ballot(good);
+    batch = g0;
+    look_ahead(g0 + 64);
   };
-  // Asks for the wave's share of 64 tokens; the granules that are there, a bit each.
-  auto ask = [&](int at) {
-    const unsigned g0 = (unsigned)at / 16;
-    int page[4], place[4], there = 0;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int index = (int)page_index(a, g0 + u);
-      if (index >= entry + 64) turn_table(index);
-      const int p = __builtin_amdgcn_readlane(page_of_lane, index - entry);
-      const bool good = at + 16 * u < seq.length && (unsigned)p < (unsigned)a.pages;
-      there |= good << u;
-      page[u] = good ? p : 0;
-      place[u] = (int)(g0 + u) - index * a.granules;
-    }
-    auto granule = [&](int page, int place) { return head + (int64_t)page * a.page_bytes + place * (17 * D); };
-    const bool odd = wave & 1, high = wave & 2;
-    share.load(granule(high ? (odd ? page[3] : page[2]) : odd ? page[1] : page[0], high ? (odd ? place[3] : place[2]) : odd ? place[1] : place[0]),
-               granule(odd ? page[2] : page[0], odd ? place[2] : place[0]), granule(odd ? page[3] : page[1], odd ? place[3] : place[1]), lane);
-    return there;
+  auto ask = [&](int at) {  // for the wave's share of 64 tokens
+    const int g = at / 16;
+    if (g >= batch + 64) turn_table(g);
+    auto granule = [&](int u) {
+      const int l = g - batch + u;
+      const int64_t offset = (int64_t)__builtin_amdgcn_readlane(offset_high, l) << 32 | (unsigned)__builtin_amdgcn_readlane(offset_low, l);
+      return head + offset;
+    };
+    const int v = 2 * (wave & 1);
+    share.load(granule(wave), granule(v), granule(v + 1), lane);
   };
-  int next = 0;
-  if (from < to) {
-    turn_table((int)page_index(a, (unsigned)from / 16));
-    next = ask(from);
-  }
+  auto begin = [&] {
+    if (from >= to) return;
+    look_ahead(from / 16);
+    turn_table(from / 16);
+    ask(from);
+  };
+  begin();
   R rows;
   rows.begin(a, seq, kv, r0, all, lane);
   unsigned lost[NT] = {};  // outputs that are NaN: bit i for elements of row 4 (lane / 16) + i of all products, or 4 c + i for those of products 2 c and 2 c + 1
-  int buffer = 0;
-  for (int at = from; at < to; at += kTurn, buffer ^= 1) {
-    const int granules = __builtin_amdgcn_readfirstlane(next), behind = seq.length - at;
-    int upto[4];
+  // turns from plain_from on, up to plain_to, have tokens that all rows of the wave see
+  const int plain_from = a.window ? p0 + t1 - a.window + 1 : 0, plain_to = p0 + t0 + 1 - kTurn;
+  // All turns.  HALF: values and weights are multiplied as f16; false where some values are not exact in it.
+  auto turns = [&](auto as_half) {
+    constexpr bool HALF = decltype(as_half)::value;
+    int buffer = 0;
+    unsigned next = from < to ? (unsigned)(there >> (from / 16 - batch)) & 15u : 0u;  // which of the four granules asked for are there
+    for (int at = from; at < to; at += kTurn, buffer ^= 1) {
+      const unsigned here = next;
+      const int behind = seq.length - at;
+      int upto[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) upto[u] = granules >> u & 1 ? min(behind - 16 * u, 16) : 0;
-    share.store(keys[buffer], values[buffer], nans[buffer], nan_of[buffer], upto, wave, lane);
-    if (at + kTurn < to) next = ask(at + kTurn);
-    lds_barrier();
-#pragma unroll 1
-    for (int h = 0; h < 2; ++h) {
-      const int begin = at + h * kStep;
-      if (begin >= mine_to || begin + kStep <= mine_from) continue;
-      const int there[2] = {h ? upto[2] : upto[0], h ? upto[3] : upto[1]};
-      const bool plain = there[0] == 16 && there[1] == 16 && begin + kStep - 1 <= p0 + t0 && (!a.window || begin > p0 + t1 - a.window);
-      f32x4 x[NT][2];
+      for (int u = 0; u < 4; ++u) upto[u] = here >> u & 1 ? min(behind - 16 * u, 16) : 0;
+      share.template store<HALF>(keys[buffer], values[buffer], forms[buffer], nan_of[buffer], upto, wave, lane);
+      if (at + kTurn < to) {
+        ask(at + kTurn);
+        next = (unsigned)(there >> ((at + kTurn) / 16 - batch)) & 15u;
+      }
+      lds_barrier();
+      const int form[2] = {__builtin_amdgcn_readfirstlane(forms[buffer][0]), __builtin_amdgcn_readfirstlane(forms[buffer][1])};
+      if (HALF && ((form[0] | form[1]) & kBf16)) return false;
+      if (at >= mine_to || at + kTurn <= mine_from) continue;
+      f32x4 x[NT][4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 4; ++u)
 #pragma unroll
         for (int w = 0; w < N; ++w) {
-          const i32x4 key = keys[buffer][((2 * h + u) * N + w) * 64 + lane];
+          const i32x4 key = keys[buffer][(u * N + w) * 64 + lane];
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = QP - 1; i >= 0; --i) x[n][u] = product(key, rows.q[i][n][w], w == 0 && i == QP - 1 ? f32x4{0.f, 0.f, 0.f, 0.f} : x[n][u]);
         }
-      // (used before the branch: see Rows::weights)
+      // (used before the branch: see Rows::raise)
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float v = x[n][u][i];
-            asm volatile("" : "+v"(v));
-            x[n][u][i] = v;
-          }
-      if (!plain) rows.mask(a, x, begin, there, lane);
-      i32x4 p[PP][NT];
-      rows.weights(a, x, p);
-      if (__builtin_amdgcn_readfirstlane(nans[buffer][h])) {
+        for (int u = 0; u < 4; ++u) asm volatile("" : "+v"(x[n][u]));
+      if (here != 15u || behind < kTurn || at < plain_from || at > plain_to) rows.mask(a, x, at, upto, lane);
+      if ((form[0] | form[1]) & kNan) {
         // A NaN that some rows see and others do not: those that see it are found by a product of a one for each NaN value by a one for each token
         // that is seen.  The value itself is zero in LDS.
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          if (!(forms[buffer][h] & kNan)) continue;
+          const int there[2] = {h ? upto[2] : upto[0], h ? upto[3] : upto[1]};
 #pragma unroll
-        for (int c = 0; c < (neighbours(D) ? 1 : N); ++c) {
-          i32x4 ones{};
+          for (int c = 0; c < (neighbours(D) ? 1 : N); ++c) {
+            i32x4 ones{};
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              ones[2 * u + i / 2] |= nan_of[buffer][(h * 32 + u * 16 + 4 * quad + i) * N + (neighbours(D) ? r16 * (D / 16) / 32 : c)] ? 0x3f80 << (16 * (i & 1)) : 0;
+              for (int i = 0; i < 4; ++i)
+                ones[2 * u + i / 2] |= nan_of[buffer][(h * 32 + u * 16 + 4 * quad + i) * N + (neighbours(D) ? r16 * (D / 16) / 32 : c)] ? 0x3f80 << (16 * (i & 1)) : 0;
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const f32x4 hit = product(ones, rows.seen(a, n, begin, there, lane), f32x4{0.f, 0.f, 0.f, 0.f});
+            for (int n = 0; n < NT; ++n) {
+              const f32x4 hit = product(ones, rows.seen(a, n, 0, at + h * kStep, there, lane), f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-            for (int i = 0; i < 4; ++i) lost[n] |= (hit[i] > 0.f ? 1u : 0u) << (4 * c + i);
+              for (int i = 0; i < 4; ++i) lost[n] |= (hit[i] > 0.f ? 1u : 0u) << (4 * c + i);
+            }
           }
         }
       }
-      const i32x4* value = values[buffer] + h * 2 * N * 64 + lane;
+      rows.raise(a, x);
+      if constexpr (HALF) {
+        i32x4 p[NT][2];
 #pragma unroll
-      for (int j = 0; j < S; ++j) {
-        const i32x4 v = value[j * 64];
+        for (int n = 0; n < NT; ++n) {
+          const float base = (float)kShift - (rows.m[n] == -__builtin_inff() ? 0.f : rows.m[n]);
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+          for (int u = 0; u < 4; ++u)
 #pragma unroll
-          for (int k = PP - 1; k >= 0; --k) rows.o[n][j] = product(v, p[k][n], rows.o[n][j]);
+            for (int i = 0; i < 2; ++i) {
+              const float v = __builtin_amdgcn_exp2f(fmaf(x[n][u][2 * i], a.scale, base)), w = __builtin_amdgcn_exp2f(fmaf(x[n][u][2 * i + 1], a.scale, base));
+              p[n][u / 2][2 * (u % 2) + i] = __builtin_bit_cast(int, f16x2{(_Float16)v, (_Float16)w});
+            }
+        }
+        const i32x4 ones = {0x3c003c00, 0x3c003c00, 0x3c003c00, 0x3c003c00};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) rows.sums[n] = half_product(ones, p[n][h], rows.sums[n]);
+#pragma unroll
+          for (int j = 0; j < S; ++j) {
+            const i32x4 v = values[buffer][(h * S + j) * 64 + lane];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) rows.o[n][j] = half_product(v, p[n][h], rows.o[n][j]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          f32x4 y[NT][2];
+          i32x4 p[PP][NT];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) y[n][0] = x[n][2 * h], y[n][1] = x[n][2 * h + 1];
+          rows.parts(a, y, p);
+#pragma unroll
+          for (int j = 0; j < S; ++j) {
+            const i32x4 v = values[buffer][(h * S + j) * 64 + lane];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int k = PP - 1; k >= 0; --k) rows.o[n][j] = product(v, p[k][n], rows.o[n][j]);
+          }
+        }
       }
     }
+    return true;
+  };
+  bool done = false;
+  if constexpr (TYPE == TETRIS_BF16) {
+    done = turns(std::true_type{});
+    if (!done) {  // (all waves see the same forms, so they are all here)
+      __syncthreads();
+      rows.reset();
+#pragma unroll
+      for (int n = 0; n < NT; ++n) lost[n] = 0;
+      begin();
+    }
   }
+  if (!done) turns(std::false_type{});
 
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const float sum = sum_of_row(rows.l[n]);
+    const float sum = sum_of_row(rows.l[n]) + rows.sums[n][0];
     const int r = r0 + n * 16 + r16;
     if (r >= all) continue;
     const int t = r / a.group, h = kv * a.group + r - t * a.group;
