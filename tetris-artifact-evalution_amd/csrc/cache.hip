@@ -44,6 +44,8 @@ __device__ inline int value_byte(int token, int m, int c) {
   return ((token / 4 * 16 + m) * 4 + token % 4) * (D / 32) + c;
 }
 
+constexpr int kAtOnce = 2;  // pieces that a lane has under way
+
 // A lane has eight elements, four lanes a block.  blockIdx.y: keys, values.
 template <int TYPE, int D, bool VEC>
 __global__ __launch_bounds__(256) void append_kernel(Slots a, const typename Elem<TYPE>::type* __restrict__ k,
@@ -51,53 +53,64 @@ __global__ __launch_bounds__(256) void append_kernel(Slots a, const typename Ele
   constexpr int N = D / 32;
   const bool value = blockIdx.y;
   const auto* x = value ? v : k;
-  const int64_t waves = ((int64_t)a.tokens * per_row + 63) / 64;
-  for (int64_t w = wave_of(); w < waves; w += (int64_t)gridDim.x * (blockDim.x >> 6)) {
-    const Place p = place_of(w, per_row);
-    const Spot s = spot_of<D>(a, p);
-    if (!s.in) continue;  // (the lanes of a block are in or out together)
-    float e[8];
-    load8<typename Elem<TYPE>::type, VEC>(x + p.row * a.ld[blockIdx.y], p.piece * 8, (int)per_row * 8, e);
-    unsigned top = 0;
+  const int64_t waves = ((int64_t)a.tokens * per_row + 63) / 64, stride = (int64_t)gridDim.x * (blockDim.x >> 6);
+  for (int64_t w = wave_of(); w < waves; w += kAtOnce * stride) {
+    float es[kAtOnce][8];
+    Spot spots[kAtOnce];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(e[i]) & 0x7fffffffu);
-    top = quad_max(top);
-    const bool fine = top < 0x7f800000u;
-    const int scale = max((int)(top >> 23) - 2, 0);
-    const float by = __uint_as_float((unsigned)scale << 23);
-    unsigned c = 0;
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, e[0], e[1], by, 0);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, e[2], e[3], by, 1);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, e[4], e[5], by, 2);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, e[6], e[7], by, 3);
-    if (!fine) c = 0;
-    const uint8_t byte = fine ? (uint8_t)scale : 255;
-    const int block = s.piece / 4, q = s.piece & 3;
-    if (!value) {
-      *reinterpret_cast<unsigned*>(s.granule + key_word<D>(s.token, s.piece)) = c;
-      if (q == 0) s.granule[16 * D + s.token * N + block] = byte;
-      continue;
+    for (int n = 0; n < kAtOnce; ++n) {  // (all loads first)
+      const Place p = place_of(w + n * stride, per_row);
+      spots[n].in = false;
+      if (p.row >= a.tokens) continue;
+      load8<typename Elem<TYPE>::type, VEC>(x + p.row * a.ld[blockIdx.y], p.piece * 8, (int)per_row * 8, es[n]);
+      spots[n] = spot_of<D>(a, p);
     }
-    uint8_t* to = s.granule + 8 * D;
-    if constexpr (!neighbours(D)) {
-      // lanes q and q ^ 2 have the low and the high halves of bytes; each writes four of the eight
-      const unsigned other = (unsigned)__builtin_amdgcn_mov_dpp((int)c, 0x4e, 0xf, 0xf, true);
-      const unsigned low = q < 2 ? c : other >> 16, high = q < 2 ? other : c >> 16;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        to[value_byte<D>(s.token, 8 * (q & 1) + (q & 2) * 2 + i, block)] = (uint8_t)((low >> (4 * i) & 15) | (high >> (4 * i) & 15) << 4);
-    } else if constexpr (D >= 128) {
-      *reinterpret_cast<unsigned*>(to + value_byte<D>(s.token, s.piece * 8 / (D / 16), s.piece * 8 % (D / 16) / 2)) = c;
-    } else {
-      constexpr int M = 128 / D;  // lanes that the eight go to
-#pragma unroll
-      for (int i = 0; i < M; ++i) {
-        uint8_t* at = to + value_byte<D>(s.token, s.piece * M + i, 0);
-        if constexpr (M == 2) *reinterpret_cast<unsigned short*>(at) = (unsigned short)(c >> (16 * i));
-        else *at = (uint8_t)(c >> (8 * i));
+    for (int n = 0; n < kAtOnce; ++n) {
+      const Spot& s = spots[n];
+      float(&e)[8] = es[n];
+      if (!s.in) continue;  // (the lanes of a block are in or out together)
+      unsigned top = 0;
+  #pragma unroll
+      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(e[i]) & 0x7fffffffu);
+      top = quad_max(top);
+      const bool fine = top < 0x7f800000u;
+      const int scale = max((int)(top >> 23) - 2, 0);
+      const float by = __uint_as_float((unsigned)scale << 23);
+      unsigned c = 0;
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, e[0], e[1], by, 0);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, e[2], e[3], by, 1);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, e[4], e[5], by, 2);
+      c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, e[6], e[7], by, 3);
+      if (!fine) c = 0;
+      const uint8_t byte = fine ? (uint8_t)scale : 255;
+      const int block = s.piece / 4, q = s.piece & 3;
+      if (!value) {
+        *reinterpret_cast<unsigned*>(s.granule + key_word<D>(s.token, s.piece)) = c;
+        if (q == 0) s.granule[16 * D + s.token * N + block] = byte;
+        continue;
       }
+      uint8_t* to = s.granule + 8 * D;
+      if constexpr (!neighbours(D)) {
+        // lanes q and q ^ 2 have the low and the high halves of bytes; each writes four of the eight
+        const unsigned other = (unsigned)__builtin_amdgcn_mov_dpp((int)c, 0x4e, 0xf, 0xf, true);
+        const unsigned low = q < 2 ? c : other >> 16, high = q < 2 ? other : c >> 16;
+  #pragma unroll
+        for (int i = 0; i < 4; ++i)
+          to[value_byte<D>(s.token, 8 * (q & 1) + (q & 2) * 2 + i, block)] = (uint8_t)((low >> (4 * i) & 15) | (high >> (4 * i) & 15) << 4);
+      } else if constexpr (D >= 128) {
+        *reinterpret_cast<unsigned*>(to + value_byte<D>(s.token, s.piece * 8 / (D / 16), s.piece * 8 % (D / 16) / 2)) = c;
+      } else {
+        constexpr int M = 128 / D;  // lanes that the eight go to
+  #pragma unroll
+        for (int i = 0; i < M; ++i) {
+          uint8_t* at = to + value_byte<D>(s.token, s.piece * M + i, 0);
+          if constexpr (M == 2) *reinterpret_cast<unsigned short*>(at) = (unsigned short)(c >> (16 * i));
+          else *at = (uint8_t)(c >> (8 * i));
+        }
+      }
+      if (q == 0) s.granule[16 * D + D / 2 + (s.token / 4 * N + block) * 4 + s.token % 4] = byte;
     }
-    if (q == 0) s.granule[16 * D + D / 2 + (s.token / 4 * N + block) * 4 + s.token % 4] = byte;
   }
 }
 
@@ -107,56 +120,73 @@ __global__ __launch_bounds__(256) void read_kernel(Slots a, typename Elem<TYPE>:
   using T = typename Elem<TYPE>::type;
   constexpr int N = D / 32;
   const bool value = blockIdx.y;
-  const int64_t waves = ((int64_t)a.tokens * per_row + 63) / 64;
-  for (int64_t w = wave_of(); w < waves; w += (int64_t)gridDim.x * (blockDim.x >> 6)) {
-    const Place p = place_of(w, per_row);
-    if (p.row >= a.tokens) continue;
-    const Spot s = spot_of<D>(a, p);
-    unsigned c = 0, byte = 127;
-    const int block = s.piece / 4;
-    if (s.in && !value) {
-      c = *reinterpret_cast<const unsigned*>(s.granule + key_word<D>(s.token, s.piece));
-      byte = s.granule[16 * D + s.token * N + block];
-    } else if (s.in) {
-      const uint8_t* from = s.granule + 8 * D;
-      if constexpr (!neighbours(D)) {
-        const int q = s.piece & 3;
+  const int64_t waves = ((int64_t)a.tokens * per_row + 63) / 64, stride = (int64_t)gridDim.x * (blockDim.x >> 6);
+  for (int64_t w = wave_of(); w < waves; w += kAtOnce * stride) {
+    unsigned codes[kAtOnce], scales[kAtOnce];
+    Place places[kAtOnce];
+    Spot spots[kAtOnce];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) c |= ((unsigned)from[value_byte<D>(s.token, 8 * (q & 1) + i, block)] >> (q & 2) * 2 & 15u) << (4 * i);
-      } else if constexpr (D >= 128) {
-        c = *reinterpret_cast<const unsigned*>(from + value_byte<D>(s.token, s.piece * 8 / (D / 16), s.piece * 8 % (D / 16) / 2));
-      } else {
-        constexpr int M = 128 / D;
+    for (int n = 0; n < kAtOnce; ++n) {
+      places[n] = place_of(w + n * stride, per_row);
+      spots[n] = spot_of<D>(a, places[n]);
+    }
 #pragma unroll
-        for (int i = 0; i < M; ++i) {
-          const uint8_t* at = from + value_byte<D>(s.token, s.piece * M + i, 0);
-          if constexpr (M == 2) c |= (unsigned)*reinterpret_cast<const unsigned short*>(at) << (16 * i);
-          else c |= (unsigned)*at << (8 * i);
+    for (int n = 0; n < kAtOnce; ++n) {
+      const Spot& s = spots[n];
+      unsigned c = 0, byte = 127;
+      const int block = s.piece / 4;
+      if (s.in && !value) {
+        c = *reinterpret_cast<const unsigned*>(s.granule + key_word<D>(s.token, s.piece));
+        byte = s.granule[16 * D + s.token * N + block];
+      } else if (s.in) {
+        const uint8_t* from = s.granule + 8 * D;
+        if constexpr (!neighbours(D)) {
+          const int q = s.piece & 3;
+  #pragma unroll
+          for (int i = 0; i < 8; ++i) c |= ((unsigned)from[value_byte<D>(s.token, 8 * (q & 1) + i, block)] >> (q & 2) * 2 & 15u) << (4 * i);
+        } else if constexpr (D >= 128) {
+          c = *reinterpret_cast<const unsigned*>(from + value_byte<D>(s.token, s.piece * 8 / (D / 16), s.piece * 8 % (D / 16) / 2));
+        } else {
+          constexpr int M = 128 / D;
+  #pragma unroll
+          for (int i = 0; i < M; ++i) {
+            const uint8_t* at = from + value_byte<D>(s.token, s.piece * M + i, 0);
+            if constexpr (M == 2) c |= (unsigned)*reinterpret_cast<const unsigned short*>(at) << (16 * i);
+            else c |= (unsigned)*at << (8 * i);
+          }
         }
+        byte = s.granule[16 * D + D / 2 + (s.token / 4 * N + block) * 4 + s.token % 4];
       }
-      byte = s.granule[16 * D + D / 2 + (s.token / 4 * N + block) * 4 + s.token % 4];
+      codes[n] = c;
+      scales[n] = byte;
     }
-    const float by = __uint_as_float(byte << 23);
-    T t[8];
-    if (TYPE == TETRIS_BF16) {
-      int* o = reinterpret_cast<int*>(t);
-      o[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, by, 0));
-      o[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, by, 1));
-      o[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, by, 2));
-      o[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, by, 3));
-    } else {
-      const f32x2 e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, by, 0), f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, by, 1);
-      const f32x2 g = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, by, 2), h = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, by, 3);
-      t[0] = (T)e.x; t[1] = (T)e.y; t[2] = (T)f.x; t[3] = (T)f.y;
-      t[4] = (T)g.x; t[5] = (T)g.y; t[6] = (T)h.x; t[7] = (T)h.y;
-    }
-    T* out = (value ? v : k) + p.row * a.ld[blockIdx.y] + p.piece * 8;
-    if (VEC) {
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<int4*>(out)[i] = reinterpret_cast<const int4*>(t)[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) out[i] = t[i];
+    for (int n = 0; n < kAtOnce; ++n) {
+      const Place& p = places[n];
+      const unsigned c = codes[n], byte = scales[n];
+      if (p.row >= a.tokens) continue;
+      const float by = __uint_as_float(byte << 23);
+      T t[8];
+      if (TYPE == TETRIS_BF16) {
+        int* o = reinterpret_cast<int*>(t);
+        o[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, by, 0));
+        o[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, by, 1));
+        o[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, by, 2));
+        o[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, by, 3));
+      } else {
+        const f32x2 e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, by, 0), f = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, by, 1);
+        const f32x2 g = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, by, 2), h = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, by, 3);
+        t[0] = (T)e.x; t[1] = (T)e.y; t[2] = (T)f.x; t[3] = (T)f.y;
+        t[4] = (T)g.x; t[5] = (T)g.y; t[6] = (T)h.x; t[7] = (T)h.y;
+      }
+      T* out = (value ? v : k) + p.row * a.ld[blockIdx.y] + p.piece * 8;
+      if (VEC) {
+  #pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<int4*>(out)[i] = reinterpret_cast<const int4*>(t)[i];
+      } else {
+  #pragma unroll
+        for (int i = 0; i < 8; ++i) out[i] = t[i];
+      }
     }
   }
 }
@@ -165,7 +195,8 @@ template <int TYPE, bool APPEND, int D, bool VEC>
 void launch(const Slots& a, void* k, void* v, hipStream_t s) {
   using T = typename Elem<TYPE>::type;
   const unsigned per_row = (unsigned)(a.kv_heads * (D / 8));
-  const dim3 grid((unsigned)std::min<int64_t>(((int64_t)a.tokens * per_row + 255) / 256, 256 * 64), 2), block(256);
+  const int few = (int64_t)a.tokens * per_row > 256 * 1024 ? kAtOnce : 1;  // pieces of a lane: one where that does not fill the chip
+  const dim3 grid((unsigned)std::min<int64_t>(((int64_t)a.tokens * per_row + 256 * few - 1) / (256 * few), 256 * 64), 2), block(256);
   if constexpr (APPEND)
     hipLaunchKernelGGL((append_kernel<TYPE, D, VEC>), grid, block, 0, s, a, static_cast<const T*>(k), static_cast<const T*>(v), per_row);
   else

@@ -2,6 +2,7 @@
 // stays in registers between the sum of squares and the outputs, so that memory is passed once; bound by HBM, and for few rows by
 // the launch.
 #include <algorithm>
+#include <type_traits>
 
 #include "mx4.h"
 #include "tetris_attention.h"
@@ -22,50 +23,58 @@ struct NormRows {
   float eps;
 };
 
-// Eight elements of a thread: neighbours where rows lie on 16 bytes (VEC), else every THREADS-th, so that a wave's loads are whole lines.
-template <int THREADS, bool VEC>
-__device__ inline int first_of(int piece) {
-  return VEC ? (piece * THREADS + (int)threadIdx.x) * 8 : piece * THREADS * 8 + (int)threadIdx.x;
-}
+// Eight elements of a thread: neighbours where rows lie on 16 bytes (VEC), else every THREADS-th, so that a wave's loads are whole lines.  All loads of a
+// row are asked for before any is used: those past its end read its last elements, which count as zeros then.
 template <typename T, int THREADS, bool VEC>
-__device__ inline void load_piece(const T* row, int at, int cols, float (&v)[8]) {
-  if constexpr (VEC) {
-    if (at < cols) {
-      int4 raw[sizeof(T) / 2];
+struct Piece {
+  static constexpr int Q = sizeof(T) / 2;
+  int4 raw[VEC ? Q : 1];
+  T one[VEC ? 1 : 8];
+  __device__ static inline int first(int piece) { return VEC ? (piece * THREADS + (int)threadIdx.x) * 8 : piece * THREADS * 8 + (int)threadIdx.x; }
+  __device__ inline void load(const T* row, int piece, int cols) {
+    if constexpr (VEC) {
+      const int4* from = reinterpret_cast<const int4*>(row + min(first(piece), cols - 8));
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = reinterpret_cast<const int4*>(row + at)[i];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = (float)reinterpret_cast<const T*>(raw)[i];
+      for (int i = 0; i < Q; ++i) raw[i] = from[i];
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+      for (int i = 0; i < 8; ++i) one[i] = row[min(first(piece) + i * THREADS, cols - 1)];
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = at + i * THREADS < cols ? (float)row[at + i * THREADS] : 0.f;
   }
-}
-template <typename T, int THREADS, bool VEC>
-__device__ inline void store_piece(T* row, int at, int cols, const float (&v)[8]) {
-  if constexpr (VEC) {
-    if (at >= cols) return;
-    T t[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = (T)v[i];
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<int4*>(row + at)[i] = reinterpret_cast<const int4*>(t)[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (at + i * THREADS < cols) row[at + i * THREADS] = (T)v[i];
+  __device__ inline float at(int i) const {
+    if constexpr (VEC) return (float)reinterpret_cast<const T*>(raw)[i];
+    else return (float)one[i];
   }
-}
+  __device__ static inline bool in(int piece, int i, int cols) { return VEC ? first(piece) < cols : first(piece) + i * THREADS < cols; }
+  __device__ static inline void store(T* row, int piece, int cols, const float (&v)[8]) {
+    if constexpr (VEC) {
+      if (first(piece) >= cols) return;
+      T t[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = (T)v[i];
+#pragma unroll
+      for (int i = 0; i < Q; ++i) reinterpret_cast<int4*>(row + first(piece))[i] = reinterpret_cast<const int4*>(t)[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (first(piece) + i * THREADS < cols) row[first(piece) + i * THREADS] = (T)v[i];
+    }
+  }
+};
 
 // The sum of v over the workgroup, in all threads, always added in the same order.
 template <int THREADS>
 __device__ inline float sum_of_all(float v, float* shared) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+  auto step = [&](auto ctrl, auto rows) {
+    v += __uint_as_float((unsigned)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+  };
+  step(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});  // from 1, 2, 4 and 8 lanes below in rows of sixteen
+  step(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
+  step(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
+  step(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
+  step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});  // a row's last to the next row, the second row's to the upper half
+  step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
+  v = __uint_as_float((unsigned)__builtin_amdgcn_readlane((int)__float_as_uint(v), 63));
   if constexpr (THREADS > 64) {
     if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
     __syncthreads();
@@ -80,6 +89,8 @@ __device__ inline float sum_of_all(float v, float* shared) {
 template <int TYPE, int THREADS, int KEPT, bool VEC>
 __global__ __launch_bounds__(THREADS) void rms_norm_kernel(NormRows a) {
   using T = typename Elem<TYPE>::type;
+  using P = Piece<T, THREADS, VEC>;
+  using W = Piece<float, THREADS, VEC>;
   __shared__ float shared[THREADS / 64];
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(a.x) + row * a.ldx;
@@ -87,45 +98,57 @@ __global__ __launch_bounds__(THREADS) void rms_norm_kernel(NormRows a) {
   T* sum = a.sum ? static_cast<T*>(a.sum) + row * a.lds : nullptr;
   T* y = static_cast<T*>(a.y) + row * a.ldy;
   const int pieces = (a.cols + THREADS * 8 - 1) / (THREADS * 8);
-  auto total = [&](int piece, float (&v)[8]) {
-    const int at = first_of<THREADS, VEC>(piece);
-    load_piece<T, THREADS, VEC>(x, at, a.cols, v);
-    if (r) {
-      float u[8];
-      load_piece<T, THREADS, VEC>(r, at, a.cols, u);
+  P xs[KEPT], rs[KEPT];
+  W ws[KEPT];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] += u[i];
-    }
+  for (int p = 0; p < KEPT; ++p) xs[p].load(x, p, a.cols);
+  if (r) {
+#pragma unroll
+    for (int p = 0; p < KEPT; ++p) rs[p].load(r, p, a.cols);
+  }
+  if (a.weight) {
+#pragma unroll
+    for (int p = 0; p < KEPT; ++p) ws[p].load(a.weight, p, a.cols);
+  }
+  auto total = [&](const P& u, const P& v, int p, float (&out)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = P::in(p, i, a.cols) ? (r ? u.at(i) + v.at(i) : u.at(i)) : 0.f;
   };
   float kept[KEPT][8], squares = 0.f;
 #pragma unroll
-  for (int p = 0; p < KEPT; ++p) total(p, kept[p]);
-#pragma unroll
-  for (int p = 0; p < KEPT; ++p)
+  for (int p = 0; p < KEPT; ++p) {
+    total(xs[p], rs[p], p, kept[p]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) squares = fmaf(kept[p][i], kept[p][i], squares);
+  }
   for (int p = KEPT; p < pieces; ++p) {
-    float v[8];
-    total(p, v);
+    P u, v;
+    float t[8];
+    u.load(x, p, a.cols);
+    if (r) v.load(r, p, a.cols);
+    total(u, v, p, t);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) squares = fmaf(v[i], v[i], squares);
+    for (int i = 0; i < 8; ++i) squares = fmaf(t[i], t[i], squares);
   }
   const float by = 1.f / sqrtf(sum_of_all<THREADS>(squares, shared) / (float)a.cols + a.eps);
-  auto finish = [&](int piece, const float (&v)[8]) {
-    const int at = first_of<THREADS, VEC>(piece);
-    if (sum) store_piece<T, THREADS, VEC>(sum, at, a.cols, v);
-    float w[8], out[8];
-    if (a.weight) load_piece<float, THREADS, VEC>(a.weight, at, a.cols, w);
+  auto finish = [&](int p, const W& w, const float (&v)[8]) {
+    if (sum) P::store(sum, p, a.cols, v);
+    float out[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out[i] = a.weight ? v[i] * by * w[i] : v[i] * by;
-    store_piece<T, THREADS, VEC>(y, at, a.cols, out);
+    for (int i = 0; i < 8; ++i) out[i] = a.weight ? v[i] * by * w.at(i) : v[i] * by;
+    P::store(y, p, a.cols, out);
   };
 #pragma unroll
-  for (int p = 0; p < KEPT; ++p) finish(p, kept[p]);
+  for (int p = 0; p < KEPT; ++p) finish(p, ws[p], kept[p]);
   for (int p = KEPT; p < pieces; ++p) {
-    float v[8];
-    total(p, v);
-    finish(p, v);
+    P u, v;
+    W w;
+    float t[8];
+    u.load(x, p, a.cols);
+    if (r) v.load(r, p, a.cols);
+    if (a.weight) w.load(a.weight, p, a.cols);
+    total(u, v, p, t);
+    finish(p, w, t);
   }
 }
 
@@ -140,10 +163,13 @@ void launch(const NormRows& a, int64_t rows, hipStream_t s) {
     if (a.sum) b.sum = static_cast<char*>(a.sum) + from * a.lds * size;
     b.y = static_cast<char*>(a.y) + from * a.ldy * size;
     const dim3 grid((unsigned)std::min(kMost, rows - from));
-    if (a.cols <= 512) hipLaunchKernelGGL((rms_norm_kernel<TYPE, 64, 1, VEC>), grid, dim3(64), 0, s, b);
-    else if (a.cols <= 2048) hipLaunchKernelGGL((rms_norm_kernel<TYPE, 256, 1, VEC>), grid, dim3(256), 0, s, b);
-    else if (a.cols <= 4096) hipLaunchKernelGGL((rms_norm_kernel<TYPE, 256, 2, VEC>), grid, dim3(256), 0, s, b);
-    else hipLaunchKernelGGL((rms_norm_kernel<TYPE, 256, 4, VEC>), grid, dim3(256), 0, s, b);
+#define TETRIS_NORM(THREADS, KEPT) hipLaunchKernelGGL((rms_norm_kernel<TYPE, THREADS, KEPT, VEC>), grid, dim3(THREADS), 0, s, b)
+    if (a.cols <= 512) TETRIS_NORM(64, 1);
+    else if (a.cols <= 2048) TETRIS_NORM(256, 1);
+    else if (a.cols <= 4096 && rows >= 512) TETRIS_NORM(256, 2);
+    else if (a.cols <= 8192 && rows >= 512) TETRIS_NORM(512, 2);
+    else TETRIS_NORM(1024, 1);  // few rows: all of a row's loads at once
+#undef TETRIS_NORM
   }
 }
 

@@ -28,22 +28,21 @@ struct Rotary {
   double turns;  // log2 of the base
 };
 
+// Eight elements as they lie.
 template <typename T>
-__device__ inline void load_eight(const T* p, float (&v)[8]) {
+struct Eight {
   int4 raw[sizeof(T) / 2];
+  __device__ inline void load(const T* p) {
 #pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = reinterpret_cast<const int4*>(p)[i];
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = reinterpret_cast<const int4*>(p)[i];
+  }
+  __device__ inline void store(T* p) const {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = (float)reinterpret_cast<const T*>(raw)[i];
-}
-template <typename T>
-__device__ inline void store_eight(T* p, const float (&v)[8]) {
-  T t[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) t[i] = (T)v[i];
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<int4*>(p)[i] = reinterpret_cast<const int4*>(t)[i];
-}
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<int4*>(p)[i] = raw[i];
+  }
+  __device__ inline float get(int i) const { return (float)reinterpret_cast<const T*>(raw)[i]; }
+  __device__ inline void set(int i, float v) { reinterpret_cast<T*>(raw)[i] = (T)v; }
+};
 
 // VEC: rows lie on 16 bytes, and a unit of work is eight elements, or eight pairs of halves.  Otherwise it is a pair, or an element past the pairs.
 template <int TYPE, bool VEC, bool HALVES>
@@ -76,52 +75,61 @@ __global__ __launch_bounds__(256) void rotary_kernel(Rotary a) {
   const int turned = VEC ? (HALVES ? a.half / 8 : a.half / 4) : a.half, units = turned + (VEC ? tail / 8 : tail);  // of a head
   const int h0 = (int)((int64_t)a.heads * split / a.splits), heads = (int)((int64_t)a.heads * (split + 1) / a.splits) - h0;
   const int all = heads * units;
-  for (int token = 0; token < count; ++token) {
-    const T* x = static_cast<const T*>(a.x) + (int64_t)(first + token) * a.ldx;
-    T* y = static_cast<T*>(a.y) + (int64_t)(first + token) * a.ldy;
-    const float2* angle = table + token * a.half;
-    for (int w = threadIdx.x; w < all; w += 256) {
-      const int h = w / units, u = w - h * units;
-      const int64_t at = (int64_t)(h0 + h) * a.head;
-      if constexpr (VEC) {
-        float p[8], q[8];
-        if (u >= turned) {  // as they are
-          const int64_t from = at + dims + (u - turned) * 8;
-          int4 raw[sizeof(T) / 2];
+  if constexpr (VEC) {
+    // two tokens' loads are under way together
+    for (int t0 = 0; t0 < count; t0 += 2) {
+      const T* x = static_cast<const T*>(a.x) + (int64_t)(first + t0) * a.ldx;
+      T* y = static_cast<T*>(a.y) + (int64_t)(first + t0) * a.ldy;
+      const int more = min(count - t0, 2);
+      for (int w = threadIdx.x; w < all; w += 256) {
+        const int h = w / units, u = w - h * units;
+        const int64_t head = (int64_t)(h0 + h) * a.head;
+        const bool copied = u >= turned;
+        const int64_t at = head + (copied ? dims + (u - turned) * 8 : u * 8);
+        Eight<T> p[2], q[2];
 #pragma unroll
-          for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = reinterpret_cast<const int4*>(x + from)[i];
-#pragma unroll
-          for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<int4*>(y + from)[i] = raw[i];
-        } else if constexpr (HALVES) {
-          load_eight(x + at + u * 8, p);
-          load_eight(x + at + a.half + u * 8, q);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float2 cs = angle[u * 8 + i];
-            const float f = p[i] * cs.x - q[i] * cs.y;
-            q[i] = p[i] * cs.y + q[i] * cs.x;
-            p[i] = f;
-          }
-          store_eight(y + at + u * 8, p);
-          store_eight(y + at + a.half + u * 8, q);
-        } else {
-          load_eight(x + at + u * 8, p);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 cs = angle[u * 4 + i];
-            q[2 * i] = p[2 * i] * cs.x - p[2 * i + 1] * cs.y;
-            q[2 * i + 1] = p[2 * i] * cs.y + p[2 * i + 1] * cs.x;
-          }
-          store_eight(y + at + u * 8, q);
+        for (int k = 0; k < 2; ++k) {
+          const T* from = x + (k < more ? k : 0) * a.ldx + at;
+          p[k].load(from);
+          if (HALVES) q[k].load(from + (copied ? 0 : a.half));
         }
-      } else if (u >= turned) {
-        y[at + dims + u - turned] = x[at + dims + u - turned];
-      } else {
-        const int64_t i = at + (HALVES ? u : 2 * u), j = HALVES ? i + a.half : i + 1;
-        const float p = (float)x[i], q = (float)x[j];
-        const float2 cs = angle[u];
-        y[i] = (T)(p * cs.x - q * cs.y);
-        y[j] = (T)(p * cs.y + q * cs.x);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if (k >= more) break;
+          T* to = y + k * a.ldy + at;
+          if (!copied) {
+            const float2* angle = table + (t0 + k) * a.half + u * (HALVES ? 8 : 4);
+#pragma unroll
+            for (int i = 0; i < (HALVES ? 8 : 4); ++i) {
+              const float2 cs = angle[i];
+              const float v = HALVES ? p[k].get(i) : p[k].get(2 * i), z = HALVES ? q[k].get(i) : p[k].get(2 * i + 1);
+              const float f = v * cs.x - z * cs.y, g = v * cs.y + z * cs.x;
+              if (HALVES) p[k].set(i, f), q[k].set(i, g);
+              else p[k].set(2 * i, f), p[k].set(2 * i + 1, g);
+            }
+            if (HALVES) q[k].store(to + a.half);
+          }
+          p[k].store(to);
+        }
+      }
+    }
+  } else {
+    for (int token = 0; token < count; ++token) {
+      const T* x = static_cast<const T*>(a.x) + (int64_t)(first + token) * a.ldx;
+      T* y = static_cast<T*>(a.y) + (int64_t)(first + token) * a.ldy;
+      const float2* angle = table + token * a.half;
+      for (int w = threadIdx.x; w < all; w += 256) {
+        const int h = w / units, u = w - h * units;
+        const int64_t at = (int64_t)(h0 + h) * a.head;
+        if (u >= turned) {
+          y[at + dims + u - turned] = x[at + dims + u - turned];
+        } else {
+          const int64_t i = at + (HALVES ? u : 2 * u), j = HALVES ? i + a.half : i + 1;
+          const float p = (float)x[i], q = (float)x[j];
+          const float2 cs = angle[u];
+          y[i] = (T)(p * cs.x - q * cs.y);
+          y[j] = (T)(p * cs.y + q * cs.x);
+        }
       }
     }
   }
@@ -180,7 +188,7 @@ extern "C" int tetris_rotate(const tetris_rotary* r, const void* d_x, int type, 
                    r->head % 8 == 0 && a.half % (a.halves ? 8 : 4) == 0;
   // Few tokens: a workgroup each, or several that share its heads.  Many: as many as fill the table, so that every thread makes an angle or two.
   a.each = 1;
-  while (a.each * 2 * a.half <= kRotaryEntries / 2 && (int64_t)(tokens / (a.each * 2)) >= 1024) a.each *= 2;
+  while (a.each * 2 * a.half <= kRotaryEntries / 2 && tokens / (a.each * 2) >= 2048) a.each *= 2;
   int64_t groups = ceil_div(tokens, a.each);
   a.splits = 1;
   while (a.splits * 2 <= heads && groups * a.splits < 512 && width / (a.splits * 2) >= 1024) a.splits *= 2;
