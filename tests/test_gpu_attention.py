@@ -412,7 +412,106 @@ def test_pages_far_into_a_large_pool():
     within(case.run(), *case.want())
 
 
+# ---- prompts: rows that share what is made of the values ----
+
+
+def many(kind, lengths, fresh, heads, kv_heads, head, page, copies, **how):
+    """Few sequences in the cache, each `copies` times in the call: enough rows for the kernel of prompts.  The case, its outputs and theirs."""
+    c = Case(kind, lengths, fresh, heads, kv_heads, head, page, **how)
+    one = c.lengths, c.fresh, c.table, c.first, c.q, c.k, c.v
+    c.lengths, c.fresh = c.lengths * copies, c.fresh * copies
+    c.table, c.q = np.tile(c.table, (copies, 1)), np.tile(c.q[:c.first[-1]], (copies, 1))
+    c.first = np.concatenate([[0], np.cumsum(c.fresh)]).astype(np.int32)
+    return c, one
+
+
+def check_many(c, one, copies, **how):
+    got = c.run(**how)
+    c.lengths, c.fresh, c.table, c.first, c.q, c.k, c.v = one
+    want, far = c.want(**{k: v for k, v in how.items() if k in ("window", "scale")})
+    got = got.reshape(copies, *want.shape)
+    within(got[0], want, far)
+    assert all(np.array_equal(got[0], g, equal_nan=True) for g in got)
+    return got[0]
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("head", [32, 64, 96, 128, 160, 192, 224, 256])
+def test_prompts(kind, head):
+    c, one = many(kind, [130, 64, 97], [130, 64, 40], 4, 2, head, 16, 40, seed=head)
+    check_many(c, one, 40)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,page,window,pad,offset", [(3, 3, 48, 0, 0, 0), (5, 1, 64, 33, 1, 3), (16, 2, 32, 100, 8, 8), (8, 1, 128, 1, 0, 0)])
+def test_prompts_groups_pages_and_windows(kind, heads, kv_heads, page, window, pad, offset):
+    c, one = many(kind, [150, 0, 65], [90, 3, 65], heads, kv_heads, 64, page, 64, seed=heads)
+    check_many(c, one, 64, window=window, pad=pad, offset=offset)
+
+
+def test_prompts_of_strong_scores():
+    c, one = many("bf16", [200], [200], 4, 1, 128, 16, 64, strength=8.0)
+    check_many(c, one, 64, scale=2.0)
+
+
+def test_prompts_with_values_beyond_f16():
+    """Values of 2^20, 2^-30 and zero next to ordinary ones: some workgroups multiply in bf16, none loses a bit of them."""
+    for big in (2.0 ** 20, 2.0 ** -30, 0.0):
+        c, one = many("bf16", [140], [140], 4, 2, 64, 16, 64)
+        v = rounded_to(c.rng.normal(size=(140, 128)), "bf16")
+        v[70:75, :64] *= big
+        c.put(0, range(140), rounded_to(c.k[0].reshape(140, -1), "bf16"), v)
+        one[6][0] = of_mx4(v).reshape(140, 2, 64)
+        check_many(c, one, 64)
+
+
+@pytest.mark.parametrize("head", [64, 96, 128])
+def test_prompts_with_nan_that_some_rows_see(head):
+    c, one = many("bf16", [100], [100], 4, 2, head, 16, 64)
+    clean = check_many(c, one, 64).reshape(100, 4, head)
+    c, one = many("bf16", [100], [100], 4, 2, head, 16, 64)
+    v = rounded_to(c.v[0].reshape(100, -1), "bf16")
+    v[40, head + 33] = np.nan  # kv head 1, block 1: rows 40 .. see it
+    c.put(0, range(100), rounded_to(c.k[0].reshape(100, -1), "bf16"), v)
+    got = c.run().reshape(64, 100, 4, head)
+    hit = np.zeros(clean.shape, bool)
+    hit[40:, 2:, 32:64] = True
+    for g in got[[0, 63]]:
+        assert np.isnan(g[hit]).all() and np.array_equal(g[~hit], clean[~hit])
+
+
+def test_prompts_pages_outside_of_the_pool():
+    c, one = many("bf16", [130], [130], 4, 2, 64, 16, 64)
+    c.table[:, 3], c.table[:, 7] = -7, c.pages
+    got = c.run().reshape(64, 130, -1)
+    c.lengths, c.fresh, c.table, c.first, c.q, c.k, c.v = one
+    want, far = c.want(absent={0: list(range(48, 64)) + list(range(112, 128))})
+    within(got[0], want, far)
+    within(got[63], want, far)
+
+
 # ---- streams, graphs, workspaces ----
+
+
+def test_a_workspace_made_for_some_sequences_serves_fewer():
+    c = Case("bf16", [2000, 900, 3], [1, 1, 1], 8, 2, 128, 32)
+    stream = torch.cuda.Stream()
+    q, (y, _) = on_gpu(c.q, "bf16"), out_like(3, 1024, "bf16")
+    length, table = torch.tensor(c.lengths, dtype=torch.int32, device="cuda"), torch.from_numpy(c.table).cuda()
+    torch.cuda.synchronize()
+    c.cache.handle.prepare(8, 400, 2000, T.BF16, rows=2000, most_rows=5, stream=stream.cuda_stream)
+    with torch.cuda.stream(stream):
+        for n, most in ((3, 2000), (1, 2000), (2, 2000)):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                c.cache.handle.attend(q.data_ptr(), y.data_ptr(), T.BF16, 8, n, length.data_ptr(), table.data_ptr(), most, ld_table=table.shape[1],
+                                      stream=stream.cuda_stream)
+            y.fill_(77.0)
+            graph.replay()
+            stream.synchronize()
+            want, far = c.want()
+            within(numbers(y)[:n], want[:n], far[:n])
+            assert (y[n:] == 77.0).all()
 
 
 def test_captured_and_replayed():

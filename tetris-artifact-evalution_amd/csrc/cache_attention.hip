@@ -1077,23 +1077,40 @@ constexpr int kMostTiles = most_tiles(kParts<TYPE>, D);
 
 // How a call is cut: by its sizes alone, so that its workspace can be made ahead.
 struct Cut { bool prompt; int tiles, blocks, workgroups, chunk, chunks; int64_t units, most; size_t part, shares, space; };
+
+// Whether rows share what is made of the values (attend_prompt_kernel) or each block of 16 NT rows makes its own (the others), by the microseconds that each is
+// expected to take.  Measured, and what these fit within a fifth: 4 prompts of 300, 16 by 4 heads of 128: 19 us against 27; 16 of 128 16 against 30; 32 newest
+// rows of 32 sequences of 4096 126 against 148; one prompt of 1024 of 8 by 8 heads, whose last workgroups are long alone, 38 against 28; 16 newest rows of 8
+// sequences of 4096 120 against 36.
+bool shares_values(const tetris_attention* a, int kv_heads, int head, int type, int64_t rows, int tiles) {
+  if (rows <= 32) return false;
+  const double parts = type == TETRIS_BF16 ? 1.0 : type == TETRIS_F16 ? 1.5 : 2.0, size = tiles * head / 128.0 * parts;
+  const double length = a->window ? std::min<double>(a->most_length, (double)a->window + a->most_rows) : a->most_length;
+  const double seen = std::max(length - std::min<double>(a->most_rows, length) / 2, 1.0), units = (double)a->sequences * kv_heads;
+  // turns of 64 tokens: the longest workgroup's alone, all of them with two on a compute unit
+  const double turn = (0.7 + 0.58 * size) * (head > 128 ? 1.4 : 1.0), groups = units * std::ceil(rows / (16.0 * tiles * kPromptWaves));
+  const double prompt = 8 + std::max(turn * std::ceil(length / kTurn), groups * seen / kTurn * turn * 1.25 / (head > 128 ? 256 : 512));
+  // steps of 32 tokens by a block, on 1024 SIMDs, and a workgroup's beginning and end
+  const double blocks = units * std::ceil(rows / (16.0 * tiles));
+  const double other = 8 + 8 * std::max(1.0, blocks / (256 * waves_of(parts_of(type), head, tiles))) + blocks * seen / kStep * (0.4 + 0.38 * size) / 1024;
+  return prompt < other;
+}
+
 Cut cut_of(const tetris_cache* c, const tetris_attention* a, int type) {
   Cut k{};
   const int64_t rows = (int64_t)std::min(a->most_rows, a->rows) * (a->heads / c->kv_heads);
   k.tiles = rows <= 16 ? 1 : most_tiles(parts_of(type), c->head);
   k.blocks = (int)((rows + 16 * k.tiles - 1) / (16 * k.tiles));
-  const int64_t span = a->window ? std::min<int64_t>(a->most_length, (int64_t)a->window + a->most_rows + kStep) : a->most_length;
-  const int64_t quanta = std::max<int64_t>((span + kQuantum - 1) / kQuantum, 1);
   k.units = (int64_t)a->sequences * c->kv_heads * k.blocks;
-  k.most = k.units * (quanta + kBegin);
-  const int64_t turns = (int64_t)a->sequences * c->kv_heads * ((k.blocks + kPromptWaves - 1) / kPromptWaves);
-  const int PR=getenv("PR")?atoi(getenv("PR")):64, PW=getenv("PW")?atoi(getenv("PW")):64;
-  k.prompt = rows > PR && turns >= PW;
+  k.prompt = shares_values(a, c->kv_heads, c->head, type, rows, k.tiles);
   if (k.prompt) {
-    k.tiles = most_tiles(parts_of(type), c->head);
-    k.workgroups = (int)std::min<int64_t>(turns, 0x7fffffff);
+    k.most = (int64_t)a->sequences * c->kv_heads * ((k.blocks + kPromptWaves - 1) / kPromptWaves);
+    k.workgroups = (int)std::min<int64_t>(k.most, 0x7fffffff);
     return k;
   }
+  const int64_t span = a->window ? std::min<int64_t>(a->most_length, (int64_t)a->window + a->most_rows + kStep) : a->most_length;
+  const int64_t quanta = std::max<int64_t>((span + kQuantum - 1) / kQuantum, 1);
+  k.most = k.units * (quanta + kBegin);
   const int resident = 256 * waves_of(parts_of(type), c->head, k.tiles);
   if (a->sequences > 1 && k.most >= 16 * (int64_t)resident) {
     k.workgroups = resident;
@@ -1103,8 +1120,7 @@ Cut cut_of(const tetris_cache* c, const tetris_attention* a, int type) {
     k.chunks = (int)((quanta + k.chunk - 1) / k.chunk);
     k.workgroups = (int)std::min<int64_t>(k.units * k.chunks, 0x7fffffff);
   }
-  if (k.chunks != 1) k.part = (size_t)k.workgroups * 2 * 16 * k.tiles * (c->head + 2) * sizeof(float);
-  k.part = (k.part + 15) / 16 * 16;
+  if (k.chunks != 1) k.part = ((size_t)k.workgroups * 2 * 16 * k.tiles * (c->head + 2) * sizeof(float) + 15) / 16 * 16;
   k.shares = (size_t)k.units * sizeof(int2);
   k.space = k.part + k.shares;
   return k;
@@ -1167,8 +1183,13 @@ extern "C" int tetris_cache_prepare(tetris_cache* c, const tetris_attention* a, 
   int rc = check_attention(c, a, type);
   if (!rc) rc = check_cache(c);
   if (rc) return rc;
+  // what a call of these sizes or smaller ones may take: parts of as many workgroups as run at once
+  size_t part = 0;
+  for (int tiles = 1; tiles <= most_tiles(parts_of(type), c->head); ++tiles)
+    part = std::max(part, (size_t)256 * waves_of(parts_of(type), c->head, tiles) * 2 * 16 * tiles * (c->head + 2) * sizeof(float));
+  const int64_t rows = (int64_t)std::min(a->most_rows, a->rows) * (a->heads / c->kv_heads);
   uint8_t* d;
-  return c->space.get(static_cast<hipStream_t>(stream), cut_of(c, a, type).space, &d);
+  return c->space.get(static_cast<hipStream_t>(stream), part + (size_t)a->sequences * c->kv_heads * ((rows + 15) / 16) * sizeof(int2), &d);
 }
 
 extern "C" int tetris_cache_attend(tetris_cache* c, const tetris_attention* a, const void* d_q, int64_t ldq, int type, const int32_t* d_first,
