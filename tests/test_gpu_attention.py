@@ -631,3 +631,16 @@ def test_a_step_of_the_whole_half():
         step()
         torch.cuda.synchronize()
         assert np.array_equal(eager, numbers(y))
+
+
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("tokens,context", [(1, 1), (5, 70), (33, 129)])
+def test_the_block_with_its_attention(tokens, context, graph):
+    """python -m tetris_amd.expert_block: each operator from what the one before it gave; a rounding to bf16 bounds each error, 2^-8, and the sums
+    and weights in 32 or 11 bits a sixteenth of that."""
+    from tetris_amd import expert_block
+
+    args = ["--tokens", str(tokens), "--width", "256", "--hidden", "96", "--experts", "12", "--top", "3", "--classes", "50", "--steps", "3", "--context", str(context)]
+    out = expert_block.main(args + (["--graph"] if graph else []))
+    assert out["query_error"] <= 2.0 ** -8 and out["sum_error"] <= 2.0 ** -8 and out["attention_error"] <= 17 / 16 * 2.0 ** -8
+    assert out["block_error"] <= 3 * 2.0 ** -8 and out["scores_error"] <= 2.0 ** -8
