@@ -65,8 +65,8 @@ int tetris_cache_read(tetris_cache* c, const int64_t* d_slot, int tokens, void* 
  * h / (heads / kv_heads)) of `sequences` sequences: sequence s has rows d_first[s] .. d_first[s + 1] - 1, the newest tokens of
  * the d_length[s] that are cached of it, or without d_first row s alone.  Token j of a sequence lies in page d_table[s][j / page]
  * at place j % page.  Row i of n of a sequence of length L is at position p = L - n + i, sees tokens j with j <= p and, with a window,
- * j > p - window, and becomes  y = sum_j softmax_j(scale * q.k_j) v_j; a row that sees nothing becomes zeros.  Keys and values
- * that a row does not see do not touch it, whatever they are.
+ * j > p - window, and becomes  y = sum_j softmax_j(scale * q.k_j) v_j; a row that sees nothing becomes zeros (a score of
+ * minus infinity counts as not seen).  Keys and values that a row does not see do not touch it, whatever they are.
  * most_length (up to 2^28) and most_rows: no sequence is longer, nor has more rows; what is longer counts as most_length, rows beyond most_rows are left as they
  * are, as are those of no sequence.  d_table: a row of ceil(most_length / page) page numbers for each sequence, ld_table
  * apart; a number outside of the pool stands for a page that no row sees.  The lengths, tables and offsets are read on the device: a captured

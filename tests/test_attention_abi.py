@@ -94,6 +94,12 @@ def test_attend_refusals():
     attend(rows=0, d_first=A)()
 
 
+def test_scales_that_are_not_finite_are_refused():
+    c = T.MX4Cache(A, 4, 2, 64, page=16)
+    for scale in (float("nan"), float("inf"), -float("inf"), 3e38):
+        refused(lambda: c.attend(A, B, T.F32, 4, 3, A, A, 40, scale=scale))
+
+
 def test_plain_forms_of_worked_numbers():
     s, _, y, _ = P.rms_norm(np.array([[3.0, 3.0]]), np.array([[0.0, 1.0]]), np.array([1.0, 2.0]), 0.0, "f32")
     assert list(s[0]) == [3, 4] and np.allclose(y, [[3 / 12.5 ** 0.5, 8 / 12.5 ** 0.5]])

@@ -644,3 +644,54 @@ def test_the_block_with_its_attention(tokens, context, graph):
     out = expert_block.main(args + (["--graph"] if graph else []))
     assert out["query_error"] <= 2.0 ** -8 and out["sum_error"] <= 2.0 ** -8 and out["attention_error"] <= 17 / 16 * 2.0 ** -8
     assert out["block_error"] <= 3 * 2.0 ** -8 and out["scores_error"] <= 2.0 ** -8
+
+
+# ---- more rows than a launch has, more rows than the call says ----
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("most_rows", [1, 3])
+@pytest.mark.parametrize("length,fresh,window", [(3000, 500, 100), (900, 900, 40), (20, 400, 7)])
+def test_most_rows_below_the_rows_of_a_window(kind, most_rows, length, fresh, window):
+    """The rows' window begins far before the newest token: what is cut by most_rows has as many parts as the launch is made for."""
+    c = Case(kind, [length, 50], [fresh, 1], 4, 2, 64, 16)
+    want, far = c.want(window=window)
+    got = c.run(window=window, most_rows=most_rows)
+    done = list(range(most_rows)) + [fresh]
+    within(got[done], want[done], far[done])
+    assert (got[most_rows:fresh] == 77.0).all()
+
+
+def test_most_rows_below_the_rows_of_a_window_in_equal_shares():
+    c, one = many("bf16", [300], [40], 4, 2, 64, 16, 1700)
+    got = c.run(window=100, most_rows=2).reshape(1700, 40, -1)
+    c.lengths, c.fresh, c.table, c.first, c.q, c.k, c.v = one
+    want, far = c.want(window=100)
+    within(got[0, :2], want[:2], far[:2])
+    within(got[-1, :2], want[:2], far[:2])
+    assert (got[:, 2:] == 77.0).all() and (got[:, :2] == got[:1, :2]).all()
+
+
+def test_norm_of_more_rows_than_a_launch_has():
+    """2^26 rows of a wave each are 2^32 threads."""
+    rows = (1 << 26) + 5
+    x = torch.randn(rows, 1, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    y = torch.full_like(x, 77.0)
+    T.rms_norm(x.data_ptr(), y.data_ptr(), T.F32, rows, 1, eps=0.5)
+    x = x.double()
+    # the square and the sum's division half a step each, halved by the root; the root, the reciprocal and the product as much again each
+    assert ((y - x / (x * x + 0.5).sqrt()).abs() <= 5 * 2.0 ** -24).all()
+
+
+def test_rotary_of_more_tokens_than_a_launch_has():
+    """2^24 tokens of a workgroup each are 2^32 threads; in place.  A turn by 1 or 2 radians of (1, 0)."""
+    tokens, head = (1 << 24) + 3, 1024
+    x = torch.zeros(tokens, head, dtype=torch.float16, device="cuda")
+    x[:, 0] = 1
+    position = torch.ones(tokens, dtype=torch.int32, device="cuda")
+    position[-1] = 2
+    T.Rotary(head).rotate(x.data_ptr(), x.data_ptr(), T.F16, tokens, 1, position.data_ptr())
+    for part in (x[:1 << 22], x[1 << 22:-1]):
+        assert (part[:, 0] == float(np.float16(np.cos(1)))).all() and (part[:, head // 2] == float(np.float16(np.sin(1)))).all()
+    assert float(x[-1, 0]) == np.float16(np.cos(2)) and float(x[-1, head // 2]) == np.float16(np.sin(2))
+    assert not x[-5:, 1:head // 2].any() and not x[-5:, head // 2 + 1:].any()

@@ -419,7 +419,7 @@ struct Pages { int page[2]; };
 __device__ inline unsigned page_index(const Attend& a, unsigned granule) { return a.page_magic ? __umulhi(granule, a.page_magic) : granule; }
 
 // How the work is dealt out.  A unit is a block of 16 NT rows of a sequence and kv head; it is as many quanta of four steps as its sequence
-// has tokens for (one at least: rows that see nothing become zeros).  What a workgroup does of a unit that it does not do all of it leaves to join_kernel.
+// tokens that its rows see (one at least: rows that see nothing become zeros).  What a workgroup does of a unit that it does not do all of it leaves to join_kernel.
 //   little work     a.chunk quanta of one unit each; chunks that a sequence is too short for end at once.  It begins without looking at the
 //                   other sequences: one token of 4000 tokens by 32 heads takes 10 us in place of 13.
 //   much work       the units' quanta, sequence after sequence, in equal shares, whatever the lengths are: 64 sequences of up to 8192 tokens, 3700 on
@@ -428,8 +428,9 @@ constexpr int kQuantum = 4 * kStep;
 constexpr int kBegin = 3;  // quanta's time that a unit takes besides: queries, the first loads, joining the waves' outputs
 struct Units { int quanta, blocks; };
 __device__ inline Units units_of(const Attend& a, const Sequence& q) {
-  const int rows = min(q.rows, a.most_rows) * a.group, size = 16 * a.tiles;
-  return {max((q.length - q.base + kQuantum - 1) / kQuantum, 1), (rows + size - 1) / size};
+  const int count = min(q.rows, a.most_rows), rows = count * a.group, size = 16 * a.tiles;
+  const int seen = q.length - q.rows + count - q.base;  // (up to the last row that is worked on: no more than the launch is cut for, with a window too)
+  return {max((seen + kQuantum - 1) / kQuantum, 1), (rows + size - 1) / size};
 }
 __device__ inline int quanta_of(const Attend& a, int s) {
   if (s >= a.sequences) return 0;
@@ -1171,6 +1172,7 @@ int check_attention(const tetris_cache* c, const tetris_attention* a, int type) 
   if (a->sequences < 0 || a->rows < 0 || a->most_rows < 0 || a->most_length < 0 || a->window < 0)
     return fail(TETRIS_EINVAL, "%d sequences, %d rows (at most %d each), %d tokens, window %d", a->sequences, a->rows, a->most_rows, a->most_length, a->window);
   if (a->most_length > kCacheLength || a->rows > 0x40000000 / a->heads) return fail(TETRIS_EINVAL, "%d rows of %d heads, %d tokens (up to 2^30 and 2^28)", a->rows, a->heads, a->most_length);
+  if (!std::isfinite(a->scale * 1.44269504088896340736f)) return fail(TETRIS_EINVAL, "scale %g is not finite in powers of two", (double)a->scale);
   return TETRIS_OK;
 }
 
@@ -1210,7 +1212,8 @@ extern "C" int tetris_cache_attend(tetris_cache* c, const tetris_attention* a, c
   if (d_q == d_y) return fail(TETRIS_EINVAL, "the output is the input");
   if ((rc = check_cache(c))) return rc;
   const Cut k = cut_of(c, a, type);
-  if (k.most > 0x7fffffff || k.units * 4 * k.tiles > 0x7fffffff)
+  // a launch has fewer than 2^32 threads
+  if (k.most > 0x7fffffff || k.workgroups >= 1 << 24 || (!k.prompt && k.chunks != 1 && k.units * 4 * k.tiles >= 1 << 24))
     return fail(TETRIS_EUNSUPPORTED, "%d sequences of up to %d rows and %d tokens are more than a launch has", a->sequences, a->most_rows, a->most_length);
   uint8_t* d = nullptr;
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -154,7 +154,7 @@ __global__ __launch_bounds__(THREADS) void rms_norm_kernel(NormRows a) {
 
 template <int TYPE, bool VEC>
 void launch(const NormRows& a, int64_t rows, hipStream_t s) {
-  constexpr int64_t kMost = 1 << 30;  // rows of a launch
+  constexpr int64_t kMost = 1 << 21;  // rows of a launch, which has fewer than 2^32 threads
   constexpr int size = TYPE == TETRIS_F32 ? 4 : 2;
   for (int64_t from = 0; from < rows; from += kMost) {
     NormRows b = a;

@@ -4,6 +4,7 @@
 // A pair's angle in turns is formed in 64 bits and its whole turns taken off, which leaves a far position's angle exact to about
 // 2^-49 of the position.  What is left goes to 32 bits as t + d with d below 2^-25 t, and cos(t + d) = cos t - d sin t, so that the cosine is
 // as near as one rounded from 64 bits.
+#include <algorithm>
 #include <cmath>
 
 #include "mx4.h"
@@ -189,14 +190,22 @@ extern "C" int tetris_rotate(const tetris_rotary* r, const void* d_x, int type, 
   // Few tokens: a workgroup each, or several that share its heads.  Many: as many as fill the table, so that every thread makes an angle or two.
   a.each = 1;
   while (a.each * 2 * a.half <= kRotaryEntries / 2 && tokens / (a.each * 2) >= 2048) a.each *= 2;
-  int64_t groups = ceil_div(tokens, a.each);
+  constexpr int kMost = 1 << 22;  // tokens of a launch, which has fewer than 2^32 threads
+  const int64_t groups = ceil_div(std::min(tokens, kMost), a.each);
   a.splits = 1;
   while (a.splits * 2 <= heads && groups * a.splits < 512 && width / (a.splits * 2) >= 1024) a.splits *= 2;
-  if (groups * a.splits > 0x7fffffff) a.splits = 1;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (type == TETRIS_F32) launch<TETRIS_F32>(a, vec, groups * a.splits, s);
-  else if (type == TETRIS_F16) launch<TETRIS_F16>(a, vec, groups * a.splits, s);
-  else launch<TETRIS_BF16>(a, vec, groups * a.splits, s);
+  for (int from = 0; from < tokens; from += std::min(kMost, tokens - from)) {
+    Rotary b = a;
+    b.x = static_cast<const char*>(d_x) + from * ldx * size;
+    b.y = static_cast<char*>(d_y) + from * ldy * size;
+    b.position = d_position + from;
+    b.tokens = std::min(kMost, tokens - from);
+    const int64_t grid = (int64_t)ceil_div(b.tokens, b.each) * b.splits;
+    if (type == TETRIS_F32) launch<TETRIS_F32>(b, vec, grid, s);
+    else if (type == TETRIS_F16) launch<TETRIS_F16>(b, vec, grid, s);
+    else launch<TETRIS_BF16>(b, vec, grid, s);
+  }
   TETRIS_HIP(hipGetLastError());
   return TETRIS_OK;
 }
