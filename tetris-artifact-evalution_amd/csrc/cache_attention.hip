@@ -774,11 +774,12 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void attend_prompt_kernel(Att
   __shared__ uint8_t nan_of[2][kTurn * N];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, quad = lane >> 4;
   // (kv heads first: the workgroups of one kv head are a multiple of 8 apart where there are 8, 16, .. kv heads, on one of the eight dies, whose cache then
-  // holds this kv head's tokens; the last rows first, which see the most)
+  // holds this kv head's tokens; the last rows first, which see the most.  Sequences take turns in another order from one row of workgroups to the next: a die
+  // deals its workgroups to its four shader engines in turn, each of which would have one sequence of four, however long they are)
   int id = blockIdx.x;
   const int kv = id % a.kv_heads;
   id /= a.kv_heads;
-  const int s = id % a.sequences, group = (a.blocks + W - 1) / W - 1 - id / a.sequences;
+  const int turn = id / a.sequences, s = (int)((unsigned)(id + turn + turn / 4) % (unsigned)a.sequences), group = (a.blocks + W - 1) / W - 1 - turn;
   const Sequence seq = sequence_of(a, s);
   const int all = min(seq.rows, a.most_rows) * a.group, w0 = group * W * (16 * NT), r0 = w0 + wave * (16 * NT);
   if (w0 >= all) return;
