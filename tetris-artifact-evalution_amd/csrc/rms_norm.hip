@@ -204,7 +204,7 @@ extern "C" int tetris_rms_norm(const void* d_x, int type, int64_t rows, int cols
   hipStream_t s = static_cast<hipStream_t>(stream);
   const size_t size = elem_size(type);
   auto whole = [&](const void* p, int64_t ld) { return !p || ((reinterpret_cast<size_t>(p) & 15) == 0 && ld * size % 16 == 0); };
-  const bool vec = cols % 8 == 0 && whole(d_x, ldx) && whole(d_residual, ld_residual) && whole(d_sum, ld_sum) && whole(d_y, ldy) && whole(d_weight, 4);
+  const bool vec = cols % 8 == 0 && whole(d_x, ldx) && whole(d_residual, ld_residual) && whole(d_sum, ld_sum) && whole(d_y, ldy) && (reinterpret_cast<size_t>(d_weight) & 15) == 0;
   if (type == TETRIS_F32) vec ? launch<TETRIS_F32, true>(a, rows, s) : launch<TETRIS_F32, false>(a, rows, s);
   else if (type == TETRIS_F16) vec ? launch<TETRIS_F16, true>(a, rows, s) : launch<TETRIS_F16, false>(a, rows, s);
   else vec ? launch<TETRIS_BF16, true>(a, rows, s) : launch<TETRIS_BF16, false>(a, rows, s);
