@@ -6,9 +6,13 @@
 //   outputs   O^T [elements][rows] += V^T P^T     the same instruction; the page's layout (csrc/cache.h) gives a lane the values of the tokens whose
 //                                               weights it holds, so that weights go from one product to the next without leaving the lane
 // A key or value has two significant bits and its scale's exponent: exact in bf16.  q comes in 1, 2 or 3 bf16 parts (bf16, f16, f32), which hold
-// all of its bits, and P in two (16 bits; f32: three), so outputs are those of 32-bit arithmetic rounded once.
+// all of its bits, and P in two (16 bits; f32: three; attend_prompt_kernel has one of 11 bits for bf16), so outputs are those of 32-bit arithmetic rounded once.
 // m is raised only to a score that is more than 8 above it (weights are at most 2^8, far from overflow); most steps need no exchange
 // between lanes for it.  A row's sum stays apart in four lanes until the end.
+//
+// One token a sequence is bound by the cache's bytes: 64 sequences of 8192 tokens by 8 kv heads of 128 (570 MB) take 122 us with the joining, 4.7 TB/s, where a
+// copy reaches 4.9; of up to 8192 tokens, 3700 on average (259 MB), 61.  Small calls are bound by their chain: page number, granule, two products with the
+// softmax between them, the waves' join, the chunks' join: 4000 tokens 7 + 4 us.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -423,7 +427,7 @@ __device__ inline unsigned page_index(const Attend& a, unsigned granule) { retur
 //   little work     a.chunk quanta of one unit each; chunks that a sequence is too short for end at once.  It begins without looking at the
 //                   other sequences: one token of 4000 tokens by 32 heads takes 10 us in place of 13.
 //   much work       the units' quanta, sequence after sequence, in equal shares, whatever the lengths are: 64 sequences of up to 8192 tokens, 3700 on
-//                   average, take 68 us in place of 86.
+//                   average, take 61 us (68 in place of 86 when both were measured).
 constexpr int kQuantum = 4 * kStep;
 constexpr int kBegin = 3;  // quanta's time that a unit takes besides: queries, the first loads, joining the waves' outputs
 struct Units { int quanta, blocks; };
@@ -642,8 +646,11 @@ __global__ __launch_bounds__(256, waves_of(kParts<TYPE>, D, NT)) void attend_sha
 // All waves' writes to LDS are done; loads from memory may be under way (__syncthreads would wait for them too).
 __device__ inline void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// Many rows of a sequence: four waves, each with 16 NT rows of its own, share what is made of the keys and values of 64 tokens: each makes a quarter of it
-// bf16, in the form in which the products take it, and leaves it in LDS (8 KiB for 32 elements of a head, twice, so that one barrier a turn is enough).
+// Many rows of a sequence (prompts, drafts of many tokens).  Four waves, each with 16 NT rows of its own, share what is made of the keys and values of 64
+// tokens: each makes a quarter of it bf16, in the form in which the products take it, and leaves it in LDS (8 KiB for 32 elements of a head, twice, so that
+// one barrier a turn is enough).  What bounds it is the vector instructions around the products (softmax, conversions, addresses), which hide little behind them:
+// four prompts of 1030, 1791, 3917 and 4096 tokens, 32 by 8 heads of 128, take 373 us, 800 TFLOP/s of what their rows see, with the matrix cores busy
+// a third of the time.  (128 fma beside 32 products of 16x16x32 cost two thirds of what they cost alone, four waves a SIMD; exponentials cost nothing.)
 //
 // A weight of bf16 operators enters the second product as f16, 2^7 as large as it is (2^15 at most), with values that are exact in f16: one
 // product in place of two, and one conversion of a pair of weights in place of six instructions.  It is within 2^-12 of itself, or 2^-32 of the row's
@@ -765,7 +772,7 @@ struct Share {
 };
 
 template <int TYPE, int D, int NT>
-__global__ __launch_bounds__(64 * kPromptWaves, 2) void attend_prompt_kernel(Attend a) {
+__global__ __launch_bounds__(64 * kPromptWaves, D <= 128 ? 2 : 1) void attend_prompt_kernel(Attend a) {
   using T = typename Elem<TYPE>::type;
   using R = Rows<TYPE, D, NT>;
   constexpr int N = D / 32, S = D / 16, W = kPromptWaves, QP = R::QP, PP = R::PP;

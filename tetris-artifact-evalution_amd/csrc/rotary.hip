@@ -1,5 +1,7 @@
 // Rotary positions: pairs of a head's elements turned by position * rate, each pair by the position of its section's axis.  A workgroup
-// makes the cosines and sines of a few tokens once, in LDS, and turns all heads of these tokens with them; one pass over memory.
+// makes the cosines and sines of a few tokens once, in LDS, and turns all heads of these tokens with them; one pass over memory, which
+// bounds it: 4096 tokens of 32 heads of 128 f32 29 us (134 MB, 4.7 TB/s), 15000 of 16 of 80 f16 with three axes 14.7 (77 MB, 5.2 TB/s); 8 tokens
+// are a launch, 3.3 us.
 //
 // A pair's angle in turns is formed in 64 bits and its whole turns taken off, which leaves a far position's angle exact to about
 // 2^-49 of the position.  What is left goes to 32 bits as t + d with d below 2^-25 t, and cos(t + d) = cos t - d sin t, so that the cosine is
