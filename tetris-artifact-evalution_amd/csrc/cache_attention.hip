@@ -648,9 +648,9 @@ __device__ inline void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_b
 
 // Many rows of a sequence (prompts, drafts of many tokens).  Four waves, each with 16 NT rows of its own, share what is made of the keys and values of 64
 // tokens: each makes a quarter of it bf16, in the form in which the products take it, and leaves it in LDS (8 KiB for 32 elements of a head, twice, so that
-// one barrier a turn is enough).  What bounds it is the vector instructions around the products (softmax, conversions, addresses), which hide little behind them:
-// four prompts of 1030, 1791, 3917 and 4096 tokens, 32 by 8 heads of 128, take 373 us, 800 TFLOP/s of what their rows see, with the matrix cores busy
-// a third of the time.  (128 fma beside 32 products of 16x16x32 cost two thirds of what they cost alone, four waves a SIMD; exponentials cost nothing.)
+// one barrier a turn is enough).  Four prompts of 1030, 1791, 3917 and 4096 tokens, 32 by 8 heads of 128, take 373 us, 800 TFLOP/s of what their rows see.
+// No unit is full: the products alone would take 145 us at the rate that a loop of them reaches, the vector instructions (softmax, conversions,
+// addresses) 112, LDS 100; a wave needs them one after another, and the registers leave room for two waves a SIMD.
 //
 // A weight of bf16 operators enters the second product as f16, 2^7 as large as it is (2^15 at most), with values that are exact in f16: one
 // product in place of two, and one conversion of a pair of weights in place of six instructions.  It is within 2^-12 of itself, or 2^-32 of the row's
