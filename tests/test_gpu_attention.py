@@ -695,3 +695,28 @@ def test_rotary_of_more_tokens_than_a_launch_has():
         assert (part[:, 0] == float(np.float16(np.cos(1)))).all() and (part[:, head // 2] == float(np.float16(np.sin(1)))).all()
     assert float(x[-1, 0]) == np.float16(np.cos(2)) and float(x[-1, head // 2]) == np.float16(np.sin(2))
     assert not x[-5:, 1:head // 2].any() and not x[-5:, head // 2 + 1:].any()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,heads", [(1, 4), (3, 4), (200, 16)])
+def test_calls_for_no_tokens_at_all(kind, rows, heads):
+    """most_length 0, with which there is no table: every row sees nothing."""
+    c = Cache(1, 2, 64, 16)
+    q = on_gpu(np.ones((2 * rows, heads * 64)), kind, heads * 64)
+    y, around = out_like(2 * rows, heads * 64, kind, heads * 64)
+    first, length = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([0, rows, 2 * rows], [0, 9]))
+    c.handle.attend(q.data_ptr(), y.data_ptr(), TYPES[kind][0], heads, 2, length.data_ptr(), 0, 0, d_first=first.data_ptr(), rows=2 * rows, most_rows=rows)
+    assert (numbers(y) == 0).all()
+    untouched(around, y)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("lengths,kv_heads", [([40], 1), ([4100, 70], 2)])
+def test_calls_made_for_the_longest_sequences(kind, lengths, kv_heads):
+    """most_length 2^28, where sequences are short: few quanta of many, by chunks and by equal shares."""
+    c = Case(kind, lengths, [1] * len(lengths), 2, kv_heads, 64, 4096)
+    want, far = c.want()
+    table = np.full((len(lengths), (1 << 28) // 4096), -1, np.int32)
+    table[:, : c.table.shape[1]] = c.table
+    c.table, c.most = table, 1 << 28
+    within(c.run(), want, far)
