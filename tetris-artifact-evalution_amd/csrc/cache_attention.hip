@@ -319,7 +319,7 @@ struct Rows {
         for (int i = 0; i < 4; ++i) top[n] = fmaxf(top[n], x[n][u][i]);
       top[n] *= a.scale;
       // Taken before the branch: where a branch comes between a matrix instruction and the first use of its result, the compiler has left out
-      // the wait that the instruction needs (tests/test_matrix_waits.py looks for that in the built library).
+      // the wait that the instruction needs (tests/test_matrix_waits_of_every_kernel.py looks for that in the built library).
       asm volatile("" : "+v"(top[n]));
       above = above || top[n] > m[n] + kRoom;
     }
