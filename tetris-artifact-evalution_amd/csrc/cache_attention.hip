@@ -591,6 +591,7 @@ __device__ inline void attend_unit(const Attend& a, const Sequence& seq, int qua
 }
 
 // Waves of a SIMD, and so workgroups of a compute unit, that the registers of a wave leave room for.
+constexpr int kResidentMost = 256 * 4;  // workgroups that run at once, for any of them
 constexpr int waves_of(int parts, int head, int tiles) { return parts * tiles * head <= 64 ? 4 : tiles * head <= 128 && parts * tiles * head <= 256 ? 3 : 2; }
 // (Two waves a SIMD at least: with 256 registers or fewer the products' sums stay in ordinary registers, not in those that have to be copied for the rest.)
 template <int TYPE, int D, int NT>
@@ -1218,11 +1219,11 @@ extern "C" int tetris_cache_attend(tetris_cache* c, const tetris_attention* a, c
   if ((reinterpret_cast<size_t>(d_first) | reinterpret_cast<size_t>(d_length) | reinterpret_cast<size_t>(d_table)) & 3)
     return fail(TETRIS_EINVAL, "offsets, lengths or table not aligned to their elements");
   if (d_q == d_y) return fail(TETRIS_EINVAL, "the output is the input");
-  if ((rc = check_cache(c))) return rc;
   const Cut k = cut_of(c, a, type);
-  // a launch has fewer than 2^32 threads
-  if (k.most > 0x7fffffff || k.workgroups >= 1 << 24 || (!k.prompt && k.chunks != 1 && k.units * 4 * k.tiles >= 1 << 24))
+  // a launch has fewer than 2^32 threads; attend_shares_kernel's quanta are numbered in 31 bits, up to its last workgroup's share, which may pass their end
+  if (k.most > 0x7fffffff - kResidentMost || k.workgroups >= 1 << 24 || (!k.prompt && k.chunks != 1 && k.units * 4 * k.tiles >= 1 << 24))
     return fail(TETRIS_EUNSUPPORTED, "%d sequences of up to %d rows and %d tokens are more than a launch has", a->sequences, a->most_rows, a->most_length);
+  if ((rc = check_cache(c))) return rc;
   uint8_t* d = nullptr;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if ((rc = c->space.get(s, k.space, &d))) return rc;
