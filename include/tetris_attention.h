@@ -14,7 +14,7 @@ extern "C" {
 /* ------------------------------------------------------------------------------------------------
  * s = x + residual and y = s / sqrt(mean(s^2) + eps) * weight, row by row.  d_residual NULL: s = x.  d_weight: cols floats, or
  * NULL for ones.  d_sum, NULL or rows of `type` for s rounded; d_sum may be d_residual (with ld_sum = ld_residual), nothing else overlaps.
- * The norm is of s in 32 bits, before it is rounded.  Columns up to 2^20.
+ * The norm is of s in 32 bits, before it is rounded, also where its squares are beyond them or vanish in them.  Columns up to 2^20.
  * ---------------------------------------------------------------------------------------------- */
 int tetris_rms_norm(const void* d_x, int type, int64_t rows, int cols, int64_t ldx, const void* d_residual, int64_t ld_residual,
                     const float* d_weight, float eps, void* d_sum, int64_t ld_sum, void* d_y, int64_t ldy, void* stream);

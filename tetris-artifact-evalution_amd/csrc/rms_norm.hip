@@ -130,7 +130,43 @@ __global__ __launch_bounds__(THREADS) void rms_norm_kernel(NormRows a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) squares = fmaf(t[i], t[i], squares);
   }
-  const float by = 1.f / sqrtf(sum_of_all<THREADS>(squares, shared) / (float)a.cols + a.eps);
+  const float under = sum_of_all<THREADS>(squares, shared) / (float)a.cols + a.eps;
+  if (__builtin_expect(!(under >= 0x1p-100f && under < __builtin_inff()), 0)) {
+    // Squares that 32 bits do not hold are taken of the row scaled by a power of two: elements up to 2^128 by 2^-80, and where what is under the root is
+    // below 2^-100, elements from 2^-149 on by 2^96.  The row is read again for that, so that the registers of ordinary ones are what they were.
+    const bool small = under < 1.f;
+    const float scale = small ? 0x1p96f : 0x1p-80f;
+    auto again = [&](auto each) {
+#pragma unroll 1
+      for (int p = 0; p < pieces; ++p) {
+        P u, v;
+        float t[8];
+        u.load(x, p, a.cols);
+        if (r) v.load(r, p, a.cols);
+        total(u, v, p, t);
+        each(p, t);
+      }
+    };
+    if constexpr (THREADS > 64) __syncthreads();  // (the waves' sums have been read)
+    float scaled = 0.f;
+    again([&](int, const float (&t)[8]) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) scaled = fmaf(t[i] * scale, t[i] * scale, scaled);
+    });
+    const float by = 1.f / sqrtf(sum_of_all<THREADS>(scaled, shared) / (float)a.cols + a.eps * scale * scale);
+    const float first = small ? scale : by, second = small ? by : scale;  // (in this order products of elements that matter stay within 32 bits' range)
+    again([&](int p, const float (&t)[8]) {
+      W w;
+      float out[8];
+      if (a.weight) w.load(a.weight, p, a.cols);
+      if (sum) P::store(sum, p, a.cols, t);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) out[i] = a.weight ? t[i] * first * second * w.at(i) : t[i] * first * second;
+      P::store(y, p, a.cols, out);
+    });
+    return;
+  }
+  const float by = 1.f / sqrtf(under);
   auto finish = [&](int p, const W& w, const float (&v)[8]) {
     if (sum) P::store(sum, p, a.cols, v);
     float out[8];
