@@ -18,3 +18,12 @@ def test_shares_that_would_pass_31_bits(sequences, quanta):
     with pytest.raises(T.TetrisError) as e:
         c.attend(A, B, T.BF16, kv_heads, sequences, A, A, 128 * quanta)
     assert e.value.code == T.EUNSUPPORTED
+
+
+@pytest.mark.parametrize("sequences,heads,most_rows,most_length", [(2 ** 31 - 1, 1024, 40, 2 ** 28), (2 ** 31 - 1, 1, 2 ** 30, 2 ** 28), (2 ** 31 - 1, 1024, 1, 0)])
+def test_more_units_than_31_bits_hold(sequences, heads, most_rows, most_length):
+    """Units times quanta of the first pass 64 bits; the size that is refused may not be what is left of that."""
+    c = T.MX4Cache(A, 4, heads, 32, page=16)
+    with pytest.raises(T.TetrisError) as e:
+        c.attend(A, B, T.BF16, heads, sequences, A, A, most_length, d_first=A, rows=2 ** 30 // heads, most_rows=most_rows)
+    assert e.value.code == T.EUNSUPPORTED

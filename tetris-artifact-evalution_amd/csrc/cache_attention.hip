@@ -1120,7 +1120,7 @@ Cut cut_of(const tetris_cache* c, const tetris_attention* a, int type) {
   }
   const int64_t span = a->window ? std::min<int64_t>(a->most_length, (int64_t)a->window + a->most_rows + kStep) : a->most_length;
   const int64_t quanta = std::max<int64_t>((span + kQuantum - 1) / kQuantum, 1);
-  k.most = k.units * (quanta + kBegin);
+  k.most = k.units > 0x7fffffff ? k.units : k.units * (quanta + kBegin);  // (a call of so many units is refused, and the product of both may pass 64 bits)
   const int resident = 256 * waves_of(parts_of(type), c->head, k.tiles);
   if (a->sequences > 1 && k.most >= 16 * (int64_t)resident) {
     k.workgroups = resident;
