@@ -40,7 +40,7 @@ struct Attend {
   float* part;  // [2 workgroups][16 NT rows]: maximum and sum, then outputs (struct Slot)
   int2* shares; // of a unit: the first workgroup that has some of it, and how many have
   int64_t page_bytes, ldt, ldq, ldy;
-  int pages, page, granules, kv_heads, heads, group, sequences, rows, most_rows, most_length, window;
+  int pages, granules, kv_heads, group, sequences, rows, most_rows, most_length, window;
   int tiles;   // NT
   int blocks;  // most blocks of 16 NT rows of a sequence and kv head
   int workgroups;
@@ -1233,8 +1233,8 @@ extern "C" int tetris_cache_attend(tetris_cache* c, const tetris_attention* a, c
   t.part = reinterpret_cast<float*>(d);
   t.shares = reinterpret_cast<int2*>(d + k.part);
   t.page_bytes = c->page_bytes; t.ldt = ld_table; t.ldq = ldq; t.ldy = ldy;
-  t.pages = c->pages; t.page = c->page; t.granules = c->page / kGranule;
-  t.kv_heads = c->kv_heads; t.heads = a->heads; t.group = a->heads / c->kv_heads;
+  t.pages = c->pages; t.granules = c->page / kGranule;
+  t.kv_heads = c->kv_heads; t.group = a->heads / c->kv_heads;
   t.sequences = a->sequences; t.rows = a->rows; t.most_rows = std::min(a->most_rows, a->rows); t.most_length = a->most_length;
   t.window = std::min(a->window, a->most_length);
   t.tiles = k.tiles; t.blocks = k.blocks; t.workgroups = k.workgroups; t.chunk = k.chunk; t.chunks = k.chunks;
