@@ -72,10 +72,12 @@ int tetris_cache_read(tetris_cache* c, const int64_t* d_slot, int tokens, void* 
  * apart; a number outside of the pool stands for a page that no row sees.  The lengths, tables and offsets are read on the device: a captured
  * launch serves whatever they hold when it is replayed.
  * Products are of the cache's exact values and of q in 1, 2 or 3 bf16 parts (bf16, f16, f32: no bit is lost), summed in 32 bits, as are
- * the softmax and its sums.  Its weights enter the second product with 16 bits, for f32 with 24; where a call has many rows in bf16, with 11, which is a
- * sixteenth of what the output is rounded by.  Results do not depend on the order in which anything runs.
+ * the softmax and its sums.  Its weights enter the second product with 16 bits, for f32 with 24; where a call has many rows in bf16, with 11 (2^-11 of a weight),
+ * an eighth of what the output is rounded by.  Results do not depend on the order in which anything runs.
  * Workspace is the cache's, one per stream as in tetris_mx4.h; tetris_cache_prepare makes it ahead of a graph capture, for calls of
  * these sizes or smaller sequences, most_rows and most_length with as many or fewer rows.
+ * Sizes that are more than a launch has (2^24 workgroups, or for all sequences' kv heads and rows together some 2^31 times 128 tokens) are refused with
+ * TETRIS_EUNSUPPORTED.
  * ---------------------------------------------------------------------------------------------- */
 typedef struct {
   int32_t heads, sequences, rows, most_rows, most_length, window; /* window 0: none */

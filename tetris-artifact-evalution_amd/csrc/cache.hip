@@ -1,6 +1,8 @@
 // The cache of keys and values in MX4: keys and values rounded into their slots, and read back.  One pass over memory, bound by HBM and by stores of
-// 4 bytes that are spread over a granule: 16384 tokens of 8 heads of 128 bf16 written and read take 45 us together (170 MB, 3.8 TB/s); a token of each of
-// 64 sequences is two launches, 5.4 us.
+// 4 bytes that are spread over a granule: 16384 tokens of 8 heads of 128 bf16 written and read take 45 us together (170 MB, 3.8 TB/s; 41 where the last-level cache
+// has some of it); a token of each of 64 sequences is two launches, 5.4 us.  A lane's eight elements of a value are one word only in heads of 128 and 256, which take 1.13 to
+// 1.17 times what the bytes do at a copy's rate; heads of 64 go by two bytes and those of 96, 160, 192 and 224 by one, 1.31 to 1.41 times (23 us at 64, 69 at 192), and those of
+// 32 by one at 1.75 (15 us).
 #include <new>
 
 #include "cache.h"

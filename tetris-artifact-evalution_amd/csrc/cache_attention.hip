@@ -6,7 +6,8 @@
 //   outputs   O^T [elements][rows] += V^T P^T     the same instruction; the page's layout (csrc/cache.h) gives a lane the values of the tokens whose
 //                                               weights it holds, so that weights go from one product to the next without leaving the lane
 // A key or value has two significant bits and its scale's exponent: exact in bf16.  q comes in 1, 2 or 3 bf16 parts (bf16, f16, f32), which hold
-// all of its bits, and P in two (16 bits; f32: three; attend_prompt_kernel has one of 11 bits for bf16), so outputs are those of 32-bit arithmetic rounded once.
+// all of its bits.  P comes in three for f32, which hold all of it, else in two, within 2^-16 of it (attend_prompt_kernel has one f16 for bf16, within 2^-11):
+// a product an output costs less, and an output of f16 or bf16 is rounded by up to 2^-11 or 2^-8.  Sums, the softmax's statistics and outputs are of 32 bits until then.
 // m is raised only to a score that is more than 8 above it (weights are at most 2^8, far from overflow); most steps need no exchange
 // between lanes for it.  A row's sum stays apart in four lanes until the end.
 //
@@ -425,7 +426,8 @@ __device__ inline unsigned page_index(const Attend& a, unsigned granule) { retur
 // How the work is dealt out.  A unit is a block of 16 NT rows of a sequence and kv head; it is as many quanta of four steps as its sequence
 // tokens that its rows see (one at least: rows that see nothing become zeros).  What a workgroup does of a unit that it does not do all of it leaves to join_kernel.
 //   little work     a.chunk quanta of one unit each; chunks that a sequence is too short for end at once.  It begins without looking at the
-//                   other sequences: one token of 4000 tokens by 32 heads takes 10 us in place of 13.
+//                   other sequences: one token of 4000 tokens by 32 heads takes 11 us in place of 13.  A chunk goes by most_length, which
+//                   may be far more than there is: the same in a call made for 131072 tokens takes 17, with 32 kv heads 36 in place of 12.
 //   much work       the units' quanta, sequence after sequence, in equal shares, whatever the lengths are: 64 sequences of up to 8192 tokens, 3700 on
 //                   average, take 61 us (68 in place of 86 when both were measured).
 constexpr int kQuantum = 4 * kStep;
@@ -593,7 +595,10 @@ __device__ inline void attend_unit(const Attend& a, const Sequence& seq, int qua
 // Waves of a SIMD, and so workgroups of a compute unit, that the registers of a wave leave room for.
 constexpr int kResidentMost = 256 * 4;  // workgroups that run at once, for any of them
 constexpr int waves_of(int parts, int head, int tiles) { return parts * tiles * head <= 64 ? 4 : tiles * head <= 128 && parts * tiles * head <= 256 ? 3 : 2; }
-// (Two waves a SIMD at least: with 256 registers or fewer the products' sums stay in ordinary registers, not in those that have to be copied for the rest.)
+// (Two waves a SIMD at least: with 256 registers or fewer the products' sums stay in ordinary registers, not in those that have to be copied for the rest.
+// 21 of the 94 forms keep some of theirs in memory for that: of f32 heads of 96 by two tiles and of 160 to 256, of f16 heads of 64 by two tiles (6 registers), of
+// 192 to 256 and prompts of 128, of bf16 heads of 192 and 224.  f32 at 224 has the most, 263 and 320: 64 sequences of 4096 tokens by 4 kv heads take 309 us, at
+// 256, with 105 and 43, 131, and 97 and 72 in bf16.)
 template <int TYPE, int D, int NT>
 __global__ __launch_bounds__(256, waves_of(kParts<TYPE>, D, NT)) void attend_chunks_kernel(Attend a) {
   int id = blockIdx.x / a.chunks;
@@ -654,8 +659,8 @@ __device__ inline void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_b
 // addresses) 112, LDS 100; a wave needs them one after another, and the registers leave room for two waves a SIMD.
 //
 // A weight of bf16 operators enters the second product as f16, 2^7 as large as it is (2^15 at most), with values that are exact in f16: one
-// product in place of two, and one conversion of a pair of weights in place of six instructions.  It is within 2^-12 of itself, or 2^-32 of the row's
-// largest; a row's sum is of the weights as they are multiplied.  Where some
+// product in place of two, and one conversion of a pair of weights in place of six instructions.  It is within 2^-11 of the weight, an eighth of what the
+// output's own rounding may be off by, or within 2^-32 of the row's largest; a row's sum is of the weights as they are multiplied.  Where some
 // values are beyond f16's range a workgroup begins again with bf16, and weights in two parts.
 constexpr int kPromptWaves = 4, kTurn = 64, kShift = 7;
 constexpr int kNan = 1, kBf16 = 2;
@@ -1154,6 +1159,9 @@ int launch(Attend a, const Cut& k, hipStream_t s) {
   TETRIS_HIP(hipGetLastError());
   if (k.chunks == 1) return TETRIS_OK;
   const dim3 joins((unsigned)(k.units * 4 * k.tiles));
+  // Four waves to join the parts of rows that have few, sixteen for more: 64 sequences of up to 8192 tokens (768 workgroups of 512 units) 68 us against 75, 24 of
+  // drafts (432 of 144) 26 against 29, 24 of 4000 (768 of 192) 32 against 34; two of 131072 (752 of 8) 50 against 44, one of 4000 (256 of 8) 12.3 against 11.1; as fast
+  // either way where a unit has 6 (16 of 2048).
   if (k.workgroups <= 4 * k.units) hipLaunchKernelGGL((join_kernel<TYPE, D, 4>), joins, block, 0, s, a);
   else hipLaunchKernelGGL((join_kernel<TYPE, D, 16>), joins, dim3(1024), 0, s, a);
   TETRIS_HIP(hipGetLastError());

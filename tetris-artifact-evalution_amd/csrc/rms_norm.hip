@@ -1,6 +1,8 @@
 // The residual's addition with a root-mean-square norm: s = x + r, y = s / sqrt(mean(s^2) + eps) * w.  A workgroup has a row, which
-// stays in registers between the sum of squares and the outputs, so that memory is passed once; bound by HBM (8192 rows of 4096 bf16, with
-// residual and sum: 49 us for 268 MB, 5.5 TB/s, some of it from the last-level cache), and for few rows by the launch (8 rows: 3.3 us).
+// stays in registers between the sum of squares and the outputs up to 8192 columns, so that memory is passed once (what lies beyond is read twice, mostly from the caches: 8192
+// rows of 16384 bf16 193 us, 5.6 TB/s of what has to pass); bound by HBM (8192 rows of 4096 bf16, with
+// residual and sum: 50 us for 268 MB, 5.4 TB/s, some of it from the last-level cache), for few rows by the launch (8 rows: 3.3 us), and for rows of a head by a workgroup's
+// beginning (262144 of 128: 80 us, 3.4 TB/s).
 #include <algorithm>
 #include <type_traits>
 
@@ -200,11 +202,13 @@ void launch(const NormRows& a, int64_t rows, hipStream_t s) {
     b.y = static_cast<char*>(a.y) + from * a.ldy * size;
     const dim3 grid((unsigned)std::min(kMost, rows - from));
 #define TETRIS_NORM(THREADS, KEPT) hipLaunchKernelGGL((rms_norm_kernel<TYPE, THREADS, KEPT, VEC>), grid, dim3(THREADS), 0, s, b)
+    // Many rows: fewer threads with two pieces each, so that a compute unit has several rows under way.  512 rows of 4096 bf16 4.95 us against 5.5 with 1024 threads, 2048
+    // 12.4 against 14.2, 2048 of f32 27.9 against 29.4, 1024 of 8192 bf16 13.1 against 14.0; at 64 rows the two are as fast.
     if (a.cols <= 512) TETRIS_NORM(64, 1);
     else if (a.cols <= 2048) TETRIS_NORM(256, 1);
     else if (a.cols <= 4096 && rows >= 512) TETRIS_NORM(256, 2);
     else if (a.cols <= 8192 && rows >= 512) TETRIS_NORM(512, 2);
-    else TETRIS_NORM(1024, 1);  // few rows: all of a row's loads at once
+    else TETRIS_NORM(1024, 1);  // all of a row's loads at once
 #undef TETRIS_NORM
   }
 }

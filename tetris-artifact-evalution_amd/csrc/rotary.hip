@@ -4,7 +4,7 @@
 // are a launch, 3.3 us.
 //
 // A pair's angle in turns is formed in 64 bits and its whole turns taken off, which leaves a far position's angle exact to about
-// 2^-49 of the position.  What is left goes to 32 bits as t + d with d below 2^-25 t, and cos(t + d) = cos t - d sin t, so that the cosine is
+// 2^-49 of the position.  What is left goes to 32 bits as t + d with |d| at most 2^-25 (half turns, |t| at most 1), and cos(t + d) = cos t - d sin t, so that the cosine is
 // as near as one rounded from 64 bits.
 #include <algorithm>
 #include <cmath>
