@@ -8,6 +8,7 @@ T = pytest.importorskip("tetris_amd")
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
+from test_gpu_attention import out_like, untouched  # noqa: E402
 from test_gpu_mx4 import TYPES, numbers, on_gpu, rounded_to, within  # noqa: E402
 
 
@@ -59,3 +60,26 @@ def test_rows_that_have_no_norm():
     T.rms_norm(x.data_ptr(), y.data_ptr(), T.F32, 3, 4096, eps=0.0)
     assert y[0].isnan().all() and y[2].isnan().all()  # 0 / 0
     assert y[1, 5].isnan() and (y[1, :5] == 0).all() and (y[1, 6:] == 0).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols,pad,offset", [(3, 100, 3, 1), (4, 2048, 8, 8), (512, 4096, 0, 0), (514, 4100, 1, 0), (600, 8192, 0, 0), (5, 8200, 8, 0), (3, 20001, 0, 3)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_their_sums(kind, rows, cols, pad, offset, in_place):
+    """Every third row large and every third small, their sums written beside the norm or in the residual's place, nothing around them."""
+    rng = np.random.default_rng(rows + cols)
+    by = np.exp2(np.array([0.0, 80.0, -70.0]))[np.arange(rows) % 3, None]
+    x, r = (rounded_to(rng.normal(size=(rows, cols)) * by, kind) for _ in range(2))
+    w = rounded_to(rng.normal(size=cols), "f32")
+    dw = torch.from_numpy(w).float().cuda()
+    ld = cols + pad
+    dx, dr = on_gpu(x, kind, ld, offset), on_gpu(r, kind, ld, offset)
+    (y, around), (other, around_other) = (out_like(rows, cols, kind, ld, offset) for _ in range(2))
+    total = dr if in_place else other
+    T.rms_norm(dx.data_ptr(), y.data_ptr(), TYPES[kind][0], rows, cols, d_weight=dw.data_ptr(), eps=0.0, d_residual=dr.data_ptr(), d_sum=total.data_ptr(), ldx=ld,
+               ldy=ld, ld_residual=ld, ld_sum=ld)
+    s, far_s, want, far = P.rms_norm(x, r, w, 0.0, kind)
+    within(numbers(y), want, far)
+    within(numbers(total), s, far_s)
+    untouched(around, y)
+    untouched(around_other, other)
